@@ -45,6 +45,22 @@ I64 = ctypes.c_int64
 I32 = ctypes.c_int32
 SZ = ctypes.c_size_t
 
+
+class KvCache(ctypes.Structure):
+    """hm_kv_cache."""
+
+    _fields_ = [("k", P), ("v", P), ("pages", I64), ("page_size", I64), ("page_stride", I64), ("head_stride", I64), ("token_stride", I64),
+                ("kv_heads", I32), ("head_dim", I32), ("dtype", I32)]
+
+
+class QkNormRopeArgs(ctypes.Structure):
+    """hm_qk_norm_rope_args."""
+
+    _fields_ = [("qkv", P), ("ldqkv", I64), ("q", P), ("ldq", I64), ("k", P), ("ldk", I64), ("bias", P), ("q_weight", P), ("k_weight", P),
+                ("frequencies", P), ("positions", P), ("slots", P), ("rows", I64), ("q_heads", I32), ("kv_heads", I32), ("head_dim", I32),
+                ("rotary_dim", I32), ("eps", ctypes.c_float), ("interleaved", I32), ("dtype", I32)]
+
+
 # name: (restype, argtypes)
 _SIGNATURES = {
     "hm_abi_version": (ctypes.c_int, []),
@@ -92,6 +108,10 @@ _SIGNATURES = {
     "hm_residual_add2_mixed": (ctypes.c_int, [P, I64, P, I64, I32, P, I64, I32, I64, I64, ctypes.c_int, P]),
     "hm_find_nonfinite": (I64, [P, I64, I64, I64, ctypes.c_int, I32]),
     "hm_find_nonfinite_device": (ctypes.c_int, [P, I64, I64, I64, ctypes.c_int, I32, P, P]),
+    "hm_page_plan": (ctypes.c_int, [P, P, I64, P, I64, I64, I64, P, I64, P, P, P, P, I64, P, P, P, P]),
+    "hm_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(QkNormRopeArgs), ctypes.POINTER(KvCache), P]),
+    "hm_paged_attention_workspace_bytes": (SZ, [ctypes.POINTER(KvCache), I64]),
+    "hm_paged_attention": (ctypes.c_int, [ctypes.POINTER(KvCache), P, I64, P, I64, I64, I64, P, I64, I64, I64, P, P, ctypes.c_float, I64, P, SZ, P]),
     "hm_partition_check": (ctypes.c_int, [I64, I64, I64]),
     "hm_partition_from_ratio": (ctypes.c_int, [I64, ctypes.c_double, I64, ctypes.POINTER(I64)]),
     "hm_split_type": (I32, [I32, I32, I32, I32, I32, I32]),

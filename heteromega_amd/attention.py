@@ -1,0 +1,278 @@
+"""Attention over a paged key-value cache: the operators between a layer's Q/K/V projection and its O projection, over the
+C ABI (include/hm_w4a16.h), and a layer's attention block made of them.
+
+The reference's model keeps one contiguous cache per sequence and runs RoPE and decode attention on it
+(src/hipkernels/flash_attn_decode.cu); here a step's requests share a cache of pages. A serving loop calls page_plan once
+per step, and each layer then qk_norm_rope and paged_attention (or AttnLayer.block_forward, which calls both). Nothing waits for
+the host: lengths, page ids and counters stay in device memory, so a step can be captured in a graph.
+"""
+
+import contextlib
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .ffn import (_DTYPES, _aligned, _call, _handed_over, _hm_dtype, _on, _stream, _workspace, packed_linear, residual_add2, rmsnorm)
+
+kPagePlanMaxRequests = 4096
+
+
+def _guard(device):
+    """The device of the tensors as the current one: a launch goes to the current device."""
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _device_of(t, what):
+    device = t.device
+    if device.type != "cuda":
+        raise ValueError(f"{what}: needs device tensors, got one on {device}")
+    return device
+
+
+def _ints(t, dtype, n, device, what, name):
+    """Address of a contiguous vector of at least n integers."""
+    if t.dtype != dtype or t.dim() != 1 or t.size(0) < n or (t.size(0) > 1 and t.stride(0) != 1) or t.device != device:
+        raise ValueError(f"{what}: {name} must be a contiguous {dtype} vector of {n} or more elements on {device}")
+    return t.data_ptr()
+
+
+def _vector(t, dtype, n, device, what, name):
+    if t is None:
+        return None
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{what}: {name} must be a contiguous {dtype} vector of {n} elements on {device}")
+    return t.data_ptr()
+
+
+def _rows(t, rows, heads, d, dtype, device, what, name):
+    """(address, leading dimension) of [rows, heads * d] or [rows, heads, d] with packed heads."""
+    width = heads * d
+    if t.dim() == 3:
+        ok = t.size(1) == heads and t.size(2) == d and (d == 1 or t.stride(2) == 1) and (heads == 1 or t.stride(1) == d)
+    else:
+        ok = t.dim() == 2 and t.size(1) == width and t.stride(1) == 1
+    if not ok or t.size(0) != rows or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{what}: {name} must be {dtype} [{rows}, {heads} x {d}] with contiguous rows on {device}")
+    return t.data_ptr(), (t.stride(0) if rows > 1 else width)
+
+
+def _table(t, device, what):
+    if t.dtype != torch.int32 or t.dim() != 2 or (t.size(1) > 1 and t.stride(1) != 1) or t.device != device:
+        raise ValueError(f"{what}: block_table must be int32 [requests, pages of a request] with contiguous rows on {device}")
+    return t.data_ptr(), max(t.stride(0), t.size(1)) if t.size(0) == 1 else t.stride(0), t.size(0), t.size(1)
+
+
+def rope_frequencies(rotary_dim, base=10000.0, device=None, llama3_scaling=None):
+    """Radians per position of the rotary_dim / 2 pairs, base^(-2 i / rotary_dim), fp64 (qk_norm_rope's frequencies).
+    llama3_scaling: (factor, low_freq_factor, high_freq_factor, original_context), as in the configuration of Llama 3.1 and 3.2
+    models: pairs that turn less than low_freq_factor times in the original context are slowed down by factor, those that turn more than
+    high_freq_factor times are kept, and those between are interpolated."""
+    freq = []
+    for i in range(rotary_dim // 2):
+        f = base ** (-2.0 * i / rotary_dim)
+        if llama3_scaling is not None:
+            factor, low, high, context = llama3_scaling
+            turns = context * f / (2.0 * math.pi)
+            keep = min(1.0, max(0.0, (turns - low) / (high - low)))
+            f = f * keep + f / factor * (1.0 - keep)
+        freq.append(f)
+    return torch.tensor(freq, dtype=torch.float64, device=device)
+
+
+class PagedCache:
+    """One layer's keys and values in pages, k and v [pages, kv_heads, page_size, head_dim] of one shape and one set of strides, the
+    last dimension contiguous (a [pages, page_size, kv_heads, head_dim] array fits as its transpose(1, 2))."""
+
+    def __init__(self, k, v):
+        device = _device_of(k, "PagedCache")
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or v.device != device:
+            raise ValueError("PagedCache: k and v must be [pages, kv_heads, page_size, head_dim] alike in shape, strides, type and device")
+        if k.stride(3) != 1:
+            raise ValueError("PagedCache: the head dimension must be contiguous")
+        self.k, self.v, self.device, self.dtype = k, v, device, k.dtype
+        self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        # a dimension of one element may have any stride
+        strides = [s if n > 1 else self.head_dim for s, n in zip(k.stride()[:3], k.shape[:3])]
+        self._c = _lib.KvCache(k.data_ptr(), v.data_ptr(), self.pages, self.page_size, *strides, self.kv_heads, self.head_dim, _hm_dtype(k.dtype))
+        self._ref = ctypes.byref(self._c)
+
+    @classmethod
+    def empty(cls, pages, page_size, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda"):
+        """A new cache; its contents are read only where tokens were written."""
+        device = torch.device(device)
+        return cls(*(torch.empty((pages, kv_heads, page_size, head_dim), dtype=dtype, device=device) for _ in range(2)))
+
+    def attention_workspace_bytes(self, q_heads):
+        return _lib.load().hm_paged_attention_workspace_bytes(self._ref, q_heads)
+
+    def attention_workspace(self, q_heads, stream=None):
+        """A workspace for paged_attention calls on one stream, for any rows and lengths."""
+        with _guard(self.device):
+            return _workspace(self.attention_workspace_bytes(q_heads), self.device, stream)
+
+
+class PagePlan:
+    """What page_plan works out for a step of up to `rows` new tokens of `requests` requests, kept from step to step (a captured
+    step's layers read these tensors): slots, positions and requests of each row, starts of the requests' rows, and their lengths
+    and the page queue's counters after the step."""
+
+    def __init__(self, requests, rows, page_size, device="cuda"):
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        new = lambda n, t: torch.full((n,), -1, dtype=t, device=device)
+        self.page_size, self.device = page_size, device
+        self.slots, self.positions, self.requests = new(rows, torch.int64), new(rows, torch.int32), new(rows, torch.int32)
+        self.starts, self.lengths, self.queue = new(requests + 1, torch.int32), new(requests, torch.int32), new(4, torch.int64)
+
+
+def page_plan(plan, lengths, added, block_table, free_pages, queue, lengths_out=None, queue_out=None, stream=None):
+    """Pages, cache slots and positions of a step's new tokens (hm_page_plan), into `plan`. lengths, added int32 [requests]: cached tokens
+    and new ones (0: none, -1: the request has ended and gives its pages back); block_table int32 [requests, pages of a request] and
+    the ring of free pages free_pages int32 are updated in place; queue int64 [4] holds the ring's head and tail. The lengths
+    and counters after the step go to plan.lengths and plan.queue, or to lengths_out and queue_out, which may be lengths and queue.
+    plan.queue[2] counts the requests that got nothing because pages, rows or table entries did not suffice."""
+    device = _device_of(lengths, "page_plan")
+    table, ld, count, width = _table(block_table, device, "page_plan")
+    rows = plan.slots.size(0)
+    lengths_out = plan.lengths if lengths_out is None else lengths_out
+    queue_out = plan.queue if queue_out is None else queue_out
+    if plan.device != device or plan.starts.size(0) != count + 1 or lengths.size(0) != count or added.size(0) != count:
+        raise ValueError(f"page_plan: the plan, lengths and added must be of the table's {count} requests and on {device}")
+    i32, i64 = torch.int32, torch.int64
+    args = (_ints(lengths, i32, count, device, "page_plan", "lengths"), _ints(added, i32, count, device, "page_plan", "added"), count, table, ld, width,
+            plan.page_size, _ints(free_pages, i32, 1, device, "page_plan", "free_pages"), free_pages.size(0),
+            _ints(queue, i64, 2, device, "page_plan", "queue"), plan.slots.data_ptr(), plan.positions.data_ptr(), plan.requests.data_ptr(), rows,
+            plan.starts.data_ptr(), _ints(lengths_out, i32, count, device, "page_plan", "lengths_out"),
+            _ints(queue_out, i64, 4, device, "page_plan", "queue_out"))
+    with _guard(device):
+        _call(_lib.load().hm_page_plan(*args, _stream(stream, device)))
+    return plan
+
+
+def qk_norm_rope(q_out, qkv, frequencies, positions, cache=None, slots=None, k_out=None, kv_heads=None, head_dim=None, q_weight=None, k_weight=None,
+                 bias=None, eps=1e-6, interleaved=False, stream=None):
+    """Q/K/V rows made ready for attention (hm_qk_norm_rope): bias, RMSNorm of each query and key head (q_weight, k_weight
+    [head_dim]; None: no norm), rotation by position * frequencies (fp64 radians per position; fewer than head_dim / 2: only that part of the head),
+    fp32 with one rounding. qkv [rows, (q_heads + 2 kv_heads) * head_dim]; queries go to q_out [rows, q_heads (x) head_dim]. With a
+    cache, keys and values go to their slots; without one, keys go to k_out and kv_heads and head_dim are given. q_out and
+    k_out may be their columns of qkv. Rows with a negative position are left as they are."""
+    device = _device_of(qkv, "qk_norm_rope")
+    dtype = qkv.dtype
+    if cache is not None:
+        if k_out is not None or slots is None:
+            raise ValueError("qk_norm_rope: a cache takes slots and no k_out")
+        kv_heads, head_dim = cache.kv_heads, cache.head_dim
+        if cache.dtype != dtype or cache.device != device:
+            raise ValueError(f"qk_norm_rope: the cache must be {dtype} on {device}")
+    elif k_out is None or slots is not None or not kv_heads or not head_dim:
+        raise ValueError("qk_norm_rope: without a cache, needs k_out, kv_heads and head_dim and no slots")
+    if qkv.dim() != 2 or head_dim <= 0 or qkv.size(1) % head_dim or qkv.size(1) // head_dim <= 2 * kv_heads:
+        raise ValueError(f"qk_norm_rope: qkv must be [rows, (q_heads + 2 x {kv_heads}) x {head_dim}]")
+    rows, heads = qkv.size(0), qkv.size(1) // head_dim
+    q_heads = heads - 2 * kv_heads
+    what = "qk_norm_rope"
+    a = _lib.QkNormRopeArgs()
+    a.qkv, a.ldqkv = _rows(qkv, rows, heads, head_dim, dtype, device, what, "qkv")
+    a.q, a.ldq = _rows(q_out, rows, q_heads, head_dim, dtype, device, what, "q_out")
+    if cache is None:
+        a.k, a.ldk = _rows(k_out, rows, kv_heads, head_dim, dtype, device, what, "k_out")
+    else:
+        a.slots = _ints(slots, torch.int64, rows, device, what, "slots")
+    a.positions = _ints(positions, torch.int32, rows, device, what, "positions")
+    a.rotary_dim = 2 * frequencies.numel()
+    a.frequencies = _vector(frequencies, torch.float64, frequencies.numel(), device, what, "frequencies")
+    a.bias = _vector(bias, dtype, heads * head_dim, device, what, "bias")
+    a.q_weight = _vector(q_weight, dtype, head_dim, device, what, "q_weight")
+    a.k_weight = _vector(k_weight, dtype, head_dim, device, what, "k_weight")
+    a.rows, a.q_heads, a.kv_heads, a.head_dim = rows, q_heads, kv_heads, head_dim
+    a.eps, a.interleaved, a.dtype = eps, bool(interleaved), _hm_dtype(dtype)
+    with _guard(device):
+        _call(_lib.load().hm_qk_norm_rope(ctypes.byref(a), cache._ref if cache is not None else None, _stream(stream, device)))
+    return q_out
+
+
+def paged_attention(out, q, cache, block_table, positions, requests=None, scale=None, window=0, stream=None, workspace=None):
+    """out[t, h] = softmax(scale q[t, h] K^T) V over keys 0..positions[t] (its last `window` ones, if not 0) of row t's request in the
+    paged cache (hm_paged_attention). q, out [rows, q_heads, head_dim]; block_table int32 [requests, pages of a request]; row t is of request
+    requests[t], or t. Position -1: zeros; a negative request: the row is left as it is; a row outside the table or the
+    cache: NaN. scale: 1 / sqrt(head_dim) by default. workspace: cache.attention_workspace(q_heads), one per stream."""
+    what = "paged_attention"
+    device = cache.device
+    d = cache.head_dim
+    rows = q.size(0)
+    q_heads = q.size(1) if q.dim() == 3 else q.size(-1) // d
+    qp, ldq = _rows(q, rows, q_heads, d, cache.dtype, device, what, "q")
+    op, ldo = _rows(out, rows, q_heads, d, cache.dtype, device, what, "out")
+    table, ld, count, width = _table(block_table, device, what)
+    pp = _ints(positions, torch.int32, rows, device, what, "positions")
+    rp = _ints(requests, torch.int32, rows, device, what, "requests") if requests is not None else None
+    with _guard(device):
+        if workspace is None:
+            workspace = cache.attention_workspace(q_heads, stream)
+        wp, wb = _aligned(workspace)
+        _call(_lib.load().hm_paged_attention(cache._ref, op, ldo, qp, ldq, rows, q_heads, table, ld, count, width, pp, rp,
+                                             1.0 / math.sqrt(d) if scale is None else scale, window, wp, wb, _stream(stream, device)))
+    return out
+
+
+class AttnLayer:
+    """A layer's attention block over its paged cache, the counterpart of FfnLayer.block_forward: x += attention(RMSNorm(x)) Wo.
+    wqkv [hidden, (q_heads + 2 kv_heads) * head_dim] and wo [q_heads * head_dim, hidden] are RepackedMatrix (RepackedMatrix.concat makes
+    wqkv of three); frequencies as rope_frequencies gives them; bias of the Q/K/V columns, q_weight and k_weight of normed heads or None."""
+
+    def __init__(self, wqkv, wo, q_heads, kv_heads, head_dim, frequencies, bias=None, q_weight=None, k_weight=None, qk_eps=1e-6, scale=None, window=0,
+                 interleaved=False):
+        if wqkv.n != (q_heads + 2 * kv_heads) * head_dim or wo.k != q_heads * head_dim or wo.n != wqkv.k or wo.dtype != wqkv.dtype:
+            raise ValueError(f"AttnLayer: wqkv [{wqkv.k}, {wqkv.n}] and wo [{wo.k}, {wo.n}] do not fit {q_heads} + 2 x {kv_heads} heads of {head_dim}")
+        if wqkv.dtype not in _DTYPES or q_heads % kv_heads:
+            raise ValueError("AttnLayer: query heads must be a multiple of key heads")
+        self.wqkv, self.wo, self.q_heads, self.kv_heads, self.head_dim = wqkv, wo, q_heads, kv_heads, head_dim
+        self.hidden, self.dtype, self.device = wqkv.k, wqkv.dtype, wqkv.device
+        self.frequencies, self.bias, self.q_weight, self.k_weight, self.qk_eps = frequencies, bias, q_weight, k_weight, qk_eps
+        self.scale, self.window, self.interleaved = scale, window, interleaved
+        self._buffers = {}
+
+    def _scratch(self, rows, cache, stream):
+        """(normed or projected rows, Q/K/V rows, attention rows, workspaces) of calls on this stream, grown as needed."""
+        key = _stream(stream, self.device)
+        kept = self._buffers.get(key)
+        if kept is None or kept[0].size(0) < rows:
+            with _on(stream, self.device):
+                new = lambda n: torch.empty((rows, n), dtype=self.dtype, device=self.device)
+                linear = max(w.workspace_bytes(m) for w in (self.wqkv, self.wo) for m in (rows, min(rows, 16)))
+                kept = self._buffers[key] = (new(self.hidden), new(self.wqkv.n), new(self.wo.k), _workspace(linear, self.device, stream),
+                                             cache.attention_workspace(self.q_heads, stream))
+        return tuple(t[:rows] for t in kept[:3]) + kept[3:]
+
+    def block_forward(self, x, norm_weight, cache, plan, block_table, eps=1e-5, stream=None):
+        """In place: x [rows, hidden] += attention(RMSNorm(x) * norm_weight) Wo. The rows are those of `plan` (page_plan of this step): their keys and values
+        are written to `cache` first, and each row sees its request's tokens up to its own. Rows that the plan left empty stay as they are.
+        Each row reads the cache by itself, so long prompts cost the square of their length in cache reads."""
+        rows = plan.slots.size(0)
+        if x.dim() != 2 or x.size(0) != rows or x.size(1) != self.hidden or x.stride(1) != 1 or x.dtype != self.dtype or x.device != plan.device:
+            raise ValueError(f"AttnLayer.block_forward: x must be {self.dtype} [{rows}, {self.hidden}] on {plan.device}")
+        if norm_weight.numel() != self.hidden or norm_weight.dtype != x.dtype or not norm_weight.is_contiguous():
+            raise ValueError(f"norm_weight must be a contiguous {x.dtype} vector of {self.hidden} elements")
+        if (cache.kv_heads, cache.head_dim, cache.page_size) != (self.kv_heads, self.head_dim, plan.page_size):
+            raise ValueError("AttnLayer.block_forward: the cache's heads and page size must be the layer's and the plan's")
+        with _guard(self.device):
+            normed, qkv, heads, linear_ws, attention_ws = self._scratch(rows, cache, stream)
+            rmsnorm(normed, x, norm_weight, eps, stream)
+            packed_linear(qkv, normed, self.wqkv, stream=stream, workspace=linear_ws)
+            q = qkv[:, :self.q_heads * self.head_dim]
+            qk_norm_rope(q, qkv, self.frequencies, plan.positions, cache=cache, slots=plan.slots, q_weight=self.q_weight, k_weight=self.k_weight,
+                         bias=self.bias, eps=self.qk_eps, interleaved=self.interleaved, stream=stream)
+            with _on(stream, self.device):
+                heads.zero_()  # the rows that the plan left empty add nothing
+            paged_attention(heads, q, cache, block_table, plan.positions, plan.requests, self.scale, self.window, stream, attention_ws)
+            packed_linear(normed, heads, self.wo, stream=stream, workspace=linear_ws)
+            residual_add2(x, normed, stream=stream)
+        return x
+
+
+__all__ = ["kPagePlanMaxRequests", "rope_frequencies", "PagedCache", "PagePlan", "page_plan", "qk_norm_rope", "paged_attention", "AttnLayer"]

@@ -128,6 +128,18 @@ __device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t r, uint8_t *lds
 #endif
 }
 
+// Four 16-bit elements per lane of LDS, transposed over each 16 lanes (ds_read_b64_tr_b16): lane l of the 16 names 8 bytes, the
+// columns 4 (l % 4) .. + 3 of row l / 4 of a 4 x 16 block, and gets column l of its rows 0..3. Only the device pass sees the builtin.
+__device__ __forceinline__ uint2 lds_read_transposed(const uint8_t *lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef short short4_t __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t *)lds));
+#else
+    (void)lds;
+    return uint2{};
+#endif
+}
+
 // Workgroup barrier for LDS traffic only: waits for this wave's LDS operations and is a compiler memory
 // barrier, but unlike __syncthreads() it does not wait for the wave's outstanding global loads (the
 // workgroup-scope fence of __syncthreads() waits for vmcnt(0)).

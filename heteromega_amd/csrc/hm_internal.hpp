@@ -172,4 +172,68 @@ hipError_t launch_residual_add2_mixed(uint16_t *x, int64_t ldx, const void *a, i
 hipError_t launch_find_nonfinite(const uint16_t *x, int64_t ld, int64_t rows, int64_t cols, int64_t stride, int dtype, int64_t *first,
                                  hipStream_t stream);
 
+// One step's page plan (hm_page_plan).
+struct PagePlanArgs {
+    const int32_t *lengths, *added;
+    int64_t requests_count;
+    int32_t *block_table;
+    int64_t ld_table, width;
+    int page_shift;
+    int32_t *free_pages;
+    int64_t ring_size;
+    const int64_t *queue_in;
+    int64_t *slots;
+    int32_t *positions, *requests;
+    int64_t rows;
+    int32_t *starts, *lengths_out;
+    int64_t *queue_out;
+};
+hipError_t launch_page_plan(const PagePlanArgs &a, hipStream_t stream);
+
+// Q/K/V rows made ready for attention (hm_qk_norm_rope). heads: those worked on (queries, keys and, with slots, values).
+struct QkNormRopeArgs {
+    const uint16_t *qkv;
+    int64_t ldqkv;
+    uint16_t *q;
+    int64_t ldq;
+    uint16_t *k;
+    int64_t ldk;
+    const uint16_t *bias, *q_weight, *k_weight;
+    const double *frequencies;
+    const int32_t *positions;
+    const int64_t *slots; // null: keys to k
+    uint16_t *cache_k, *cache_v;
+    int64_t pages, page_stride, head_stride, token_stride;
+    int page_shift;
+    int64_t rows;
+    int q_heads, kv_heads, heads, head_dim, rotary_dim;
+    float eps;
+    bool interleaved;
+    int dtype;
+};
+hipError_t launch_qk_norm_rope(const QkNormRopeArgs &a, hipStream_t stream);
+
+// One-token attention over a paged cache (hm_paged_attention).
+struct PagedAttentionArgs {
+    const uint16_t *k, *v;
+    int64_t pages, page_stride, head_stride;
+    int64_t token_stride;
+    int page_shift;
+    uint16_t *out;
+    int64_t ldo;
+    const uint16_t *q;
+    int64_t ldq;
+    int64_t rows;
+    int q_heads, kv_heads, head_dim;
+    const int32_t *block_table;
+    int64_t ld_table, requests_count, width;
+    const int32_t *positions, *requests;
+    float scale;
+    int64_t window;
+    void *workspace;
+    int dtype;
+};
+size_t paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t head_dim);
+hipError_t launch_paged_attention(const PagedAttentionArgs &a, hipStream_t stream);
+
 } // namespace hm

@@ -334,6 +334,108 @@ hm_status hm_residual_add2_mixed(void *x, int64_t ldx, const void *a, int64_t ld
                                  int64_t ldb, int32_t b_fp32, int64_t rows, int64_t cols, hm_dtype dtype, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Attention over a paged key-value cache: what a decoder layer runs between its
+ * Q/K/V projection and its O projection (the reference's RoPE and decode
+ * attention, src/hipkernels/flash_attn_decode.cu, keep one contiguous cache per
+ * sequence instead). A step of a serving loop calls hm_page_plan once; then
+ * each layer calls hm_qk_norm_rope (queries, and keys and values into its cache)
+ * and hm_paged_attention. A step's tokens are rows, in the order of their
+ * requests; the plan's rows behind the last token, and those of a request that
+ * it refused, carry -1 as position and request and are left as they were by
+ * the layer calls. Nothing here waits for the host, so a step can be captured
+ * in a graph and replayed with other lengths.
+ * ------------------------------------------------------------------------- */
+
+/* One layer's cache: keys and values of `pages` pages of `page_size` tokens. Token t of page p of key head h has its
+ * head_dim contiguous elements at p * page_stride + h * head_stride + t * token_stride (in elements, the same for k and
+ * v), so [page, head, token, d] and [page, token, head, d] arrays and slices of a larger one all fit. page_size: a power
+ * of two, 16 or more. k and v 16-byte aligned, strides multiples of 8, heads at least head_dim apart; a page's tokens of
+ * one head span less than 2 GiB. */
+typedef struct hm_kv_cache {
+    void *k, *v;
+    int64_t pages, page_size;
+    int64_t page_stride, head_stride, token_stride;
+    int32_t kv_heads, head_dim;
+    int32_t dtype; /* hm_dtype of the cache, of the rows next to it and of outputs */
+} hm_kv_cache;
+
+/* A step's pages, cache slots and positions from the requests' lengths, all arrays in device memory.
+ *   lengths [R]       tokens of each request that the cache holds
+ *   added [R]         new tokens of each request in this step; 0: none, negative: the request has ended
+ *   block_table [R, W] page ids of each request (leading dimension ld_table); the entries of new pages are written
+ *   free_pages [Q]    ring of free page ids: those at (i mod Q), head <= i < tail, are free
+ *   queue_in [4]      {head, tail, ...}: the counters of the ring; they only grow
+ * Results:
+ *   slots [rows]      page * page_size + offset of each row's token in the cache
+ *   positions [rows]  its position in its request (0 for the first token)
+ *   requests [rows]   its request
+ *   starts [R + 1]    first row of each request: the sum of the new tokens before it (at most `rows`)
+ *   lengths_out [R]   lengths after the step: + added, 0 for an ended request
+ *   queue_out [4]     {head, tail, requests refused, rows asked for} after the step
+ * New pages come from the head of the ring, in the order of requests and positions. An ended request's pages go
+ * behind its tail, in that order too, and can be handed out from the next call on. A request with new tokens is refused,
+ * keeping its length and its place among the rows (slots, positions and requests -1), if its length is negative or above W * page_size,
+ * if it would outgrow W pages, if its rows would end behind `rows`, or if it needs pages and it or a request before it
+ * needs more than are left. Rows behind the last token get -1 too. lengths_out may be lengths and queue_out may be
+ * queue_in; other arrays must not overlap. R up to HM_PAGE_PLAN_MAX_REQUESTS. Page ids are taken as they stand in the
+ * ring and the table; the layer calls check them against their cache. */
+#define HM_PAGE_PLAN_MAX_REQUESTS 4096
+hm_status hm_page_plan(const int32_t *lengths, const int32_t *added, int64_t R, int32_t *block_table, int64_t ld_table, int64_t W,
+                       int64_t page_size, int32_t *free_pages, int64_t Q, const int64_t *queue_in, int64_t *slots, int32_t *positions,
+                       int32_t *requests, int64_t rows, int32_t *starts, int32_t *lengths_out, int64_t *queue_out, void *stream);
+
+/* The rows of a Q/K/V projection, qkv [rows, (q_heads + 2 kv_heads) * head_dim] (ldqkv; hm_weights_concat's column
+ * order), made ready for attention. Per row, in fp32 with one rounding at the end:
+ *   x = qkv + bias                                   (bias may be NULL)
+ *   h = h * rsqrt(mean(h^2) + eps) * weight          for each query head (q_weight) and key head (k_weight); NULL: no norm
+ *   (a, b) -> (a cos - b sin, b cos + a sin)         for each query and key head; angle i = position * frequencies[i],
+ *                                                    radians, fp64, i < rotary_dim / 2; the pair of i is elements i and
+ *                                                    i + rotary_dim / 2, or 2 i and 2 i + 1 (interleaved != 0)
+ * Elements from rotary_dim on are not rotated. Queries go to q [rows, q_heads * head_dim] (ldq). With a cache, keys and
+ * values go to their slots (slots [rows], as hm_page_plan gives them; a slot outside the cache is not written; two rows
+ * must not have the same slot); without one (NULL), keys go to k [rows, kv_heads * head_dim] (ldk) and values are left
+ * where they are. Each of q and k may be its columns of qkv itself (then with ldqkv); otherwise they must not overlap
+ * it. A row with a negative position is skipped whole. head_dim: a multiple of 16 up to 512, of 16 for rotary_dim (at
+ * most head_dim; 0: no rotation). All row arrays 16-byte aligned with leading dimensions that are multiples of 8. */
+typedef struct hm_qk_norm_rope_args {
+    const void *qkv;
+    int64_t ldqkv;
+    void *q;
+    int64_t ldq;
+    void *k; /* only without a cache */
+    int64_t ldk;
+    const void *bias, *q_weight, *k_weight;
+    const double *frequencies;
+    const int32_t *positions;
+    const int64_t *slots; /* only with a cache */
+    int64_t rows;
+    int32_t q_heads, kv_heads, head_dim, rotary_dim;
+    float eps;
+    int32_t interleaved;
+    int32_t dtype;
+} hm_qk_norm_rope_args;
+hm_status hm_qk_norm_rope(const hm_qk_norm_rope_args *args, const hm_kv_cache *cache, void *stream);
+
+/* Attention of one query token per row over its request's cached keys and values:
+ *   out[t, h] = sum_j p_j v_j, p = softmax over j of scale * (q[t, h] . k_j), j = first..positions[t],
+ *   first = 0, or max(0, positions[t] - window + 1) with a window > 0.
+ * q and out are [rows, q_heads * head_dim] (ldq, ldo; multiples of 8, 16-byte aligned); query head h reads key head
+ * h / (q_heads / kv_heads). block_table [R, W] (ld_table) holds the page ids; row t belongs to request requests[t], or to
+ * request t without requests (NULL). Position -1 sees no key: its output is zero. A negative request is a row to leave as
+ * it is. Keys and values behind a row's position or before its window are not read for it, whatever they hold. A row whose
+ * request, position or one of whose page ids lies outside the table or the cache comes out as NaN, and nothing outside
+ * them is read. Several rows may belong to one request (drafted tokens, a prompt: each row reads the cache by itself).
+ * fp32 scores, statistics and sums; the weights p enter the second product as the sum of two 16-bit floats.
+ * head_dim: 64, 96, 128 or 256; q_heads a multiple of kv_heads. The workspace (hm_paged_attention_workspace_bytes, 256-byte
+ * aligned, nothing in it has to start at zero) holds the parts of rows that several workgroups share; calls that may
+ * overlap in time need workspaces of their own. */
+size_t hm_paged_attention_workspace_bytes(const hm_kv_cache *cache, int64_t q_heads);
+hm_status hm_paged_attention(const hm_kv_cache *cache, void *out, int64_t ldo, const void *q, int64_t ldq, int64_t rows, int64_t q_heads,
+                             const int32_t *block_table, int64_t ld_table, int64_t R, int64_t W, const int32_t *positions,
+                             const int32_t *requests, float scale, int64_t window, void *workspace, size_t workspace_bytes,
+                             void *stream);
+
+/* ---------------------------------------------------------------------------
  * Nonfinite scan (the merged FFN's failure check).
  * ------------------------------------------------------------------------- */
 

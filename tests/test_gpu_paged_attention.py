@@ -1,0 +1,265 @@
+"""GPU: one-token attention over a paged cache against its float64 form."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import attention_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+class Case:
+    """A cache of shuffled pages holding `lengths` tokens of each request; what no request holds is NaN."""
+
+    def __init__(self, seed, lengths, q_heads, kv_heads, d, page_size, dtype, width=None, layout="page_head_token", q_scale=1.5):
+        rng = np.random.default_rng(seed)
+        gen = torch.Generator().manual_seed(seed)
+        self.dtype, self.page_size, self.q_heads = dtype, page_size, q_heads
+        held = [ref.pages_of(n, page_size) for n in lengths]
+        pages = sum(held) + 3
+        ids = rng.permutation(pages)
+        width = max(max(held), 1) if width is None else width
+        self.table = torch.full((len(lengths), width), -1, dtype=torch.int32)
+        self.k = torch.full((pages, kv_heads, page_size, d), float("nan"), dtype=dtype)
+        self.v = self.k.clone()
+        at = 0
+        for r, (n, h) in enumerate(zip(lengths, held)):
+            self.table[r, :h] = torch.from_numpy(ids[at:at + h].astype(np.int32))
+            at += h
+            pos = torch.arange(n)
+            for c in (self.k, self.v):
+                c[self.table[r, pos // page_size].long(), :, pos % page_size] = torch.randn((n, kv_heads, d), generator=gen).to(dtype)
+        self.q = (q_scale * torch.randn((len(lengths), q_heads, d), generator=gen)).to(dtype)
+        self.lengths, self.layout = lengths, layout
+
+    def cache(self, hm, device):
+        if self.layout == "page_token_head":
+            k, v = (c.transpose(1, 2).contiguous().to(device).transpose(1, 2) for c in (self.k, self.v))
+        elif self.layout == "sliced":  # one allocation for k and v, with room between the tokens and heads
+            both = torch.full((self.k.size(0), 2, self.k.size(1) + 1, self.page_size, self.k.size(3) + 8), float("nan"), dtype=self.dtype, device=device)
+            for i, c in enumerate((self.k, self.v)):
+                both[:, i, :-1, :, :-8] = c.to(device)
+            k, v = both[:, 0, :-1, :, :-8], both[:, 1, :-1, :, :-8]
+        else:
+            k, v = self.k.to(device), self.v.to(device)
+        return hm.PagedCache(k, v)
+
+
+def _check(hm, device, c, positions=None, requests=None, q=None, scale=None, window=0, tag="", **kw):
+    q = c.q if q is None else q
+    pos = torch.tensor([n - 1 for n in c.lengths] if positions is None else positions, dtype=torch.int32)
+    req = None if requests is None else torch.tensor(requests, dtype=torch.int32)
+    scale = 1 / math.sqrt(q.size(2)) if scale is None else scale
+    want, bound = ref.attention(q, c.k, c.v, c.table, pos, req, scale, window, c.page_size)
+    out = torch.full(q.shape, 7.0, dtype=c.dtype, device=device)
+    print(f"{tag}: rows={q.size(0)} heads={c.q_heads}/{c.k.size(1)} d={q.size(2)} page={c.page_size} window={window} longest={int(pos.max()) + 1}", flush=True)
+    got = hm.paged_attention(out, q.to(device), c.cache(hm, device), c.table.to(device), pos.to(device), None if req is None else req.to(device),
+                             scale=scale, window=window, **kw)
+    torch.cuda.synchronize()
+    live = torch.ones(q.size(0), dtype=torch.bool) if req is None else req >= 0
+    ref.assert_within(got[live.to(device)], want[live], bound[live], c.dtype, tag)
+    assert (got[~live.to(device)] == 7.0).all(), "rows of no request are left as they are"
+    return got
+
+
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_lengths_around_the_tiles(hm, device, d, dtype):
+    lengths = [1, 2, 15, 16, 17, 31, 32, 33, 47, 64, 127, 128, 129, 160, 255, 256, 257, 1000]
+    _check(hm, device, Case(d, lengths, 8, 2, d, 16, DT[dtype]), tag="lengths")
+
+
+@pytest.mark.parametrize("heads", [(1, 1), (2, 2), (5, 1), (12, 4), (16, 1), (17, 1), (40, 1), (28, 4), (40, 8), (64, 8), (32, 32)])
+def test_head_layouts(hm, device, heads):
+    _check(hm, device, Case(2, [70, 1, 333], heads[0], heads[1], 128, 16, torch.bfloat16), tag="heads")
+
+
+@pytest.mark.parametrize("page_size", [16, 32, 64, 128, 256, 1024])
+@pytest.mark.parametrize("layout", ["page_head_token", "page_token_head", "sliced"])
+def test_pages_and_strides(hm, device, page_size, layout):
+    _check(hm, device, Case(3, [5, 777, 64, 1500], 8, 4, 64, page_size, torch.float16, layout=layout), tag=layout)
+
+
+@pytest.mark.parametrize("window", [1, 2, 15, 16, 17, 100, 128, 129, 1000, 5000])
+def test_windows(hm, device, window):
+    lengths = [1, 16, 17, 100, 129, 300, 1023, 2000]
+    c = Case(4, lengths, 8, 2, 128, 32, torch.bfloat16)
+    # what lies before the window may hold anything
+    for r, n in enumerate(lengths):
+        for at in range(0, max(0, n - window)):
+            for t in (c.k, c.v):
+                t[int(c.table[r, at // 32]), :, at % 32] = float("nan") if at % 2 else float("inf")
+    _check(hm, device, c, window=window, tag="window")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_one_long_row_split_over_the_card(hm, device, d):
+    _check(hm, device, Case(5, [20011], 8, 2, d, 16, torch.float16), tag="long row")
+
+
+def test_ragged_batch_with_shared_parts(hm, device):
+    rng = np.random.default_rng(6)
+    lengths = [int(v) for v in np.exp(rng.uniform(0, np.log(6000), 40))] + [9001]
+    _check(hm, device, Case(6, lengths, 20, 4, 128, 16, torch.bfloat16), tag="ragged")
+
+
+def test_many_short_rows(hm, device):
+    rng = np.random.default_rng(7)
+    _check(hm, device, Case(7, [int(v) for v in rng.integers(1, 40, 700)], 4, 2, 64, 16, torch.float16), tag="short rows")
+
+
+def test_rows_of_requests(hm, device):
+    # several rows of one request (drafted tokens), empty rows, rows of no request in runs longer than a wave, requests out of order
+    c = Case(8, [300, 40, 1025], 8, 2, 128, 16, torch.bfloat16)
+    requests = [2, 2, 2, 0, 0] + [-1] * 200 + [1, 1, 0] + [-1] * 70
+    positions = [1022, 1023, 1024, 0, 299] + [-1] * 200 + [39, -1, 17] + [-1] * 70
+    q = torch.randn((len(requests), 8, 128), generator=torch.Generator().manual_seed(9)).to(torch.bfloat16)
+    got = _check(hm, device, c, positions, requests, q, tag="rows of requests")
+    assert (got[206] == 0).all(), "a row that sees no key is zero"
+
+
+def test_no_rows_to_work_on(hm, device):
+    c = Case(10, [40], 8, 2, 64, 16, torch.float16)
+    q = torch.zeros((3, 8, 64), dtype=torch.float16)
+    _check(hm, device, c, [-1, -1, -1], [-1, -1, -1], q, tag="only rows of no request")
+    _check(hm, device, c, [-1, -1, -1], [0, 0, 0], q, tag="only empty rows")
+    out = torch.empty((0, 8, 64), dtype=torch.float16, device=device)
+    assert hm.paged_attention(out, out, c.cache(hm, device), c.table.to(device), torch.empty(0, dtype=torch.int32, device=device)).numel() == 0
+
+
+def test_extreme_scores(hm, device):
+    # one key that outweighs the rest, scores far apart and far below zero, a zero scale
+    for dtype in (torch.float16, torch.bfloat16):
+        c = Case(11, [600, 600, 600], 4, 2, 64, 16, dtype, q_scale=12.0)
+        c.k[int(c.table[0, 3]), :, 5] *= 8
+        _check(hm, device, c, scale=1.0, tag="large scores")
+        _check(hm, device, c, scale=-1.0, tag="negative scale")
+        _check(hm, device, c, scale=0.0, tag="zero scale")
+
+
+def test_small_weights_add_up(hm, device):
+    # a key of weight 1 next to thousands of weight 2^-26 with values 2^9 times as large: fp16 weights would lose them all
+    n, d = 4097, 64
+    c = Case(12, [n], 1, 1, d, 16, torch.float16)
+    q = torch.zeros((1, 1, d), dtype=torch.float16)
+    q[..., 0] = 26.0
+    for at in range(n):
+        page, o = int(c.table[0, at // 16]), at % 16
+        c.k[page, 0, o] = 0.0
+        c.k[page, 0, o, 0] = 0.0 if at == 1000 else -1.0
+        c.v[page, 0, o] = 1.0 if at == 1000 else 512.0
+    got = _check(hm, device, c, q=q, scale=math.log(2.0), tag="small weights")
+    assert float(got.float().mean()) > 1.02
+
+
+def test_infinities_and_nan_stay_in_their_row(hm, device):
+    c = Case(13, [100, 200, 300], 4, 2, 128, 16, torch.float16)
+    c.k[int(c.table[1, 3]), 0, 4, 7] = float("nan")
+    c.v[int(c.table[2, 5]), 1, 2, 9] = float("inf")
+    want, bound = ref.attention(c.q, c.k, c.v, c.table, torch.tensor([99, 199, 299]), None, 0.1, 0, 16)
+    out = torch.zeros(c.q.shape, dtype=c.dtype, device=device)
+    got = hm.paged_attention(out, c.q.to(device), c.cache(hm, device), c.table.to(device), torch.tensor([99, 199, 299], dtype=torch.int32, device=device),
+                             scale=0.1).cpu().double()
+    assert torch.isnan(got[1, :2]).all() and torch.isposinf(got[2, 2:, 9]).all()
+    fine = torch.isfinite(want)
+    assert torch.isfinite(got[fine]).all()
+    ref.assert_within(got[0], want[0], bound[0], c.dtype, "row without them")
+
+
+def test_rows_outside_the_table_or_cache_are_nan(hm, device):
+    c = Case(14, [100, 200, 300, 400], 4, 2, 64, 16, torch.bfloat16)
+    table = c.table.clone()
+    table[1, 4] = c.k.size(0)
+    table[2, 18] = -1
+    pos = torch.tensor([99, 199, 299, 399, 399, 16 * table.size(1), -2], dtype=torch.int32, device=device)
+    req = torch.tensor([0, 1, 2, 3, 4, 3, 3], dtype=torch.int32, device=device)
+    q = torch.randn((7, 4, 64)).to(c.dtype)
+    out = torch.zeros(q.shape, dtype=c.dtype, device=device)
+    got = hm.paged_attention(out, q.to(device), c.cache(hm, device), table.to(device), pos, req).cpu()
+    for t in (1, 2, 4, 5, 6):
+        assert torch.isnan(got[t]).all(), t
+    want, bound = ref.attention(q[[0, 3]], c.k, c.v, c.table, [99, 399], [0, 3], 1 / 8, 0, 16)
+    ref.assert_within(got[[0, 3]], want, bound, c.dtype, "rows inside")
+
+
+def test_strided_queries_and_outputs(hm, device):
+    c = Case(15, [90, 33], 8, 2, 64, 16, torch.float16)
+    want, bound = ref.attention(c.q, c.k, c.v, c.table, [89, 32], None, 0.125, 0, 16)
+    qkv = torch.full((2, 12 * 64), float("nan"), dtype=c.dtype, device=device)
+    qkv[:, :512] = c.q.view(2, 512).to(device)
+    out = torch.full((2, 1024), 3.0, dtype=c.dtype, device=device)
+    hm.paged_attention(out[:, 8:520], qkv[:, :512], c.cache(hm, device), c.table.to(device), torch.tensor([89, 32], dtype=torch.int32, device=device))
+    ref.assert_within(out[:, 8:520].reshape(2, 8, 64), want, bound, c.dtype, "strided")
+    assert (out[:, :8] == 3.0).all() and (out[:, 520:] == 3.0).all()
+
+
+def test_a_replayed_graph_follows_lengths_and_pages(hm, device):
+    c = Case(16, [1500, 700, 90], 8, 2, 128, 16, torch.bfloat16)
+    cache, table = c.cache(hm, device), c.table.to(device)
+    q, pos = c.q.to(device), torch.tensor([1499, 699, 89], dtype=torch.int32, device=device)
+    out = torch.zeros(c.q.shape, dtype=c.dtype, device=device)
+    ws = cache.attention_workspace(8)
+    hm.paged_attention(out, q, cache, table, pos, workspace=ws)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        hm.paged_attention(out, q, cache, table, pos, workspace=ws)
+    for positions in ([1499, 699, 89], [0, 1, 2], [777, -1, 60], [1499, 699, 89]):
+        pos.copy_(torch.tensor(positions, dtype=torch.int32))
+        out.fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        eager = hm.paged_attention(torch.zeros_like(out), q, cache, table, pos)
+        assert torch.equal(out, eager)
+        want, bound = ref.attention(c.q, c.k, c.v, c.table, positions, None, 1 / math.sqrt(128), 0, 16)
+        ref.assert_within(out, want, bound, c.dtype, f"replay at {positions}")
+
+
+def test_two_streams_with_their_own_workspaces(hm, device):
+    a, b = Case(17, [5000], 8, 2, 128, 16, torch.float16), Case(18, [3000, 41], 8, 2, 128, 16, torch.float16)
+    runs = []
+    for c in (a, b):
+        s = torch.cuda.Stream()
+        cache, table, q = c.cache(hm, device), c.table.to(device), c.q.to(device)
+        pos = torch.tensor([n - 1 for n in c.lengths], dtype=torch.int32, device=device)
+        runs.append((c, s, cache, table, q, pos, torch.zeros(q.shape, dtype=q.dtype, device=device)))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for c, s, cache, table, q, pos, out in runs:
+            hm.paged_attention(out, q, cache, table, pos, stream=s)
+    torch.cuda.synchronize()
+    for c, s, cache, table, q, pos, out in runs:
+        want, bound = ref.attention(c.q, c.k, c.v, c.table, pos.cpu(), None, 1 / math.sqrt(128), 0, 16)
+        ref.assert_within(out, want, bound, c.dtype, "on its stream")
+
+
+def test_the_same_bits_on_every_call(hm, device):
+    c = Case(19, [3000, 17, 800], 8, 2, 128, 16, torch.bfloat16)
+    cache, table, q = c.cache(hm, device), c.table.to(device), c.q.to(device)
+    pos = torch.tensor([2999, 16, 799], dtype=torch.int32, device=device)
+    first = hm.paged_attention(torch.zeros_like(q), q, cache, table, pos)
+    for _ in range(5):
+        assert torch.equal(first, hm.paged_attention(torch.zeros_like(q), q, cache, table, pos))
+
+
+def test_a_cache_past_32_bits_of_elements(hm, device):
+    # pages at both ends of a cache of 2^32 + elements per tensor (8.6 GB each)
+    pages = (1 << 32) // (16 * 8 * 128) + 64
+    k = torch.zeros((pages, 8, 16, 128), dtype=torch.float16, device=device)
+    v = torch.zeros((pages, 8, 16, 128), dtype=torch.float16, device=device)
+    cache = hm.PagedCache(k, v)
+    gen = torch.Generator().manual_seed(20)
+    table = torch.tensor([[pages - 1, 0, pages - 40, 1]], dtype=torch.int32)
+    small_k, small_v = (torch.randn((4, 8, 16, 128), generator=gen).half() for _ in range(2))
+    for i, p in enumerate(table[0].tolist()):
+        k[p], v[p] = small_k[i].to(device), small_v[i].to(device)
+    q = torch.randn((1, 32, 128), generator=gen).half()
+    got = hm.paged_attention(torch.zeros((1, 32, 128), dtype=torch.float16, device=device), q.to(device), cache, table.to(device),
+                             torch.tensor([60], dtype=torch.int32, device=device))
+    want, bound = ref.attention(q, small_k, small_v, torch.arange(4)[None], [60], None, 1 / math.sqrt(128), 0, 16)
+    ref.assert_within(got, want, bound, torch.float16, "far pages")
