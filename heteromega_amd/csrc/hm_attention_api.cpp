@@ -209,10 +209,11 @@ hm_status hm_paged_attention(const hm_kv_cache *cache, void *out, int64_t ldo, c
         return set_error(HM_INVALID_ARGUMENT, "%s: %lld rows need `requests` or a table row each, the table has %lld", what, static_cast<long long>(rows),
                          static_cast<long long>(R));
     }
-    // A row's tiles over all heads are counted in 32 bits.
+    // The tiles of all rows and heads are counted in 32 bits.
     const int64_t units = cache->kv_heads * ((q_heads / cache->kv_heads + 15) / 16);
-    if ((W * cache->page_size / 128 + 2) * units > INT32_MAX) {
-        return set_error(HM_UNSUPPORTED, "%s: W * page_size * key heads is too large", what);
+    const int64_t tiles = (W * cache->page_size / 128 + 2) * units;
+    if (tiles > INT32_MAX || rows > INT32_MAX / tiles) {
+        return set_error(HM_UNSUPPORTED, "%s: rows * key heads * (W * page_size / 128 + 2) must stay below 2^31 (fewer rows per call)", what);
     }
     if (rows == 0) {
         return HM_OK;

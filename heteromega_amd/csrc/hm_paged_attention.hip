@@ -4,9 +4,11 @@
 // the query heads of a key head (G, up to 16 at a time) are the columns of one MFMA tile, so that they share the reads.
 //
 // A wave takes 32 keys at a time, as two sub-tiles of 16 keys (a page holds whole sub-tiles):
-//   S^T [key, q] = K Q^T   v_mfma_f32_16x16x32: A = K, lane L holds key L & 15 and 8 consecutive elements, straight from
-//                          memory in 16-byte loads; B = Q^T, kept in registers.
-//   O^T [d, q] += V^T P^T  A = V^T: the rows of V go through LDS and come back transposed (ds_read_b64_tr_b16); B = P^T.
+//   S^T [key, q] = K Q^T   v_mfma_f32_16x16x32: A = K, lane L holds key L & 15 and 8 consecutive elements; B = Q^T, kept in
+//                          registers.
+//   O^T [d, q] += V^T P^T  A = V^T, read from LDS transposed (ds_read_b64_tr_b16); B = P^T.
+// Rows of K and V are loaded whole by neighbouring lanes and pass through LDS, K as well as V: loads in A's own order touch 64
+// bytes of 16 rows each, and took 394 us instead of 362 (64 rows of 8192 keys, 8 key heads of 128).
 // In S^T a lane holds, for one column q = L & 15, keys 4 (L >> 4) + i of each sub-tile. The k index of the second product may
 // be dealt in any order that A and B share, so those eight weights are its B operand as they are: no weight crosses
 // lanes. O^T keeps one q per lane too, so rescaling by a new maximum is one factor per lane.
@@ -30,7 +32,8 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kWaveKeys = 32;
 constexpr int kTileKeys = kWaveKeys * kWaves;
-constexpr int kPerCu = 3; // workgroups per CU
+constexpr int kPerCu = 2; // workgroups per CU
+constexpr int kStream = 2; // cache policy of the keys and values, read once: non-temporal
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
@@ -42,7 +45,7 @@ struct Descriptor { // of a workgroup's last unit, when it begins there and is n
 // The workspace of `groups` workgroups with `cols` columns (query heads of a unit).
 struct Workspace {
     Descriptor *desc;
-    float2 *stats; // [2 groups][cols]: m, l of each part; part 2 w: the unit that workgroup w goes on with, 2 w + 1: the one it begins
+    float2 *stats; // [2 groups][cols]: m, l of each part; part 2 w: of the unit that workgroup w goes on with, 2 w + 1: of the one it begins
     float *o;      // [2 groups][cols][D]
 };
 
@@ -82,6 +85,12 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
     return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
 
+// A row that all lanes hold, in scalar registers: page addresses must be known to be uniform, or each load becomes a loop over
+// the lanes' addresses (which took 374 us instead of 358 at 64 rows of 8192 keys).
+__device__ __forceinline__ Row uniform_row(const Row &r) {
+    return Row{uniform(r.request), uniform(r.first), uniform(r.start), uniform(r.end), uniform(r.tiles), uniform(r.bad) != 0};
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 template <class T> __device__ __forceinline__ void store4(uint16_t *p, float4_t v) {
@@ -113,71 +122,91 @@ template <class T, int D> struct Shape {
     static constexpr int kSteps = D / 32;         // K steps of the first product, and 16-byte pieces of V per lane and sub-tile
     static constexpr int kDTiles = D / 16;        // row tiles of O^T
     static constexpr int kRowBytes = 2 * D + 32;  // a row of V in LDS: 32 bytes of padding turn the banks of successive rows
-    static constexpr int kVBytes = kWaveKeys * kRowBytes;
+    static constexpr int kRegion = kWaveKeys * kRowBytes;
     static constexpr int kORow = D + 4;           // floats of a column of O in LDS
-    static_assert(16 * kORow * 4 <= kVBytes, "O takes the place of V");
+    static_assert(16 * kORow * 4 <= kRegion, "O takes the place of V");
+};
+
+// Piece i * 64 + lane of a sub-tile's 16 rows of D / 8 pieces: its key, its offset in memory and its place in LDS. Where rows are a
+// power of two of pieces, piece i lies a constant number of rows behind piece 0.
+template <int D> struct Pieces {
+    static constexpr int kPerRow = D / 8;
+    static constexpr bool kEven = 64 % kPerRow == 0;
+    static constexpr int kKept = kEven ? 1 : D / 32;
+    int keys[kKept];
+    uint32_t offsets[kKept], places[kKept];
+    uint32_t step;
+
+    __device__ __forceinline__ Pieces(int lane, uint32_t row_bytes) : step(64 / kPerRow * row_bytes) {
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) {
+            const int piece = i * 64 + lane;
+            keys[i] = piece / kPerRow;
+            const int c = piece - keys[i] * kPerRow;
+            offsets[i] = keys[i] * row_bytes + c * 16;
+            places[i] = keys[i] * (2 * D + 32) + c * 16;
+        }
+    }
+    __device__ __forceinline__ int key(int i) const { return kEven ? keys[0] + i * (64 / kPerRow) : keys[i % kKept]; }
+    __device__ __forceinline__ uint32_t offset(int i) const { return kEven ? offsets[0] + i * step : offsets[i % kKept]; }
+    __device__ __forceinline__ uint32_t lds_offset() const { return kEven ? places[0] : 0; }
+    __device__ __forceinline__ uint32_t lds_step(int i) const { return kEven ? i * (64 / kPerRow) * (2 * D + 32) : places[i % kKept]; }
 };
 
 template <class T, int D>
-__global__ void __launch_bounds__(kThreads, D <= 128 ? 3 : 1) paged_attention_kernel(PagedAttentionArgs a, int groups, int cols, int col_tiles) {
+__global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_kernel(PagedAttentionArgs a, int groups, int cols, int col_tiles) {
     using S = Shape<T, D>;
     using vec = typename Split<T>::vec;
     using elem = typename Split<T>::elem;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * S::kVBytes];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * S::kRegion];
     __shared__ float2 wave_stats[kWaves][16];
-    __shared__ int64_t scan[kWaves];
-    __shared__ int64_t found[2];
+    __shared__ int scan[kWaves];
+    __shared__ int found, found_base;
 
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int col = lane & 15, quad = lane >> 4;
     const int units = a.kv_heads * col_tiles;
-    const Workspace ws = carve(a.workspace, groups, cols);
-    const int w = blockIdx.x;
+    const int w = blockIdx.x, rows = static_cast<int>(a.rows);
 
-    // ---- this workgroup's run of tiles ----
-    int64_t x, x_end, base, total, per_run, longer;
-    int64_t t;
+    // ---- this workgroup's run of tiles, [x, x_end) ----
+    int x, x_end, per_run, longer; // the first `longer` runs have per_run + 1 tiles, the others per_run
+    int t = 0, base = 0;           // the row that x lies in, and the row's first tile
+    Row r{};
     {
-        const int64_t per = (a.rows + kThreads - 1) / kThreads;
-        const int64_t t0 = min(static_cast<int64_t>(threadIdx.x) * per, a.rows), t1 = min(t0 + per, a.rows);
-        int64_t own = 0;
-        for (int64_t i = t0; i < t1; ++i) {
+        const int per = (rows + kThreads - 1) / kThreads;
+        const int t0 = min(static_cast<int>(threadIdx.x) * per, rows), t1 = min(t0 + per, rows);
+        int own = 0;
+        for (int i = t0; i < t1; ++i) {
             own += row_of(a, i).tiles;
         }
-        int64_t upto = own;
+        int upto = own;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
-            const int64_t v = __shfl_up(upto, off);
+            const int v = __shfl_up(upto, off);
             upto += lane >= off ? v : 0;
         }
         if (lane == 63) {
             scan[wave] = upto;
         }
         __syncthreads();
-        int64_t before = 0;
-        total = 0;
+        int before = upto - own, total = 0;
 #pragma unroll
         for (int i = 0; i < kWaves; ++i) {
             before += i < wave ? scan[i] : 0;
             total += scan[i];
         }
-        before += upto - own;
-        total = uniform64(total * units);
-        if ((static_cast<uint64_t>(total) >> 32) == 0) {
-            per_run = static_cast<uint32_t>(total) / static_cast<uint32_t>(groups);
-        } else {
-            per_run = total / groups;
-        }
-        longer = total - per_run * groups; // the first `longer` runs have a tile more
-        x = w * per_run + min(static_cast<int64_t>(w), longer);
+        total = uniform(total) * units;
+        per_run = static_cast<uint32_t>(total) / static_cast<uint32_t>(groups);
+        longer = total - per_run * groups;
+        x = w * per_run + min(w, longer);
         x_end = x + per_run + (w < longer ? 1 : 0);
         if (x < x_end && before * units <= x && x < (before + own) * units) {
-            int64_t b = before * units;
-            for (int64_t i = t0; i < t1; ++i) {
-                const int64_t n = static_cast<int64_t>(row_of(a, i).tiles) * units;
+            int b = before * units;
+            for (int i = t0; i < t1; ++i) {
+                const int n = (per == 1 ? own : row_of(a, i).tiles) * units;
                 if (x < b + n) {
-                    found[0] = i;
-                    found[1] = b;
+                    found = i;
+                    found_base = b;
                     break;
                 }
                 b += n;
@@ -187,54 +216,45 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 3 : 1) paged_attention_ke
     }
     Descriptor begun{0, 0, 0, 0};
     if (x < x_end) {
-        t = uniform64(found[0]);
-        base = uniform64(found[1]);
+        t = uniform(found);
+        base = uniform(found_base);
+        r = uniform_row(row_of(a, t));
     }
 
     // ---- constants of the lane ----
     const uint32_t row_bytes = static_cast<uint32_t>(a.token_stride) * 2;
-    const uint32_t k_off = col * row_bytes + quad * 16;
-    uint32_t v_off[S::kSteps], v_lds[S::kSteps];
-    int v_key[S::kSteps];
-#pragma unroll
-    for (int i = 0; i < S::kSteps; ++i) {
-        const int piece = i * 64 + lane;
-        v_key[i] = piece / (D / 8);
-        const int c = piece - v_key[i] * (D / 8);
-        v_off[i] = v_key[i] * row_bytes + c * 16;
-        v_lds[i] = wave * S::kVBytes + v_key[i] * S::kRowBytes + c * 16;
-    }
-    const uint32_t tr_base = wave * S::kVBytes + (4 * quad + (col >> 2)) * S::kRowBytes + (col & 3) * 8;
+    // Pieces of 16 bytes of a sub-tile's rows as the lanes load them, whole rows by neighbouring lanes.
+    const Pieces<D> pieces(lane, row_bytes);
+    const uint32_t to_lds = wave * S::kRegion + pieces.lds_offset();
+    const uint32_t k_lds = wave * S::kRegion + col * S::kRowBytes + quad * 16;
+    const uint32_t v_lds = wave * S::kRegion + (4 * quad + (col >> 2)) * S::kRowBytes + (col & 3) * 8;
     const float c_scale = a.scale * 1.4426950408889634f;
+    const int group_heads = a.q_heads / a.kv_heads;
 
     while (x < x_end) {
-        Row r = row_of(a, t);
-        while (x >= base + static_cast<int64_t>(r.tiles) * units) { // on to the next row with tiles, 64 at a time
-            base += static_cast<int64_t>(r.tiles) * units;
-            int64_t from = t + 1;
+        while (x >= base + r.tiles * units) { // on to the next row with tiles, 64 at a time
+            base = uniform(base + r.tiles * units);
+            int from = t + 1;
             uint64_t some = 0;
-            for (; from < a.rows; from += 64) {
-                some = __ballot(from + lane < a.rows && row_of(a, min(from + lane, a.rows - 1)).tiles > 0);
+            for (; from < rows; from += 64) {
+                some = __ballot(from + lane < rows && row_of(a, min(from + lane, rows - 1)).tiles > 0);
                 if (some != 0) {
                     break;
                 }
             }
-            t = some != 0 ? from + __builtin_ctzll(some) : a.rows - 1; // a run ends before the rows do
-            r = row_of(a, t);
+            t = uniform(some != 0 ? from + static_cast<int>(__builtin_ctzll(some)) : rows - 1); // a run ends before the rows do
+            r = uniform_row(row_of(a, t));
         }
-        r.request = uniform(r.request), r.first = uniform(r.first), r.start = uniform(r.start), r.end = uniform(r.end), r.tiles = uniform(r.tiles);
-        const int in_row = static_cast<int>(x - base);
-        const int unit = in_row / r.tiles;
-        const int tile0 = in_row - unit * r.tiles;
-        const int tile1 = static_cast<int>(min(static_cast<int64_t>(r.tiles), tile0 + (x_end - x)));
-        const int kv_head = unit / col_tiles;
+        const int unit = uniform(static_cast<uint32_t>(x - base) / static_cast<uint32_t>(r.tiles));
+        const int tile0 = x - base - unit * r.tiles;
+        const int tile1 = min(r.tiles, tile0 + (x_end - x));
+        const int kv_head = uniform(col_tiles == 1 ? unit : unit / col_tiles);
         const int head_in_group = (unit - kv_head * col_tiles) * 16;
-        const int group_heads = a.q_heads / a.kv_heads;
         const int used = min(16, group_heads - head_in_group);
         const int q_head = kv_head * group_heads + head_in_group;
 
         u32x4_t q[S::kSteps];
-        const uint16_t *q_row = a.q + t * a.ldq + static_cast<int64_t>(q_head + (col < used ? col : 0)) * D + 8 * quad;
+        const uint16_t *q_row = a.q + static_cast<int64_t>(t) * a.ldq + static_cast<int64_t>(q_head + (col < used ? col : 0)) * D + 8 * quad;
 #pragma unroll
         for (int s = 0; s < S::kSteps; ++s) {
             q[s] = col < used ? *reinterpret_cast<const u32x4_t *>(q_row + 32 * s) : u32x4_t{0, 0, 0, 0};
@@ -249,13 +269,17 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 3 : 1) paged_attention_ke
         bool poisoned = false;
 
         u32x4_t k_reg[2][S::kSteps], v_reg[2][S::kSteps];
-        const int32_t *table = a.block_table + (r.bad ? 0 : r.request) * a.ld_table;
+        const int32_t *table = a.block_table + uniform64((r.bad ? 0 : r.request) * a.ld_table);
+        const uint16_t *k_head = a.k + uniform64(kv_head * a.head_stride), *v_head = a.v + uniform64(kv_head * a.head_stride);
+        const int64_t page_stride = uniform64(a.page_stride);
+        const int shift = uniform(a.page_shift), offset_mask = (1 << shift) - 1;
+        const uint32_t pages = uniform(static_cast<int>(a.pages));
         int32_t id[2];
         const auto page_ids = [&](int tile) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 const int key = r.start + tile * kTileKeys + wave * kWaveKeys + 16 * s;
-                id[s] = key < r.end ? table[key >> a.page_shift] : 0;
+                id[s] = key < r.end ? table[key >> shift] : 0;
             }
         };
         const auto request = [&](int tile) {
@@ -264,23 +288,21 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 3 : 1) paged_attention_ke
                 const int key = r.start + tile * kTileKeys + wave * kWaveKeys + 16 * s;
                 const int32_t page = uniform(id[s]);
                 int seen = max(0, min(16, r.end - key));
-                if (page < 0 || page >= a.pages) {
+                if (static_cast<uint32_t>(page) >= pages) {
                     poisoned |= seen > 0;
                     seen = 0;
                 }
                 // Past the row's last key the buffer ends, and its loads return zero.
-                const uint32_t bytes = seen > 0 ? (seen - 1) * row_bytes + 2 * D : 0;
-                const int64_t at = seen > 0 ? page * a.page_stride + kv_head * a.head_stride +
-                                                  (key & ((1 << a.page_shift) - 1)) * a.token_stride
-                                            : 0;
-                const __amdgpu_buffer_rsrc_t kr = buffer_rsrc(a.k + at, bytes), vr = buffer_rsrc(a.v + at, bytes);
+                const uint32_t bytes = uniform(seen > 0 ? (seen - 1) * row_bytes + 2 * D : 0);
+                const int64_t at = uniform64(seen > 0 ? page * page_stride + static_cast<int64_t>(key & offset_mask) * (row_bytes / 2) : 0);
+                const __amdgpu_buffer_rsrc_t kr = buffer_rsrc(k_head + at, bytes), vr = buffer_rsrc(v_head + at, bytes);
 #pragma unroll
                 for (int i = 0; i < S::kSteps; ++i) {
-                    k_reg[s][i] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_off + 64 * i, 0, 0);
+                    k_reg[s][i] = __builtin_amdgcn_raw_buffer_load_b128(kr, pieces.offset(i), 0, kStream);
                 }
 #pragma unroll
                 for (int i = 0; i < S::kSteps; ++i) {
-                    v_reg[s][i] = __builtin_amdgcn_raw_buffer_load_b128(vr, v_off[i], 0, 0);
+                    v_reg[s][i] = __builtin_amdgcn_raw_buffer_load_b128(vr, pieces.offset(i), 0, kStream);
                 }
             }
         };
@@ -297,10 +319,18 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 3 : 1) paged_attention_ke
                 for (int s = 0; s < 2; ++s) {
 #pragma unroll
                     for (int i = 0; i < S::kSteps; ++i) {
-                        if (key0 + 16 * s + v_key[i] < r.first) {
+                        if (key0 + 16 * s + pieces.key(i) < r.first) {
                             v_reg[s][i] = u32x4_t{0, 0, 0, 0};
                         }
                     }
+                }
+            }
+            // K and then V pass through the wave's own region of LDS; a wave's LDS accesses are carried out in order.
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+#pragma unroll
+                for (int i = 0; i < S::kSteps; ++i) {
+                    *reinterpret_cast<u32x4_t *>(lds + to_lds + pieces.lds_step(i) + s * 16 * S::kRowBytes) = k_reg[s][i];
                 }
             }
             float4_t score[2] = {float4_t{0.0f, 0.0f, 0.0f, 0.0f}, float4_t{0.0f, 0.0f, 0.0f, 0.0f}};
@@ -308,14 +338,15 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 3 : 1) paged_attention_ke
             for (int i = 0; i < S::kSteps; ++i) {
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    score[s] = T::mfma16(__builtin_bit_cast(uint4, k_reg[s][i]), __builtin_bit_cast(uint4, q[i]), score[s]);
+                    const uint4 k = *reinterpret_cast<const uint4 *>(lds + k_lds + s * 16 * S::kRowBytes + 64 * i);
+                    score[s] = T::mfma16(k, __builtin_bit_cast(uint4, q[i]), score[s]);
                 }
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
 #pragma unroll
                 for (int i = 0; i < S::kSteps; ++i) {
-                    *reinterpret_cast<u32x4_t *>(lds + v_lds[i] + s * 16 * S::kRowBytes) = v_reg[s][i];
+                    *reinterpret_cast<u32x4_t *>(lds + to_lds + pieces.lds_step(i) + s * 16 * S::kRowBytes) = v_reg[s][i];
                 }
             }
             if (tile + 1 < tile1) {
@@ -364,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 3 : 1) paged_attention_ke
                 uint2 half[2];
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    half[s] = lds_read_transposed(lds + tr_base + s * 16 * S::kRowBytes + i * 32);
+                    half[s] = lds_read_transposed(lds + v_lds + s * 16 * S::kRowBytes + i * 32);
                 }
                 const uint4 vt = make_uint4(half[0].x, half[0].y, half[1].x, half[1].y);
                 o[i] = T::mfma16(vt, __builtin_bit_cast(uint4, hi), o[i]);
@@ -389,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 3 : 1) paged_attention_ke
                 top = fmaxf(top, wave_stats[i][col].x);
             }
             const float f = top == -INFINITY ? 0.0f : exp2_fast(m - top);
-            float *mine = reinterpret_cast<float *>(lds + wave * S::kVBytes);
+            float *mine = reinterpret_cast<float *>(lds + wave * S::kRegion);
             if (col < used) {
 #pragma unroll
                 for (int i = 0; i < S::kDTiles; ++i) {
@@ -399,7 +430,8 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 3 : 1) paged_attention_ke
         }
         __syncthreads();
         const bool whole = tile0 == 0 && tile1 == r.tiles;
-        const int64_t part = 2 * static_cast<int64_t>(w) + (tile0 == 0 ? 1 : 0);
+        const int64_t part = 2 * w + (tile0 == 0 ? 1 : 0);
+        const Workspace ws = carve(a.workspace, groups, cols);
         for (int i = threadIdx.x; i < used * (D / 4); i += kThreads) {
             const int j = i / (D / 4), d = (i - j * (D / 4)) * 4;
             float top = -INFINITY, sum = 0.0f;
@@ -412,14 +444,14 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 3 : 1) paged_attention_ke
             for (int k = 0; k < kWaves; ++k) {
                 const float2 st = wave_stats[k][j];
                 sum += st.y * (top == -INFINITY ? 1.0f : exp2_fast(st.x - top));
-                v += *reinterpret_cast<const float4_t *>(reinterpret_cast<const float *>(lds + k * S::kVBytes) + j * S::kORow + d);
+                v += *reinterpret_cast<const float4_t *>(reinterpret_cast<const float *>(lds + k * S::kRegion) + j * S::kORow + d);
             }
             if (whole) {
                 if (r.bad) {
                     sum = NAN;
                 }
                 v = r.end == r.first && !r.bad ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : v / sum;
-                store4<T>(a.out + t * a.ldo + static_cast<int64_t>(q_head + j) * D + d, v);
+                store4<T>(a.out + static_cast<int64_t>(t) * a.ldo + static_cast<int64_t>(q_head + j) * D + d, v);
             } else {
                 *reinterpret_cast<float4_t *>(ws.o + (part * cols + j) * D + d) = v;
                 if (d == 0) {
@@ -428,24 +460,27 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 3 : 1) paged_attention_ke
             }
         }
         __syncthreads();
-        if (tile0 == 0 && tile1 < r.tiles) {
-            const int64_t last = x - tile0 + r.tiles - 1; // the unit's last tile, and the workgroup that has it
-            const int64_t head_tiles = longer * (per_run + 1);
-            const int64_t last_w = last < head_tiles ? last / (per_run + 1) : longer + (last - head_tiles) / per_run;
-            begun = Descriptor{static_cast<int32_t>(t), unit, static_cast<int32_t>(last_w - w), 0};
+        if (tile0 == 0 && !whole) {
+            const uint32_t last = x + r.tiles - 1; // the unit's last tile, and the workgroup that has it
+            const uint32_t long_tiles = longer * (per_run + 1);
+            const int last_w = last < long_tiles ? last / (per_run + 1) : longer + (last - long_tiles) / per_run;
+            begun = Descriptor{t, unit, last_w - w, 0};
         }
-        x += tile1 - tile0;
+        x = uniform(x + tile1 - tile0);
     }
     if (threadIdx.x == 0) {
-        ws.desc[w] = begun;
+        carve(a.workspace, groups, cols).desc[w] = begun;
     }
 }
 
 // Joins the parts of the unit that workgroup blockIdx.x began and others went on with: columns blockIdx.y, blockIdx.y + gridDim.y, ...
-template <class T, int D>
-__global__ void __launch_bounds__(kThreads) join_kernel(PagedAttentionArgs a, int groups, int cols, int col_tiles) {
-    constexpr int kItems = D / 4;                // float4 elements of a column
-    constexpr int kLanes = kThreads / kItems;    // parts read at a time
+// A launch of its own: the count of arrivals that would let the last workgroup join in the first launch costs more, since its
+// stores, count and loads each go to memory and back past the XCDs' L2s (one row of 1037 keys: 17.5 us instead of 12.3).
+template <class T, int D, int THREADS>
+__global__ void __launch_bounds__(THREADS) join_kernel(PagedAttentionArgs a, int groups, int cols, int col_tiles) {
+    constexpr int kItems = D / 4;            // float4 elements of a column
+    constexpr int kLanes = THREADS / kItems; // parts that the workgroup reads at a time, kAhead times
+    constexpr int kAhead = 4;
     __shared__ float4_t acc[kLanes][kItems];
     __shared__ float2 stat[kLanes];
     const Workspace ws = carve(a.workspace, groups, cols);
@@ -463,15 +498,33 @@ __global__ void __launch_bounds__(kThreads) join_kernel(PagedAttentionArgs a, in
         float m = -INFINITY, l = 0.0f;
         float4_t v = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
         if (y < kLanes) {
-#pragma unroll 4
-            for (int i = y; i <= d.pieces; i += kLanes) {
-                const int64_t part = 2 * static_cast<int64_t>(w + i) + (i == 0 ? 1 : 0);
-                const float2 st = ws.stats[part * cols + j];
-                const float4_t o = *reinterpret_cast<const float4_t *>(ws.o + (part * cols + j) * D + 4 * e);
-                const float top = fmaxf(m, st.x);
-                const float f = top == -INFINITY ? 1.0f : exp2_fast(m - top), g = top == -INFINITY ? 1.0f : exp2_fast(st.x - top);
-                v = v * f + o * g;
-                l = l * f + st.y * g;
+            for (int i = y; i <= d.pieces; i += kAhead * kLanes) {
+                float2 st[kAhead];
+                float4_t o[kAhead];
+                float top = m;
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const int p = min(i + k * kLanes, d.pieces);
+                    const int64_t part = 2 * (w + p) + (p == 0 ? 1 : 0);
+                    st[k] = ws.stats[part * cols + j];
+                    o[k] = *reinterpret_cast<const float4_t *>(ws.o + (part * cols + j) * D + 4 * e);
+                }
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    top = fmaxf(top, st[k].x); // the last part may count twice here
+                }
+                const float from = top == -INFINITY ? 0.0f : top; // no finite score yet: weights of zero
+                const float f = exp2_fast(m - from);
+                v *= f;
+                l *= f;
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    if (i + k * kLanes <= d.pieces) {
+                        const float g = exp2_fast(st[k].x - from);
+                        v += o[k] * g;
+                        l += st[k].y * g;
+                    }
+                }
                 m = top;
             }
             acc[y][e] = v;
@@ -489,7 +542,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(PagedAttentionArgs a, in
             }
 #pragma unroll
             for (int i = 0; i < kLanes; ++i) {
-                const float f = top == -INFINITY ? 1.0f : exp2_fast(stat[i].x - top);
+                const float f = exp2_fast(stat[i].x - (top == -INFINITY ? 0.0f : top));
                 out += acc[i][e] * f;
                 sum += stat[i].y * f;
             }
@@ -508,8 +561,13 @@ template <class T, int D> hipError_t launch(const PagedAttentionArgs &a, int64_t
     if (e != hipSuccess) {
         return e;
     }
-    hipLaunchKernelGGL((join_kernel<T, D>), dim3(static_cast<unsigned>(groups), static_cast<unsigned>(std::min(cols, 4))), dim3(kThreads), 0,
-                       stream, a, static_cast<int>(groups), cols, col_tiles);
+    // Most of these workgroups find nothing to join and leave, so one wave each; four where few units have many parts.
+    const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>(std::min(cols, 4)));
+    if (groups <= 16 * a.rows * a.kv_heads * col_tiles) {
+        hipLaunchKernelGGL((join_kernel<T, D, 64>), grid, dim3(64), 0, stream, a, static_cast<int>(groups), cols, col_tiles);
+    } else {
+        hipLaunchKernelGGL((join_kernel<T, D, 256>), grid, dim3(256), 0, stream, a, static_cast<int>(groups), cols, col_tiles);
+    }
     return hipGetLastError();
 }
 
@@ -530,8 +588,7 @@ template <class T> hipError_t launch_type(const PagedAttentionArgs &a, int64_t g
 
 size_t paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
     const int64_t groups = max_groups(), cols = std::min<int64_t>(16, q_heads / kv_heads);
-    return static_cast<size_t>(groups * static_cast<int64_t>(sizeof(Descriptor)) + (2 * groups * cols * 8 + 15) / 16 * 16 +
-                               2 * groups * cols * head_dim * 4);
+    return static_cast<size_t>(groups * static_cast<int64_t>(sizeof(Descriptor)) + (2 * groups * cols * 8 + 15) / 16 * 16 + 2 * groups * cols * head_dim * 4);
 }
 
 hipError_t launch_paged_attention(const PagedAttentionArgs &a, hipStream_t stream) {
