@@ -19,11 +19,27 @@ from .ffn import (_DTYPES, _aligned, _call, _handed_over, _hm_dtype, _on, _strea
 kPagePlanMaxRequests = 4096
 
 
+# The current device's index without torch.cuda's check that it is initialized (device tensors are at hand): not part of torch's public
+# interface, so a torch without it takes the public call.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _guard(device):
     """The device of the tensors as the current one: a launch goes to the current device."""
-    if device.index == torch.cuda.current_device():
+    if device.index == _current_device():
         return contextlib.nullcontext()
     return torch.cuda.device(device)
+
+
+def _on_device(device, call, *args):
+    """call(*args) with `device` current, its status checked. (A with statement costs 0.5 us, a tenth of a small call.)"""
+    if device.index == _current_device():
+        status = call(*args)
+    else:
+        with torch.cuda.device(device):
+            status = call(*args)
+    if status != _lib.HM_OK:
+        _call(status)
 
 
 def _device_of(t, what):
@@ -33,37 +49,33 @@ def _device_of(t, what):
     return device
 
 
-def _ints(t, dtype, n, device, what, name):
-    """Address of a contiguous vector of at least n integers."""
-    if t.dtype != dtype or t.dim() != 1 or t.size(0) < n or (t.size(0) > 1 and t.stride(0) != 1) or t.device != device:
-        raise ValueError(f"{what}: {name} must be a contiguous {dtype} vector of {n} or more elements on {device}")
-    return t.data_ptr()
-
-
-def _vector(t, dtype, n, device, what, name):
-    if t is None:
-        return None
-    if t.dtype != dtype or t.numel() != n or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{what}: {name} must be a contiguous {dtype} vector of {n} elements on {device}")
+def _vector(t, dtype, n, device, what, name, more=False):
+    """Address of a contiguous vector of n elements (or more)."""
+    if t.dtype is not dtype or t.device != device or not t.is_contiguous() or t.dim() != 1 or (t.size(0) < n if more else t.size(0) != n):
+        raise ValueError(f"{what}: {name} must be a contiguous {dtype} vector of {n}{' or more' if more else ''} elements on {device}, got {t.dtype} "
+                         f"{list(t.shape)} with strides {t.stride()} on {t.device}")
     return t.data_ptr()
 
 
 def _rows(t, rows, heads, d, dtype, device, what, name):
     """(address, leading dimension) of [rows, heads * d] or [rows, heads, d] with packed heads."""
-    width = heads * d
-    if t.dim() == 3:
-        ok = t.size(1) == heads and t.size(2) == d and (d == 1 or t.stride(2) == 1) and (heads == 1 or t.stride(1) == d)
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 3:
+        ok = shape == (rows, heads, d) and (d == 1 or stride[2] == 1) and (heads == 1 or stride[1] == d)
     else:
-        ok = t.dim() == 2 and t.size(1) == width and t.stride(1) == 1
-    if not ok or t.size(0) != rows or t.dtype != dtype or t.device != device:
-        raise ValueError(f"{what}: {name} must be {dtype} [{rows}, {heads} x {d}] with contiguous rows on {device}")
-    return t.data_ptr(), (t.stride(0) if rows > 1 else width)
+        ok = shape == (rows, heads * d) and stride[1] == 1
+    if not ok or t.dtype is not dtype or t.device != device:
+        raise ValueError(f"{what}: {name} must be {dtype} [{rows}, {heads} x {d}] with contiguous rows on {device}, got {t.dtype} {list(shape)} with strides "
+                         f"{stride} on {t.device}")
+    return t.data_ptr(), (stride[0] if rows > 1 else heads * d)
 
 
 def _table(t, device, what):
-    if t.dtype != torch.int32 or t.dim() != 2 or (t.size(1) > 1 and t.stride(1) != 1) or t.device != device:
+    """(address, leading dimension, requests, pages of a request) of a block table."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not torch.int32 or len(shape) != 2 or (stride[1] != 1 and shape[1] > 1) or t.device != device:
         raise ValueError(f"{what}: block_table must be int32 [requests, pages of a request] with contiguous rows on {device}")
-    return t.data_ptr(), max(t.stride(0), t.size(1)) if t.size(0) == 1 else t.stride(0), t.size(0), t.size(1)
+    return t.data_ptr(), (stride[0] if shape[0] > 1 else shape[1]), shape[0], shape[1]
 
 
 def rope_frequencies(rotary_dim, base=10000.0, device=None, llama3_scaling=None):
@@ -136,21 +148,19 @@ def page_plan(plan, lengths, added, block_table, free_pages, queue, lengths_out=
     the ring of free pages free_pages int32 are updated in place; queue int64 [4] holds the ring's head and tail. The lengths
     and counters after the step go to plan.lengths and plan.queue, or to lengths_out and queue_out, which may be lengths and queue.
     plan.queue[2] counts the requests that got nothing because pages, rows or table entries did not suffice."""
-    device = _device_of(lengths, "page_plan")
-    table, ld, count, width = _table(block_table, device, "page_plan")
-    rows = plan.slots.size(0)
-    lengths_out = plan.lengths if lengths_out is None else lengths_out
-    queue_out = plan.queue if queue_out is None else queue_out
-    if plan.device != device or plan.starts.size(0) != count + 1 or lengths.size(0) != count or added.size(0) != count:
-        raise ValueError(f"page_plan: the plan, lengths and added must be of the table's {count} requests and on {device}")
+    what = "page_plan"
+    device = _device_of(lengths, what)
+    table, ld, count, width = _table(block_table, device, what)
+    if plan.device != device or plan.starts.size(0) != count + 1:
+        raise ValueError(f"page_plan: the plan must be of the table's {count} requests and on {device}")
     i32, i64 = torch.int32, torch.int64
-    args = (_ints(lengths, i32, count, device, "page_plan", "lengths"), _ints(added, i32, count, device, "page_plan", "added"), count, table, ld, width,
-            plan.page_size, _ints(free_pages, i32, 1, device, "page_plan", "free_pages"), free_pages.size(0),
-            _ints(queue, i64, 2, device, "page_plan", "queue"), plan.slots.data_ptr(), plan.positions.data_ptr(), plan.requests.data_ptr(), rows,
-            plan.starts.data_ptr(), _ints(lengths_out, i32, count, device, "page_plan", "lengths_out"),
-            _ints(queue_out, i64, 4, device, "page_plan", "queue_out"))
-    with _guard(device):
-        _call(_lib.load().hm_page_plan(*args, _stream(stream, device)))
+    n = _vector(lengths, i32, count, device, what, "lengths")
+    q = _vector(queue, i64, 4, device, what, "queue")
+    n_out = plan.lengths.data_ptr() if lengths_out is None else n if lengths_out is lengths else _vector(lengths_out, i32, count, device, what, "lengths_out")
+    q_out = plan.queue.data_ptr() if queue_out is None else q if queue_out is queue else _vector(queue_out, i64, 4, device, what, "queue_out")
+    _on_device(device, _lib.load().hm_page_plan, n, _vector(added, i32, count, device, what, "added"), count, table, ld, width, plan.page_size,
+               _vector(free_pages, i32, 1, device, what, "free_pages", True), free_pages.size(0), q, plan.slots.data_ptr(), plan.positions.data_ptr(),
+               plan.requests.data_ptr(), plan.slots.size(0), plan.starts.data_ptr(), n_out, q_out, _stream(stream, device))
     return plan
 
 
@@ -176,23 +186,20 @@ def qk_norm_rope(q_out, qkv, frequencies, positions, cache=None, slots=None, k_o
     rows, heads = qkv.size(0), qkv.size(1) // head_dim
     q_heads = heads - 2 * kv_heads
     what = "qk_norm_rope"
-    a = _lib.QkNormRopeArgs()
-    a.qkv, a.ldqkv = _rows(qkv, rows, heads, head_dim, dtype, device, what, "qkv")
-    a.q, a.ldq = _rows(q_out, rows, q_heads, head_dim, dtype, device, what, "q_out")
+    pairs = frequencies.numel()
+    k, ldk, s = None, 0, None
     if cache is None:
-        a.k, a.ldk = _rows(k_out, rows, kv_heads, head_dim, dtype, device, what, "k_out")
+        k, ldk = _rows(k_out, rows, kv_heads, head_dim, dtype, device, what, "k_out")
     else:
-        a.slots = _ints(slots, torch.int64, rows, device, what, "slots")
-    a.positions = _ints(positions, torch.int32, rows, device, what, "positions")
-    a.rotary_dim = 2 * frequencies.numel()
-    a.frequencies = _vector(frequencies, torch.float64, frequencies.numel(), device, what, "frequencies")
-    a.bias = _vector(bias, dtype, heads * head_dim, device, what, "bias")
-    a.q_weight = _vector(q_weight, dtype, head_dim, device, what, "q_weight")
-    a.k_weight = _vector(k_weight, dtype, head_dim, device, what, "k_weight")
-    a.rows, a.q_heads, a.kv_heads, a.head_dim = rows, q_heads, kv_heads, head_dim
-    a.eps, a.interleaved, a.dtype = eps, bool(interleaved), _hm_dtype(dtype)
-    with _guard(device):
-        _call(_lib.load().hm_qk_norm_rope(ctypes.byref(a), cache._ref if cache is not None else None, _stream(stream, device)))
+        s = _vector(slots, torch.int64, rows, device, what, "slots", True)
+    a = _lib.QkNormRopeArgs(*_rows(qkv, rows, heads, head_dim, dtype, device, what, "qkv"), *_rows(q_out, rows, q_heads, head_dim, dtype, device, what, "q_out"),
+                            k, ldk, None if bias is None else _vector(bias, dtype, heads * head_dim, device, what, "bias"),
+                            None if q_weight is None else _vector(q_weight, dtype, head_dim, device, what, "q_weight"),
+                            None if k_weight is None else _vector(k_weight, dtype, head_dim, device, what, "k_weight"),
+                            _vector(frequencies, torch.float64, pairs, device, what, "frequencies"),
+                            _vector(positions, torch.int32, rows, device, what, "positions", True), s, rows, q_heads, kv_heads, head_dim, 2 * pairs, eps,
+                            bool(interleaved), _hm_dtype(dtype))
+    _on_device(device, _lib.load().hm_qk_norm_rope, ctypes.byref(a), None if cache is None else cache._ref, _stream(stream, device))
     return q_out
 
 
@@ -209,14 +216,13 @@ def paged_attention(out, q, cache, block_table, positions, requests=None, scale=
     qp, ldq = _rows(q, rows, q_heads, d, cache.dtype, device, what, "q")
     op, ldo = _rows(out, rows, q_heads, d, cache.dtype, device, what, "out")
     table, ld, count, width = _table(block_table, device, what)
-    pp = _ints(positions, torch.int32, rows, device, what, "positions")
-    rp = _ints(requests, torch.int32, rows, device, what, "requests") if requests is not None else None
-    with _guard(device):
-        if workspace is None:
-            workspace = cache.attention_workspace(q_heads, stream)
-        wp, wb = _aligned(workspace)
-        _call(_lib.load().hm_paged_attention(cache._ref, op, ldo, qp, ldq, rows, q_heads, table, ld, count, width, pp, rp,
-                                             1.0 / math.sqrt(d) if scale is None else scale, window, wp, wb, _stream(stream, device)))
+    pp = _vector(positions, torch.int32, rows, device, what, "positions", True)
+    rp = None if requests is None else _vector(requests, torch.int32, rows, device, what, "requests", True)
+    if workspace is None:
+        workspace = cache.attention_workspace(q_heads, stream)
+    wp, wb = _aligned(workspace)
+    _on_device(device, _lib.load().hm_paged_attention, cache._ref, op, ldo, qp, ldq, rows, q_heads, table, ld, count, width, pp, rp,
+               1.0 / math.sqrt(d) if scale is None else scale, window, wp, wb, _stream(stream, device))
     return out
 
 
