@@ -17,7 +17,7 @@ LIB_NAME = "libhmw4a16.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 
 SOURCES = ["hm_api.cpp", "hm_split.cpp", "hm_layout.hip", "hm_gemv.hip", "hm_gemm.hip", "hm_gemm_f16.hip", "hm_gemm_bf16.hip", "hm_elementwise.hip", "hm_static.hip", "hm_pages.hip",
-           "hm_rope.hip", "hm_paged_attention.hip", "hm_attention_api.cpp"]
+           "hm_rope.hip", "hm_paged_attention.hip", "hm_paged_attention_f16.hip", "hm_paged_attention_bf16.hip", "hm_attention_api.cpp"]
 ARCH = "gfx950"
 
 COMMON_FLAGS = [

@@ -1,0 +1,74 @@
+// One-token attention over a paged cache: the launch plan and the workspace, shared by the planner (hm_paged_attention.hip) and the
+// kernels (hm_paged_attention_kernel.hpp).
+#pragma once
+
+#include "hm_internal.hpp"
+
+namespace hm {
+
+constexpr int kAttentionWaves = 4; // of a workgroup
+
+// The query heads of one unit: `count` heads from q_head on, all of one key head.
+struct UnitHeads {
+    int kv_head, q_head, count;
+};
+
+struct AttentionPlan {
+    int runs;        // equal shares of the tiles
+    int team;        // waves that share a run: 4 or 1
+    int cols;        // columns of a unit: query heads, up to 32
+    int units;       // of a row: key heads times shares of their query heads
+    int shares;      // units of one key head
+    int group_heads; // query heads of one key head
+    bool few_units;  // join with a workgroup per unit and column
+
+    __host__ __device__ UnitHeads heads_of(int unit) const {
+        const int kv = shares == 1 ? unit : unit / shares, first = (unit - kv * shares) * cols;
+        const int left = group_heads - first;
+        return {kv, kv * group_heads + first, left < cols ? left : cols};
+    }
+};
+
+// Tiles dealt in equal runs: the first `longer` runs have per_run + 1 tiles, the others per_run.
+struct Runs {
+    int per_run, longer;
+
+    static __host__ __device__ Runs deal(int tiles, int runs) {
+        const int n = static_cast<int>(static_cast<uint32_t>(tiles) / static_cast<uint32_t>(runs));
+        return {n, tiles - n * runs};
+    }
+    __host__ __device__ int begin(int w) const { return w * per_run + (w < longer ? w : longer); }
+    // The run of a tile.
+    __host__ __device__ int of(int tile) const {
+        const uint32_t t = static_cast<uint32_t>(tile), n = static_cast<uint32_t>(per_run), in_longer = static_cast<uint32_t>(longer) * (n + 1);
+        return static_cast<int>(t < in_longer ? t / (n + 1) : static_cast<uint32_t>(longer) + (t - in_longer) / n);
+    }
+};
+
+struct AttentionDescriptor { // of the unit that a run begins and does not finish
+    int32_t row, unit, pieces, pad; // pieces: runs behind this one that hold its other parts; 0: there is none
+};
+
+// The workspace of `runs` runs with units of `cols` columns.
+struct AttentionWorkspace {
+    AttentionDescriptor *desc; // [runs]
+    float2 *stats;             // [2 runs][cols]: m, l of each part; part 2 w: of the unit that run w goes on with, 2 w + 1: of the one it begins
+    float *o;                  // [2 runs][cols][D]
+};
+
+__host__ __device__ __forceinline__ int64_t attention_workspace_bytes(int64_t runs, int64_t cols, int64_t head_dim) {
+    return runs * static_cast<int64_t>(sizeof(AttentionDescriptor)) + (2 * runs * cols * 8 + 15) / 16 * 16 + 2 * runs * cols * head_dim * 4;
+}
+
+__host__ __device__ __forceinline__ AttentionWorkspace carve(void *p, int64_t runs, int64_t cols) {
+    uint8_t *b = static_cast<uint8_t *>(p);
+    uint8_t *stats = b + runs * static_cast<int64_t>(sizeof(AttentionDescriptor));
+    return {reinterpret_cast<AttentionDescriptor *>(b), reinterpret_cast<float2 *>(stats),
+            reinterpret_cast<float *>(stats + (2 * runs * cols * 8 + 15) / 16 * 16)};
+}
+
+// The launches of one type (hm_paged_attention_f16.hip, hm_paged_attention_bf16.hip).
+hipError_t launch_paged_attention_f16(const PagedAttentionArgs &a, const AttentionPlan &plan, hipStream_t stream);
+hipError_t launch_paged_attention_bf16(const PagedAttentionArgs &a, const AttentionPlan &plan, hipStream_t stream);
+
+} // namespace hm

@@ -113,6 +113,45 @@ def test_many_short_rows(hm, device):
     _check(hm, device, Case(7, [int(v) for v in rng.integers(1, 40, 700)], 4, 2, 64, 16, torch.float16), tag="short rows")
 
 
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("window", [0, 50])
+def test_rows_enough_for_a_run_per_wave(hm, device, d, window):
+    # 2050 and more units: runs of single waves, that end inside long rows; with empty rows, rows of no request and rows outside the cache
+    rng = np.random.default_rng(d)
+    lengths = [int(v) for v in rng.integers(1, 70, 1025)]
+    for r in (0, 3, 500, 1024):
+        lengths[r] = int(rng.integers(1000, 3000))
+    c = Case(d, lengths, 4, 2, d, 16, torch.bfloat16)
+    if window:  # what lies before the window may hold anything
+        for r in (0, 500):
+            at = torch.arange(lengths[r] - window)
+            for t in (c.k, c.v):
+                t[c.table[r, at // 16].long(), :, at % 16] = float("nan")
+    positions = [n - 1 for n in lengths]
+    requests = list(range(1025))
+    for r in range(700, 900):
+        requests[r] = -1
+    positions[10] = positions[901] = -1
+    _check(hm, device, c, positions, requests, window=window, tag="a run per wave")
+    c.table[20, (lengths[20] - 1) // 16] = c.k.size(0) + 7  # the page of its last key, which every window holds
+    positions[30] = 16 * c.table.size(1)
+    pos, req = (torch.tensor(v, dtype=torch.int32) for v in (positions, requests))
+    got = hm.paged_attention(torch.zeros(c.q.shape, dtype=c.dtype, device=device), c.q.to(device), c.cache(hm, device), c.table.to(device), pos.to(device),
+                             req.to(device), window=window).cpu()
+    assert torch.isnan(got[[20, 30]]).all() and torch.isfinite(got[:20]).all() and torch.isfinite(got[21:30]).all() and torch.isfinite(got[31:]).all()
+
+
+@pytest.mark.parametrize("heads", [(24, 1), (32, 1), (33, 1), (64, 2), (100, 1)])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+def test_many_query_heads_of_a_key_head(hm, device, heads, d):
+    _check(hm, device, Case(22, [1, 100, 2500, 31], heads[0], heads[1], d, 32, torch.float16), tag="many query heads")
+
+
+@pytest.mark.parametrize("lengths", [[1], [129], [128 * 512], [3, 70000], [1, 2, 40000, 5, 3000]])
+def test_few_rows(hm, device, lengths):
+    _check(hm, device, Case(23, lengths, 6, 2, 64, 256, torch.bfloat16), tag="few rows")
+
+
 def test_rows_of_requests(hm, device):
     # several rows of one request (drafted tokens), empty rows, rows of no request in runs longer than a wave, requests out of order
     c = Case(8, [300, 40, 1025], 8, 2, 128, 16, torch.bfloat16)
