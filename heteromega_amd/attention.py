@@ -257,8 +257,7 @@ class AttnLayer:
 
     def block_forward(self, x, norm_weight, cache, plan, block_table, eps=1e-5, stream=None):
         """In place: x [rows, hidden] += attention(RMSNorm(x) * norm_weight) Wo. The rows are those of `plan` (page_plan of this step): their keys and values
-        are written to `cache` first, and each row sees its request's tokens up to its own. Rows that the plan left empty stay as they are.
-        Each row reads the cache by itself, so long prompts cost the square of their length in cache reads."""
+        are written to `cache` first, and each row sees its request's tokens up to its own. Rows that the plan left empty stay as they are."""
         rows = plan.slots.size(0)
         if x.dim() != 2 or x.size(0) != rows or x.size(1) != self.hidden or x.stride(1) != 1 or x.dtype != self.dtype or x.device != plan.device:
             raise ValueError(f"AttnLayer.block_forward: x must be {self.dtype} [{rows}, {self.hidden}] on {plan.device}")

@@ -8,24 +8,37 @@ namespace hm {
 
 constexpr int kAttentionWaves = 4; // of a workgroup
 
-// The query heads of one unit: `count` heads from q_head on, all of one key head.
-struct UnitHeads {
-    int kv_head, q_head, count;
+// A unit's columns are query heads of one key head: of one row, heads of it; or of several rows of one request, all heads of each.
+struct Column {
+    int row, q_head; // row: behind the unit's first
 };
 
 struct AttentionPlan {
     int runs;        // equal shares of the tiles
     int team;        // waves that share a run: 4 or 1
-    int cols;        // columns of a unit: query heads, up to 32
-    int units;       // of a row: key heads times shares of their query heads
+    int cols;        // columns of a unit, up to 32
+    int rows;        // rows that a unit may have; 1: it has `cols` heads of one
+    int units;       // of a row, or of a unit's rows: key heads times shares of their query heads
     int shares;      // units of one key head
     int group_heads; // query heads of one key head
     bool few_units;  // join with a workgroup per unit and column
 
-    __host__ __device__ UnitHeads heads_of(int unit) const {
-        const int kv = shares == 1 ? unit : unit / shares, first = (unit - kv * shares) * cols;
-        const int left = group_heads - first;
-        return {kv, kv * group_heads + first, left < cols ? left : cols};
+    __host__ __device__ int kv_head(int unit) const { return shares == 1 ? unit : unit / shares; }
+    // Columns of a unit that has `count` rows. GROUPED: rows > 1.
+    template <bool GROUPED> __host__ __device__ int columns(int unit, int count) const {
+        if (GROUPED) {
+            return count * group_heads;
+        }
+        const int left = group_heads - (unit - kv_head(unit) * shares) * cols;
+        return left < cols ? left : cols;
+    }
+    template <bool GROUPED> __host__ __device__ Column column(int unit, int j) const {
+        const int kv = kv_head(unit);
+        if (GROUPED) {
+            const int row = j / group_heads;
+            return {row, kv * group_heads + j - row * group_heads};
+        }
+        return {0, kv * group_heads + (unit - kv * shares) * cols + j};
     }
 };
 
@@ -46,7 +59,7 @@ struct Runs {
 };
 
 struct AttentionDescriptor { // of the unit that a run begins and does not finish
-    int32_t row, unit, pieces, pad; // pieces: runs behind this one that hold its other parts; 0: there is none
+    int32_t row, unit, pieces, count; // pieces: runs behind this one that hold its other parts; 0: there is none. count: rows
 };
 
 // The workspace of `runs` runs with units of `cols` columns.

@@ -14,22 +14,57 @@ constexpr int kStream = 2; // cache policy of the keys and values, read once: no
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 
-// The keys of one row: [first, end) are seen, the tiles begin at start.
-struct Row {
-    int32_t request, first, start, end, tiles;
+// One row's request and keys [first, end).
+struct Keys {
+    int32_t request, first, end;
     bool bad; // request or position outside the table
 };
 
-__device__ __forceinline__ Row row_of(const PagedAttentionArgs &a, int64_t t, int tile_keys) {
-    Row r;
-    r.request = a.requests != nullptr ? a.requests[t] : static_cast<int32_t>(t);
+__device__ __forceinline__ Keys keys_of(const PagedAttentionArgs &a, int64_t t) {
+    Keys k;
+    k.request = a.requests != nullptr ? a.requests[t] : static_cast<int32_t>(t);
     const int32_t pos = a.positions[t];
-    r.bad = r.request >= a.requests_count || pos < -1 || pos >= (a.width << a.page_shift);
-    r.end = r.bad ? 0 : pos + 1;
-    r.first = a.window > 0 && a.window < r.end ? r.end - static_cast<int32_t>(a.window) : 0;
+    k.bad = k.request >= a.requests_count || pos < -1 || pos >= (a.width << a.page_shift);
+    k.end = k.bad ? 0 : pos + 1;
+    k.first = a.window > 0 && a.window < k.end ? k.end - static_cast<int32_t>(a.window) : 0;
+    return k;
+}
+
+// The rows of a unit, `count` from this one on: keys [first, end) are seen by some of them, [all_first, all_end) by all; the tiles begin
+// at start.
+struct Row {
+    int32_t request, first, end, all_first, all_end, start, tiles, count;
+    bool bad;
+};
+
+// Row t with those that share units with it. Rows that belong to another row's units have no tiles, like rows of no request. With
+// `rows` > 1, a unit's rows lie within an aligned block of so many, follow each other, are of one request and none is bad.
+template <bool GROUPED> __device__ __forceinline__ Row row_of(const PagedAttentionArgs &a, int64_t t, int tile_keys, int rows) {
+    const Keys k = keys_of(a, t);
+    Row r{k.request, k.first, k.end, k.first, k.end, 0, 0, 1, k.bad};
+    if (k.request < 0) {
+        return r;
+    }
+    if constexpr (GROUPED) {
+        if (t % rows != 0 && !k.bad) {
+            const Keys before = keys_of(a, t - 1);
+            if (before.request == k.request && !before.bad) {
+                return r;
+            }
+        }
+        const int64_t stop = min(a.rows, t - t % rows + rows);
+        for (int64_t u = t + 1; u < stop && !k.bad; ++u) {
+            const Keys next = keys_of(a, u);
+            if (next.request != k.request || next.bad) {
+                break;
+            }
+            r.first = min(r.first, next.first), r.end = max(r.end, next.end);
+            r.all_first = max(r.all_first, next.first), r.all_end = min(r.all_end, next.end);
+            ++r.count;
+        }
+    }
     r.start = r.first & ~15;
-    // A row without keys still has an output to write.
-    r.tiles = r.request < 0 ? 0 : max(1, (r.end - r.start + tile_keys - 1) / tile_keys);
+    r.tiles = max(1, (r.end - r.start + tile_keys - 1) / tile_keys); // a row without keys still has an output to write
     return r;
 }
 
@@ -42,7 +77,8 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
 // A row that all lanes hold, in scalar registers: page addresses must be known to be uniform, or each load becomes a loop over
 // the lanes' addresses (which took 374 us instead of 358 at 64 rows of 8192 keys).
 __device__ __forceinline__ Row uniform_row(const Row &r) {
-    return Row{uniform(r.request), uniform(r.first), uniform(r.start), uniform(r.end), uniform(r.tiles), uniform(r.bad) != 0};
+    return Row{uniform(r.request), uniform(r.first), uniform(r.end),   uniform(r.all_first), uniform(r.all_end),
+               uniform(r.start),   uniform(r.tiles), uniform(r.count), uniform(r.bad) != 0};
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -64,12 +100,14 @@ template <> struct Split<F16> {
     typedef _Float16 elem;
     static constexpr float kTop = 15.0f;
     static constexpr float kBelow = 1.0f - 0x1p-11f;
+    static constexpr uint32_t kExponent = 0x7C00u; // all bits set: an infinity or NaN
 };
 template <> struct Split<BF16> {
     typedef bf16x8_t vec;
     typedef __bf16 elem;
     static constexpr float kTop = 0.0f;
     static constexpr float kBelow = 1.0f - 0x1p-8f;
+    static constexpr uint32_t kExponent = 0x7F80u;
 };
 
 template <class T, int D> struct Shape {
@@ -107,9 +145,9 @@ template <int D> struct Pieces {
     __device__ __forceinline__ uint32_t lds_step(int i) const { return kEven ? i * (64 / kPerRow) * (2 * D + 32) : places[i % kKept]; }
 };
 
-// TEAM waves of a workgroup (4 or 1) share a run of tiles of TEAM * 32 keys; a workgroup has 4 / TEAM runs. CT: column tiles of
-// 16 query heads that a unit has at most.
-template <class T, int D, int TEAM, int CT>
+// TEAM waves of a workgroup (4 or 1) share a run of tiles of TEAM * 32 keys; a workgroup has 4 / TEAM runs. CT: tiles of 16 columns that
+// a unit has at most. GROUPED: units of several rows.
+template <class T, int D, int TEAM, int CT, bool GROUPED>
 __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_kernel(PagedAttentionArgs a, AttentionPlan plan) {
     using S = Shape<T, D>;
     using vec = typename Split<T>::vec;
@@ -136,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
         const int t0 = min(static_cast<int>(threadIdx.x) * per, rows), t1 = min(t0 + per, rows);
         int own = 0;
         for (int i = t0; i < t1; ++i) {
-            own += row_of(a, i, kTileKeys).tiles;
+            own += row_of<GROUPED>(a, i, kTileKeys, plan.rows).tiles;
         }
         int upto = own;
 #pragma unroll
@@ -164,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
                 int b = before * units;
                 for (int i = t0; i < t1; ++i) {
                     // The row is read again below, by scalar loads: handed on over LDS it cost 5 us of a call's 11.
-                    const int n = (per == 1 ? own : row_of(a, i, kTileKeys).tiles) * units;
+                    const int n = (per == 1 ? own : row_of<GROUPED>(a, i, kTileKeys, plan.rows).tiles) * units;
                     if (xj < b + n) {
                         found[j][0] = i;
                         found[j][1] = b;
@@ -180,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
     if (x < x_end) {
         t = uniform(found[TEAM == 1 ? wave : 0][0]);
         base = uniform(found[TEAM == 1 ? wave : 0][1]);
-        r = uniform_row(row_of(a, t, kTileKeys));
+        r = uniform_row(row_of<GROUPED>(a, t, kTileKeys, plan.rows));
     }
 
     // ---- constants of the lane ----
@@ -198,24 +236,33 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
             int from = t + 1;
             uint64_t some = 0;
             for (; from < rows; from += 64) {
-                some = __ballot(from + lane < rows && row_of(a, min(from + lane, rows - 1), kTileKeys).tiles > 0);
+                some = __ballot(from + lane < rows && row_of<GROUPED>(a, min(from + lane, rows - 1), kTileKeys, plan.rows).tiles > 0);
                 if (some != 0) {
                     break;
                 }
             }
             t = uniform(some != 0 ? from + static_cast<int>(__builtin_ctzll(some)) : rows - 1); // a run ends before the rows do
-            r = uniform_row(row_of(a, t, kTileKeys));
+            r = uniform_row(row_of<GROUPED>(a, t, kTileKeys, plan.rows));
         }
         const int unit = uniform(static_cast<uint32_t>(x - base) / static_cast<uint32_t>(r.tiles));
         const int tile0 = x - base - unit * r.tiles;
         const int tile1 = min(r.tiles, tile0 + (x_end - x));
-        const UnitHeads heads = plan.heads_of(unit);
+        const int columns = plan.columns<GROUPED>(unit, r.count), kv_head = uniform(plan.kv_head(unit));
 
         u32x4_t q[CT][S::kSteps];
+        int first[GROUPED ? CT : 1], end[GROUPED ? CT : 1], row_in_unit[GROUPED ? CT : 1]; // of the lane's column
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-            const bool live = 16 * c + col < heads.count;
-            const uint16_t *q_row = a.q + static_cast<int64_t>(t) * a.ldq + static_cast<int64_t>(heads.q_head + (live ? 16 * c + col : 0)) * D + 8 * quad;
+            const bool live = 16 * c + col < columns;
+            const Column at = plan.column<GROUPED>(unit, live ? 16 * c + col : 0);
+            const uint16_t *q_row = a.q + static_cast<int64_t>(t + at.row) * a.ldq + static_cast<int64_t>(at.q_head) * D + 8 * quad;
+            if constexpr (GROUPED) {
+                first[c] = r.first, end[c] = r.end, row_in_unit[c] = at.row;
+                if (!r.bad) {
+                    const Keys k = keys_of(a, t + at.row);
+                    first[c] = k.first, end[c] = k.end;
+                }
+            }
 #pragma unroll
             for (int s = 0; s < S::kSteps; ++s) {
                 q[c][s] = live ? *reinterpret_cast<const u32x4_t *>(q_row + 32 * s) : u32x4_t{0, 0, 0, 0};
@@ -232,11 +279,11 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
             }
             m[c] = -INFINITY, l[c] = 0.0f;
         }
-        bool poisoned = false;
+        bool poisoned[GROUPED ? CT : 1] = {}; // a page outside the cache among those that the column (GROUPED) or the row sees
 
         u32x4_t k_reg[2][S::kSteps], v_reg[2][S::kSteps];
         const int32_t *table = a.block_table + uniform64((r.bad ? 0 : r.request) * a.ld_table);
-        const uint16_t *k_head = a.k + uniform64(heads.kv_head * a.head_stride), *v_head = a.v + uniform64(heads.kv_head * a.head_stride);
+        const uint16_t *k_head = a.k + uniform64(kv_head * a.head_stride), *v_head = a.v + uniform64(kv_head * a.head_stride);
         const int64_t page_stride = uniform64(a.page_stride);
         const int shift = uniform(a.page_shift), offset_mask = (1 << shift) - 1;
         const uint32_t pages = uniform(static_cast<int>(a.pages));
@@ -255,7 +302,14 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
                 const int32_t page = uniform(id[s]);
                 int seen = max(0, min(16, r.end - key));
                 if (static_cast<uint32_t>(page) >= pages) {
-                    poisoned |= seen > 0;
+                    if constexpr (GROUPED) {
+#pragma unroll
+                        for (int c = 0; c < CT; ++c) {
+                            poisoned[c] |= key < end[c] && key + 16 > first[c];
+                        }
+                    } else {
+                        poisoned[0] |= seen > 0;
+                    }
                     seen = 0;
                 }
                 // Past the row's last key the buffer ends, and its loads return zero.
@@ -264,11 +318,11 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
                 const __amdgpu_buffer_rsrc_t kr = buffer_rsrc(k_head + at, bytes), vr = buffer_rsrc(v_head + at, bytes);
 #pragma unroll
                 for (int i = 0; i < S::kSteps; ++i) {
-                    k_reg[s][i] = __builtin_amdgcn_raw_buffer_load_b128(kr, pieces.offset(i), 0, kStream);
+                    k_reg[s][i] = __builtin_amdgcn_raw_buffer_load_b128(kr, pieces.offset(i), 0, GROUPED ? 0 : kStream);
                 }
 #pragma unroll
                 for (int i = 0; i < S::kSteps; ++i) {
-                    v_reg[s][i] = __builtin_amdgcn_raw_buffer_load_b128(vr, pieces.offset(i), 0, kStream);
+                    v_reg[s][i] = __builtin_amdgcn_raw_buffer_load_b128(vr, pieces.offset(i), 0, GROUPED ? 0 : kStream);
                 }
             }
         };
@@ -289,6 +343,26 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
                             v_reg[s][i] = u32x4_t{0, 0, 0, 0};
                         }
                     }
+                }
+            }
+            const bool some_masked = key0 < r.all_first || key0 + kWaveKeys > r.all_end;
+            // Keys that some of the unit's rows see and others do not: their weight is zero where they are not seen, but zero times an infinity or
+            // NaN among the values would still show there. Then the rows go one by one.
+            bool apart = false;
+            if constexpr (GROUPED) {
+                if (some_masked) {
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+                        for (int i = 0; i < S::kSteps; ++i) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t v = v_reg[s][i][k], e = Split<T>::kExponent;
+                                apart |= (v & e) == e || (v >> 16 & e) == e;
+                            }
+                        }
+                    }
+                    apart = __any(apart);
                 }
             }
             // K and then V pass through the wave's own region of LDS; a wave's LDS accesses are carried out in order.
@@ -334,11 +408,11 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
                 for (int e = 0; e < 8; ++e) {
                     p[e] = score[c][e >> 2][e & 3] * c_scale;
                 }
-                if (key0 < r.first || key0 + kWaveKeys > r.end) {
+                if (some_masked) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const int key = key0 + 16 * (e >> 2) + 4 * quad + (e & 3);
-                        p[e] = key >= r.first && key < r.end ? p[e] : -INFINITY;
+                        p[e] = key >= (GROUPED ? first[c] : r.first) && key < (GROUPED ? end[c] : r.end) ? p[e] : -INFINITY;
                     }
                 }
                 float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
@@ -371,6 +445,29 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
                     half[s] = lds_read_transposed(lds + v_lds + s * 16 * S::kRowBytes + i * 32);
                 }
                 const uint4 vt = make_uint4(half[0].x, half[0].y, half[1].x, half[1].y);
+                if constexpr (GROUPED) {
+                    if (apart) {
+                        for (int u = 0; u < r.count; ++u) {
+                            const Keys seen = keys_of(a, t + u);
+                            uint32_t mine[4] = {vt.x, vt.y, vt.z, vt.w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const int key = key0 + 16 * (k >> 1) + 4 * quad + 2 * (k & 1);
+                                mine[k] &= (key >= seen.first && key < seen.end ? 0xFFFFu : 0u) |
+                                           (key + 1 >= seen.first && key + 1 < seen.end ? 0xFFFF0000u : 0u);
+                            }
+                            const uint4 vu = make_uint4(mine[0], mine[1], mine[2], mine[3]);
+#pragma unroll
+                            for (int c = 0; c < CT; ++c) {
+                                float4_t sum = o[c][i];
+                                sum = T::mfma16(vu, __builtin_bit_cast(uint4, hi[c]), sum);
+                                sum = T::mfma16(vu, __builtin_bit_cast(uint4, lo[c]), sum);
+                                o[c][i] = row_in_unit[c] == u ? sum : o[c][i];
+                            }
+                        }
+                        continue;
+                    }
+                }
 #pragma unroll
                 for (int c = 0; c < CT; ++c) {
                     o[c][i] = T::mfma16(vt, __builtin_bit_cast(uint4, hi[c]), o[c][i]);
@@ -383,31 +480,35 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
         const bool whole = tile0 == 0 && tile1 == r.tiles;
         const int64_t part = 2 * w + (tile0 == 0 ? 1 : 0);
         const AttentionWorkspace ws = carve(a.workspace, plan.runs, plan.cols);
-        uint16_t *out = a.out + static_cast<int64_t>(t) * a.ldo + static_cast<int64_t>(heads.q_head) * D;
+        const auto out = [&](int j) {
+            const Column at = plan.column<GROUPED>(unit, j);
+            return a.out + static_cast<int64_t>(t + at.row) * a.ldo + static_cast<int64_t>(at.q_head) * D;
+        };
         // What a whole unit's sums are divided by: NaN outside the table; a row that sees no key is zero over one.
-        const auto divisor = [&](float sum) { return r.bad ? NAN : r.end == 0 ? 1.0f : sum; };
+        const auto divisor = [&](float sum, int keys_end) { return r.bad ? NAN : keys_end == 0 ? 1.0f : sum; };
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
             l[c] += __shfl_xor(l[c], 16);
             l[c] += __shfl_xor(l[c], 32);
-            if (poisoned) {
+            if (poisoned[GROUPED ? c : 0]) {
                 l[c] = NAN;
             }
-            const int first = 16 * c, used = min(16, heads.count - first);
+            const int before = 16 * c, used = min(16, columns - before);
             if constexpr (TEAM == 1) {
                 if (col < used) {
-                    const float over = divisor(l[c]);
+                    const float over = divisor(l[c], GROUPED ? end[c] : r.end);
+                    uint16_t *to = out(before + col);
 #pragma unroll
                     for (int i = 0; i < S::kDTiles; ++i) {
                         const int d = 16 * i + 4 * quad;
                         if (whole) {
-                            store4<T>(out + static_cast<int64_t>(first + col) * D + d, o[c][i] / over);
+                            store4<T>(to + d, o[c][i] / over);
                         } else {
-                            *reinterpret_cast<float4_t *>(ws.o + (part * plan.cols + first + col) * D + d) = o[c][i];
+                            *reinterpret_cast<float4_t *>(ws.o + (part * plan.cols + before + col) * D + d) = o[c][i];
                         }
                     }
                     if (!whole && quad == 0) {
-                        ws.stats[part * plan.cols + first + col] = make_float2(m[c], l[c]);
+                        ws.stats[part * plan.cols + before + col] = make_float2(m[c], l[c]);
                     }
                 }
             } else {
@@ -446,11 +547,12 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
                         v += *reinterpret_cast<const float4_t *>(reinterpret_cast<const float *>(lds + k * S::kRegion) + j * S::kORow + d);
                     }
                     if (whole) {
-                        store4<T>(out + static_cast<int64_t>(first + j) * D + d, v / divisor(sum));
+                        const int keys_end = GROUPED && !r.bad ? keys_of(a, t + plan.column<GROUPED>(unit, before + j).row).end : r.end;
+                        store4<T>(out(before + j) + d, v / divisor(sum, keys_end));
                     } else {
-                        *reinterpret_cast<float4_t *>(ws.o + (part * plan.cols + first + j) * D + d) = v;
+                        *reinterpret_cast<float4_t *>(ws.o + (part * plan.cols + before + j) * D + d) = v;
                         if (d == 0) {
-                            ws.stats[part * plan.cols + first + j] = make_float2(top, sum);
+                            ws.stats[part * plan.cols + before + j] = make_float2(top, sum);
                         }
                     }
                 }
@@ -458,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
             }
         }
         if (tile0 == 0 && !whole) {
-            begun = AttentionDescriptor{t, unit, runs.of(x + r.tiles - 1) - w, 0};
+            begun = AttentionDescriptor{t, unit, runs.of(x + r.tiles - 1) - w, r.count};
         }
         x = uniform(x + tile1 - tile0);
     }
@@ -467,10 +569,10 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
     }
 }
 
-// The parts of column j of one unit, of runs w .. w + pieces, joined into `out`: THREADS threads, kLanes parts at a time for each of its
+// The parts of column j of one unit, of runs w .. w + pieces, joined into `out` (zero if the column sees no key): THREADS threads, kLanes parts at a time for each of its
 // float4 elements, kAhead of them requested before the first is used.
 template <class T, int D, int THREADS>
-__device__ __forceinline__ void join_column(uint16_t *out, const AttentionWorkspace &ws, int cols, int w, int pieces, int j) {
+__device__ __forceinline__ void join_column(uint16_t *out, bool empty, const AttentionWorkspace &ws, int cols, int w, int pieces, int j) {
     constexpr int kItems = D / 4;
     constexpr int kLanes = THREADS / kItems;
     constexpr int kAhead = 4;
@@ -528,7 +630,7 @@ __device__ __forceinline__ void join_column(uint16_t *out, const AttentionWorksp
             all += acc[i][e] * f;
             sum += stat[i].y * f;
         }
-        store4<T>(out + 4 * e, all / sum);
+        store4<T>(out + 4 * e, empty ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : all / sum);
     }
     __syncthreads();
 }
@@ -538,64 +640,75 @@ __device__ __forceinline__ void join_column(uint16_t *out, const AttentionWorksp
 // The joins are a launch of their own: the count of arrivals that would let the last workgroup join in the first launch costs
 // as much, since its stores, count and loads each go to memory and back past the XCDs' L2s, one after the other (and with fences of that
 // scope instead, which write back and drop a whole L2, 64 rows of 8192 keys took 670 us).
-template <class T, int D> __global__ void __launch_bounds__(64) join_kernel(PagedAttentionArgs a, AttentionPlan plan) {
+template <class T, int D, bool GROUPED> __global__ void __launch_bounds__(64) join_kernel(PagedAttentionArgs a, AttentionPlan plan) {
     const AttentionWorkspace ws = carve(a.workspace, plan.runs, plan.cols);
     const AttentionDescriptor d = ws.desc[blockIdx.x];
     if (d.pieces == 0) {
         return;
     }
-    const UnitHeads heads = plan.heads_of(d.unit);
-    for (int j = blockIdx.y; j < heads.count; j += gridDim.y) {
-        join_column<T, D, 64>(a.out + d.row * a.ldo + static_cast<int64_t>(heads.q_head + j) * D, ws, plan.cols, blockIdx.x, d.pieces, j);
+    const int columns = plan.columns<GROUPED>(d.unit, d.count);
+    for (int j = blockIdx.y; j < columns; j += gridDim.y) {
+        const Column at = plan.column<GROUPED>(d.unit, j);
+        const int64_t row = d.row + at.row;
+        join_column<T, D, 64>(a.out + row * a.ldo + static_cast<int64_t>(at.q_head) * D, a.positions[row] < 0, ws, plan.cols, blockIdx.x, d.pieces, j);
     }
 }
 
 // The same for few units, which have many parts each: a workgroup per unit and column, which finds the parts from the lengths.
 constexpr int kFewThreads = 512;
-template <class T, int D> __global__ void __launch_bounds__(kFewThreads) join_few_kernel(PagedAttentionArgs a, AttentionPlan plan) {
+template <class T, int D, bool GROUPED> __global__ void __launch_bounds__(kFewThreads) join_few_kernel(PagedAttentionArgs a, AttentionPlan plan) {
     constexpr int kTileKeys = kAttentionWaves * kWaveKeys; // few units are dealt in tiles of whole workgroups
     const int t = blockIdx.x / plan.units, unit = blockIdx.x - t * plan.units;
-    int before = 0, own = 0, total = 0;
+    int before = 0, total = 0;
+    Row own{};
     for (int i = 0; i < static_cast<int>(a.rows); ++i) { // a handful
-        const int n = row_of(a, i, kTileKeys).tiles;
-        before += i < t ? n : 0;
-        own = i == t ? n : own;
-        total += n;
+        const Row r = row_of<GROUPED>(a, i, kTileKeys, plan.rows);
+        before += i < t ? r.tiles : 0;
+        if (i == t) {
+            own = r;
+        }
+        total += r.tiles;
     }
-    if (own == 0) {
+    if (own.tiles == 0) {
         return;
     }
     const Runs runs = Runs::deal(total * plan.units, plan.runs);
-    const int first = before * plan.units + unit * own;
-    const int w = runs.of(first), pieces = runs.of(first + own - 1) - w;
-    const UnitHeads heads = plan.heads_of(unit);
+    const int first = before * plan.units + unit * own.tiles;
+    const int w = runs.of(first), pieces = runs.of(first + own.tiles - 1) - w;
     const int j = blockIdx.y;
-    if (pieces == 0 || j >= heads.count) {
+    if (pieces == 0 || j >= plan.columns<GROUPED>(unit, own.count)) {
         return;
     }
-    join_column<T, D, kFewThreads>(a.out + t * a.ldo + static_cast<int64_t>(heads.q_head + j) * D, carve(a.workspace, plan.runs, plan.cols), plan.cols, w, pieces,
-                                   j);
+    const Column at = plan.column<GROUPED>(unit, j);
+    const int64_t row = t + at.row;
+    join_column<T, D, kFewThreads>(a.out + row * a.ldo + static_cast<int64_t>(at.q_head) * D, a.positions[row] < 0,
+                                   carve(a.workspace, plan.runs, plan.cols), plan.cols, w, pieces, j);
 }
 
-template <class T, int D, int TEAM, int CT> hipError_t launch(const PagedAttentionArgs &a, const AttentionPlan &plan, hipStream_t stream) {
+template <class T, int D, int TEAM, int CT, bool GROUPED> hipError_t launch(const PagedAttentionArgs &a, const AttentionPlan &plan, hipStream_t stream) {
     const unsigned blocks = static_cast<unsigned>((plan.runs * TEAM + kAttentionWaves - 1) / kAttentionWaves);
-    hipLaunchKernelGGL((paged_attention_kernel<T, D, TEAM, CT>), dim3(blocks), dim3(kThreads), 0, stream, a, plan);
+    hipLaunchKernelGGL((paged_attention_kernel<T, D, TEAM, CT, GROUPED>), dim3(blocks), dim3(kThreads), 0, stream, a, plan);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {
         return e;
     }
     if (plan.few_units) {
-        hipLaunchKernelGGL((join_few_kernel<T, D>), dim3(static_cast<unsigned>(a.rows * plan.units), static_cast<unsigned>(plan.cols)),
+        hipLaunchKernelGGL((join_few_kernel<T, D, GROUPED>), dim3(static_cast<unsigned>(a.rows * plan.units), static_cast<unsigned>(plan.cols)),
                            dim3(kFewThreads), 0, stream, a, plan);
     } else {
-        hipLaunchKernelGGL((join_kernel<T, D>), dim3(static_cast<unsigned>(plan.runs), static_cast<unsigned>(plan.cols < 4 ? plan.cols : 4)), dim3(64), 0,
+        hipLaunchKernelGGL((join_kernel<T, D, GROUPED>), dim3(static_cast<unsigned>(plan.runs), static_cast<unsigned>(plan.cols < 4 ? plan.cols : 4)), dim3(64), 0,
                            stream, a, plan);
     }
     return hipGetLastError();
 }
 
 template <class T, int D> hipError_t launch_d(const PagedAttentionArgs &a, const AttentionPlan &plan, hipStream_t stream) {
-    return plan.team == 1 ? launch<T, D, 1, 1>(a, plan, stream) : plan.cols <= 16 ? launch<T, D, 4, 1>(a, plan, stream) : launch<T, D, 4, 2>(a, plan, stream);
+    if (plan.rows > 1) {
+        return plan.team == 1 ? launch<T, D, 1, 1, true>(a, plan, stream) : launch<T, D, 4, 1, true>(a, plan, stream);
+    }
+    return plan.team == 1     ? launch<T, D, 1, 1, false>(a, plan, stream)
+           : plan.cols <= 16 ? launch<T, D, 4, 1, false>(a, plan, stream)
+                              : launch<T, D, 4, 2, false>(a, plan, stream);
 }
 
 template <class T> hipError_t launch_t(const PagedAttentionArgs &a, const AttentionPlan &plan, hipStream_t stream) {

@@ -152,6 +152,119 @@ def test_few_rows(hm, device, lengths):
     _check(hm, device, Case(23, lengths, 6, 2, 64, 256, torch.bfloat16), tag="few rows")
 
 
+def _prompt_rows(seed):
+    """(positions, requests) of more rows than requests: chunks of prompts, drafted tokens, decodes, positions out of order and twice, empty
+    rows and rows of no request, at places that fall in and across blocks of 2 to 16 rows."""
+    rng = np.random.default_rng(seed)
+    rows = [(p, 2) for p in range(800, 1025)] + [(p, 1) for p in range(40)] + [(299, 0), (298, 0), (299, 0)] + [(-1, 0), (5, 0)] + [(0, 3)] * 2
+    rows += [(-1, -1)] * 5 + [(int(p), 2) for p in rng.integers(-1, 1025, 30)] + [(6, 3), (39, 1), (299, 0), (1024, 2)] * 3 + [(-1, -1)] * 100 + [(250, 0)]
+    return [r[0] for r in rows], [r[1] for r in rows]
+
+
+def _group_case(seed, heads, d, dtype):
+    return Case(seed, [300, 40, 1025, 7], heads[0], heads[1], d, 16, dtype)
+
+
+def _queries(c, rows, seed=30):
+    return (1.5 * torch.randn((rows, c.q_heads, c.k.size(3)), generator=torch.Generator().manual_seed(seed))).to(c.dtype)
+
+
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("heads", [(4, 4), (6, 2), (8, 2), (7, 1), (16, 1), (20, 1)])
+@pytest.mark.parametrize("window", [0, 37])
+def test_prompts_and_drafts(hm, device, heads, d, window):
+    c = _group_case(24, heads, d, torch.float16 if d == 96 else torch.bfloat16)
+    positions, requests = _prompt_rows(25)
+    got = _check(hm, device, c, positions, requests, _queries(c, len(positions)), window=window, tag="prompts and drafts")
+    for t, p in enumerate(positions):
+        if requests[t] >= 0 and p < 0:
+            assert (got[t] == 0).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompts_enough_for_a_run_per_wave(hm, device, d):
+    # as many blocks of rows and heads as waves fit the card
+    rng = np.random.default_rng(26)
+    c = Case(26, [int(v) for v in rng.integers(20, 90, 60)], 32, 16, d, 16, torch.bfloat16)
+    rows = [(p, r) for r, n in enumerate(c.lengths) for p in range(0 if r % 3 else n - 1, n)]
+    rows += [(-1, -1)] * 20
+    assert len(rows) >= 1040
+    positions, requests = zip(*rows)
+    _check(hm, device, c, list(positions), list(requests), _queries(c, len(rows)), tag="prompts, a run per wave")
+
+
+@pytest.mark.parametrize("window", [0, 64])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_later_tokens_do_not_show_in_earlier_rows(hm, device, dtype, window):
+    # an infinite value, a NaN value and a NaN key in the middle of a prompt: the rows before them, and behind their window, know nothing of them
+    c = _group_case(27, (8, 2), 128, DT[dtype])
+    at = lambda t, p: t[int(c.table[2, p // 16]), :, p % 16]
+    clean = [t.clone() for t in (c.k, c.v)]
+    at(c.v, 850)[0, 5] = float("inf")
+    at(c.v, 853)[1, 7] = float("nan")
+    at(c.k, 901)[0, 3] = float("nan")
+    positions = list(range(800, 1025))
+    q = _queries(c, len(positions))
+    pos, req = torch.tensor(positions, dtype=torch.int32), torch.full((len(positions),), 2, dtype=torch.int32)
+    out = torch.zeros(q.shape, dtype=c.dtype, device=device)
+    got = hm.paged_attention(out, q.to(device), c.cache(hm, device), c.table.to(device), pos.to(device), req.to(device), window=window).cpu()
+    c.k, c.v = clean
+    want, bound = ref.attention(q, c.k, c.v, c.table, pos, req, 1 / math.sqrt(128), window, 16)
+    sees = lambda p: torch.tensor([x >= p and (not window or x < p + window) for x in positions])
+    hit = torch.zeros(q.shape, dtype=torch.bool)
+    hit[sees(850), :4, 5] = True
+    hit[sees(853), 4:, 7] = True
+    assert torch.isposinf(got[sees(850) & ~sees(901)][:, :4, 5]).all()
+    assert torch.isnan(got[sees(853)][:, 4:, 7]).all()
+    assert torch.isnan(got[sees(901)][:, :4]).all()
+    hit[sees(901), :4] = True
+    assert torch.isfinite(got[~hit]).all()
+    ref.assert_within(torch.where(hit, 0, got), torch.where(hit, 0.0, want), bound, c.dtype, "the others")
+
+
+@pytest.mark.parametrize("window", [0, 40])
+def test_rows_that_see_a_bad_page_are_nan_and_their_neighbours_not(hm, device, window):
+    c = _group_case(28, (8, 2), 64, torch.bfloat16)
+    table = c.table.clone()
+    table[2, 52] = -3  # tokens 832..847
+    rows = [(p, 2) for p in range(801, 900)] + [(100, 0), (16 * table.size(1), 0), (101, 0), (-2, 0), (102, 0), (103, 4), (103, 0)]
+    positions, requests = zip(*rows)
+    q = _queries(c, len(rows))
+    pos, req = torch.tensor(positions, dtype=torch.int32), torch.tensor(requests, dtype=torch.int32)
+    got = hm.paged_attention(torch.zeros(q.shape, dtype=c.dtype, device=device), q.to(device), c.cache(hm, device), table.to(device), pos.to(device), req.to(device),
+                             window=window).cpu()
+    sees = torch.tensor([(r == 2 and p >= 832 and (not window or p - window < 847)) or r == 4 or p in (-2, 16 * table.size(1)) for p, r in rows])
+    assert torch.isnan(got[sees]).all()
+    fine = ~sees
+    want, bound = ref.attention(q[fine], c.k, c.v, c.table, pos[fine], req[fine], 1 / 8, window, 16)
+    ref.assert_within(got[fine], want, bound, c.dtype, "rows that do not see it")
+
+
+def test_prompts_in_a_replayed_graph(hm, device):
+    c = _group_case(29, (8, 2), 128, torch.bfloat16)
+    cache, table = c.cache(hm, device), c.table.to(device)
+    pos, req = (torch.zeros(64, dtype=torch.int32, device=device) for _ in range(2))
+    q, out, ws = _queries(c, 64).to(device), torch.zeros((64, 8, 128), dtype=c.dtype, device=device), cache.attention_workspace(8)
+    hm.paged_attention(out, q, cache, table, pos, req, workspace=ws)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        hm.paged_attention(out, q, cache, table, pos, req, workspace=ws)
+    rng = np.random.default_rng(29)
+    for _ in range(4):
+        r = np.sort(rng.integers(-1, 4, 64))
+        p = np.array([rng.integers(-1, c.lengths[x]) if x >= 0 else -1 for x in r])
+        pos.copy_(torch.tensor(p, dtype=torch.int32))
+        req.copy_(torch.tensor(r, dtype=torch.int32))
+        out.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        live = torch.tensor(r >= 0)
+        want, bound = ref.attention(q.cpu(), c.k, c.v, c.table, p, r, 1 / math.sqrt(128), 0, 16)
+        ref.assert_within(out[live.to(device)], want[live], bound[live], c.dtype, "replay")
+        assert (out[~live.to(device)] == 7.0).all()
+
+
 def test_rows_of_requests(hm, device):
     # several rows of one request (drafted tokens), empty rows, rows of no request in runs longer than a wave, requests out of order
     c = Case(8, [300, 40, 1025], 8, 2, 128, 16, torch.bfloat16)
