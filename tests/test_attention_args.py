@@ -64,8 +64,9 @@ def test_workspace_bytes(hm):
     lib = hm._lib.load()
     assert lib.hm_paged_attention_workspace_bytes(None, 8) == 0
     assert lib.hm_paged_attention_workspace_bytes(ctypes.byref(_cache(hm)), 7) == 0
-    small, large = (lib.hm_paged_attention_workspace_bytes(ctypes.byref(_cache(hm)), h) for h in (2, 32))
-    assert 0 < small < large == lib.hm_paged_attention_workspace_bytes(ctypes.byref(_cache(hm)), 80)
+    size = lambda h, **over: lib.hm_paged_attention_workspace_bytes(ctypes.byref(_cache(hm, **over)), h)
+    assert size(2) > 0 and size(2) == size(32) == size(16)  # units of 16 columns: rows of a request, or query heads
+    assert size(80) > 0 and size(8, head_dim=128) > size(8)
 
 
 def _rope_args(hm, **over):
