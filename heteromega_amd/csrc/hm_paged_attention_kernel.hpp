@@ -659,15 +659,29 @@ constexpr int kFewThreads = 512;
 template <class T, int D, bool GROUPED> __global__ void __launch_bounds__(kFewThreads) join_few_kernel(PagedAttentionArgs a, AttentionPlan plan) {
     constexpr int kTileKeys = kAttentionWaves * kWaveKeys; // few units are dealt in tiles of whole workgroups
     const int t = blockIdx.x / plan.units, unit = blockIdx.x - t * plan.units;
+    __shared__ int sums[kFewThreads / 64][2];
+    const Row own = row_of<GROUPED>(a, t, kTileKeys, plan.rows);
     int before = 0, total = 0;
-    Row own{};
-    for (int i = 0; i < static_cast<int>(a.rows); ++i) { // a handful
-        const Row r = row_of<GROUPED>(a, i, kTileKeys, plan.rows);
-        before += i < t ? r.tiles : 0;
-        if (i == t) {
-            own = r;
-        }
-        total += r.tiles;
+    for (int i = threadIdx.x; i < static_cast<int>(a.rows); i += kFewThreads) {
+        const int n = row_of<GROUPED>(a, i, kTileKeys, plan.rows).tiles;
+        before += i < t ? n : 0;
+        total += n;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        before += __shfl_xor(before, off);
+        total += __shfl_xor(total, off);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        sums[threadIdx.x >> 6][0] = before;
+        sums[threadIdx.x >> 6][1] = total;
+    }
+    __syncthreads();
+    before = total = 0;
+#pragma unroll
+    for (int i = 0; i < kFewThreads / 64; ++i) {
+        before += sums[i][0];
+        total += sums[i][1];
     }
     if (own.tiles == 0) {
         return;
