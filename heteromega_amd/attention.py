@@ -14,68 +14,32 @@ import math
 import torch
 
 from . import _lib
-from .ffn import (_DTYPES, _aligned, _call, _handed_over, _hm_dtype, _on, _stream, _workspace, packed_linear, residual_add2, rmsnorm)
+from .ffn import (_DTYPES, _call, _current_raw_stream, _hm_dtype, _on, _stream, _workspace, packed_linear, residual_add2, rmsnorm)
+
+try:
+    # The checks and calls of the three operators, compiled: at few rows they took longer in Python than the kernels run.
+    from . import _attention_host as _host
+except ImportError as e:
+    raise ImportError("heteromega_amd._attention_host is missing: run `python heteromega_amd/build.py` (or __graft_entry__.build()) first") from e
 
 kPagePlanMaxRequests = 4096
 
 
-# The current device's index without torch.cuda's check that it is initialized (device tensors are at hand): not part of torch's public
-# interface, so a torch without it takes the public call.
-_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+def _bind():
+    L = _lib.load()
+    address = lambda f: ctypes.cast(f, ctypes.c_void_p).value
+    current = _current_raw_stream or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _host.bind(address(L.hm_page_plan), address(L.hm_qk_norm_rope), address(L.hm_paged_attention), current, _stream)
+
+
+_bind()
 
 
 def _guard(device):
-    """The device of the tensors as the current one: a launch goes to the current device."""
-    if device.index == _current_device():
+    """`device` as the current one, for a call that allocates or launches there."""
+    if device.index == torch.cuda.current_device():
         return contextlib.nullcontext()
     return torch.cuda.device(device)
-
-
-def _on_device(device, call, *args):
-    """call(*args) with `device` current, its status checked. (A with statement costs 0.5 us, a tenth of a small call.)"""
-    if device.index == _current_device():
-        status = call(*args)
-    else:
-        with torch.cuda.device(device):
-            status = call(*args)
-    if status != _lib.HM_OK:
-        _call(status)
-
-
-def _device_of(t, what):
-    device = t.device
-    if device.type != "cuda":
-        raise ValueError(f"{what}: needs device tensors, got one on {device}")
-    return device
-
-
-def _vector(t, dtype, n, device, what, name, more=False):
-    """Address of a contiguous vector of n elements (or more)."""
-    if t.dtype is not dtype or t.device != device or not t.is_contiguous() or t.dim() != 1 or (t.size(0) < n if more else t.size(0) != n):
-        raise ValueError(f"{what}: {name} must be a contiguous {dtype} vector of {n}{' or more' if more else ''} elements on {device}, got {t.dtype} "
-                         f"{list(t.shape)} with strides {t.stride()} on {t.device}")
-    return t.data_ptr()
-
-
-def _rows(t, rows, heads, d, dtype, device, what, name):
-    """(address, leading dimension) of [rows, heads * d] or [rows, heads, d] with packed heads."""
-    shape, stride = t.shape, t.stride()
-    if len(shape) == 3:
-        ok = shape == (rows, heads, d) and (d == 1 or stride[2] == 1) and (heads == 1 or stride[1] == d)
-    else:
-        ok = shape == (rows, heads * d) and stride[1] == 1
-    if not ok or t.dtype is not dtype or t.device != device:
-        raise ValueError(f"{what}: {name} must be {dtype} [{rows}, {heads} x {d}] with contiguous rows on {device}, got {t.dtype} {list(shape)} with strides "
-                         f"{stride} on {t.device}")
-    return t.data_ptr(), (stride[0] if rows > 1 else heads * d)
-
-
-def _table(t, device, what):
-    """(address, leading dimension, requests, pages of a request) of a block table."""
-    shape, stride = t.shape, t.stride()
-    if t.dtype is not torch.int32 or len(shape) != 2 or (stride[1] != 1 and shape[1] > 1) or t.device != device:
-        raise ValueError(f"{what}: block_table must be int32 [requests, pages of a request] with contiguous rows on {device}")
-    return t.data_ptr(), (stride[0] if shape[0] > 1 else shape[1]), shape[0], shape[1]
 
 
 def rope_frequencies(rotary_dim, base=10000.0, device=None, llama3_scaling=None):
@@ -100,7 +64,9 @@ class PagedCache:
     last dimension contiguous (a [pages, page_size, kv_heads, head_dim] array fits as its transpose(1, 2))."""
 
     def __init__(self, k, v):
-        device = _device_of(k, "PagedCache")
+        device = k.device
+        if device.type != "cuda":
+            raise ValueError(f"PagedCache: needs device tensors, got one on {device}")
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or v.device != device:
             raise ValueError("PagedCache: k and v must be [pages, kv_heads, page_size, head_dim] alike in shape, strides, type and device")
         if k.stride(3) != 1:
@@ -110,7 +76,7 @@ class PagedCache:
         # a dimension of one element may have any stride
         strides = [s if n > 1 else self.head_dim for s, n in zip(k.stride()[:3], k.shape[:3])]
         self._c = _lib.KvCache(k.data_ptr(), v.data_ptr(), self.pages, self.page_size, *strides, self.kv_heads, self.head_dim, _hm_dtype(k.dtype))
-        self._ref = ctypes.byref(self._c)
+        self._ref, self._address = ctypes.byref(self._c), ctypes.addressof(self._c)
 
     @classmethod
     def empty(cls, pages, page_size, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda"):
@@ -148,19 +114,10 @@ def page_plan(plan, lengths, added, block_table, free_pages, queue, lengths_out=
     the ring of free pages free_pages int32 are updated in place; queue int64 [4] holds the ring's head and tail. The lengths
     and counters after the step go to plan.lengths and plan.queue, or to lengths_out and queue_out, which may be lengths and queue.
     plan.queue[2] counts the requests that got nothing because pages, rows or table entries did not suffice."""
-    what = "page_plan"
-    device = _device_of(lengths, what)
-    table, ld, count, width = _table(block_table, device, what)
-    if plan.device != device or plan.starts.size(0) != count + 1:
-        raise ValueError(f"page_plan: the plan must be of the table's {count} requests and on {device}")
-    i32, i64 = torch.int32, torch.int64
-    n = _vector(lengths, i32, count, device, what, "lengths")
-    q = _vector(queue, i64, 4, device, what, "queue")
-    n_out = plan.lengths.data_ptr() if lengths_out is None else n if lengths_out is lengths else _vector(lengths_out, i32, count, device, what, "lengths_out")
-    q_out = plan.queue.data_ptr() if queue_out is None else q if queue_out is queue else _vector(queue_out, i64, 4, device, what, "queue_out")
-    _on_device(device, _lib.load().hm_page_plan, n, _vector(added, i32, count, device, what, "added"), count, table, ld, width, plan.page_size,
-               _vector(free_pages, i32, 1, device, what, "free_pages", True), free_pages.size(0), q, plan.slots.data_ptr(), plan.positions.data_ptr(),
-               plan.requests.data_ptr(), plan.slots.size(0), plan.starts.data_ptr(), n_out, q_out, _stream(stream, device))
+    status = _host.page_plan(plan.slots, plan.positions, plan.requests, plan.starts, plan.lengths, plan.queue, plan.page_size, lengths, added,
+                             block_table, free_pages, queue, lengths_out, queue_out, stream)
+    if status != _lib.HM_OK:
+        _call(status)
     return plan
 
 
@@ -171,35 +128,11 @@ def qk_norm_rope(q_out, qkv, frequencies, positions, cache=None, slots=None, k_o
     fp32 with one rounding. qkv [rows, (q_heads + 2 kv_heads) * head_dim]; queries go to q_out [rows, q_heads (x) head_dim]. With a
     cache, keys and values go to their slots; without one, keys go to k_out and kv_heads and head_dim are given. q_out and
     k_out may be their columns of qkv. Rows with a negative position are left as they are."""
-    device = _device_of(qkv, "qk_norm_rope")
-    dtype = qkv.dtype
-    if cache is not None:
-        if k_out is not None or slots is None:
-            raise ValueError("qk_norm_rope: a cache takes slots and no k_out")
-        kv_heads, head_dim = cache.kv_heads, cache.head_dim
-        if cache.dtype != dtype or cache.device != device:
-            raise ValueError(f"qk_norm_rope: the cache must be {dtype} on {device}")
-    elif k_out is None or slots is not None or not kv_heads or not head_dim:
-        raise ValueError("qk_norm_rope: without a cache, needs k_out, kv_heads and head_dim and no slots")
-    if qkv.dim() != 2 or head_dim <= 0 or qkv.size(1) % head_dim or qkv.size(1) // head_dim <= 2 * kv_heads:
-        raise ValueError(f"qk_norm_rope: qkv must be [rows, (q_heads + 2 x {kv_heads}) x {head_dim}]")
-    rows, heads = qkv.size(0), qkv.size(1) // head_dim
-    q_heads = heads - 2 * kv_heads
-    what = "qk_norm_rope"
-    pairs = frequencies.numel()
-    k, ldk, s = None, 0, None
-    if cache is None:
-        k, ldk = _rows(k_out, rows, kv_heads, head_dim, dtype, device, what, "k_out")
-    else:
-        s = _vector(slots, torch.int64, rows, device, what, "slots", True)
-    a = _lib.QkNormRopeArgs(*_rows(qkv, rows, heads, head_dim, dtype, device, what, "qkv"), *_rows(q_out, rows, q_heads, head_dim, dtype, device, what, "q_out"),
-                            k, ldk, None if bias is None else _vector(bias, dtype, heads * head_dim, device, what, "bias"),
-                            None if q_weight is None else _vector(q_weight, dtype, head_dim, device, what, "q_weight"),
-                            None if k_weight is None else _vector(k_weight, dtype, head_dim, device, what, "k_weight"),
-                            _vector(frequencies, torch.float64, pairs, device, what, "frequencies"),
-                            _vector(positions, torch.int32, rows, device, what, "positions", True), s, rows, q_heads, kv_heads, head_dim, 2 * pairs, eps,
-                            bool(interleaved), _hm_dtype(dtype))
-    _on_device(device, _lib.load().hm_qk_norm_rope, ctypes.byref(a), None if cache is None else cache._ref, _stream(stream, device))
+    address, index = (0, 0) if cache is None else (cache._address, cache.device.index)
+    status = _host.qk_norm_rope(q_out, qkv, frequencies, positions, address, index, slots, k_out, kv_heads or 0, head_dim or 0, q_weight, k_weight, bias, eps,
+                                interleaved, stream)
+    if status != _lib.HM_OK:
+        _call(status)
     return q_out
 
 
@@ -208,21 +141,13 @@ def paged_attention(out, q, cache, block_table, positions, requests=None, scale=
     paged cache (hm_paged_attention). q, out [rows, q_heads, head_dim]; block_table int32 [requests, pages of a request]; row t is of request
     requests[t], or t. Position -1: zeros; a negative request: the row is left as it is; a row outside the table or the
     cache: NaN. scale: 1 / sqrt(head_dim) by default. workspace: cache.attention_workspace(q_heads), one per stream."""
-    what = "paged_attention"
-    device = cache.device
     d = cache.head_dim
-    rows = q.size(0)
-    q_heads = q.size(1) if q.dim() == 3 else q.size(-1) // d
-    qp, ldq = _rows(q, rows, q_heads, d, cache.dtype, device, what, "q")
-    op, ldo = _rows(out, rows, q_heads, d, cache.dtype, device, what, "out")
-    table, ld, count, width = _table(block_table, device, what)
-    pp = _vector(positions, torch.int32, rows, device, what, "positions", True)
-    rp = None if requests is None else _vector(requests, torch.int32, rows, device, what, "requests", True)
     if workspace is None:
-        workspace = cache.attention_workspace(q_heads, stream)
-    wp, wb = _aligned(workspace)
-    _on_device(device, _lib.load().hm_paged_attention, cache._ref, op, ldo, qp, ldq, rows, q_heads, table, ld, count, width, pp, rp,
-               1.0 / math.sqrt(d) if scale is None else scale, window, wp, wb, _stream(stream, device))
+        workspace = cache.attention_workspace(q.size(1) if q.dim() == 3 else q.size(-1) // d, stream)
+    status = _host.paged_attention(out, q, cache._address, cache.device.index, block_table, positions, requests, 1.0 / math.sqrt(d) if scale is None else scale,
+                                   window, workspace, stream)
+    if status != _lib.HM_OK:
+        _call(status)
     return out
 
 

@@ -60,43 +60,54 @@ def _compile(src, verbose):
 SHIM_DIR = os.path.join(HERE, "shim")
 SHIM_SOURCES = ["hm_reference_api.cpp", "py_module.cpp"]
 SHIM_NAME = "_reference_shim"
+HOST_SOURCES = ["hm_attention_host.cpp"]
+HOST_NAME = "_attention_host"
 
 
-def build_shim(verbose=False):
-    """The reference-signature C++ operators (shim/hm_reference_api.cpp) against torch's C++ headers, as a Python
-    module over libhmw4a16.so. Host code only (g++): it calls the C ABI and launches nothing itself."""
+def _build_extension(name, directory, sources, libs, verbose):
+    """A Python module of host code (g++) against torch's C++ headers, next to the package's own."""
     import sysconfig
 
+    import torch
     import torch.utils.cpp_extension as ext
 
     torch_lib = ext.library_paths()[0]
-    out = os.path.join(HERE, SHIM_NAME + sysconfig.get_config_var("EXT_SUFFIX"))
-    import torch
-
+    out = os.path.join(HERE, name + sysconfig.get_config_var("EXT_SUFFIX"))
     flags = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-             f"-DTORCH_EXTENSION_NAME={SHIM_NAME}", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", f"-I{sysconfig.get_paths()['include']}",
+             f"-DTORCH_EXTENSION_NAME={name}", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", f"-I{sysconfig.get_paths()['include']}",
              *[f"-I{p}" for p in ext.include_paths()], f"-I{os.path.join(ROOT, 'include')}"]
     os.makedirs(BUILD_DIR, exist_ok=True)
 
     def compile_one(src):
         obj = os.path.join(BUILD_DIR, os.path.splitext(src)[0] + ".o")
-        cmd = ["g++", *flags, "-c", os.path.join(SHIM_DIR, src), "-o", obj]
+        cmd = ["g++", *flags, "-c", os.path.join(directory, src), "-o", obj]
         if verbose:
             print(" ".join(cmd), flush=True)
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
-            raise RuntimeError(f"shim build failed on {src}:\n{res.stdout}\n{res.stderr}")
+            raise RuntimeError(f"build of {name} failed on {src}:\n{res.stdout}\n{res.stderr}")
         return obj
 
-    with ThreadPoolExecutor(max_workers=len(SHIM_SOURCES)) as pool:
-        objs = list(pool.map(compile_one, SHIM_SOURCES))
-    cmd = ["g++", "-shared", *objs, f"-L{torch_lib}", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", f"-L{HERE}", "-lhmw4a16",
+    with ThreadPoolExecutor(max_workers=len(sources)) as pool:
+        objs = list(pool.map(compile_one, sources))
+    cmd = ["g++", "-shared", *objs, f"-L{torch_lib}", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", f"-L{HERE}", *libs,
            "-L/opt/rocm/lib", "-lamdhip64", f"-Wl,-rpath,{torch_lib}", "-Wl,-rpath,$ORIGIN", "-o", out + ".tmp"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"shim link failed:\n{res.stdout}\n{res.stderr}")
+        raise RuntimeError(f"link of {name} failed:\n{res.stdout}\n{res.stderr}")
     os.replace(out + ".tmp", out)
     return out
+
+
+def build_shim(verbose=False):
+    """The reference-signature C++ operators (shim/hm_reference_api.cpp) against torch's C++ headers, as a Python
+    module over libhmw4a16.so. Host code only (g++): it calls the C ABI and launches nothing itself."""
+    return _build_extension(SHIM_NAME, SHIM_DIR, SHIM_SOURCES, ["-lhmw4a16"], verbose)
+
+
+def build_host(verbose=False):
+    """The compiled host side of the attention operators' Python calls (csrc/hm_attention_host.cpp)."""
+    return _build_extension(HOST_NAME, CSRC, HOST_SOURCES, [], verbose)
 
 
 def build(verbose=False):
@@ -115,6 +126,10 @@ def build(verbose=False):
 
 
 if __name__ == "__main__":
-    print(build(verbose="--verbose" in sys.argv))
+    verbose = "--verbose" in sys.argv
+    with ThreadPoolExecutor(max_workers=2) as pool:  # the module builds beside the library: it does not link with it
+        host = pool.submit(build_host, verbose)
+        print(build(verbose))
+        print(host.result())
     if "--no-shim" not in sys.argv:
-        print(build_shim(verbose="--verbose" in sys.argv))
+        print(build_shim(verbose))
