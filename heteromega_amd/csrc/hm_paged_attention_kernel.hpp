@@ -81,6 +81,12 @@ __device__ __forceinline__ Row uniform_row(const Row &r) {
                uniform(r.start),   uniform(r.tiles), uniform(r.count), uniform(r.bad) != 0};
 }
 
+// The row that a lane holds, in scalar registers.
+__device__ __forceinline__ Row row_of_lane(const Row &r, int lane) {
+    const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, lane); };
+    return Row{of(r.request), of(r.first), of(r.end), of(r.all_first), of(r.all_end), of(r.start), of(r.tiles), of(r.count), of(r.bad) != 0};
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 template <class T> __device__ __forceinline__ void store4(uint16_t *p, float4_t v) {
@@ -169,7 +175,23 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
     Runs runs{};
     int t = 0, base = 0; // the row that x lies in, and the row's first tile
     Row r{};
-    {
+    if (rows <= 64) { // a lane per row: each wave finds its place by itself
+        const Row mine = lane < rows ? row_of<GROUPED>(a, lane, kTileKeys, plan.rows) : Row{};
+        int upto = mine.tiles;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int v = __shfl_up(upto, off);
+            upto += lane >= off ? v : 0;
+        }
+        runs = Runs::deal(__builtin_amdgcn_readlane(upto, 63) * units, plan.runs);
+        x = runs.begin(w);
+        x_end = w < plan.runs ? runs.begin(w + 1) : x;
+        if (x < x_end) {
+            t = __builtin_ctzll(__ballot(x < upto * units));
+            r = row_of_lane(mine, t);
+            base = (__builtin_amdgcn_readlane(upto, t) - r.tiles) * units;
+        }
+    } else {
         const int per = (rows + kThreads - 1) / kThreads;
         const int t0 = min(static_cast<int>(threadIdx.x) * per, rows), t1 = min(t0 + per, rows);
         int own = 0;
@@ -213,13 +235,13 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
             }
         }
         __syncthreads();
+        if (x < x_end) {
+            t = uniform(found[TEAM == 1 ? wave : 0][0]);
+            base = uniform(found[TEAM == 1 ? wave : 0][1]);
+            r = uniform_row(row_of<GROUPED>(a, t, kTileKeys, plan.rows));
+        }
     }
     AttentionDescriptor begun{0, 0, 0, 0};
-    if (x < x_end) {
-        t = uniform(found[TEAM == 1 ? wave : 0][0]);
-        base = uniform(found[TEAM == 1 ? wave : 0][1]);
-        r = uniform_row(row_of<GROUPED>(a, t, kTileKeys, plan.rows));
-    }
 
     // ---- constants of the lane ----
     const uint32_t row_bytes = static_cast<uint32_t>(a.token_stride) * 2;
