@@ -167,12 +167,14 @@ class AttnLayer:
         self.frequencies, self.bias, self.q_weight, self.k_weight, self.qk_eps = frequencies, bias, q_weight, k_weight, qk_eps
         self.scale, self.window, self.interleaved = scale, window, interleaved
         self._buffers = {}
+        self._outgrown = []  # a captured step may still use them
 
     def _scratch(self, rows, cache, stream):
         """(normed or projected rows, Q/K/V rows, attention rows, workspaces) of calls on this stream, grown as needed."""
         key = _stream(stream, self.device)
         kept = self._buffers.get(key)
         if kept is None or kept[0].size(0) < rows:
+            self._outgrown.append(kept)
             with _on(stream, self.device):
                 new = lambda n: torch.empty((rows, n), dtype=self.dtype, device=self.device)
                 linear = max(w.workspace_bytes(m) for w in (self.wqkv, self.wo) for m in (rows, min(rows, 16)))

@@ -8,7 +8,7 @@
 //                          registers.
 //   O^T [d, q] += V^T P^T  A = V^T, read from LDS transposed (ds_read_b64_tr_b16); B = P^T.
 // Rows of K and V are loaded whole by neighbouring lanes and pass through LDS, K as well as V: loads in A's own order touch 64
-// bytes of 16 rows each, and took 394 us instead of 362 (64 rows of 8192 keys, 8 key heads of 128).
+// bytes of 16 rows each, and took 381 us instead of 362 (64 rows of 8192 keys, 8 key heads of 128).
 // In S^T a lane holds, for one column q = L & 15, keys 4 (L >> 4) + i of each sub-tile. The k index of the second product may
 // be dealt in any order that A and B share, so those eight weights are its B operand as they are: no weight crosses
 // lanes. O^T keeps one q per lane too, so rescaling by a new maximum is one factor per lane.
