@@ -73,6 +73,8 @@ hipError_t launch_paged_attention(const PagedAttentionArgs &a, hipStream_t strea
     const int64_t most = most_tiles(32 * p.team);
     p.runs = static_cast<int>(std::min(groups * kAttentionWaves / p.team, most));
     p.few_units = 16 * all_units < p.runs;
+    // Units may have many parts each where there are fewer of them than runs: then a wave per column.
+    p.join_cols = std::min(p.cols, 2 * all_units < p.runs ? kMaxCols : 4);
     return a.dtype == HM_FP16 ? launch_paged_attention_f16(a, p, stream) : launch_paged_attention_bf16(a, p, stream);
 }
 

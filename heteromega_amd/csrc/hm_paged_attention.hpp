@@ -22,6 +22,7 @@ struct AttentionPlan {
     int shares;      // units of one key head
     int group_heads; // query heads of one key head
     bool few_units;  // join with a workgroup per unit and column
+    int join_cols;   // else: workgroups that share the columns of a unit's join
 
     __host__ __device__ int kv_head(int unit) const { return shares == 1 ? unit : unit / shares; }
     // Columns of a unit that has `count` rows. GROUPED: rows > 1.

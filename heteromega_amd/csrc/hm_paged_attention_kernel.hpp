@@ -9,6 +9,7 @@ namespace {
 
 constexpr int kThreads = 64 * kAttentionWaves;
 constexpr int kWaveKeys = 32;
+constexpr int kLaneRows = 4;
 constexpr int kStream = 2; // cache policy of the keys and values, read once: non-temporal
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
@@ -175,9 +176,17 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
     Runs runs{};
     int t = 0, base = 0; // the row that x lies in, and the row's first tile
     Row r{};
-    if (rows <= 64) { // a lane per row: each wave finds its place by itself
-        const Row mine = lane < rows ? row_of<GROUPED>(a, lane, kTileKeys, plan.rows) : Row{};
-        int upto = mine.tiles;
+    if (rows <= 64 * kLaneRows) { // each wave finds its place by itself, kLaneRows rows a lane or one
+        const int per = rows <= 64 ? 1 : kLaneRows;
+        Row mine[kLaneRows];
+        int own = 0;
+#pragma unroll
+        for (int i = 0; i < kLaneRows; ++i) {
+            const bool some = i < per && lane * per + i < rows;
+            mine[i] = some ? row_of<GROUPED>(a, lane * per + i, kTileKeys, plan.rows) : Row{};
+            own += mine[i].tiles;
+        }
+        int upto = own;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
             const int v = __shfl_up(upto, off);
@@ -187,9 +196,20 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
         x = runs.begin(w);
         x_end = w < plan.runs ? runs.begin(w + 1) : x;
         if (x < x_end) {
-            t = __builtin_ctzll(__ballot(x < upto * units));
-            r = row_of_lane(mine, t);
-            base = (__builtin_amdgcn_readlane(upto, t) - r.tiles) * units;
+            const int from = __builtin_ctzll(__ballot(x < upto * units));
+            base = (__builtin_amdgcn_readlane(upto, from) - __builtin_amdgcn_readlane(own, from)) * units;
+            t = from * per;
+#pragma unroll
+            for (int i = 0; i < kLaneRows; ++i) {
+                if (i < per) {
+                    r = row_of_lane(mine[i], from);
+                    if (x < base + r.tiles * units) {
+                        break;
+                    }
+                    base += r.tiles * units;
+                    ++t;
+                }
+            }
         }
     } else {
         const int per = (rows + kThreads - 1) / kThreads;
@@ -597,7 +617,7 @@ template <class T, int D, int THREADS>
 __device__ __forceinline__ void join_column(uint16_t *out, bool empty, const AttentionWorkspace &ws, int cols, int w, int pieces, int j) {
     constexpr int kItems = D / 4;
     constexpr int kLanes = THREADS / kItems;
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 8;
     __shared__ float4_t acc[kLanes][kItems];
     __shared__ float2 stat[kLanes];
     const int y = threadIdx.x / kItems, e = threadIdx.x - y * kItems;
@@ -732,7 +752,7 @@ template <class T, int D, int TEAM, int CT, bool GROUPED> hipError_t launch(cons
         hipLaunchKernelGGL((join_few_kernel<T, D, GROUPED>), dim3(static_cast<unsigned>(a.rows * plan.units), static_cast<unsigned>(plan.cols)),
                            dim3(kFewThreads), 0, stream, a, plan);
     } else {
-        hipLaunchKernelGGL((join_kernel<T, D, GROUPED>), dim3(static_cast<unsigned>(plan.runs), static_cast<unsigned>(plan.cols < 4 ? plan.cols : 4)), dim3(64), 0,
+        hipLaunchKernelGGL((join_kernel<T, D, GROUPED>), dim3(static_cast<unsigned>(plan.runs), static_cast<unsigned>(plan.join_cols)), dim3(64), 0,
                            stream, a, plan);
     }
     return hipGetLastError();

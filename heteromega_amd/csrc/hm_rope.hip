@@ -2,8 +2,8 @@
 // values to their cache slots, in one pass over the rows.
 //
 // A head of D elements is handled by D / 16 lanes (of a group of the next power of two), 16 elements each in two 16-byte
-// pieces. For the split-half pairing a lane takes pieces c of both halves, so that both elements of a pair are its own and
-// only the norm's sum crosses lanes. The angles depend on the row alone: a workgroup forms cos and sin of its rows once
+// pieces. A lane takes pieces c of both halves, so that with either pairing both elements
+// of a pair are its own and only the norm's sum crosses lanes. The angles depend on the row alone: a workgroup forms cos and sin of its rows once
 // (position times frequency in turns in fp64, the fraction of a turn in fp32, so that far positions lose nothing) and all
 // heads read them from LDS.
 //
@@ -73,8 +73,10 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(QkNormRopeArgs a
     const int items = rows * heads;
     const bool lane_used = c < D / 16;
     const bool rotated = 16 * c < rd;
-    const int off_a = INTERLEAVED || !rotated ? 16 * c : 8 * c;
-    const int off_b = INTERLEAVED || !rotated ? 16 * c + 8 : half + 8 * c;
+    // A lane's two pieces lie half of its part of the head apart (the rotated part or the rest): neighbouring lanes load neighbouring pieces.
+    const int part = rotated ? 0 : rd, part_c = rotated ? c : c - rd / 16;
+    const int off_a = part + 8 * part_c;
+    const int off_b = off_a + (rotated ? half : (D - rd) / 2);
 
     int item = threadIdx.x >> group_log;
     uint4 next_a = {}, next_b = {};
@@ -184,10 +186,11 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(QkNormRopeArgs a
             continue;
         }
         if (rotated && (is_q || is_k)) {
-            const float2 *t = turn + r * half + 8 * c;
+            // The pairs of pieces a and b: pair 8 c + k across them, or, interleaved, pairs 4 c + k of a and half / 2 + 4 c + k of b.
+            const float2 *t = turn + r * half + (INTERLEAVED ? 4 : 8) * c;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float2 cs = t[k];
+                const float2 cs = INTERLEAVED ? (k < 4 ? t[k] : t[half / 2 + k - 4]) : t[k];
                 float &p = INTERLEAVED ? (k < 4 ? x[2 * k] : y[2 * k - 8]) : x[k];
                 float &q = INTERLEAVED ? (k < 4 ? x[2 * k + 1] : y[2 * k - 7]) : y[k];
                 const float p0 = p, q0 = q;
