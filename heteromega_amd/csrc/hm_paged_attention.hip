@@ -25,8 +25,9 @@
 // 1349 -> 408 us (84 TFLOP/s). They are masked one by one.
 // A run is shared by the four waves of a workgroup, 32 keys of a 128-key tile each, which join over LDS, or is one wave's own. The first
 // keeps the parts few; the second wastes nothing on rows shorter than a tile and lets waves go on to their next unit by
-// themselves, and is taken where there is a unit for each wave that fits the card (32 query and 8 key heads of 128: 1024 rows of up to 60
-// keys 75 -> 46 us, 256 rows of up to 500 keys 61 -> 56 us).
+// themselves. It is taken where there are units for three of four waves that fit the card (32 query and 8 key heads of 128: 1024 rows of up to 60
+// keys 75 -> 46 us, 256 rows of up to 500 keys 61 -> 56 us; 1824 units of up to 218 keys of 64 24 -> 21 us; 1024 units of 2040 keys would
+// take 67 us instead of 65).
 // Of 6.3 TB/s that plain reads of 2 GB reach, 64 rows of 8192 keys take 331 us (6.3 TB/s), one row of 130987 keys 92 us (5.8 TB/s); one row of
 // 1037 keys takes 10.6 us, of which the join's launch is 4.
 #include "hm_paged_attention.hpp"
@@ -69,7 +70,7 @@ hipError_t launch_paged_attention(const PagedAttentionArgs &a, hipStream_t strea
     const int64_t capacity = a.width << a.page_shift;
     const auto most_tiles = [&](int64_t keys) { return a.rows * p.units * ((capacity + keys - 1) / keys + 1); };
     // All tiles are counted in 32 bits.
-    p.team = p.cols <= 16 && all_units >= groups * kAttentionWaves && most_tiles(32) <= INT32_MAX ? 1 : kAttentionWaves;
+    p.team = p.cols <= 16 && all_units >= 3 * groups && most_tiles(32) <= INT32_MAX ? 1 : kAttentionWaves;
     const int64_t most = most_tiles(32 * p.team);
     p.runs = static_cast<int>(std::min(groups * kAttentionWaves / p.team, most));
     p.few_units = 16 * all_units < p.runs;
