@@ -73,6 +73,7 @@ hipError_t launch_paged_attention(const PagedAttentionArgs &a, hipStream_t strea
     p.team = p.cols <= 16 && all_units >= 3 * groups && most_tiles(32) <= INT32_MAX ? 1 : kAttentionWaves;
     const int64_t most = most_tiles(32 * p.team);
     p.runs = static_cast<int>(std::min(groups * kAttentionWaves / p.team, most));
+    p.joins = capacity > 32 * p.team;
     p.few_units = 16 * all_units < p.runs;
     // Units may have many parts each where there are fewer of them than runs: then a wave per column.
     p.join_cols = std::min(p.cols, 2 * all_units < p.runs ? kMaxCols : 4);

@@ -21,6 +21,7 @@ struct AttentionPlan {
     int units;       // of a row, or of a unit's rows: key heads times shares of their query heads
     int shares;      // units of one key head
     int group_heads; // query heads of one key head
+    bool joins;      // units may have more than one tile, and so parts
     bool few_units;  // join with a workgroup per unit and column
     int join_cols;   // else: workgroups that share the columns of a unit's join
 

@@ -745,7 +745,7 @@ template <class T, int D, int TEAM, int CT, bool GROUPED> hipError_t launch(cons
     const unsigned blocks = static_cast<unsigned>((plan.runs * TEAM + kAttentionWaves - 1) / kAttentionWaves);
     hipLaunchKernelGGL((paged_attention_kernel<T, D, TEAM, CT, GROUPED>), dim3(blocks), dim3(kThreads), 0, stream, a, plan);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) {
+    if (e != hipSuccess || !plan.joins) {
         return e;
     }
     if (plan.few_units) {

@@ -18,8 +18,7 @@ namespace hm {
 namespace {
 
 constexpr int kMaxRequests = HM_PAGE_PLAN_MAX_REQUESTS;
-constexpr int kPerThread = 4; // requests, and consecutive rows, of a thread
-constexpr int kSmall = 256, kLarge = kMaxRequests / kPerThread;
+constexpr int kSmall = 1024; // requests that 256 threads take; more take 512 (2048 requests 7.8 us, with 256 threads 9.9, with 1024 8.5)
 constexpr int64_t kOneBlockRows = 1024;
 
 __device__ __forceinline__ int64_t pages_of(int64_t tokens, int shift) { return (tokens + (int64_t(1) << shift) - 1) >> shift; }
@@ -87,10 +86,10 @@ __device__ __forceinline__ int last_from(const int32_t *first, int count, int32_
     return lo;
 }
 
-// Workgroups before `row_blocks` write rows, starts, the table and the freed pages; the one behind them, or with `all` the only
+// PER: requests of a thread at most. Workgroups before `row_blocks` write rows, starts, the table and the freed pages; the one behind them, or with `all` the only
 // one too, lengths and queue after the step.
-template <int THREADS> __global__ void __launch_bounds__(THREADS) page_plan_kernel(PagePlanArgs a, int row_blocks, bool all) {
-    constexpr int kRequests = THREADS * kPerThread;
+template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) page_plan_kernel(PagePlanArgs a, int row_blocks, bool all) {
+    constexpr int kRequests = THREADS * PER;
     __shared__ int32_t first_row[kRequests];  // of each request
     __shared__ int32_t length[kRequests];     // its length, or -1 if it gets nothing
     __shared__ int32_t first_page[kRequests]; // place of its first page in the ring, behind the head
@@ -102,9 +101,9 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) page_plan_kern
     const int64_t capacity = a.width << shift;
     const uint64_t head = static_cast<uint64_t>(a.queue_in[0]), tail = static_cast<uint64_t>(a.queue_in[1]);
     const int per = (R + THREADS - 1) / THREADS, r0 = static_cast<int>(threadIdx.x) * per;
-    int32_t n[kPerThread], add[kPerThread];
+    int32_t n[PER], add[PER];
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
+    for (int i = 0; i < PER; ++i) {
         const bool mine = i < per && r0 + i < R;
         n[i] = mine ? a.lengths[r0 + i] : 0;
         add[i] = mine ? a.added[r0 + i] : 0;
@@ -116,7 +115,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) page_plan_kern
     const int32_t left = static_cast<int32_t>(max(int64_t(0), min(static_cast<int64_t>(tail - head), a.ring_size)));
 
     // The pages that a request needs count only if its rows fit: first as if all do, again if their sum shows that some do not.
-    int32_t need[kPerThread], back[kPerThread];
+    int32_t need[PER], back[PER];
     Sums before, total;
     bool again = false;
     int64_t row_before = 0;
@@ -124,7 +123,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) page_plan_kern
         Sums own{0, 0, 0};
         int64_t row = row_before;
 #pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
+        for (int i = 0; i < PER; ++i) {
             const int64_t known = min(max(int64_t(n[i]), int64_t(0)), capacity);
             const int64_t held = pages_of(known, shift);
             const int32_t more = max(add[i], 0);
@@ -142,7 +141,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) page_plan_kern
     int32_t page = before.need;
     int32_t my_taken = 0, my_refused = 0;
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
+    for (int i = 0; i < PER; ++i) {
         if (i >= per || r0 + i >= R) {
             break;
         }
@@ -217,7 +216,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) page_plan_kern
         int32_t *first_back = first_page;
         int32_t to = before.back;
 #pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
+        for (int i = 0; i < PER; ++i) {
             if (i < per && r0 + i < R) {
                 first_back[r0 + i] = to;
             }
@@ -239,26 +238,26 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) page_plan_kern
     }
 }
 
-template <int THREADS> hipError_t launch(const PagePlanArgs &a, hipStream_t stream) {
+template <int THREADS, int PER> hipError_t launch(const PagePlanArgs &a, hipStream_t stream) {
     if (a.rows <= kOneBlockRows) {
-        hipLaunchKernelGGL((page_plan_kernel<THREADS>), dim3(1), dim3(THREADS), 0, stream, a, 1, true);
+        hipLaunchKernelGGL((page_plan_kernel<THREADS, PER>), dim3(1), dim3(THREADS), 0, stream, a, 1, true);
         return hipGetLastError();
     }
     const int blocks = static_cast<int>(std::min<int64_t>((a.rows + THREADS - 1) / THREADS, device_topology().cus));
     const bool in_place = a.lengths_out == a.lengths || a.queue_out == a.queue_in;
-    hipLaunchKernelGGL((page_plan_kernel<THREADS>), dim3(blocks + (in_place ? 0 : 1)), dim3(THREADS), 0, stream, a, blocks, false);
+    hipLaunchKernelGGL((page_plan_kernel<THREADS, PER>), dim3(blocks + (in_place ? 0 : 1)), dim3(THREADS), 0, stream, a, blocks, false);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !in_place) {
         return e;
     }
-    hipLaunchKernelGGL((page_plan_kernel<THREADS>), dim3(1), dim3(THREADS), 0, stream, a, 0, false);
+    hipLaunchKernelGGL((page_plan_kernel<THREADS, PER>), dim3(1), dim3(THREADS), 0, stream, a, 0, false);
     return hipGetLastError();
 }
 
 } // namespace
 
 hipError_t launch_page_plan(const PagePlanArgs &a, hipStream_t stream) {
-    return a.requests_count <= kSmall * kPerThread ? launch<kSmall>(a, stream) : launch<kLarge>(a, stream);
+    return a.requests_count <= kSmall ? launch<256, kSmall / 256>(a, stream) : launch<512, kMaxRequests / 512>(a, stream);
 }
 
 } // namespace hm
