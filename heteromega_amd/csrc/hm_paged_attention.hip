@@ -28,8 +28,8 @@
 // themselves. It is taken where there are units for three of four waves that fit the card (32 query and 8 key heads of 128: 1024 rows of up to 60
 // keys 75 -> 46 us, 256 rows of up to 500 keys 61 -> 56 us; 1824 units of up to 218 keys of 64 24 -> 21 us; 1024 units of 2040 keys would
 // take 67 us instead of 65).
-// Of 6.3 TB/s that plain reads of 2 GB reach, 64 rows of 8192 keys take 331 us (6.3 TB/s), one row of 130987 keys 92 us (5.8 TB/s); one row of
-// 1037 keys takes 10.6 us, of which the join's launch is 4.
+// Plain reads of 2 GB reach 6.3 TB/s: 64 rows of 8192 keys take 325 us (6.4 TB/s), one row of 130987 keys 91 us (5.9 TB/s with the join); one row
+// of 1037 keys takes 10.1 us, of which the join's launch is 3.
 #include "hm_paged_attention.hpp"
 
 #include <algorithm>

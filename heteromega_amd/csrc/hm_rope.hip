@@ -8,7 +8,7 @@
 // heads read them from LDS.
 //
 // Bound by memory: each element is read and written once (4 bytes of traffic, about 10 fp32 operations). 8192 rows of 32 + 2 * 8 heads of
-// 128, normed: 201 MB in 41 us (4.9 TB/s; a copy of 4 GB runs at 4.75). One row: 3.1 us, a launch.
+// 128, normed: 201 MB in 39.4 us (5.1 TB/s; a copy of 4 GB runs at 4.75). One row: 3.1 us, a launch.
 #include "hm_device.hpp"
 #include "hm_internal.hpp"
 
@@ -18,7 +18,7 @@ namespace hm {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxRows = 2; // rows of one workgroup (8192 rows: 44 us, with 1 row 45, with 4 and 8 rows 48)
+constexpr int kMaxRows = 2; // rows of one workgroup (8192 rows, with plain loads and stores: 44 us, with 1 row 45, with 4 and 8 rows 48)
 
 template <class T> __device__ __forceinline__ void unpack8(const uint4 v, float o[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
