@@ -65,6 +65,8 @@ class PagedCache:
 
     def __init__(self, k, v):
         device = k.device
+        if k.numel() == 0:
+            raise ValueError(f"PagedCache: k and v must not be empty, got {list(k.shape)}")
         if device.type != "cuda":
             raise ValueError(f"PagedCache: needs device tensors, got one on {device}")
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or v.device != device:

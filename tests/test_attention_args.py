@@ -126,6 +126,14 @@ def test_host_tensors_are_refused(hm):
         hm.qk_norm_rope(q[:, :512], q, hm.rope_frequencies(64), i, k_out=q[:, 512:640], kv_heads=2, head_dim=64)
 
 
+@pytest.mark.parametrize("shape", [(0, 2, 16, 64), (4, 0, 16, 64), (4, 2, 0, 64), (4, 2, 16, 0)])
+def test_empty_caches_are_refused(hm, shape):
+    # before the device is looked at: heads of no elements would be divided by
+    k = torch.zeros(shape, dtype=torch.float16)
+    with pytest.raises(ValueError, match="must not be empty"):
+        hm.PagedCache(k, k.clone())
+
+
 def test_rope_frequencies(hm):
     f = hm.rope_frequencies(128, 500000.0).numpy()
     np.testing.assert_allclose(f, 500000.0 ** (-np.arange(64) / 64), rtol=1e-15)
