@@ -120,6 +120,9 @@ hm_status hm_qk_norm_rope(const hm_qk_norm_rope_args *args, const hm_kv_cache *c
         return set_error(HM_INVALID_ARGUMENT, "%s: rows must fit 31 bits, heads lie in 1..65536, got %lld, %d, %d", what, static_cast<long long>(p.rows),
                          static_cast<int>(p.q_heads), static_cast<int>(p.kv_heads));
     }
+    if (p.rows > int64_t(1) << 24) { // a launch has less than 2^32 threads, 128 a row
+        return set_error(HM_UNSUPPORTED, "%s: at most 2^24 rows, got %lld", what, static_cast<long long>(p.rows));
+    }
     if (p.head_dim <= 0 || p.head_dim % 16 || p.head_dim > 512 || p.rotary_dim < 0 || p.rotary_dim % 16 || p.rotary_dim > p.head_dim) {
         return set_error(HM_INVALID_ARGUMENT, "%s: head_dim must be a multiple of 16 up to 512 and rotary_dim one within it, got %d, %d", what,
                          static_cast<int>(p.head_dim), static_cast<int>(p.rotary_dim));

@@ -395,8 +395,9 @@ hm_status hm_page_plan(const int32_t *lengths, const int32_t *added, int64_t R, 
  * values go to their slots (slots [rows], as hm_page_plan gives them; a slot outside the cache is not written; two rows
  * must not have the same slot); without one (NULL), keys go to k [rows, kv_heads * head_dim] (ldk) and values are left
  * where they are. Each of q and k may be its columns of qkv itself (then with ldqkv); otherwise they must not overlap
- * it. A row with a negative position is skipped whole. head_dim: a multiple of 16 up to 512, of 16 for rotary_dim (at
- * most head_dim; 0: no rotation). All row arrays 16-byte aligned with leading dimensions that are multiples of 8. */
+ * it. A row with a negative position is skipped whole. Up to 2^24 rows. head_dim: a multiple of 16 up to 512, of 16 for
+ * rotary_dim (at most head_dim; 0: no rotation). All row arrays 16-byte aligned with leading dimensions that are multiples
+ * of 8. */
 typedef struct hm_qk_norm_rope_args {
     const void *qkv;
     int64_t ldqkv;

@@ -88,6 +88,12 @@ def test_rope_calls_that_are_refused(hm, over):
     assert "hm_qk_norm_rope" in hm._lib.last_error()
 
 
+@pytest.mark.parametrize("rows", [2 ** 24 + 1, 2 ** 31 - 1])
+def test_rope_rows_beyond_a_launch(hm, rows):
+    assert hm._lib.load().hm_qk_norm_rope(ctypes.byref(_rope_args(hm, rows=rows)), ctypes.byref(_cache(hm)), None) == hm._lib.HM_UNSUPPORTED
+    assert "2^24 rows" in hm._lib.last_error()
+
+
 def test_rope_without_a_cache(hm):
     lib = hm._lib.load()
     assert lib.hm_qk_norm_rope(None, None, None) == hm._lib.HM_INVALID_ARGUMENT
