@@ -208,7 +208,8 @@ int qk_norm_rope(const at::Tensor &q_out, const at::Tensor &qkv, const at::Tenso
 }
 
 int paged_attention(const at::Tensor &out, const at::Tensor &q, uintptr_t cache, int device, const at::Tensor &block_table, const at::Tensor &positions,
-                    const std::optional<at::Tensor> &requests, double scale, int64_t window, const at::Tensor &workspace, py::handle stream) {
+                    const std::optional<at::Tensor> &requests, double scale, int64_t window, const std::optional<at::Tensor> &workspace,
+                    py::handle stream) {
     const char *what = "paged_attention";
     const auto *c = reinterpret_cast<const hm_kv_cache *>(cache);
     const int64_t d = c->head_dim;
@@ -220,15 +221,20 @@ int paged_attention(const at::Tensor &out, const at::Tensor &q, uintptr_t cache,
     const Table table = table_of(block_table, device, what);
     const auto *pos = static_cast<const int32_t *>(vector(positions, at::kInt, rows, device, what, "positions", true));
     const auto *req = static_cast<const int32_t *>(vector(requests, at::kInt, rows, device, what, "requests", true));
-    if (!workspace.is_cuda() || workspace.get_device() != device || !workspace.is_contiguous()) {
-        refuse("paged_attention: the workspace must be a contiguous tensor on cuda:", device, ", got ", described(workspace));
+    uintptr_t aligned = 0; // without a workspace the call itself refuses
+    size_t bytes = 0;
+    if (workspace.has_value()) {
+        if (!workspace->is_cuda() || workspace->get_device() != device || !workspace->is_contiguous()) {
+            refuse("paged_attention: the workspace must be a contiguous tensor on cuda:", device, ", got ", described(*workspace));
+        }
+        const uintptr_t base = reinterpret_cast<uintptr_t>(workspace->data_ptr());
+        aligned = (base + 255) / 256 * 256;
+        bytes = workspace->nbytes() > aligned - base ? workspace->nbytes() - (aligned - base) : 0;
     }
-    const uintptr_t base = reinterpret_cast<uintptr_t>(workspace.data_ptr()), aligned = (base + 255) / 256 * 256;
-    const size_t bytes = workspace.nbytes(), skipped = aligned - base;
     void *s = stream_of(stream, device);
     const OnDevice on(device);
     return c_paged_attention(c, to.p, to.ld, in.p, in.ld, rows, q_heads, table.p, table.ld, table.requests, table.width, pos, req, static_cast<float>(scale), window,
-                             reinterpret_cast<void *>(aligned), bytes > skipped ? bytes - skipped : 0, s);
+                             reinterpret_cast<void *>(aligned), bytes, s);
 }
 
 } // namespace

@@ -201,3 +201,28 @@ def test_refusals(oracle, hm, device):
         args.update(kw)
         with pytest.raises(ValueError):
             hm.paged_attention(**args)
+
+
+def test_a_wrong_number_of_heads_without_a_workspace(hm, device):
+    k = torch.zeros((2, 4, 16, 64), dtype=torch.float16, device=device)
+    cache, n = hm.PagedCache(k, k.clone()), torch.zeros(2, dtype=torch.int32, device=device)
+    for heads in (0, 3, 6):
+        q = torch.zeros((2, heads, 64), dtype=torch.float16, device=device)
+        with pytest.raises(ValueError, match="multiple of the 4 key heads"):
+            hm.paged_attention(q.clone(), q, cache, n[:, None], n)
+
+
+@pytest.mark.parametrize("shape", [(2048, 32, 8, 64), (4096, 32, 8, 128), (512, 8, 2, 64)])
+def test_a_step_of_fewer_rows_has_its_workspace(oracle, hm, device, shape):
+    hidden, q_heads, kv_heads, d = shape
+    rng = np.random.default_rng(27)
+    new = lambda k, n: hm.RepackedMatrix.from_logical(*logical_to_device(oracle.random_weights(rng, k, n, 128, "fp16", 0.002, 0.006), "fp16", device), 128,
+                                                      dtype=torch.float16)
+    wqkv, wo = new(hidden, (q_heads + 2 * kv_heads) * d), new(q_heads * d, hidden)
+    cache = hm.PagedCache.empty(2, 16, kv_heads, d, torch.float16, device)
+    for most in (1, 2, 5, 8, 16, 17, 100):
+        layer = hm.AttnLayer(wqkv, wo, q_heads, kv_heads, d, hm.rope_frequencies(d, device=device))
+        linear_ws = layer._scratch(most, cache, None)[3]
+        for rows in range(1, most + 1):
+            need = max(wqkv.workspace_bytes(rows), wo.workspace_bytes(rows))
+            assert need == 0 or linear_ws.numel() >= need + 256, (most, rows)
