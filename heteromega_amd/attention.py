@@ -176,7 +176,8 @@ class AttnLayer:
         key = _stream(stream, self.device)
         kept = self._buffers.get(key)
         if kept is None or kept[0].size(0) < rows:
-            self._outgrown.append(kept)
+            if kept is not None:
+                self._outgrown.append(kept)
             with _on(stream, self.device):
                 new = lambda n: torch.empty((rows, n), dtype=self.dtype, device=self.device)
                 linear = max(w.workspace_bytes(m) for w in (self.wqkv, self.wo) for m in (rows, min(rows, 16)))
@@ -186,10 +187,15 @@ class AttnLayer:
 
     def block_forward(self, x, norm_weight, cache, plan, block_table, eps=1e-5, stream=None):
         """In place: x [rows, hidden] += attention(RMSNorm(x) * norm_weight) Wo. The rows are those of `plan` (page_plan of this step): their keys and values
-        are written to `cache` first, and each row sees its request's tokens up to its own. Rows that the plan left empty stay as they are."""
+        are written to `cache` first, and each row sees its request's tokens up to its own. Rows that the plan left empty stay as they are. The buffers in between are
+        the stream's: steps captured on one stream must not be replayed at the same time."""
         rows = plan.slots.size(0)
-        if x.dim() != 2 or x.size(0) != rows or x.size(1) != self.hidden or x.stride(1) != 1 or x.dtype != self.dtype or x.device != plan.device:
-            raise ValueError(f"AttnLayer.block_forward: x must be {self.dtype} [{rows}, {self.hidden}] on {plan.device}")
+        if x.dim() != 2 or x.size(0) != rows or x.size(1) != self.hidden or x.stride(1) != 1 or x.dtype != self.dtype:
+            raise ValueError(f"AttnLayer.block_forward: x must be {self.dtype} [{rows}, {self.hidden}]")
+        for t in (x, norm_weight, plan, cache, block_table):
+            if t.device != self.device:
+                raise ValueError(f"AttnLayer.block_forward: needs everything on {self.device}, got x, norm_weight, plan, cache and block_table on "
+                                 f"{x.device}, {norm_weight.device}, {plan.device}, {cache.device}, {block_table.device}")
         if norm_weight.numel() != self.hidden or norm_weight.dtype != x.dtype or not norm_weight.is_contiguous():
             raise ValueError(f"norm_weight must be a contiguous {x.dtype} vector of {self.hidden} elements")
         if (cache.kv_heads, cache.head_dim, cache.page_size) != (self.kv_heads, self.head_dim, plan.page_size):

@@ -212,6 +212,17 @@ def test_a_wrong_number_of_heads_without_a_workspace(hm, device):
             hm.paged_attention(q.clone(), q, cache, n[:, None], n)
 
 
+def test_tensors_of_other_devices_are_refused(oracle, hm, device):
+    s = Serving(oracle, hm, device, "fp16", 26, 4, 16, False)
+    cpu_plan = hm.PagePlan(4, 16, PS, "cpu")
+    for x, nw, plan, table in ((s.x.cpu(), s.nw, cpu_plan, s.table), (s.x, s.nw, cpu_plan, s.table), (s.x.cpu(), s.nw, s.plan, s.table),
+                               (s.x, s.nw.cpu(), s.plan, s.table), (s.x, s.nw, s.plan, s.table.cpu())):
+        before = x.clone()
+        with pytest.raises(ValueError):
+            s.layer.block_forward(x, nw, s.cache, plan, table)
+        assert torch.equal(x, before)
+
+
 @pytest.mark.parametrize("shape", [(2048, 32, 8, 64), (4096, 32, 8, 128), (512, 8, 2, 64)])
 def test_a_step_of_fewer_rows_has_its_workspace(oracle, hm, device, shape):
     hidden, q_heads, kv_heads, d = shape
