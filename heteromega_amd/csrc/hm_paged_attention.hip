@@ -13,7 +13,7 @@
 // be dealt in any order that A and B share, so those eight weights are its B operand as they are: no weight crosses
 // lanes. O^T keeps one q per lane too, so rescaling by a new maximum is one factor per lane.
 // The scores' running maximum m and the sum l of p = 2^(c s - m) (c = scale log2 e) are fp32. p enters the second product as
-// hi + lo, two 16-bit floats of which lo holds what hi lacks (to 2^-16 of p in bf16, 2^-22 in fp16): 16-bit weights alone would add
+// hi + lo, two 16-bit floats of which lo holds what hi lacks (to 2^-16 of p in bf16, 2^-20 in fp16): 16-bit weights alone would add
 // an error the size of the output's own rounding, and the matrix cores are idle most of the time here.
 //
 // Rows differ in length, and their lengths are known on the device only. So the work is dealt in tiles of keys: all tiles of all

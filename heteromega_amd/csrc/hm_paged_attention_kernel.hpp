@@ -97,25 +97,37 @@ template <class T> __device__ __forceinline__ void store4(uint16_t *p, float4_t 
     *reinterpret_cast<uint2 *>(p) = o;
 }
 
-// The compiler's types of T, for its conversion instructions, and the power of two that the largest weight has: fp16 loses
-// weights below 2^-25, of which a long row can have enough to matter next to a weight of 1; from 2^15 down to its subnormals
-// it has 2^40 of range. kBelow keeps hi below p by more than its rounding, so that lo is positive as well: an infinite value
-// then gives an infinite output, as p alone would, where a lo of zero or below would make it NaN.
+typedef float float2_t __attribute__((ext_vector_type(2)));
+
+// Pairs of T's weights, and the power of two that the largest weight has: fp16 loses weights below 2^-25, of which a long row can have
+// enough to matter next to a weight of 1; from 2^15 down to its subnormals it has 2^40 of range. kBelow keeps hi below p by more than its
+// rounding, so that lo is positive as well: an infinite value then gives an infinite output, as p alone would, where a lo of zero or below
+// would make it NaN.
 template <class T> struct Split;
 template <> struct Split<F16> {
-    typedef half8_t vec;
-    typedef _Float16 elem;
+    typedef _Float16 pair_t __attribute__((ext_vector_type(2)));
     static constexpr float kTop = 15.0f;
     static constexpr float kBelow = 1.0f - 0x1p-11f;
     static constexpr uint32_t kExponent = 0x7C00u; // all bits set: an infinity or NaN
+    // Rounded towards zero by an instruction of its own. A plain conversion of a product is made twice by the compiler, once together with
+    // the product and once after it, with roundings that differ now and then: then lo does not belong to hi.
+    static __device__ __forceinline__ pair_t upper(float2_t p) { return __builtin_bit_cast(pair_t, __builtin_amdgcn_cvt_pkrtz(p[0] * kBelow, p[1] * kBelow)); }
 };
 template <> struct Split<BF16> {
-    typedef bf16x8_t vec;
-    typedef __bf16 elem;
+    typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
     static constexpr float kTop = 0.0f;
     static constexpr float kBelow = 1.0f - 0x1p-8f;
     static constexpr uint32_t kExponent = 0x7F80u;
+    static __device__ __forceinline__ pair_t upper(float2_t p) { return __builtin_convertvector(p * kBelow, pair_t); }
 };
+
+// Two weights, each as hi + lo.
+template <class T> __device__ __forceinline__ void split(float2_t p, uint32_t &hi, uint32_t &lo) {
+    typedef typename Split<T>::pair_t pair_t;
+    const pair_t upper = Split<T>::upper(p);
+    hi = __builtin_bit_cast(uint32_t, upper);
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(p - __builtin_convertvector(upper, float2_t), pair_t));
+}
 
 template <class T, int D> struct Shape {
     static constexpr int kSteps = D / 32;         // K steps of the first product, and 16-byte pieces of V per lane and sub-tile
@@ -157,8 +169,6 @@ template <int D> struct Pieces {
 template <class T, int D, int TEAM, int CT, bool GROUPED>
 __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_kernel(PagedAttentionArgs a, AttentionPlan plan) {
     using S = Shape<T, D>;
-    using vec = typename Split<T>::vec;
-    using elem = typename Split<T>::elem;
     constexpr int kRuns = kAttentionWaves / TEAM, kTileKeys = TEAM * kWaveKeys;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kAttentionWaves * S::kRegion];
     __shared__ float2 wave_stats[kAttentionWaves][16];
@@ -442,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
                 request(tile + 1);
                 page_ids(min(tile + 2, tile1 - 1));
             }
-            vec hi[CT], lo[CT];
+            u32x4_t hi[CT], lo[CT];
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
                 float p[8];
@@ -475,8 +485,12 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
                 for (int e = 0; e < 8; ++e) {
                     p[e] = exp2_fast(p[e] - m_used);
                     l[c] += p[e];
-                    hi[c][e] = static_cast<elem>(p[e] * Split<T>::kBelow);
-                    lo[c][e] = static_cast<elem>(p[e] - static_cast<float>(hi[c][e]));
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t upper, lower;
+                    split<T>(float2_t{p[2 * e], p[2 * e + 1]}, upper, lower);
+                    hi[c][e] = upper, lo[c][e] = lower;
                 }
             }
 #pragma unroll

@@ -415,3 +415,11 @@ def test_a_cache_past_32_bits_of_elements(hm, device):
                              torch.tensor([60], dtype=torch.int32, device=device))
     want, bound = ref.attention(q, small_k, small_v, torch.arange(4)[None], [60], None, 1 / math.sqrt(128), 0, 16)
     ref.assert_within(got, want, bound, torch.float16, "far pages")
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_the_halves_of_a_weight_fit_together(hm, device, dtype):
+    # two keys of about the same weight, a hundred thousand times: a weight whose lower half belongs to another rounding of its upper one is
+    # 2^-10 (fp16) off, which shows where the two values nearly cancel
+    c = Case(19, [2] * 2000, 64, 16, 64, 16, DT[dtype], q_scale=0.5)
+    _check(hm, device, c, tag="two keys")
