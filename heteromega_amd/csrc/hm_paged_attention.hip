@@ -21,15 +21,16 @@
 // each run's part (fp32 O, m, l) goes to the workspace and a second launch joins the parts. Every workgroup finds its place by
 // summing the rows' tile counts itself.
 // Where rows share requests (prompts, drafted tokens; more rows than requests), the heads of up to 16 / G rows that follow each other
-// in one request are a unit, and read the cache once: 16 requests of 4096 keys with 4 rows each 110 -> 59 us, 2048 rows of one prompt
-// 1349 -> 408 us (84 TFLOP/s). They are masked one by one.
+// in one request are a unit, and read the cache once: 16 requests of 4096 keys with 4 rows each 110 -> 59 us. They are masked one by one.
+// Blocks of many rows of one request go to a kernel of their own (hm_paged_attention_prompt.hpp), in a launch before; what is one is found
+// out on the device, by every workgroup of both, from the blocks' first and last rows.
 // A run is shared by the four waves of a workgroup, 32 keys of a 128-key tile each, which join over LDS, or is one wave's own. The first
 // keeps the parts few; the second wastes nothing on rows shorter than a tile and lets waves go on to their next unit by
 // themselves. It is taken where there are units for three of four waves that fit the card (32 query and 8 key heads of 128: 1024 rows of up to 60
 // keys 75 -> 46 us, 256 rows of up to 500 keys 61 -> 56 us; 1824 units of up to 218 keys of 64 24 -> 21 us; 1024 units of 2040 keys would
 // take 67 us instead of 65).
 // Plain reads of 2 GB reach 6.3 TB/s: 64 rows of 8192 keys take 325 us (6.4 TB/s), one row of 130987 keys 91 us (5.9 TB/s with the join); one row
-// of 1037 keys takes 10.1 us, of which the join's launch is 3.
+// of 1037 keys takes 9.7 us, of which the join's launch is 3.
 #include "hm_paged_attention.hpp"
 
 #include <algorithm>
@@ -44,6 +45,9 @@ int64_t workgroups(int64_t head_dim) { return (head_dim > 128 ? 1 : 2) * device_
 // Columns of a unit: 16 rows' heads, or up to 32 heads of a row. Units of several rows with 32 columns do not fit the registers: 2048 rows
 // of a prompt took 687 us with them and 415 with 16.
 constexpr int kMaxCols = 32, kGroupedCols = 16;
+
+// A launch has less than 2^32 threads.
+constexpr int64_t kMostPromptUnits = int64_t(1) << 23;
 
 // Rows that a unit may have, where rows share requests.
 int unit_rows(int64_t group_heads) { return static_cast<int>(std::max<int64_t>(1, kGroupedCols / group_heads)); }
@@ -77,6 +81,13 @@ hipError_t launch_paged_attention(const PagedAttentionArgs &a, hipStream_t strea
     p.few_units = 16 * all_units < p.runs;
     // Units may have many parts each where there are fewer of them than runs: then a wave per column.
     p.join_cols = std::min(p.cols, 2 * all_units < p.runs ? kMaxCols : 4);
+    // Blocks of rows of the prompts' kernel, if there may be enough of them (which are some is found out there).
+    const int prompt_rows = 16 * kAttentionWaves * prompt_tiles(a.head_dim) / p.group_heads / p.rows * p.rows;
+    const int64_t prompt_units = prompt_rows < 2 ? 0 : a.rows / prompt_rows * a.kv_heads;
+    const bool prompts = a.requests != nullptr && a.rows > a.requests_count && p.group_heads <= kGroupedCols && kPromptShare * prompt_units > groups &&
+                         prompt_units <= kMostPromptUnits;
+    p.prompt_rows = prompts ? prompt_rows : 0;
+    p.prompt_slots = static_cast<int>(std::max<int64_t>(1, groups / a.kv_heads));
     return a.dtype == HM_FP16 ? launch_paged_attention_f16(a, p, stream) : launch_paged_attention_bf16(a, p, stream);
 }
 

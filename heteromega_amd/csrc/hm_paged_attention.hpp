@@ -8,6 +8,14 @@ namespace hm {
 
 constexpr int kAttentionWaves = 4; // of a workgroup
 
+// The prompts' kernel does not split keys: a block of its goes there if it takes less than so many times what all of them take on average per
+// place on the card. With an eighth of the places in use both kernels are about as fast (a prompt of 512 rows 38 us, of 256 rows 40, by the
+// other kernel 49 and 27; 256 rows behind 32512 tokens 1508 and 1035, 512 rows 1244 and 2172; 32 query and 8 key heads of 128).
+constexpr int kPromptShare = 8;
+
+// Tiles of 16 columns that a wave of the prompts' kernel has: two do not fit the registers next to 256 rows of outputs.
+constexpr int prompt_tiles(int64_t head_dim) { return head_dim <= 128 ? 2 : 1; }
+
 // A unit's columns are query heads of one key head: of one row, heads of it; or of several rows of one request, all heads of each.
 struct Column {
     int row, q_head; // row: behind the unit's first
@@ -24,6 +32,8 @@ struct AttentionPlan {
     bool joins;      // units may have more than one tile, and so parts
     bool few_units;  // join with a workgroup per unit and column
     int join_cols;   // else: workgroups that share the columns of a unit's join
+    int prompt_rows; // rows of a block that the prompts' kernel may take; 0: it is not launched
+    int prompt_slots; // its blocks that are on the card at once
 
     __host__ __device__ int kv_head(int unit) const { return shares == 1 ? unit : unit / shares; }
     // Columns of a unit that has `count` rows. GROUPED: rows > 1.

@@ -14,7 +14,6 @@ constexpr int kStream = 2; // cache policy of the keys and values, read once: no
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
-
 // One row's request and keys [first, end).
 struct Keys {
     int32_t request, first, end;
@@ -31,6 +30,45 @@ __device__ __forceinline__ Keys keys_of(const PagedAttentionArgs &a, int64_t t) 
     return k;
 }
 
+// A prompt block's rows lie within an aligned block of `rows` rows whose first and last are of one request, and its last row sees at most
+// `limit` keys (kPromptShare): a chunk of a long request next to a few others is better split over its keys. rows 0: there are none.
+struct Prompts {
+    int rows, limit;
+};
+
+// The keys that the last row of block b sees if its first and last row are of one request, else -1.
+__device__ __forceinline__ int prompt_keys(const PagedAttentionArgs &a, int rows, int64_t b) {
+    const int64_t t0 = b * rows, t1 = t0 + rows - 1;
+    if (t1 >= a.rows) {
+        return -1;
+    }
+    const int32_t r0 = a.requests[t0], r1 = a.requests[t1], pos = a.positions[t1];
+    return r0 >= 0 && r0 == r1 && pos >= 0 && pos < (a.width << a.page_shift) ? pos + 1 : -1;
+}
+
+__device__ __forceinline__ bool of_prompt(const PagedAttentionArgs &a, const Prompts &p, int64_t b) {
+    const int keys = prompt_keys(a, p.rows, b);
+    return keys >= 0 && keys <= p.limit;
+}
+
+// Summed up by each wave for itself.
+__device__ __forceinline__ Prompts prompts_of(const PagedAttentionArgs &a, int rows, int slots) {
+    if (rows == 0) {
+        return {0, 0};
+    }
+    const int blocks = static_cast<int>(a.rows / rows);
+    int64_t sum = 0;
+#pragma unroll 4
+    for (int b = threadIdx.x & 63; b < blocks; b += 64) {
+        sum += max(prompt_keys(a, rows, b), 0);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        sum += __shfl_xor(sum, off);
+    }
+    return {rows, uniform(static_cast<int>(min((kPromptShare * sum - 1) / slots, static_cast<int64_t>(INT32_MAX))))};
+}
+
 // The rows of a unit, `count` from this one on: keys [first, end) are seen by some of them, [all_first, all_end) by all; the tiles begin
 // at start.
 struct Row {
@@ -38,15 +76,18 @@ struct Row {
     bool bad;
 };
 
-// Row t with those that share units with it. Rows that belong to another row's units have no tiles, like rows of no request. With
-// `rows` > 1, a unit's rows lie within an aligned block of so many, follow each other, are of one request and none is bad.
-template <bool GROUPED> __device__ __forceinline__ Row row_of(const PagedAttentionArgs &a, int64_t t, int tile_keys, int rows) {
+// Row t with those that share units with it. Rows that belong to another row's units or to a prompt block have no tiles, like rows of no
+// request. With `rows` > 1, a unit's rows lie within an aligned block of so many, follow each other, are of one request and none is bad.
+template <bool GROUPED> __device__ __forceinline__ Row row_of(const PagedAttentionArgs &a, int64_t t, int tile_keys, int rows, const Prompts &prompts) {
     const Keys k = keys_of(a, t);
     Row r{k.request, k.first, k.end, k.first, k.end, 0, 0, 1, k.bad};
     if (k.request < 0) {
         return r;
     }
     if constexpr (GROUPED) {
+        if (prompts.rows != 0 && of_prompt(a, prompts, t / prompts.rows)) {
+            return r;
+        }
         if (t % rows != 0 && !k.bad) {
             const Keys before = keys_of(a, t - 1);
             if (before.request == k.request && !before.bad) {
@@ -105,7 +146,8 @@ typedef float float2_t __attribute__((ext_vector_type(2)));
 // would make it NaN.
 template <class T> struct Split;
 template <> struct Split<F16> {
-    typedef _Float16 pair_t __attribute__((ext_vector_type(2)));
+    typedef _Float16 elem_t;
+    typedef elem_t pair_t __attribute__((ext_vector_type(2)));
     static constexpr float kTop = 15.0f;
     static constexpr float kBelow = 1.0f - 0x1p-11f;
     static constexpr uint32_t kExponent = 0x7C00u; // all bits set: an infinity or NaN
@@ -114,7 +156,8 @@ template <> struct Split<F16> {
     static __device__ __forceinline__ pair_t upper(float2_t p) { return __builtin_bit_cast(pair_t, __builtin_amdgcn_cvt_pkrtz(p[0] * kBelow, p[1] * kBelow)); }
 };
 template <> struct Split<BF16> {
-    typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
+    typedef __bf16 elem_t;
+    typedef elem_t pair_t __attribute__((ext_vector_type(2)));
     static constexpr float kTop = 0.0f;
     static constexpr float kBelow = 1.0f - 0x1p-8f;
     static constexpr uint32_t kExponent = 0x7F80u;
@@ -181,6 +224,11 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
     const int units = plan.units;
     const int w = blockIdx.x * kRuns + (TEAM == 1 ? wave : 0), rows = static_cast<int>(a.rows);
 
+    Prompts prompts{0, 0};
+    if constexpr (GROUPED) {
+        prompts = prompts_of(a, plan.prompt_rows, plan.prompt_slots);
+    }
+
     // ---- this run's tiles, [x, x_end) ----
     int x, x_end;
     Runs runs{};
@@ -193,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
 #pragma unroll
         for (int i = 0; i < kLaneRows; ++i) {
             const bool some = i < per && lane * per + i < rows;
-            mine[i] = some ? row_of<GROUPED>(a, lane * per + i, kTileKeys, plan.rows) : Row{};
+            mine[i] = some ? row_of<GROUPED>(a, lane * per + i, kTileKeys, plan.rows, prompts) : Row{};
             own += mine[i].tiles;
         }
         int upto = own;
@@ -226,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
         const int t0 = min(static_cast<int>(threadIdx.x) * per, rows), t1 = min(t0 + per, rows);
         int own = 0;
         for (int i = t0; i < t1; ++i) {
-            own += row_of<GROUPED>(a, i, kTileKeys, plan.rows).tiles;
+            own += row_of<GROUPED>(a, i, kTileKeys, plan.rows, prompts).tiles;
         }
         int upto = own;
 #pragma unroll
@@ -254,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
                 int b = before * units;
                 for (int i = t0; i < t1; ++i) {
                     // The row is read again below, by scalar loads: handed on over LDS it cost 5 us of a call's 11.
-                    const int n = (per == 1 ? own : row_of<GROUPED>(a, i, kTileKeys, plan.rows).tiles) * units;
+                    const int n = (per == 1 ? own : row_of<GROUPED>(a, i, kTileKeys, plan.rows, prompts).tiles) * units;
                     if (xj < b + n) {
                         found[j][0] = i;
                         found[j][1] = b;
@@ -268,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
         if (x < x_end) {
             t = uniform(found[TEAM == 1 ? wave : 0][0]);
             base = uniform(found[TEAM == 1 ? wave : 0][1]);
-            r = uniform_row(row_of<GROUPED>(a, t, kTileKeys, plan.rows));
+            r = uniform_row(row_of<GROUPED>(a, t, kTileKeys, plan.rows, prompts));
         }
     }
     AttentionDescriptor begun{0, 0, 0, 0};
@@ -288,13 +336,13 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
             int from = t + 1;
             uint64_t some = 0;
             for (; from < rows; from += 64) {
-                some = __ballot(from + lane < rows && row_of<GROUPED>(a, min(from + lane, rows - 1), kTileKeys, plan.rows).tiles > 0);
+                some = __ballot(from + lane < rows && row_of<GROUPED>(a, min(from + lane, rows - 1), kTileKeys, plan.rows, prompts).tiles > 0);
                 if (some != 0) {
                     break;
                 }
             }
             t = uniform(some != 0 ? from + static_cast<int>(__builtin_ctzll(some)) : rows - 1); // a run ends before the rows do
-            r = uniform_row(row_of<GROUPED>(a, t, kTileKeys, plan.rows));
+            r = uniform_row(row_of<GROUPED>(a, t, kTileKeys, plan.rows, prompts));
         }
         const int unit = uniform(static_cast<uint32_t>(x - base) / static_cast<uint32_t>(r.tiles));
         const int tile0 = x - base - unit * r.tiles;
@@ -625,6 +673,8 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
     }
 }
 
+#include "hm_paged_attention_prompt.hpp"
+
 // The parts of column j of one unit, of runs w .. w + pieces, joined into `out` (zero if the column sees no key): THREADS threads, kLanes parts at a time for each of its
 // float4 elements, kAhead of them requested before the first is used.
 template <class T, int D, int THREADS>
@@ -716,10 +766,11 @@ template <class T, int D, bool GROUPED> __global__ void __launch_bounds__(kFewTh
     constexpr int kTileKeys = kAttentionWaves * kWaveKeys; // few units are dealt in tiles of whole workgroups
     const int t = blockIdx.x / plan.units, unit = blockIdx.x - t * plan.units;
     __shared__ int sums[kFewThreads / 64][2];
-    const Row own = row_of<GROUPED>(a, t, kTileKeys, plan.rows);
+    const Prompts prompts{0, 0}; // enough rows for them are not few units
+    const Row own = row_of<GROUPED>(a, t, kTileKeys, plan.rows, prompts);
     int before = 0, total = 0;
     for (int i = threadIdx.x; i < static_cast<int>(a.rows); i += kFewThreads) {
-        const int n = row_of<GROUPED>(a, i, kTileKeys, plan.rows).tiles;
+        const int n = row_of<GROUPED>(a, i, kTileKeys, plan.rows, prompts).tiles;
         before += i < t ? n : 0;
         total += n;
     }
@@ -756,6 +807,16 @@ template <class T, int D, bool GROUPED> __global__ void __launch_bounds__(kFewTh
 }
 
 template <class T, int D, int TEAM, int CT, bool GROUPED> hipError_t launch(const PagedAttentionArgs &a, const AttentionPlan &plan, hipStream_t stream) {
+    if constexpr (GROUPED) {
+        if (plan.prompt_rows != 0) {
+            const unsigned prompt_blocks = static_cast<unsigned>(a.rows / plan.prompt_rows * a.kv_heads);
+            hipLaunchKernelGGL((prompt_attention_kernel<T, D>), dim3(prompt_blocks), dim3(kThreads), 0, stream, a, plan);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) {
+                return e;
+            }
+        }
+    }
     const unsigned blocks = static_cast<unsigned>((plan.runs * TEAM + kAttentionWaves - 1) / kAttentionWaves);
     hipLaunchKernelGGL((paged_attention_kernel<T, D, TEAM, CT, GROUPED>), dim3(blocks), dim3(kThreads), 0, stream, a, plan);
     const hipError_t e = hipGetLastError();
@@ -773,7 +834,7 @@ template <class T, int D, int TEAM, int CT, bool GROUPED> hipError_t launch(cons
 }
 
 template <class T, int D> hipError_t launch_d(const PagedAttentionArgs &a, const AttentionPlan &plan, hipStream_t stream) {
-    if (plan.rows > 1) {
+    if (plan.rows > 1 || plan.prompt_rows != 0) {
         return plan.team == 1 ? launch<T, D, 1, 1, true>(a, plan, stream) : launch<T, D, 4, 1, true>(a, plan, stream);
     }
     return plan.team == 1     ? launch<T, D, 1, 1, false>(a, plan, stream)

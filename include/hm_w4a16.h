@@ -426,7 +426,8 @@ hm_status hm_qk_norm_rope(const hm_qk_norm_rope_args *args, const hm_kv_cache *c
  * it is. Keys and values behind a row's position or before its window are not read for it, whatever they hold. A row whose
  * request, position or one of whose page ids lies outside the table or the cache comes out as NaN, and nothing outside
  * them is read. Several rows may belong to one request (drafted tokens, a prompt); where there are more rows than
- * requests, rows that follow each other in one request share their reads of the cache.
+ * requests, rows that follow each other in one request share their reads of the cache, and long runs of them go to a
+ * launch of their own. Infinities and NaN show in the rows that see them only.
  * fp32 scores, statistics and sums; the weights p enter the second product as the sum of two 16-bit floats. out must not
  * overlap q.
  * head_dim: 64, 96, 128 or 256; q_heads a multiple of kv_heads. The workspace (hm_paged_attention_workspace_bytes, 16-byte
