@@ -19,7 +19,7 @@
 // Rows differ in length, and their lengths are known on the device only. So the work is dealt in tiles of keys: all tiles of all
 // units (a row and a key head, with up to 32 of its query heads) in one line, cut into equal runs. A run may end inside a unit; then
 // each run's part (fp32 O, m, l) goes to the workspace and a second launch joins the parts. Every workgroup finds its place by
-// summing the rows' tile counts itself.
+// summing the rows' tile counts itself, or those of 256 chunks of rows where a launch before has summed them up.
 // Where rows share requests (prompts, drafted tokens; more rows than requests), the heads of up to 16 / G rows that follow each other
 // in one request are a unit, and read the cache once: 16 requests of 4096 keys with 4 rows each 110 -> 59 us. They are masked one by one.
 // Blocks of many rows of one request go to a kernel of their own (hm_paged_attention_prompt.hpp), in a launch before; what is one is found
@@ -45,6 +45,11 @@ int64_t workgroups(int64_t head_dim) { return (head_dim > 128 ? 1 : 2) * device_
 // Columns of a unit: 16 rows' heads, or up to 32 heads of a row. Units of several rows with 32 columns do not fit the registers: 2048 rows
 // of a prompt took 687 us with them and 415 with 16.
 constexpr int kMaxCols = 32, kGroupedCols = 16;
+
+// Rows from which their tiles are summed up in a launch before, where each is looked at once. Up to here every workgroup sums them up itself, which takes
+// 8 us per 1000 rows (32 query and 8 key heads of 128: 1100 rows of 100 keys 100 us and with the launch 102, 16 prompts of 512 rows 217 and
+// 153, 300 of 100 rows 769 and 514).
+constexpr int64_t kCountedRows = 1024;
 
 // A launch has less than 2^32 threads.
 constexpr int64_t kMostPromptUnits = int64_t(1) << 23;
@@ -77,6 +82,7 @@ hipError_t launch_paged_attention(const PagedAttentionArgs &a, hipStream_t strea
     p.team = p.cols <= 16 && all_units >= 3 * groups && most_tiles(32) <= INT32_MAX ? 1 : kAttentionWaves;
     const int64_t most = most_tiles(32 * p.team);
     p.runs = static_cast<int>(std::min(groups * kAttentionWaves / p.team, most));
+    p.counted = a.rows > kCountedRows;
     p.joins = capacity > 32 * p.team;
     p.few_units = 16 * all_units < p.runs;
     // Units may have many parts each where there are fewer of them than runs: then a wave per column.

@@ -30,6 +30,7 @@ struct AttentionPlan {
     int shares;      // units of one key head
     int group_heads; // query heads of one key head
     bool joins;      // units may have more than one tile, and so parts
+    bool counted;    // the rows' tiles are summed up in a launch before
     bool few_units;  // join with a workgroup per unit and column
     int join_cols;   // else: workgroups that share the columns of a unit's join
     int prompt_rows; // rows of a block that the prompts' kernel may take; 0: it is not launched
@@ -74,21 +75,25 @@ struct AttentionDescriptor { // of the unit that a run begins and does not finis
     int32_t row, unit, pieces, count; // pieces: runs behind this one that hold its other parts; 0: there is none. count: rows
 };
 
+constexpr int kChunks = 64 * kAttentionWaves; // of rows: a thread of a workgroup has the sum of each
+constexpr int kCountBytes = kChunks * 4 + 16;
+
 // The workspace of `runs` runs with units of `cols` columns.
 struct AttentionWorkspace {
     AttentionDescriptor *desc; // [runs]
+    int32_t *counts;           // [kChunks]: tiles of each chunk's rows, and behind them the most keys of a prompt block
     float2 *stats;             // [2 runs][cols]: m, l of each part; part 2 w: of the unit that run w goes on with, 2 w + 1: of the one it begins
     float *o;                  // [2 runs][cols][D]
 };
 
 __host__ __device__ __forceinline__ int64_t attention_workspace_bytes(int64_t runs, int64_t cols, int64_t head_dim) {
-    return runs * static_cast<int64_t>(sizeof(AttentionDescriptor)) + (2 * runs * cols * 8 + 15) / 16 * 16 + 2 * runs * cols * head_dim * 4;
+    return runs * static_cast<int64_t>(sizeof(AttentionDescriptor)) + kCountBytes + (2 * runs * cols * 8 + 15) / 16 * 16 + 2 * runs * cols * head_dim * 4;
 }
 
 __host__ __device__ __forceinline__ AttentionWorkspace carve(void *p, int64_t runs, int64_t cols) {
     uint8_t *b = static_cast<uint8_t *>(p);
-    uint8_t *stats = b + runs * static_cast<int64_t>(sizeof(AttentionDescriptor));
-    return {reinterpret_cast<AttentionDescriptor *>(b), reinterpret_cast<float2 *>(stats),
+    uint8_t *counts = b + runs * static_cast<int64_t>(sizeof(AttentionDescriptor)), *stats = counts + kCountBytes;
+    return {reinterpret_cast<AttentionDescriptor *>(b), reinterpret_cast<int32_t *>(counts), reinterpret_cast<float2 *>(stats),
             reinterpret_cast<float *>(stats + (2 * runs * cols * 8 + 15) / 16 * 16)};
 }
 

@@ -207,6 +207,45 @@ template <int D> struct Pieces {
     __device__ __forceinline__ uint32_t lds_step(int i) const { return kEven ? i * (64 / kPerRow) * (2 * D + 32) : places[i % kKept]; }
 };
 
+// The same, once they are counted, in a launch before.
+__device__ __forceinline__ Prompts prompts_known(const PagedAttentionArgs &a, const AttentionPlan &plan) {
+    return plan.counted && plan.prompt_rows != 0 ? Prompts{plan.prompt_rows, carve(a.workspace, plan.runs, plan.cols).counts[kChunks]}
+                                                 : prompts_of(a, plan.prompt_rows, plan.prompt_slots);
+}
+
+// The tiles of each chunk of rows, a workgroup per chunk, and the limit of prompt blocks.
+template <bool GROUPED> __global__ void __launch_bounds__(kThreads) count_kernel(PagedAttentionArgs a, AttentionPlan plan) {
+    __shared__ int sums[kAttentionWaves];
+    Prompts prompts{0, 0};
+    if constexpr (GROUPED) {
+        prompts = prompts_of(a, plan.prompt_rows, plan.prompt_slots);
+    }
+    const int rows = static_cast<int>(a.rows), per = (rows + kChunks - 1) / kChunks;
+    const int t0 = min(static_cast<int>(blockIdx.x) * per, rows), t1 = min(t0 + per, rows);
+    int own = 0;
+    for (int i = t0 + threadIdx.x; i < t1; i += kThreads) {
+        own += row_of<GROUPED>(a, i, plan.team * kWaveKeys, plan.rows, prompts).tiles;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        own += __shfl_xor(own, off);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        sums[threadIdx.x >> 6] = own;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < kAttentionWaves; ++i) {
+            own += sums[i];
+        }
+        int32_t *counts = carve(a.workspace, plan.runs, plan.cols).counts;
+        counts[blockIdx.x] = own;
+        if (blockIdx.x == 0) {
+            counts[kChunks] = prompts.limit;
+        }
+    }
+}
+
 // TEAM waves of a workgroup (4 or 1) share a run of tiles of TEAM * 32 keys; a workgroup has 4 / TEAM runs. CT: tiles of 16 columns that
 // a unit has at most. GROUPED: units of several rows.
 template <class T, int D, int TEAM, int CT, bool GROUPED>
@@ -226,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
 
     Prompts prompts{0, 0};
     if constexpr (GROUPED) {
-        prompts = prompts_of(a, plan.prompt_rows, plan.prompt_slots);
+        prompts = prompts_known(a, plan);
     }
 
     // ---- this run's tiles, [x, x_end) ----
@@ -270,11 +309,15 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
             }
         }
     } else {
-        const int per = (rows + kThreads - 1) / kThreads;
+        const int per = (rows + kChunks - 1) / kChunks;
         const int t0 = min(static_cast<int>(threadIdx.x) * per, rows), t1 = min(t0 + per, rows);
         int own = 0;
-        for (int i = t0; i < t1; ++i) {
-            own += row_of<GROUPED>(a, i, kTileKeys, plan.rows, prompts).tiles;
+        if (plan.counted) {
+            own = carve(a.workspace, plan.runs, plan.cols).counts[threadIdx.x];
+        } else {
+            for (int i = t0; i < t1; ++i) {
+                own += row_of<GROUPED>(a, i, kTileKeys, plan.rows, prompts).tiles;
+            }
         }
         int upto = own;
 #pragma unroll
@@ -299,24 +342,31 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_attention_ke
         for (int j = 0; j < kRuns; ++j) {
             const int xj = runs.begin(blockIdx.x * kRuns + j);
             if (before * units <= xj && xj < (before + own) * units) {
-                int b = before * units;
-                for (int i = t0; i < t1; ++i) {
-                    // The row is read again below, by scalar loads: handed on over LDS it cost 5 us of a call's 11.
-                    const int n = (per == 1 ? own : row_of<GROUPED>(a, i, kTileKeys, plan.rows, prompts).tiles) * units;
-                    if (xj < b + n) {
-                        found[j][0] = i;
-                        found[j][1] = b;
-                        break;
-                    }
-                    b += n;
-                }
+                found[j][0] = t0;
+                found[j][1] = before * units;
             }
         }
         __syncthreads();
-        if (x < x_end) {
-            t = uniform(found[TEAM == 1 ? wave : 0][0]);
+        if (x < x_end) { // the chunk's rows, 64 at a time
             base = uniform(found[TEAM == 1 ? wave : 0][1]);
-            r = uniform_row(row_of<GROUPED>(a, t, kTileKeys, plan.rows, prompts));
+            for (int from = uniform(found[TEAM == 1 ? wave : 0][0]); from < rows; from += 64) {
+                const Row mine = from + lane < rows ? row_of<GROUPED>(a, from + lane, kTileKeys, plan.rows, prompts) : Row{};
+                int to = mine.tiles;
+#pragma unroll
+                for (int off = 1; off < 64; off <<= 1) {
+                    const int v = __shfl_up(to, off);
+                    to += lane >= off ? v : 0;
+                }
+                const uint64_t behind = __ballot(x < base + to * units);
+                if (behind != 0) {
+                    const int at = __builtin_ctzll(behind);
+                    r = row_of_lane(mine, at);
+                    base += (__builtin_amdgcn_readlane(to, at) - r.tiles) * units;
+                    t = from + at;
+                    break;
+                }
+                base += __builtin_amdgcn_readlane(to, 63) * units;
+            }
         }
     }
     AttentionDescriptor begun{0, 0, 0, 0};
@@ -807,6 +857,13 @@ template <class T, int D, bool GROUPED> __global__ void __launch_bounds__(kFewTh
 }
 
 template <class T, int D, int TEAM, int CT, bool GROUPED> hipError_t launch(const PagedAttentionArgs &a, const AttentionPlan &plan, hipStream_t stream) {
+    if (plan.counted) {
+        hipLaunchKernelGGL((count_kernel<GROUPED>), dim3(kChunks), dim3(kThreads), 0, stream, a, plan);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) {
+            return e;
+        }
+    }
     if constexpr (GROUPED) {
         if (plan.prompt_rows != 0) {
             const unsigned prompt_blocks = static_cast<unsigned>(a.rows / plan.prompt_rows * a.kv_heads);

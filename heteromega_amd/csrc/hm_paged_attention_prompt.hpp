@@ -34,7 +34,7 @@ template <class T, int D> __global__ void __launch_bounds__(kThreads, D <= 128 ?
     // Longest first; if all are on the card at once, the second of a CU's two is the shorter the longer the first.
     const int place = blockIdx.x / a.kv_heads;
     const int64_t block = blocks > plan.prompt_slots || 2 * place < blocks ? blocks - 1 - place : place - (blocks + 1) / 2;
-    if (!of_prompt(a, prompts_of(a, plan.prompt_rows, plan.prompt_slots), block)) {
+    if (!of_prompt(a, prompts_known(a, plan), block)) {
         return;
     }
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);

@@ -205,3 +205,27 @@ def test_the_same_bits_on_every_call(hm, device):
     first = hm.paged_attention(torch.zeros_like(q), q, cache, table, pos, req)
     for _ in range(3):
         assert torch.equal(hm.paged_attention(torch.zeros_like(q), q, cache, table, pos, req), first)
+
+
+@pytest.mark.parametrize("rows", [1024, 1025, 1300, 3000])
+@pytest.mark.parametrize("kind", ["single", "drafts", "prompts", "empty"])
+def test_many_rows(hm, device, rows, kind):
+    # around the number of rows from which they are counted in a launch of their own, and chunks of several rows
+    rng = np.random.default_rng(66)
+    if kind == "single":
+        c = Case(67, [int(n) for n in rng.integers(1, 60, rows)], 8, 2, 64, 16, torch.float16)
+        _check(hm, device, c, tag="single tokens")
+        return
+    c = Case(68, [int(n) for n in rng.integers(100, 200, 40)], 16, 4, 64, 16, torch.bfloat16)
+    at = []
+    while len(at) < rows:
+        r = int(rng.integers(0, 40))
+        n = c.lengths[r]
+        if kind == "drafts":
+            at += [(p, r) for p in range(n - int(rng.integers(1, 6)), n)] + [(-1, -1)] * int(rng.integers(0, 2))
+        elif kind == "prompts":
+            at += [(p, r) for p in range(n)]
+        else:
+            at += [(-1, -1)] * 900 + [(n - 1, r)]
+    positions, requests = zip(*at[:rows])
+    _check(hm, device, c, list(positions), list(requests), _queries(c, rows, 69), tag=f"{kind}")
