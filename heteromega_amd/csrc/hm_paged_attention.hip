@@ -30,7 +30,7 @@
 // keys 75 -> 46 us, 256 rows of up to 500 keys 61 -> 56 us; 1824 units of up to 218 keys of 64 24 -> 21 us; 1024 units of 2040 keys would
 // take 67 us instead of 65).
 // Plain reads of 2 GB reach 6.3 TB/s: 64 rows of 8192 keys take 325 us (6.4 TB/s), one row of 130987 keys 91 us (5.9 TB/s with the join); one row
-// of 1037 keys takes 9.7 us, of which the join's launch is 3.
+// of 1037 keys takes 10 us, of which the join's launch is 3.
 #include "hm_paged_attention.hpp"
 
 #include <algorithm>
