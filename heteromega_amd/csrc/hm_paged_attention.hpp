@@ -10,7 +10,7 @@ constexpr int kAttentionWaves = 4; // of a workgroup
 
 // The prompts' kernel does not split keys: a block of its goes there if it takes less than so many times what all of them take on average per
 // place on the card. With an eighth of the places in use both kernels are about as fast (a prompt of 512 rows 38 us, of 256 rows 40, by the
-// other kernel 49 and 27; 256 rows behind 32512 tokens 1508 and 1035, 512 rows 1244 and 2172; 32 query and 8 key heads of 128).
+// other kernel 49 and 27; the last 256 of 32768 rows 1508 and 1035, the last 512 1244 and 2172; 32 query and 8 key heads of 128).
 constexpr int kPromptShare = 8;
 
 // Tiles of 16 columns that a wave of the prompts' kernel has: two do not fit the registers next to 256 rows of outputs.

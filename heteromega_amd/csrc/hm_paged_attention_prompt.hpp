@@ -9,9 +9,10 @@
 // prompt, go first.
 //
 // 32 query and 8 key heads of 128, bf16: a prompt of 2048 rows 107 us (320 TFLOP/s; 408 by units of 16 columns), of 8192 rows 922 us
-// (597; 4400), 2048 rows behind 30720 tokens 1.68 ms (635; 8.75 ms). A large matrix product reaches 1199 TFLOP/s, and the lower halves
+// (597; 4400), the last 2048 of 32768 rows 1.68 ms (635; 8.75 ms). A large matrix product reaches 1199 TFLOP/s, and the lower halves
 // make three products of two, so 800 would be all. Steps at 8192 rows: as first built 1211 us; 32 of the tile's 64 keys at a time, for
-// the registers, 1176; maximum followed late 1050; masks as branches, paired conversions 1015; page ids by vector loads 990; rows counted in a launch before 922.
+// the registers, 1176; maximum followed late 1050; masks as branches, paired conversions 1015; page ids by vector loads 990; rows
+// counted in a launch before 922.
 #pragma once
 
 constexpr int kPromptTile = 16 * kAttentionWaves;
