@@ -8,8 +8,8 @@
 // while one is worked on. A wave skips tiles that none of its rows sees. Nothing is split over keys; the last rows, the longest of a
 // prompt, go first.
 //
-// 32 query and 8 key heads of 128, bf16: a prompt of 2048 rows 107 us (320 TFLOP/s; 408 by units of 16 columns), of 8192 rows 922 us
-// (597; 4400), the last 2048 of 32768 rows 1.68 ms (635; 8.75 ms). A large matrix product reaches 1199 TFLOP/s, and the lower halves
+// 32 query and 8 key heads of 128, bf16: a prompt of 2048 rows 108 us (319 TFLOP/s; 408 us by units of 16 columns), of 8192 rows 849 us
+// (648; 4400), the last 2048 of 32768 rows 1.62 ms (656; 8.75 ms). A large matrix product reaches 1199 TFLOP/s, and the lower halves
 // make three products of two, so 800 would be all. Steps at 8192 rows: as first built 1211 us; 32 of the tile's 64 keys at a time, for
 // the registers, 1176; maximum followed late 1050; masks as branches, paired conversions 1015; page ids by vector loads 990; rows
 // counted in a launch before 922.
@@ -24,7 +24,9 @@ template <class T, int D> __global__ void __launch_bounds__(kThreads, D <= 128 ?
     typedef typename Split<T>::elem_t elem4_t __attribute__((ext_vector_type(4)));
     constexpr int CT = prompt_tiles(D), kMostRows = 16 * kAttentionWaves * CT, kSubs = kAttentionWaves;
     // The maximum that weights are relative to follows only when a score passes it by more than a factor 2^kSlack: sums and outputs are
-    // rescaled seldom, and weights stay in range by starting that much lower.
+    // rescaled seldom, and weights stay in range by starting that much lower. The maximum is one of the scores as they leave the product, and is taken from them
+    // before the factor comes in: a fused score times factor less a maximum that was rounded with its factor is off by half a step of that maximum, in
+    // the exponent (infinite fp16 weights from 2^23 on). The subtraction costs 2 %: 8192 rows 828 -> 849 us.
     constexpr float kSlack = 3.0f, kTop = Split<T>::kTop - (Split<T>::kTop > 0.0f ? kSlack : 0.0f);
     constexpr int kTileBytes = kPromptTile * S::kRowBytes; // of keys, or values
     __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][kTileBytes];
@@ -57,6 +59,7 @@ template <class T, int D> __global__ void __launch_bounds__(kThreads, D <= 128 ?
     const uint32_t v_lds = (4 * quad + (col >> 2)) * S::kRowBytes + (col & 3) * 8;
     // The sign goes to the queries. Not zero: a masked score of -infinity times it must stay one.
     const float c_scale = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 0x1p-126f);
+    const float slack = fminf(kSlack / c_scale, 0x1p126f); // of scores without the factor
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
     const int64_t page_stride = uniform64(a.page_stride);
     const int shift = uniform(a.page_shift), offset_mask = (1 << shift) - 1;
@@ -272,12 +275,11 @@ template <class T, int D> __global__ void __launch_bounds__(kThreads, D <= 128 ?
                     for (int e = 1; e < 8; ++e) {
                         top = fmaxf(top, score[c][e >> 2][e & 3]);
                     }
-                    top *= c_scale;
-                    if (__any(top > m[c] + kSlack)) {
+                    if (__any(top > m[c] + slack)) {
                         top = fmaxf(top, __shfl_xor(top, 16));
                         top = fmaxf(top, __shfl_xor(top, 32));
                         const float m_new = fmaxf(m[c], top);
-                        const float f = m_new == -INFINITY ? 1.0f : exp2_fast(m[c] - m_new);
+                        const float f = m_new == -INFINITY ? 1.0f : exp2_fast((m[c] - m_new) * c_scale);
                         m[c] = m_new;
                         l[c] *= f;
 #pragma unroll
@@ -285,13 +287,13 @@ template <class T, int D> __global__ void __launch_bounds__(kThreads, D <= 128 ?
                             o[c][i] *= f;
                         }
                     }
-                    const float m_used = m[c] == -INFINITY ? 0.0f : m[c] - kTop;
+                    const float m_used = m[c] == -INFINITY ? 0.0f : m[c];
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) {
                         float2_t p;
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
-                            p[k] = exp2_fast(__builtin_fmaf(score[c][e >> 2][(e & 3) + k], c_scale, -m_used));
+                            p[k] = exp2_fast(__builtin_fmaf(score[c][e >> 2][(e & 3) + k] - m_used, c_scale, kTop));
                             l[c] += p[k];
                         }
                         uint32_t upper, lower;

@@ -229,3 +229,33 @@ def test_many_rows(hm, device, rows, kind):
             at += [(-1, -1)] * 900 + [(n - 1, r)]
     positions, requests = zip(*at[:rows])
     _check(hm, device, c, list(positions), list(requests), _queries(c, rows, 69), tag=f"{kind}")
+
+
+@pytest.mark.parametrize("scale,order", [(1.0, "rising"), (1.0, "falling"), (-1.0, "rising")])
+@pytest.mark.parametrize("window", [0, 37])
+@pytest.mark.parametrize("dtype,k_log,q_size", [("fp16", 9, 500.0), ("fp16", 13, 8000.0), ("fp16", 16, 60000.0), ("bf16", 16, 60000.0), ("bf16", 40, 1e12)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_scores_far_from_zero(hm, device, d, dtype, k_log, q_size, window, scale, order):
+    # Scores up to 2^80 of which a row's largest is ahead of the next by more than 2^6 in base 2, so that each other weight is zero in fp32 and
+    # the output is one key's value, exactly: a weight is hi + lo to 2^-16, far less than half a step of the output.
+    n, kv, heads = 256, 16, 64
+    c = Case(70, [n], heads, kv, d, 16, DT[dtype])
+    at = torch.arange(n)
+    size = ((at + 1) / n - 0.5) * 2.0 ** k_log  # distinct, of 8 bits: exact in both types
+    where = (c.table[0, at // 16].long(), slice(None), at % 16)
+    k = torch.zeros((n, kv, d), dtype=c.dtype)
+    k[..., 0] = (size if order == "rising" else -size).to(c.dtype)[:, None]
+    c.k[where] = k
+    values = c.v[where]
+    q = torch.zeros((n, heads, d), dtype=c.dtype)
+    q[..., 0] = (q_size * (0.5 + 0.5 * torch.rand((n, heads), generator=torch.Generator().manual_seed(71)))).to(c.dtype)
+    assert _blocks(c, list(range(n)), [0] * n)[0] > 0
+    pos = torch.arange(n, dtype=torch.int32, device=device)
+    got = hm.paged_attention(torch.zeros(q.shape, dtype=c.dtype, device=device), q.to(device), c.cache(hm, device), c.table.to(device), pos, torch.zeros_like(pos),
+                             scale=scale, window=window).cpu()
+    first = (at - window + 1).clamp(min=0) if window else torch.zeros_like(at)
+    top = at if (scale > 0) == (order == "rising") else first
+    want = values[top].repeat_interleave(heads // kv, 1)
+    wrong = (got != want).any(-1)
+    print(f"{dtype} d={d} window={window}: {int(wrong.sum())} of {wrong.numel()} heads are wrong", flush=True)
+    assert not wrong.any()
