@@ -115,7 +115,8 @@ def page_plan(plan, lengths, added, block_table, free_pages, queue, lengths_out=
     and new ones (0: none, -1: the request has ended and gives its pages back); block_table int32 [requests, pages of a request] and
     the ring of free pages free_pages int32 are updated in place; queue int64 [4] holds the ring's head and tail. The lengths
     and counters after the step go to plan.lengths and plan.queue, or to lengths_out and queue_out, which may be lengths and queue.
-    plan.queue[2] counts the requests that got nothing because pages, rows or table entries did not suffice."""
+    plan.queue[2] counts the requests that got nothing because pages, rows or table entries did not suffice, and those that could not end: free_pages
+    should have an entry for every page that is free or held, or pages given back may not fit it, and their request keeps them."""
     status = _host.page_plan(plan.slots, plan.positions, plan.requests, plan.starts, plan.lengths, plan.queue, plan.page_size, lengths, added,
                              block_table, free_pages, queue, lengths_out, queue_out, stream)
     if status != _lib.HM_OK:

@@ -94,7 +94,7 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) page_
     __shared__ int32_t length[kRequests];     // its length, or -1 if it gets nothing
     __shared__ int32_t first_page[kRequests]; // place of its first page in the ring, behind the head
     __shared__ Sums waves[THREADS / 64];
-    __shared__ int32_t taken, refused;
+    __shared__ int32_t taken, given_back, refused;
     const bool does_rows = blockIdx.x < static_cast<unsigned>(row_blocks), finishes = all || !does_rows;
     const int R = static_cast<int>(a.requests_count), shift = a.page_shift;
     const uint32_t ring_size = static_cast<uint32_t>(a.ring_size);
@@ -109,7 +109,7 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) page_
         add[i] = mine ? a.added[r0 + i] : 0;
     }
     if (threadIdx.x == 0) {
-        taken = 0, refused = 0;
+        taken = 0, given_back = 0, refused = 0;
     }
     const uint32_t head_place = ring_place(head, ring_size);
     const int32_t left = static_cast<int32_t>(max(int64_t(0), min(static_cast<int64_t>(tail - head), a.ring_size)));
@@ -137,6 +137,12 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) page_
         row_before = before.rows;
         again = !again && total.rows > a.rows;
     } while (again);
+    // A ring smaller than the pages in circulation may not take all that come back: then some requests do not end (the rows and pages of others are as
+    // if they did). Pages handed out by this step make room, so entries that are read may be written too: one workgroup does both in turn.
+    const int32_t room_before = static_cast<int32_t>(ring_size) - left;
+    const bool crowded = total.back > room_before;
+    const int writers = crowded ? 1 : row_blocks;
+    const bool writes_rows = does_rows && blockIdx.x < static_cast<unsigned>(writers);
     int64_t row = before.rows;
     int32_t page = before.need;
     int32_t my_taken = 0, my_refused = 0;
@@ -158,30 +164,54 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) page_
                 a.starts[r] = first;
             }
         }
+        my_taken = served && need[i] > 0 ? page_end : my_taken;
         if (finishes) {
-            my_taken = served && need[i] > 0 ? page_end : my_taken;
             my_refused += more > 0 && !served;
-            a.lengths_out[r] = add[i] < 0 ? 0 : served ? n[i] + more : n[i];
+            if (add[i] >= 0 || !crowded) {
+                a.lengths_out[r] = add[i] < 0 ? 0 : served ? n[i] + more : n[i];
+            }
         }
         row += more;
         page = page_end;
     }
-    if (finishes) {
-        if (my_taken > 0) {
-            atomicMax(&taken, my_taken);
-        }
-        if (my_refused > 0) {
-            atomicAdd(&refused, my_refused);
-        }
+    if (my_taken > 0 && (finishes || crowded)) {
+        atomicMax(&taken, my_taken);
+    }
+    if (my_refused > 0) {
+        atomicAdd(&refused, my_refused);
     }
     __syncthreads();
-    if (does_rows) {
+    if (crowded) {
+        const int32_t room = room_before + taken;
+        int32_t to = before.back, my_back = 0, my_kept = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (i < per && r0 + i < R && add[i] < 0) {
+                to = add_pages(to, back[i]);
+                const bool ends = back[i] == 0 || to <= room;
+                my_back = ends && back[i] > 0 ? to : my_back;
+                my_kept += !ends;
+                if (finishes) {
+                    a.lengths_out[r0 + i] = ends ? 0 : n[i];
+                }
+            }
+        }
+        if (my_back > 0) {
+            atomicMax(&given_back, my_back);
+        }
+        if (my_kept > 0) {
+            atomicAdd(&refused, my_kept);
+        }
+        __syncthreads();
+    }
+    const int32_t freed = crowded ? given_back : total.back;
+    if (writes_rows) {
         if (blockIdx.x == 0 && threadIdx.x == 0) {
             a.starts[R] = static_cast<int32_t>(min(total.rows, a.rows));
         }
         const int64_t used = min(total.rows, a.rows);
         const int32_t mask = static_cast<int32_t>((int64_t(1) << shift) - 1);
-        const int64_t step = static_cast<int64_t>(row_blocks) * THREADS;
+        const int64_t step = static_cast<int64_t>(writers) * THREADS;
         for (int64_t t = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x; t < a.rows; t += step) {
             int64_t slot = -1;
             int32_t position = -1, request = -1;
@@ -211,7 +241,7 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) page_
             a.requests[t] = request;
         }
     }
-    if (does_rows && total.back > 0) { // pages of ended requests, dealt and found like rows
+    if (writes_rows && freed > 0) { // pages of ended requests, dealt and found like rows
         __syncthreads();
         int32_t *first_back = first_page;
         int32_t to = before.back;
@@ -224,15 +254,14 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) page_
         }
         __syncthreads();
         const uint32_t tail_place = ring_place(tail, ring_size);
-        const int32_t count = min(total.back, static_cast<int32_t>(ring_size));
-        for (int64_t j = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x; j < count; j += static_cast<int64_t>(row_blocks) * THREADS) {
+        for (int64_t j = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x; j < freed; j += static_cast<int64_t>(writers) * THREADS) {
             const int r = last_from(first_back, R, static_cast<int32_t>(j));
             a.free_pages[ring_after(tail_place, static_cast<uint32_t>(j), ring_size)] = a.block_table[r * a.ld_table + (j - first_back[r])];
         }
     }
     if (finishes && threadIdx.x == 0) {
         a.queue_out[0] = static_cast<int64_t>(head + taken);
-        a.queue_out[1] = static_cast<int64_t>(tail + total.back);
+        a.queue_out[1] = static_cast<int64_t>(tail + freed);
         a.queue_out[2] = refused;
         a.queue_out[3] = total.rows;
     }

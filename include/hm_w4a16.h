@@ -373,7 +373,9 @@ typedef struct hm_kv_cache {
  *   lengths_out [R]   lengths after the step: + added, 0 for an ended request
  *   queue_out [4]     {head, tail, requests refused, rows asked for} after the step
  * New pages come from the head of the ring, in the order of requests and positions. An ended request's pages go
- * behind its tail, in that order too, and can be handed out from the next call on. A request with new tokens is refused,
+ * behind its tail, in that order too, and can be handed out from the next call on. The ring needs room for them: Q of at least
+ * the pages that are free and held together is always enough. In a smaller one at most Q pages are free after the step: an ended request
+ * is refused, keeping its length and pages, if its pages or those of one before it do not fit. A request with new tokens is refused,
  * keeping its length and its place among the rows (slots, positions and requests -1), if its length is negative or above W * page_size,
  * if it would outgrow W pages, if its rows would end behind `rows`, or if it needs pages and it or a request before it
  * needs more than are left. Rows behind the last token get -1 too. lengths_out may be lengths and queue_out may be

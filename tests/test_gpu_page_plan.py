@@ -138,3 +138,83 @@ def test_a_loop_in_a_graph_takes_and_gives_back_pages(hm, device):
         live = [p for r in range(requests) for p in host["table"][r, :ref.pages_of(int(host["lengths"][r]), ps)]]
         free = [host["ring"][i % pages] for i in range(int(host["queue"][0]), int(host["queue"][1]))]
         assert sorted(live + free) == list(range(pages)), "every page is held once or free once"
+
+
+def _plan_in_a_small_ring(lengths, added, table, ring, head, tail, rows, page_size):
+    """The plan made request by request, where ended requests keep their pages that the ring has no room for behind this step's."""
+    args = (table, ring, head, tail, rows, page_size)
+    taken = int(ref.plan(lengths, added, *args)["queue"][0]) - head
+    room = len(ring) - min(max(tail - head, 0), len(ring)) + taken
+    kept, at, limited = 0, 0, np.array(added)
+    for r, (n, a) in enumerate(zip(lengths, added)):
+        if a < 0:
+            pages = ref.pages_of(min(max(int(n), 0), table.shape[1] * page_size), page_size)
+            at += pages
+            if pages and at > room:
+                kept, limited[r] = kept + 1, 0
+    want = ref.plan(lengths, limited, *args)
+    want["queue"][2] += kept
+    return want, kept
+
+
+@pytest.mark.parametrize("rows", [60, 1024, 3000])
+@pytest.mark.parametrize("requests", [6, 500, 2500])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_a_ring_smaller_than_the_pages_in_circulation(hm, device, requests, rows, in_place):
+    rng = np.random.default_rng([requests, rows])
+    ps, width = 16, 6
+    i32 = lambda v: torch.tensor(np.asarray(v), dtype=torch.int32, device=device)
+    some = 0
+    for size in (1, requests // 2 + 1, requests + 1, 3 * requests):
+        lengths = rng.integers(0, width * ps, requests)
+        free = int(rng.integers(size // 2, size + 1))
+        held = [ref.pages_of(n, ps) for n in lengths]
+        ids = rng.permutation(sum(held) + free)
+        table = np.full((requests, width), -7, np.int64)
+        at = 0
+        for r, h in enumerate(held):
+            table[r, :h] = ids[at:at + h]
+            at += h
+        ring, head = np.full(size, -9, np.int64), int(rng.integers(0, 1 << 40))
+        ring[(head + np.arange(free)) % size] = ids[at:]
+        added = np.where(rng.random(requests) < 0.4, -1, rng.integers(0, max(2, 2 * rows // requests), requests))
+        want, kept = _plan_in_a_small_ring(lengths, added, table, ring, head, head + free, rows, ps)
+        some += kept
+        t, r, n, q = i32(table), i32(ring), i32(lengths), torch.tensor([head, head + free, 99, 99], dtype=torch.int64, device=device)
+        plan = hm.PagePlan(requests, rows, ps, device)
+        print(f"{requests} requests, {rows} rows, a ring of {size} with {free} free: {kept} keep their pages", flush=True)
+        out = (n, q) if in_place else (plan.lengths, plan.queue)
+        hm.page_plan(plan, n, i32(added), t, r, q, *out)
+        torch.cuda.synchronize()
+        for name, v in {"slots": plan.slots, "positions": plan.positions, "requests": plan.requests, "starts": plan.starts, "lengths": out[0],
+                        "queue": out[1], "table": t, "ring": r}.items():
+            np.testing.assert_array_equal(v.cpu().numpy().astype(np.int64), want[name], err_msg=name)
+    assert some > 0
+
+
+def test_no_page_is_lost_in_a_small_ring(hm, device):
+    # requests that could not end are asked to end again in the next step, as a serving loop would
+    ps, width, requests, rows = 16, 8, 12, 64
+    rng = np.random.default_rng(9)
+    pages, size = 50, 14
+    table = torch.full((requests, width), -1, dtype=torch.int32, device=device)
+    ids = rng.permutation(pages)
+    lengths = torch.tensor([48] * requests, dtype=torch.int32, device=device)
+    table[:, :3] = torch.tensor(ids[:36].reshape(12, 3), dtype=torch.int32)
+    ring = torch.tensor(ids[36:], dtype=torch.int32, device=device)
+    assert len(ring) == size
+    queue = torch.tensor([0, size, 0, 0], dtype=torch.int64, device=device)
+    plan = hm.PagePlan(requests, rows, ps, device)
+    ending, refused = set(), 0
+    for step in range(80):
+        a = np.where(rng.random(requests) < 0.25, -1, rng.integers(0, 9, requests))
+        a[list(ending)] = -1
+        hm.page_plan(plan, lengths, torch.tensor(a, dtype=torch.int32, device=device), table, ring, queue, lengths, queue)
+        torch.cuda.synchronize()
+        n, t, f, q = (v.cpu().numpy().astype(np.int64) for v in (lengths, table, ring, queue))
+        ending = {r for r in range(requests) if a[r] < 0 and n[r] > 0}
+        refused += len(ending)
+        live = [p for r in range(requests) for p in t[r, :ref.pages_of(int(n[r]), ps)]]
+        free = [f[i % size] for i in range(int(q[0]), int(q[1]))]
+        assert q[1] - q[0] <= size and sorted(live + free) == list(range(pages)), f"step {step}: every page is held once or free once"
+    assert refused > 0
