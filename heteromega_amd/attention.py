@@ -16,11 +16,16 @@ import torch
 from . import _lib
 from .ffn import (_DTYPES, _call, _current_raw_stream, _hm_dtype, _on, _stream, _workspace, packed_linear, residual_add2, rmsnorm)
 
-try:
-    # The checks and calls of the three operators, compiled: at few rows they took longer in Python than the kernels run.
-    from . import _attention_host as _host
-except ImportError as e:
-    raise ImportError("heteromega_amd._attention_host is missing: run `python heteromega_amd/build.py` (or __graft_entry__.build()) first") from e
+
+class _MissingHost:
+    """In the place of the compiled module where it is not built: the attention calls say so, and the rest of the package works without it."""
+
+    def __init__(self, error):
+        self._error = error
+
+    def __getattr__(self, name):
+        raise ImportError("heteromega_amd._attention_host is missing: run `python heteromega_amd/build.py` (or __graft_entry__.build()) first") from self._error
+
 
 kPagePlanMaxRequests = 4096
 
@@ -32,7 +37,13 @@ def _bind():
     _host.bind(address(L.hm_page_plan), address(L.hm_qk_norm_rope), address(L.hm_paged_attention), current, _stream)
 
 
-_bind()
+try:
+    # The checks and calls of the three operators, compiled: at few rows they took longer in Python than the kernels run.
+    from . import _attention_host as _host
+except ImportError as e:
+    _host = _MissingHost(e)
+else:
+    _bind()
 
 
 def _guard(device):

@@ -127,9 +127,11 @@ def build(verbose=False):
 
 if __name__ == "__main__":
     verbose = "--verbose" in sys.argv
-    with ThreadPoolExecutor(max_workers=2) as pool:  # the module builds beside the library: it does not link with it
-        host = pool.submit(build_host, verbose)
+    if "--no-shim" in sys.argv:  # the library alone, which needs none of torch's headers
         print(build(verbose))
-        print(host.result())
-    if "--no-shim" not in sys.argv:
+    else:
+        with ThreadPoolExecutor(max_workers=2) as pool:  # the module builds beside the library: it does not link with it
+            host = pool.submit(build_host, verbose)
+            print(build(verbose))
+            print(host.result())
         print(build_shim(verbose))
