@@ -165,6 +165,13 @@ def paged_attention(out, q, cache, block_table, positions, requests=None, scale=
     return out
 
 
+class _Scratch:
+    """An attention block's buffers on one stream."""
+
+    def __init__(self, rows, linear, attention):
+        self.rows, self.linear, self.attention, self.captured = rows, linear, attention, False
+
+
 class AttnLayer:
     """A layer's attention block over its paged cache, the counterpart of FfnLayer.block_forward: x += attention(RMSNorm(x)) Wo.
     wqkv [hidden, (q_heads + 2 kv_heads) * head_dim] and wo [q_heads * head_dim, hidden] are RepackedMatrix (RepackedMatrix.concat makes
@@ -181,26 +188,30 @@ class AttnLayer:
         self.frequencies, self.bias, self.q_weight, self.k_weight, self.qk_eps = frequencies, bias, q_weight, k_weight, qk_eps
         self.scale, self.window, self.interleaved = scale, window, interleaved
         self._buffers = {}
-        self._outgrown = []  # a captured step may still use them
+        self._outgrown = []  # those that a captured step still uses
 
     def _scratch(self, rows, cache, stream):
         """(normed or projected rows, Q/K/V rows, attention rows, workspaces) of calls on this stream, grown as needed."""
         key = _stream(stream, self.device)
         kept = self._buffers.get(key)
-        if kept is None or kept[0].size(0) < rows:
-            if kept is not None:
-                self._outgrown.append(kept)
-            with _on(stream, self.device):
+        with _on(stream, self.device):
+            capturing = torch.cuda.is_current_stream_capturing()
+            if kept is None or kept.rows[0].size(0) < rows:
+                if kept is not None and kept.captured:
+                    self._outgrown.append(kept)
                 new = lambda n: torch.empty((rows, n), dtype=self.dtype, device=self.device)
                 linear = max(w.workspace_bytes(m) for w in (self.wqkv, self.wo) for m in (rows, min(rows, 16)))
-                kept = self._buffers[key] = (new(self.hidden), new(self.wqkv.n), new(self.wo.k), _workspace(linear, self.device, stream),
-                                             cache.attention_workspace(self.q_heads, stream))
-        return tuple(t[:rows] for t in kept[:3]) + kept[3:]
+                # attention's workspace does not depend on the rows
+                attention = cache.attention_workspace(self.q_heads) if kept is None else kept.attention
+                kept = self._buffers[key] = _Scratch((new(self.hidden), new(self.wqkv.n), new(self.wo.k)), _workspace(linear, self.device, None), attention)
+        kept.captured |= capturing
+        return tuple(t[:rows] for t in kept.rows) + (kept.linear, kept.attention)
 
     def block_forward(self, x, norm_weight, cache, plan, block_table, eps=1e-5, stream=None):
         """In place: x [rows, hidden] += attention(RMSNorm(x) * norm_weight) Wo. The rows are those of `plan` (page_plan of this step): their keys and values
         are written to `cache` first, and each row sees its request's tokens up to its own. Rows that the plan left empty stay as they are. The buffers in between are
-        the stream's: steps captured on one stream must not be replayed at the same time."""
+        the stream's, also those of a step that was captured on it: such steps, wherever they are replayed, and other calls on the stream must not run at the same
+        time."""
         rows = plan.slots.size(0)
         if x.dim() != 2 or x.size(0) != rows or x.size(1) != self.hidden or x.stride(1) != 1 or x.dtype != self.dtype:
             raise ValueError(f"AttnLayer.block_forward: x must be {self.dtype} [{rows}, {self.hidden}]")
