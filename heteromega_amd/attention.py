@@ -175,14 +175,19 @@ class _Scratch:
 class AttnLayer:
     """A layer's attention block over its paged cache, the counterpart of FfnLayer.block_forward: x += attention(RMSNorm(x)) Wo.
     wqkv [hidden, (q_heads + 2 kv_heads) * head_dim] and wo [q_heads * head_dim, hidden] are RepackedMatrix (RepackedMatrix.concat makes
-    wqkv of three); frequencies as rope_frequencies gives them; bias of the Q/K/V columns, q_weight and k_weight of normed heads or None."""
+    wqkv of three); frequencies as rope_frequencies gives them; bias of the Q/K/V columns, q_weight and k_weight of normed heads or None.
+    head_dim: 64, 96, 128 or 256."""
 
     def __init__(self, wqkv, wo, q_heads, kv_heads, head_dim, frequencies, bias=None, q_weight=None, k_weight=None, qk_eps=1e-6, scale=None, window=0,
                  interleaved=False):
+        if wqkv.dtype not in _DTYPES or min(q_heads, kv_heads) <= 0 or q_heads > 65536 or q_heads % kv_heads:
+            raise ValueError(f"AttnLayer: query heads (up to 65536) must be a multiple of key heads, got {q_heads} and {kv_heads}")
+        if head_dim not in (64, 96, 128, 256):
+            raise ValueError(f"AttnLayer: paged_attention takes heads of 64, 96, 128 or 256, got {head_dim}")
+        if (scale is not None and not math.isfinite(ctypes.c_float(scale).value)) or window < 0:
+            raise ValueError(f"AttnLayer: scale must be finite and window not negative, got {scale} and {window}")
         if wqkv.n != (q_heads + 2 * kv_heads) * head_dim or wo.k != q_heads * head_dim or wo.n != wqkv.k or wo.dtype != wqkv.dtype:
             raise ValueError(f"AttnLayer: wqkv [{wqkv.k}, {wqkv.n}] and wo [{wo.k}, {wo.n}] do not fit {q_heads} + 2 x {kv_heads} heads of {head_dim}")
-        if wqkv.dtype not in _DTYPES or q_heads % kv_heads:
-            raise ValueError("AttnLayer: query heads must be a multiple of key heads")
         self.wqkv, self.wo, self.q_heads, self.kv_heads, self.head_dim = wqkv, wo, q_heads, kv_heads, head_dim
         self.hidden, self.dtype, self.device = wqkv.k, wqkv.dtype, wqkv.device
         self.frequencies, self.bias, self.q_weight, self.k_weight, self.qk_eps = frequencies, bias, q_weight, k_weight, qk_eps

@@ -1,6 +1,7 @@
 """CPU checks of the attention operators' refusals: every call here is turned down before anything reaches a GPU."""
 
 import ctypes
+import math
 
 import numpy as np
 import pytest
@@ -160,3 +161,28 @@ def test_the_request_by_request_plan():
     assert p["positions"][:5].tolist() == [15, 16, 0, 1, 2] and p["starts"].tolist() == [0, 1, 2, 20, 20, 36]
     assert p["lengths"].tolist() == [16, 17, 18, 0, 0] and p["queue"].tolist() == [3, 5, 1, 36]
     assert p["table"].tolist() == [[4, -1], [2, 9], [8, 5], [7, 3], [-1, -1]] and p["ring"].tolist() == [9, 8, 5, 7, 3, -1]
+
+
+def _layer(hm, q_heads=8, kv_heads=2, head_dim=64, **kw):
+    from types import SimpleNamespace
+
+    cuda = torch.device("cuda", 0)
+    wqkv = SimpleNamespace(k=512, n=(q_heads + 2 * kv_heads) * head_dim, dtype=torch.float16, device=cuda)
+    wo = SimpleNamespace(k=q_heads * head_dim, n=512, dtype=torch.float16, device=cuda)
+    return hm.AttnLayer(wqkv, wo, q_heads, kv_heads, head_dim, hm.rope_frequencies(64), **kw)
+
+
+@pytest.mark.parametrize("kw,match", [
+    *[(dict(head_dim=d), "heads of 64, 96, 128 or 256") for d in (16, 32, 80, 112, 160, 512)],
+    (dict(kv_heads=0), "multiple"), (dict(q_heads=0), "multiple"), (dict(q_heads=7), "multiple"), (dict(q_heads=65538), "65536"),
+    *[(dict(scale=s), "scale") for s in (math.nan, math.inf, 1e39)], (dict(window=-1), "window"),
+], ids=str)
+def test_layers_that_no_call_would_take_are_refused_when_made(hm, kw, match):
+    # they used to fail in their first call, when keys and values had been written to the cache
+    with pytest.raises(ValueError, match=match):
+        _layer(hm, **kw)
+
+
+def test_layers_of_every_head_size(hm):
+    for d in (64, 96, 128, 256):
+        assert _layer(hm, head_dim=d, scale=0.0, window=5).head_dim == d
