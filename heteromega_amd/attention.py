@@ -186,6 +186,8 @@ class AttnLayer:
             raise ValueError(f"AttnLayer: paged_attention takes heads of 64, 96, 128 or 256, got {head_dim}")
         if (scale is not None and not math.isfinite(ctypes.c_float(scale).value)) or window < 0:
             raise ValueError(f"AttnLayer: scale must be finite and window not negative, got {scale} and {window}")
+        if wo.device != wqkv.device:
+            raise ValueError(f"AttnLayer: wqkv and wo must be on one device, got {wqkv.device} and {wo.device}")
         if wqkv.n != (q_heads + 2 * kv_heads) * head_dim or wo.k != q_heads * head_dim or wo.n != wqkv.k or wo.dtype != wqkv.dtype:
             raise ValueError(f"AttnLayer: wqkv [{wqkv.k}, {wqkv.n}] and wo [{wo.k}, {wo.n}] do not fit {q_heads} + 2 x {kv_heads} heads of {head_dim}")
         self.wqkv, self.wo, self.q_heads, self.kv_heads, self.head_dim = wqkv, wo, q_heads, kv_heads, head_dim

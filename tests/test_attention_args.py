@@ -163,22 +163,22 @@ def test_the_request_by_request_plan():
     assert p["table"].tolist() == [[4, -1], [2, 9], [8, 5], [7, 3], [-1, -1]] and p["ring"].tolist() == [9, 8, 5, 7, 3, -1]
 
 
-def _layer(hm, q_heads=8, kv_heads=2, head_dim=64, **kw):
+def _layer(hm, q_heads=8, kv_heads=2, head_dim=64, wo_device="cuda:0", **kw):
     from types import SimpleNamespace
 
     cuda = torch.device("cuda", 0)
     wqkv = SimpleNamespace(k=512, n=(q_heads + 2 * kv_heads) * head_dim, dtype=torch.float16, device=cuda)
-    wo = SimpleNamespace(k=q_heads * head_dim, n=512, dtype=torch.float16, device=cuda)
+    wo = SimpleNamespace(k=q_heads * head_dim, n=512, dtype=torch.float16, device=torch.device(wo_device))
     return hm.AttnLayer(wqkv, wo, q_heads, kv_heads, head_dim, hm.rope_frequencies(64), **kw)
 
 
 @pytest.mark.parametrize("kw,match", [
     *[(dict(head_dim=d), "heads of 64, 96, 128 or 256") for d in (16, 32, 80, 112, 160, 512)],
     (dict(kv_heads=0), "multiple"), (dict(q_heads=0), "multiple"), (dict(q_heads=7), "multiple"), (dict(q_heads=65538), "65536"),
-    *[(dict(scale=s), "scale") for s in (math.nan, math.inf, 1e39)], (dict(window=-1), "window"),
+    *[(dict(scale=s), "scale") for s in (math.nan, math.inf, 1e39)], (dict(window=-1), "window"), (dict(wo_device="cuda:1"), "device"),
 ], ids=str)
 def test_layers_that_no_call_would_take_are_refused_when_made(hm, kw, match):
-    # they used to fail in their first call, when keys and values had been written to the cache
+    # they used to fail in their first call, when keys and values had been written to the cache (or, on two devices, not at all)
     with pytest.raises(ValueError, match=match):
         _layer(hm, **kw)
 
