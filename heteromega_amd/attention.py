@@ -230,6 +230,9 @@ class AttnLayer:
             raise ValueError(f"norm_weight must be a contiguous {x.dtype} vector of {self.hidden} elements")
         if (cache.kv_heads, cache.head_dim, cache.page_size) != (self.kv_heads, self.head_dim, plan.page_size):
             raise ValueError("AttnLayer.block_forward: the cache's heads and page size must be the layer's and the plan's")
+        if block_table.dtype != torch.int32 or block_table.dim() != 2 or 0 in block_table.shape or (block_table.size(1) > 1 and block_table.stride(1) != 1):
+            raise ValueError(f"AttnLayer.block_forward: block_table must be int32 [requests, pages of a request] with contiguous rows, got {block_table.dtype} "
+                             f"{list(block_table.shape)}")
         with _guard(self.device):
             normed, qkv, heads, linear_ws, attention_ws = self._scratch(rows, cache, stream)
             rmsnorm(normed, x, norm_weight, eps, stream)

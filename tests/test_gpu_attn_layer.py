@@ -277,3 +277,14 @@ def test_a_captured_step_keeps_its_buffers_when_others_outgrow_them(oracle, hm, 
         g.replay()
         s.check(added, given, used, f"replay {i}")
     assert len(s.layer._outgrown) == 1, "the captured step's buffers alone are kept"
+
+
+def test_a_refused_table_leaves_the_cache_as_it_was(oracle, hm, device):
+    s = Serving(oracle, hm, device, "fp16", 31, 4, 16, False)
+    s.inputs([3, 1, 1, 1])
+    s.hm.page_plan(s.plan, s.lengths, s.added, s.table, s.ring, s.queue)
+    for table in (s.table.long(), s.table[0], s.table[:, ::2], s.table[:0], s.table[:, :0]):
+        with pytest.raises(ValueError, match="block_table"):
+            s.layer.block_forward(s.x, s.nw, s.cache, s.plan, table)
+    torch.cuda.synchronize()
+    assert torch.isnan(s.cache.k).all() and torch.isnan(s.cache.v).all()
