@@ -18,3 +18,13 @@ def test_cpp_host_ffn_forward():
     r = subprocess.run([BIN], capture_output=True, text=True, timeout=120)
     print(r.stdout, r.stderr, flush=True)
     assert r.returncode == 0 and "PASS" in r.stdout, (r.returncode, r.stdout, r.stderr)
+
+
+def test_cpp_host_attention_over_a_paged_cache():
+    # tests/c_abi/attention_step.cpp: a serving loop's steps of plan, rotation with cache write, and attention, against float64
+    program = os.path.join(os.path.dirname(BIN), "attention_step")
+    assert os.path.exists(program), f"{program} is missing: run __graft_entry__.build() first"
+    print("running", program, flush=True)
+    r = subprocess.run([program], capture_output=True, text=True, timeout=120)
+    print(r.stdout, r.stderr, flush=True)
+    assert r.returncode == 0 and "PASS" in r.stdout, (r.returncode, r.stdout, r.stderr)
