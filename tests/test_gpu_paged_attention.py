@@ -423,3 +423,28 @@ def test_the_halves_of_a_weight_fit_together(hm, device, dtype):
     # 2^-10 (fp16) off, which shows where the two values nearly cancel
     c = Case(19, [2] * 2000, 64, 16, 64, 16, DT[dtype], q_scale=0.5)
     _check(hm, device, c, tag="two keys")
+
+
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("window", [0, 25000])
+def test_drafts_of_a_long_request(hm, device, d, dtype, window):
+    # few units of several rows, each split over the card: drafted tokens of one request and of two, an empty row among them
+    c = Case(31, [30000], 8, 2, d, 16, DT[dtype])
+    q = _queries(c, 4)
+    _check(hm, device, c, list(range(29996, 30000)), [0] * 4, q, window=window, tag="four drafts")
+    got = _check(hm, device, c, [29996, -1, 29998, 29999], [0] * 4, q, window=window, tag="drafts and an empty row")
+    assert (got[1] == 0).all()
+    c = Case(32, [20001, 9000], 8, 2, d, 32, DT[dtype])
+    rows = [(p, 0) for p in range(19997, 20001)] + [(p, 1) for p in range(8995, 9000)] + [(-1, -1), (3, 1)]
+    positions, requests = zip(*rows)
+    _check(hm, device, c, list(positions), list(requests), _queries(c, len(rows)), window=window and 7000, tag="drafts of two")
+
+
+@pytest.mark.parametrize("height", [4, 64, 400])
+def test_the_tables_height(hm, device, height):
+    # the same rows in tables with few and many other requests
+    c = _group_case(33, (8, 2), 128, torch.bfloat16)
+    c.table = torch.cat([c.table, torch.full((height - 4, c.table.size(1)), -1, dtype=torch.int32)])
+    positions, requests = _prompt_rows(34)
+    _check(hm, device, c, positions, requests, _queries(c, len(positions)), tag=f"a table of {height} requests")

@@ -259,3 +259,22 @@ def test_scores_far_from_zero(hm, device, d, dtype, k_log, q_size, window, scale
     wrong = (got != want).any(-1)
     print(f"{dtype} d={d} window={window}: {int(wrong.sum())} of {wrong.numel()} heads are wrong", flush=True)
     assert not wrong.any()
+
+
+def test_the_limit_keeps_a_long_request_out(hm, device):
+    # Above 1024 rows the launch that counts tiles leaves the limit of prompt blocks behind 256 counts in the workspace: eight times what all blocks take
+    # on average per place on the card (256 CUs with two workgroups each, over the key heads).
+    c = Case(72, [30000] + [150] * 7, 64, 16, 64, 16, torch.bfloat16)
+    rows = [(p, 0) for p in range(30000 - 32, 30000)] + [(p, r) for r in range(1, 8) for p in range(150)]
+    positions, requests = zip(*rows)
+    assert len(rows) > 1024
+    cache, q = c.cache(hm, device), _queries(c, len(rows), 73)
+    ws = torch.zeros(cache.attention_workspace_bytes(64) + 256, dtype=torch.uint8, device=device)
+    ws = ws[-ws.data_ptr() % 256:]
+    _check(hm, device, c, list(positions), list(requests), q, tag="a long request among short ones", workspace=ws)
+    ends = [positions[b + 31] + 1 if requests[b] == requests[b + 31] else 0 for b in range(0, len(rows) - 31, 32)]
+    runs = 2048  # one per wave: more units than three for every four waves
+    left = int(ws[16 * runs + 4 * 256:16 * runs + 4 * 256 + 4].view(torch.int32))
+    print(f"limit {left}, blocks of {sorted(set(ends))} keys", flush=True)
+    assert left == (8 * sum(ends) - 1) // (512 // 16)
+    assert ends[0] == 30000 > left > max(ends[1:]) > 0

@@ -160,3 +160,29 @@ def test_a_replayed_graph_follows_positions_and_slots(hm, device):
         hm.qk_norm_rope(q2, qkv, freq, pos, cache=hm.PagedCache(k2, v2), slots=slots)
         assert torch.equal(q, q2) and torch.equal(k, k2) and torch.equal(v, v2)
         assert (q[i] == 0).all() and (q != 0).any()
+
+
+# From 2048 rows of one pass on, a workgroup takes two rows of all heads and results are stored past the caches: each form of that kernel, with rows left out
+# first and second of their pair and alone in the last.
+MANY = dict(skip=(0, 7, 20, 1001, 2050))
+
+
+@pytest.mark.parametrize("d,rotary", [(16, 16), (64, 64), (64, 32), (80, 32), (96, 96), (128, 128), (128, 0), (256, 64), (512, 512)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_head_sizes_of_many_rows(hm, device, d, rotary, interleaved, dtype):
+    _check(hm, device, d + rotary, 2051, 3, 1, d, rotary, DT[dtype], interleaved=interleaved, **MANY)
+
+
+@pytest.mark.parametrize("norm,bias", [("", False), ("", True), ("q", False), ("k", True), ("qk", True), ("qk", False)])
+@pytest.mark.parametrize("cached", [False, True])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("dtype,interleaved", [("bf16", False), ("fp16", True)])
+def test_forms_of_many_rows(hm, device, norm, bias, cached, in_place, dtype, interleaved):
+    _check(hm, device, 14, 2051, 5, 1, 64, 64, DT[dtype], norm=norm, bias=bias, interleaved=interleaved, cached=cached, in_place=in_place, pad=8, **MANY)
+
+
+@pytest.mark.parametrize("rows", [2047, 2048, 2049, 6001])
+@pytest.mark.parametrize("page_size,layout", [(16, "page_token_head"), (64, "page_head_token"), (1024, "page_token_head")])
+def test_row_counts_and_layouts_of_many_rows(hm, device, rows, page_size, layout):
+    _check(hm, device, rows, rows, 4, 2, 64, 64, torch.bfloat16, page_size=page_size, layout=layout, skip=(rows - 1,))
