@@ -154,7 +154,8 @@ def paged_attention(out, q, cache, block_table, positions, requests=None, scale=
     """out[t, h] = softmax(scale q[t, h] K^T) V over keys 0..positions[t] (its last `window` ones, if not 0) of row t's request in the
     paged cache (hm_paged_attention). q, out [rows, q_heads, head_dim]; block_table int32 [requests, pages of a request]; row t is of request
     requests[t], or t. Position -1: zeros; a negative request: the row is left as it is; a row outside the table or the
-    cache: NaN. scale: 1 / sqrt(head_dim) by default. workspace: cache.attention_workspace(q_heads), one per stream."""
+    cache: NaN. Rows of one request share their reads of the cache where there are more rows than the table has: block_table[:n] of the requests
+    in use is faster for prompts and drafts than a taller table. scale: 1 / sqrt(head_dim) by default. workspace: cache.attention_workspace(q_heads), one per stream."""
     d = cache.head_dim
     if workspace is None:
         workspace = cache.attention_workspace(q.size(1) if q.dim() == 3 else q.size(-1) // d, stream)

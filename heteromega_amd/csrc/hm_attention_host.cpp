@@ -1,5 +1,5 @@
 // The Python calls' host side of the attention operators: argument checks on torch tensors and the C ABI calls, compiled. In Python
-// the checks took 5 us of a call, more than the kernels of a few rows run (page_plan of 64 requests 4.4 us, qk_norm_rope of a row 3.9).
+// the checks took 5 us of a call, more than a call of few rows takes now (page_plan of 64 requests 4.2 us, qk_norm_rope of a row 4.2).
 // The C ABI's functions come from the library that the ctypes binding loaded (bind), so there is one of it. Host code only.
 #include "hm_w4a16.h"
 

@@ -20,10 +20,12 @@
 // units (a row and a key head, with up to 32 of its query heads) in one line, cut into equal runs. A run may end inside a unit; then
 // each run's part (fp32 O, m, l) goes to the workspace and a second launch joins the parts. Every workgroup finds its place by
 // summing the rows' tile counts itself, or those of 256 chunks of rows where a launch before has summed them up.
-// Where rows share requests (prompts, drafted tokens; more rows than requests), the heads of up to 16 / G rows that follow each other
-// in one request are a unit, and read the cache once: 16 requests of 4096 keys with 4 rows each 110 -> 59 us. They are masked one by one.
+// Where rows must share requests (prompts, drafted tokens: a call of more rows than the block table has), the heads of up to 16 / G rows that
+// follow each other in one request are a unit, and read the cache once. They are masked one by one. Which rows share is known on the device only, so calls of
+// no more rows than the table take units of one row, whatever they hold: 64 rows, 4 of each of 16 requests of 4096 keys, 58 us in a table of up to 63
+// requests and 103 to 107 in taller ones, a prompt of 2048 rows 104 us in a table of up to 2047 and 1375 in one of 2048.
 // Blocks of many rows of one request go to a kernel of their own (hm_paged_attention_prompt.hpp), in a launch before; what is one is found
-// out on the device, by every workgroup of both, from the blocks' first and last rows.
+// out on the device from the blocks' first and last rows, against a limit that every wave of both kernels sums up, or that the counting launch leaves.
 // A run is shared by the four waves of a workgroup, 32 keys of a 128-key tile each, which join over LDS, or is one wave's own. The first
 // keeps the parts few; the second wastes nothing on rows shorter than a tile and lets waves go on to their next unit by
 // themselves. It is taken where there are units for three of four waves that fit the card (32 query and 8 key heads of 128: 1024 rows of up to 60

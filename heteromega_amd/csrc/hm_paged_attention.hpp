@@ -9,8 +9,8 @@ namespace hm {
 constexpr int kAttentionWaves = 4; // of a workgroup
 
 // The prompts' kernel does not split keys: a block of its goes there if it takes less than so many times what all of them take on average per
-// place on the card. With an eighth of the places in use both kernels are about as fast (a prompt of 512 rows 38 us, of 256 rows 40, by the
-// other kernel 49 and 27; the last 256 of 32768 rows 1508 and 1035, the last 512 1244 and 2172; 32 query and 8 key heads of 128).
+// place on the card. With an eighth of the places in use both kernels are about as fast (a prompt of 512 rows 38 us, of 256 rows 29, by the
+// other kernel 49 and 26; the last 256 of 32768 rows 1296 and 1130, the last 512 1302 and 2378; 32 query and 8 key heads of 128).
 constexpr int kPromptShare = 8;
 
 // Tiles of 16 columns that a wave of the prompts' kernel has: two do not fit the registers next to 256 rows of outputs.
@@ -30,7 +30,7 @@ struct AttentionPlan {
     int shares;      // units of one key head
     int group_heads; // query heads of one key head
     bool joins;      // units may have more than one tile, and so parts
-    bool counted;    // the rows' tiles are summed up in a launch before
+    bool counted;    // the rows' tiles are summed up in a launch before, and the limit of prompt blocks
     bool few_units;  // join with a workgroup per unit and column
     int join_cols;   // else: workgroups that share the columns of a unit's join
     int prompt_rows; // rows of a block that the prompts' kernel may take; 0: it is not launched

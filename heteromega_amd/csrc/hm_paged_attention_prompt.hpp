@@ -12,7 +12,7 @@
 // (648; 4400), the last 2048 of 32768 rows 1.62 ms (656; 8.75 ms). A large matrix product reaches 1199 TFLOP/s, and the lower halves
 // make three products of two, so 800 would be all. Steps at 8192 rows: as first built 1211 us; 32 of the tile's 64 keys at a time, for
 // the registers, 1176; maximum followed late 1050; masks as branches, paired conversions 1015; page ids by vector loads 990; rows
-// counted in a launch before 922.
+// counted in a launch before 922 (828 timed as above, and 849 since the maximum is taken from scores without their factor).
 #pragma once
 
 constexpr int kPromptTile = 16 * kAttentionWaves;

@@ -427,11 +427,12 @@ hm_status hm_qk_norm_rope(const hm_qk_norm_rope_args *args, const hm_kv_cache *c
  * request t without requests (NULL). Position -1 sees no key: its output is zero. A negative request is a row to leave as
  * it is. Keys and values behind a row's position or before its window are not read for it, whatever they hold. A row whose
  * request, position or one of whose page ids lies outside the table or the cache comes out as NaN, and nothing outside
- * them is read. Several rows may belong to one request (drafted tokens, a prompt); where there are more rows than
- * requests, rows that follow each other in one request share their reads of the cache, and long runs of them go to a
- * launch of their own. Infinities and NaN show in the rows that see them only.
+ * them is read. Several rows may belong to one request (drafted tokens, a prompt). In a call of more rows than R,
+ * rows that follow each other in one request share their reads of the cache, and long runs of them go to a launch of their own; otherwise each row
+ * reads the cache for itself, so a table should not be taller than its requests' numbers need (up to 16 query heads per key head;
+ * rows of more never share). Infinities and NaN show in the rows that see them only.
  * fp32 scores, statistics and sums; the weights p enter the second product as the sum of two 16-bit floats. out must not
- * overlap q.
+ * overlap q. rows * key heads * (W * page_size / 128 + 2) must stay below 2^31.
  * head_dim: 64, 96, 128 or 256; q_heads a multiple of kv_heads. The workspace (hm_paged_attention_workspace_bytes, 16-byte
  * aligned, nothing in it has to start at zero) holds the parts of rows that several workgroups share; calls that may
  * overlap in time need workspaces of their own. */
