@@ -13,6 +13,8 @@ from .ffn import *  # noqa: E402,F401,F403
 from .ffn import __all__ as _ffn_all  # noqa: E402
 from .attention import *  # noqa: E402,F401,F403
 from .attention import __all__ as _attention_all  # noqa: E402
+from .branches import *  # noqa: E402,F401,F403
+from .branches import __all__ as _branches_all  # noqa: E402
 from . import hetero  # noqa: E402,F401
 
-__all__ = list(_ffn_all) + list(_attention_all) + ["hetero"]
+__all__ = list(_ffn_all) + list(_attention_all) + list(_branches_all) + ["hetero"]

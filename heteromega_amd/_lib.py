@@ -19,6 +19,7 @@ HM_WORKSPACE_TOO_SMALL = 5
 
 HM_BF16 = 0
 HM_FP16 = 1
+HM_LOGITS_FP32 = 2  # beside these, for beam_select's logits
 
 HM_GATE_UP_BLOCKED = 0
 HM_GATE_UP_INTERLEAVED = 1
@@ -112,6 +113,17 @@ _SIGNATURES = {
     "hm_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(QkNormRopeArgs), ctypes.POINTER(KvCache), P]),
     "hm_paged_attention_workspace_bytes": (SZ, [ctypes.POINTER(KvCache), I64]),
     "hm_paged_attention": (ctypes.c_int, [ctypes.POINTER(KvCache), P, I64, P, I64, I64, I64, P, I64, I64, I64, P, P, ctypes.c_float, I64, P, SZ, P]),
+    "hm_beam_select_workspace_bytes": (SZ, [I64, I64, I64, I64, I32]),
+    "hm_beam_select": (ctypes.c_int, [P, I64, I32, P, P, I64, I64, I64, I64, I64, P, P, P, P, P, SZ, P]),
+    "hm_page_fork_workspace_bytes": (SZ, [I64, I64]),
+    "hm_page_fork": (ctypes.c_int, [P, P, P, I64, P, I64, P, I64, I64, I64, P, I64, P, P, P, P, P, SZ, P]),
+    "hm_page_compact_workspace_bytes": (SZ, [I64]),
+    "hm_page_compact": (ctypes.c_int, [I64, I64, P, I64, P, I64, P, I64, I64, I64, P, I64, P, P, I64, P, P, SZ, P]),
+    "hm_copy_pages": (ctypes.c_int, [ctypes.POINTER(KvCache), ctypes.POINTER(KvCache), I64, P, I64, P]),
+    "hm_share_plan_bytes": (SZ, [I64]),
+    "hm_share_plan": (ctypes.c_int, [P, I64, I64, I64, I64, P, P, I64, I64, I64, I64, P, P, SZ, P]),
+    "hm_shared_attention_workspace_bytes": (SZ, [ctypes.POINTER(KvCache), I64, I64]),
+    "hm_shared_attention": (ctypes.c_int, [ctypes.POINTER(KvCache), P, I64, P, I64, I64, I64, P, I64, I64, I64, P, P, ctypes.c_float, P, SZ, P, SZ, P]),
     "hm_partition_check": (ctypes.c_int, [I64, I64, I64]),
     "hm_partition_from_ratio": (ctypes.c_int, [I64, ctypes.c_double, I64, ctypes.POINTER(I64)]),
     "hm_split_type": (I32, [I32, I32, I32, I32, I32, I32]),

@@ -106,6 +106,15 @@ class PagedCache:
             return _workspace(self.attention_workspace_bytes(q_heads), self.device, stream)
 
 
+    def shared_attention_workspace_bytes(self, q_heads, rows):
+        return _lib.load().hm_shared_attention_workspace_bytes(self._ref, q_heads, rows)
+
+    def shared_attention_workspace(self, q_heads, rows, stream=None):
+        """A workspace for shared_attention calls of so many rows on one stream, for any lengths."""
+        with _guard(self.device):
+            return _workspace(self.shared_attention_workspace_bytes(q_heads, rows), self.device, stream)
+
+
 class PagePlan:
     """What page_plan works out for a step of up to `rows` new tokens of `requests` requests, kept from step to step (a captured
     step's layers read these tensors): slots, positions and requests of each row, starts of the requests' rows, and their lengths
@@ -171,6 +180,7 @@ class _Scratch:
 
     def __init__(self, rows, linear, attention):
         self.rows, self.linear, self.attention, self.captured = rows, linear, attention, False
+        self.shared = None  # shared_attention's workspace, for as many rows as the buffers have
 
 
 class AttnLayer:
@@ -198,8 +208,9 @@ class AttnLayer:
         self._buffers = {}
         self._outgrown = []  # those that a captured step still uses
 
-    def _scratch(self, rows, cache, stream):
-        """(normed or projected rows, Q/K/V rows, attention rows, workspaces) of calls on this stream, grown as needed."""
+    def _scratch(self, rows, cache, stream, shared=False):
+        """(normed or projected rows, Q/K/V rows, attention rows, workspaces) of calls on this stream, grown as needed. shared: the attention's workspace is
+        shared_attention's."""
         key = _stream(stream, self.device)
         kept = self._buffers.get(key)
         with _on(stream, self.device):
@@ -212,13 +223,15 @@ class AttnLayer:
                 # attention's workspace does not depend on the rows
                 attention = cache.attention_workspace(self.q_heads) if kept is None else kept.attention
                 kept = self._buffers[key] = _Scratch((new(self.hidden), new(self.wqkv.n), new(self.wo.k)), _workspace(linear, self.device, None), attention)
+            if shared and kept.shared is None:
+                kept.shared = cache.shared_attention_workspace(self.q_heads, kept.rows[0].size(0))
         kept.captured |= capturing
-        return tuple(t[:rows] for t in kept.rows) + (kept.linear, kept.attention)
+        return tuple(t[:rows] for t in kept.rows) + (kept.linear, kept.shared if shared else kept.attention)
 
-    def block_forward(self, x, norm_weight, cache, plan, block_table, eps=1e-5, stream=None):
+    def block_forward(self, x, norm_weight, cache, plan, block_table, eps=1e-5, stream=None, share=None):
         """In place: x [rows, hidden] += attention(RMSNorm(x) * norm_weight) Wo. The rows are those of `plan` (page_plan of this step): their keys and values
-        are written to `cache` first, and each row sees its request's tokens up to its own. Rows that the plan left empty stay as they are. The buffers in between are
-        the stream's, also those of a step that was captured on it: such steps, wherever they are replayed, and other calls on the stream must not run at the same
+        are written to `cache` first, and each row sees its request's tokens up to its own. Rows that the plan left empty stay as they are. share: share_plan of this
+        step's positions and requests, where rows share pages (up to 4096 rows, the layer's heads and window). The buffers in between are the stream's, also those of a step that was captured on it: such steps, wherever they are replayed, and other calls on the stream must not run at the same
         time."""
         rows = plan.slots.size(0)
         if x.dim() != 2 or x.size(0) != rows or x.size(1) != self.hidden or x.stride(1) != 1 or x.dtype != self.dtype:
@@ -234,8 +247,13 @@ class AttnLayer:
         if block_table.dtype != torch.int32 or block_table.dim() != 2 or 0 in block_table.shape or (block_table.size(1) > 1 and block_table.stride(1) != 1):
             raise ValueError(f"AttnLayer.block_forward: block_table must be int32 [requests, pages of a request] with contiguous rows, got {block_table.dtype} "
                              f"{list(block_table.shape)}")
+        if share is not None:
+            made, called = (share.rows, share.page_size, share.q_heads, share.kv_heads, share.window, share.device), (rows, plan.page_size, self.q_heads, self.kv_heads,
+                                                                                                                   self.window, self.device)
+            if made != called:
+                raise ValueError(f"AttnLayer.block_forward: share must be made for (rows, page size, heads, window, device) {called}, got {made}")
         with _guard(self.device):
-            normed, qkv, heads, linear_ws, attention_ws = self._scratch(rows, cache, stream)
+            normed, qkv, heads, linear_ws, attention_ws = self._scratch(rows, cache, stream, share is not None)
             rmsnorm(normed, x, norm_weight, eps, stream)
             packed_linear(qkv, normed, self.wqkv, stream=stream, workspace=linear_ws)
             q = qkv[:, :self.q_heads * self.head_dim]
@@ -243,10 +261,15 @@ class AttnLayer:
                          bias=self.bias, eps=self.qk_eps, interleaved=self.interleaved, stream=stream)
             with _on(stream, self.device):
                 heads.zero_()  # the rows that the plan left empty add nothing
-            paged_attention(heads, q, cache, block_table, plan.positions, plan.requests, self.scale, self.window, stream, attention_ws)
+            if share is None:
+                paged_attention(heads, q, cache, block_table, plan.positions, plan.requests, self.scale, self.window, stream, attention_ws)
+            else:
+                shared_attention(heads, q, cache, block_table, plan.positions, share, plan.requests, self.scale, stream, attention_ws)
             packed_linear(normed, heads, self.wo, stream=stream, workspace=linear_ws)
             residual_add2(x, normed, stream=stream)
         return x
 
+
+from .branches import shared_attention  # noqa: E402  (which uses this module's cache)
 
 __all__ = ["kPagePlanMaxRequests", "rope_frequencies", "PagedCache", "PagePlan", "page_plan", "qk_norm_rope", "paged_attention", "AttnLayer"]

@@ -17,7 +17,8 @@ LIB_NAME = "libhmw4a16.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 
 SOURCES = ["hm_api.cpp", "hm_split.cpp", "hm_layout.hip", "hm_gemv.hip", "hm_gemm.hip", "hm_gemm_f16.hip", "hm_gemm_bf16.hip", "hm_elementwise.hip", "hm_static.hip", "hm_pages.hip",
-           "hm_rope.hip", "hm_paged_attention.hip", "hm_paged_attention_f16.hip", "hm_paged_attention_bf16.hip", "hm_attention_api.cpp"]
+           "hm_rope.hip", "hm_paged_attention.hip", "hm_paged_attention_f16.hip", "hm_paged_attention_bf16.hip", "hm_attention_api.cpp", "hm_page_fork.hip",
+           "hm_beam.hip", "hm_share_plan.hip", "hm_shared_attention.hip", "hm_shared_attention_f16.hip", "hm_shared_attention_bf16.hip", "hm_branch_api.cpp"]
 ARCH = "gfx950"
 
 COMMON_FLAGS = [
@@ -60,7 +61,7 @@ def _compile(src, verbose):
 SHIM_DIR = os.path.join(HERE, "shim")
 SHIM_SOURCES = ["hm_reference_api.cpp", "py_module.cpp"]
 SHIM_NAME = "_reference_shim"
-HOST_SOURCES = ["hm_attention_host.cpp"]
+HOST_SOURCES = ["hm_attention_host.cpp", "hm_branch_host.cpp"]
 HOST_NAME = "_attention_host"
 
 

@@ -1,21 +1,15 @@
 // The Python calls' host side of the attention operators: argument checks on torch tensors and the C ABI calls, compiled. In Python
 // the checks took 5 us of a call, more than a call of few rows takes now (page_plan of 64 requests 4.2 us, qk_norm_rope of a row 4.2).
 // The C ABI's functions come from the library that the ctypes binding loaded (bind), so there is one of it. Host code only.
-#include "hm_w4a16.h"
-
-#include <torch/extension.h>
-
-#include <hip/hip_runtime_api.h>
-
-#include <optional>
+#include "hm_host_checks.hpp"
 
 namespace {
+
+using namespace hm_host;
 
 decltype(&hm_page_plan) c_page_plan = nullptr;
 decltype(&hm_qk_norm_rope) c_qk_norm_rope = nullptr;
 decltype(&hm_paged_attention) c_paged_attention = nullptr;
-PyObject *current_stream = nullptr; // of a device index: its handle
-PyObject *handle_of = nullptr;      // of a stream argument that is not None: its handle
 
 void bind(uintptr_t page_plan, uintptr_t qk_norm_rope, uintptr_t paged_attention, py::object current, py::object handle) {
     c_page_plan = reinterpret_cast<decltype(c_page_plan)>(page_plan);
@@ -25,109 +19,6 @@ void bind(uintptr_t page_plan, uintptr_t qk_norm_rope, uintptr_t paged_attention
     current_stream = current.release().ptr();
     handle_of = handle.release().ptr();
 }
-
-template <class... Parts> [[noreturn]] void refuse(const Parts &...parts) {
-    std::ostringstream s;
-    (s << ... << parts);
-    throw py::value_error(s.str());
-}
-
-std::string described(const at::Tensor &t) {
-    std::ostringstream s;
-    s << t.scalar_type() << " " << t.sizes() << " with strides " << t.strides() << " on " << t.device();
-    return s.str();
-}
-
-int device_of(const at::Tensor &t, const char *what) {
-    if (!t.is_cuda()) {
-        refuse(what, ": needs device tensors, got one on ", t.device());
-    }
-    return t.get_device();
-}
-
-// Address of a contiguous vector of n elements (or more).
-void *vector(const at::Tensor &t, at::ScalarType type, int64_t n, int device, const char *what, const char *name, bool more = false) {
-    if (t.scalar_type() != type || t.dim() != 1 || !t.is_contiguous() || (more ? t.size(0) < n : t.size(0) != n) || !t.is_cuda() || t.get_device() != device) {
-        refuse(what, ": ", name, " must be a contiguous ", type, " vector of ", n, more ? " or more" : "", " elements on cuda:", device, ", got ", described(t));
-    }
-    return t.data_ptr();
-}
-
-void *vector(const std::optional<at::Tensor> &t, at::ScalarType type, int64_t n, int device, const char *what, const char *name, bool more = false) {
-    return t.has_value() ? vector(*t, type, n, device, what, name, more) : nullptr;
-}
-
-struct Rows {
-    void *p;
-    int64_t ld;
-};
-
-// [rows, heads * d] or [rows, heads, d] with packed heads.
-Rows row_array(const at::Tensor &t, int64_t rows, int64_t heads, int64_t d, at::ScalarType type, int device, const char *what, const char *name) {
-    bool ok = t.scalar_type() == type && t.is_cuda() && t.get_device() == device;
-    if (ok && t.dim() == 3) {
-        ok = t.size(0) == rows && t.size(1) == heads && t.size(2) == d && t.stride(2) == 1 && (heads == 1 || t.stride(1) == d);
-    } else if (ok) {
-        ok = t.dim() == 2 && t.size(0) == rows && t.size(1) == heads * d && t.stride(1) == 1;
-    }
-    if (!ok) {
-        refuse(what, ": ", name, " must be ", type, " [", rows, ", ", heads, " x ", d, "] with contiguous rows on cuda:", device, ", got ", described(t));
-    }
-    return {t.data_ptr(), rows > 1 ? t.stride(0) : heads * d}; // a single row's stride may be anything
-}
-
-struct Table {
-    int32_t *p;
-    int64_t ld, requests, width;
-};
-
-Table table_of(const at::Tensor &t, int device, const char *what) {
-    if (t.scalar_type() != at::kInt || t.dim() != 2 || (t.size(1) > 1 && t.stride(1) != 1) || !t.is_cuda() || t.get_device() != device) {
-        refuse(what, ": block_table must be int32 [requests, pages of a request] with contiguous rows on cuda:", device, ", got ", described(t));
-    }
-    return {static_cast<int32_t *>(t.data_ptr()), t.size(0) > 1 ? t.stride(0) : t.size(1), t.size(0), t.size(1)};
-}
-
-void *stream_of(py::handle stream, int device) {
-    PyObject *h = nullptr;
-    if (stream.is_none()) {
-        const auto index = py::reinterpret_steal<py::object>(PyLong_FromLong(device));
-        h = PyObject_CallOneArg(current_stream, index.ptr());
-    } else {
-        h = PyObject_CallOneArg(handle_of, stream.ptr());
-    }
-    if (h == nullptr) {
-        throw py::error_already_set();
-    }
-    const auto owned = py::reinterpret_steal<py::object>(h);
-    void *p = PyLong_AsVoidPtr(h);
-    if (p == nullptr && PyErr_Occurred()) {
-        throw py::error_already_set();
-    }
-    return p;
-}
-
-// A launch goes to the current device: the tensors' one, for as long as this lives.
-class OnDevice {
-  public:
-    explicit OnDevice(int device) {
-        if (hipGetDevice(&before_) != hipSuccess || before_ == device || hipSetDevice(device) != hipSuccess) {
-            before_ = -1;
-        }
-    }
-    ~OnDevice() {
-        if (before_ >= 0) {
-            (void)hipSetDevice(before_);
-        }
-    }
-    OnDevice(const OnDevice &) = delete;
-    OnDevice &operator=(const OnDevice &) = delete;
-
-  private:
-    int before_ = -1;
-};
-
-at::ScalarType type_of(int32_t dtype) { return dtype == HM_FP16 ? at::kHalf : at::kBFloat16; }
 
 int page_plan(const at::Tensor &slots, const at::Tensor &positions, const at::Tensor &requests, const at::Tensor &starts, const at::Tensor &plan_lengths,
               const at::Tensor &plan_queue, int64_t page_size, const at::Tensor &lengths, const at::Tensor &added, const at::Tensor &block_table,
@@ -221,20 +112,11 @@ int paged_attention(const at::Tensor &out, const at::Tensor &q, uintptr_t cache,
     const Table table = table_of(block_table, device, what);
     const auto *pos = static_cast<const int32_t *>(vector(positions, at::kInt, rows, device, what, "positions", true));
     const auto *req = static_cast<const int32_t *>(vector(requests, at::kInt, rows, device, what, "requests", true));
-    uintptr_t aligned = 0; // without a workspace the call itself refuses
-    size_t bytes = 0;
-    if (workspace.has_value()) {
-        if (!workspace->is_cuda() || workspace->get_device() != device || !workspace->is_contiguous()) {
-            refuse("paged_attention: the workspace must be a contiguous tensor on cuda:", device, ", got ", described(*workspace));
-        }
-        const uintptr_t base = reinterpret_cast<uintptr_t>(workspace->data_ptr());
-        aligned = (base + 255) / 256 * 256;
-        bytes = workspace->nbytes() > aligned - base ? workspace->nbytes() - (aligned - base) : 0;
-    }
+    const Workspace ws = workspace.has_value() ? workspace_of(*workspace, device, what) : Workspace{nullptr, 0}; // without one the call itself refuses
     void *s = stream_of(stream, device);
     const OnDevice on(device);
     return c_paged_attention(c, to.p, to.ld, in.p, in.ld, rows, q_heads, table.p, table.ld, table.requests, table.width, pos, req, static_cast<float>(scale), window,
-                             reinterpret_cast<void *>(aligned), bytes, s);
+                             ws.p, ws.bytes, s);
 }
 
 } // namespace
@@ -245,4 +127,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("page_plan", &page_plan);
     m.def("qk_norm_rope", &qk_norm_rope);
     m.def("paged_attention", &paged_attention);
+    def_branches(m);
 }

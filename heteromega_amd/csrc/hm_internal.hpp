@@ -236,4 +236,101 @@ struct PagedAttentionArgs {
 size_t paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t head_dim);
 hipError_t launch_paged_attention(const PagedAttentionArgs &a, hipStream_t stream);
 
+// Requests that become copies or prefixes of others (hm_page_fork).
+struct PageForkArgs {
+    const int32_t *sources, *keep, *lengths;
+    int64_t requests_count;
+    const int32_t *block_table;
+    int64_t ld_table;
+    int32_t *table_out;
+    int64_t ld_out, width;
+    int page_shift;
+    int32_t *free_pages;
+    int64_t ring_size;
+    const int64_t *queue_in;
+    int32_t *copies, *lengths_out;
+    int64_t *queue_out;
+    void *workspace;
+    int hash_bits; // set by the launch
+};
+size_t page_fork_workspace(int64_t requests, int64_t width);
+hipError_t launch_page_fork(const PageForkArgs &a, hipStream_t stream);
+
+// Pages in use moved below a limit (hm_page_compact).
+struct PageCompactArgs {
+    int64_t pages, limit;
+    const int32_t *lengths;
+    int64_t requests_count;
+    const int32_t *block_table;
+    int64_t ld_table;
+    int32_t *table_out;
+    int64_t ld_out, width;
+    int page_shift;
+    int32_t *free_pages;
+    int64_t ring_size;
+    const int64_t *queue_in;
+    int32_t *copies;
+    int64_t most_copies;
+    int64_t *queue_out;
+    void *workspace;
+};
+size_t page_compact_workspace(int64_t pages);
+hipError_t launch_page_compact(const PageCompactArgs &a, hipStream_t stream);
+
+// Pages copied within the caches of some layers, or from those to others (hm_copy_pages).
+constexpr int kCopyLayers = 64; // of a launch
+struct CopyPagesArgs {
+    const uint16_t *from_k[kCopyLayers], *from_v[kCopyLayers];
+    uint16_t *to_k[kCopyLayers], *to_v[kCopyLayers];
+    int layers;
+    int64_t from_pages, from_page, from_head, from_token;
+    int64_t to_pages, to_page, to_head, to_token;
+    int kv_heads, head_dim, page_shift;
+    const int32_t *copies;
+    int64_t count;
+};
+hipError_t launch_copy_pages(const CopyPagesArgs &a, hipStream_t stream);
+
+// The best continuations of beams (hm_beam_select).
+struct BeamSelectArgs {
+    const void *logits;
+    int64_t ld;
+    int dtype; // hm_dtype, or HM_LOGITS_FP32
+    const float *scores;
+    const uint8_t *ended;
+    int32_t end_token;
+    int64_t rows;
+    int beams;
+    int64_t vocabulary;
+    int k;
+    int32_t *parents, *tokens;
+    float *scores_out;
+    uint8_t *ended_out;
+    void *workspace;
+    int parts; // waves of a row; set by the launch
+};
+size_t beam_select_workspace(int64_t rows, int64_t vocabulary, int64_t k, int dtype);
+hipError_t launch_beam_select(BeamSelectArgs a, hipStream_t stream);
+
+// What rows share (hm_share_plan).
+struct SharePlanArgs {
+    const int32_t *block_table;
+    int64_t ld_table, requests_count, width;
+    int page_shift;
+    const int32_t *positions, *requests;
+    int64_t rows;
+    int group_heads, kv_heads;
+    int64_t window;
+    int32_t *shared;
+    void *plan;
+    int tree_base; // set by the launch
+};
+size_t share_plan_workspace(int64_t rows);
+hipError_t launch_share_plan(SharePlanArgs a, hipStream_t stream);
+
+// Attention over shared pages (hm_shared_attention): hm_shared_attention.hpp.
+struct SharedAttentionArgs;
+size_t shared_attention_workspace(int64_t rows, int64_t q_heads, int64_t head_dim);
+hipError_t launch_shared_attention(SharedAttentionArgs a, hipStream_t stream);
+
 } // namespace hm

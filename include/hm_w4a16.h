@@ -443,6 +443,102 @@ hm_status hm_paged_attention(const hm_kv_cache *cache, void *out, int64_t ldo, c
                              void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Requests that branch over a paged cache: the beams of a search, several samples
+ * of one prompt, requests that begin with the same system prompt. They hold the
+ * pages that they have in common together. A page that several requests hold
+ * stands in the block table as the same block of each (its keys carry their
+ * positions), and only as long as it is full: a last page that is not full, into
+ * which hm_page_plan puts the next tokens, is one request's own. The calls here
+ * keep both. They find the holders in the table, so there is nothing to count and
+ * hm_page_plan works on such a table as it is, except that a request that shares
+ * pages ends by hm_page_fork (source -1): hm_page_plan would give pages back that
+ * others still hold. Nothing here waits for the host.
+ * ------------------------------------------------------------------------- */
+
+/* The k best continuations of each request's beams. Row i of logits [R * beams, V] (leading dimension ld, 2-byte elements or with HM_LOGITS_FP32 fp32; any
+ * alignment of an element) is beam i % beams of request i / beams. A continuation of row i by token t scores
+ *   scores[i] + logits[i, t] - log(sum over u of exp(logits[i, u])),
+ * and of a row that has ended (ended [R * beams], 0 or 1; NULL: none) there is one, by end_token, at scores[i]. Per request, best first, equal scores by
+ * the lower beam * V + token:
+ *   parents [R, k]    row that it continues (hm_page_fork's sources, where k = beams and a row is a request there)
+ *   tokens [R, k], scores_out [R, k]
+ *   ended_out [R, k]  1 if its row had ended or its token is end_token
+ * Logits of -infinity are no continuations, nor are those of a row whose score is not finite (-infinity: a beam that is not in use yet) or among whose
+ * logits are NaN or +infinity. Where fewer than k are left: parent and token -1, score -infinity, ended 1. Sums are fp32 over 32 logits and fp64 from there on, candidates
+ * of different rows are compared in fp64. end_token: -1 for none, if `ended` is NULL. beams up to HM_BEAM_MAX_BEAMS, k up to HM_BEAM_MAX_K. With k = beams,
+ * scores_out may be scores and ended_out may be ended; other arrays must not overlap. Workspace (16-byte aligned, nothing in it has to start at zero):
+ * hm_beam_select_workspace_bytes. */
+#define HM_LOGITS_FP32 2
+#define HM_BEAM_MAX_BEAMS 256
+#define HM_BEAM_MAX_K 64
+size_t hm_beam_select_workspace_bytes(int64_t R, int64_t beams, int64_t V, int64_t k, int32_t logits_dtype);
+hm_status hm_beam_select(const void *logits, int64_t ld, int32_t logits_dtype, const float *scores, const uint8_t *ended, int64_t end_token, int64_t R,
+                         int64_t beams, int64_t V, int64_t k, int32_t *parents, int32_t *tokens, float *scores_out, uint8_t *ended_out, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
+/* Requests become copies of others, or of their first tokens, all at once.
+ *   sources [R]       request r becomes what request sources[r] was before the call; r: it stays; negative: it ends
+ *   keep [R]          of which it keeps the first keep[r] tokens (not negative; more than there are: all); NULL: all
+ *   lengths [R]       tokens of each request; block_table [R, W] (ld_table) its pages, as for hm_page_plan
+ *   free_pages [Q], queue_in [4]: the ring of free pages and its counters, as for hm_page_plan
+ * Results:
+ *   table_out [R, W]  (ld_out) the pages after, ceil(lengths_out[r] / page_size) entries of each row; the others are left as they are
+ *   lengths_out [R]
+ *   copies [R, 3]     (source page, target page, tokens): what hm_copy_pages has to copy in each layer's cache, before anything else is written to
+ *                     it; entries behind the last are -1
+ *   queue_out [4]     {head, tail, 1 if the call was refused, fresh pages}
+ * Full pages are shared. A last page that is not full goes to one of the requests that end in it, unless another holds it in full: to the first that
+ * had it (sources[r] = r), else the first of all; each of the others gets a fresh page from the head of the ring, in the order of requests, and an entry of
+ * `copies`. Pages that nobody holds any more go behind the ring's tail, by blocks and then by the first request that held them.
+ * The call is refused as a whole, and all stays as it is, if a source is R or more, a keep is negative, a length lies outside 0..W * page_size, the ring holds
+ * too few pages, or has no room for those that come free next to those that are free now (Q of the pages that are free and held together is
+ * always enough). table_out may be block_table, lengths_out lengths and queue_out queue_in; other arrays must not overlap. Negative entries
+ * of the table are carried along. R up to HM_PAGE_PLAN_MAX_REQUESTS. Workspace (16-byte aligned, nothing in it has to start at zero): hm_page_fork_workspace_bytes. */
+size_t hm_page_fork_workspace_bytes(int64_t R, int64_t W);
+hm_status hm_page_fork(const int32_t *sources, const int32_t *keep, const int32_t *lengths, int64_t R, const int32_t *block_table, int64_t ld_table,
+                       int32_t *table_out, int64_t ld_out, int64_t W, int64_t page_size, int32_t *free_pages, int64_t Q, const int64_t *queue_in,
+                       int32_t *copies, int32_t *lengths_out, int64_t *queue_out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The pages that requests hold move to ids below `limit`, so that a cache of `pages` pages can be cut to its first `limit`, or grown to them:
+ * each held page at limit or above, in the order of ids, to the next id below that no request holds. The ring is made anew: from its head on, all ids below
+ * limit that are then not held, in order (entries outside 0..pages - 1 of the table are carried along).
+ *   copies [n, 3]     (source page, target page, page_size) of each move, -1 behind the last; n at least 1 and min(limit, pages - limit)
+ *   table_out [R, W]  the pages after, as for hm_page_fork; may be block_table
+ *   queue_out [4]     {head, tail, 1 if the call was refused, moves}; may be queue_in
+ * Refused as a whole, all as it is, if more than `limit` pages are held, or more are free below it than the ring has entries. */
+size_t hm_page_compact_workspace_bytes(int64_t pages);
+hm_status hm_page_compact(int64_t pages, int64_t limit, const int32_t *lengths, int64_t R, const int32_t *block_table, int64_t ld_table, int32_t *table_out,
+                          int64_t ld_out, int64_t W, int64_t page_size, int32_t *free_pages, int64_t Q, const int64_t *queue_in, int32_t *copies, int64_t n,
+                          int64_t *queue_out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Copies the first `tokens` tokens (at most page_size) of keys and values, all heads, for each (source page, target page, tokens) of copies [n, 3] in device
+ * memory, in each of `layers` caches: within `from`, or from there to the cache of the same number of `to` (NULL: from). Entries with a page outside
+ * the caches (negative ones) are passed over. A target must be neither a source nor twice a target. The caches are alike in heads, type and page size, those
+ * of `from` in pages and strides too, and those of `to`. */
+hm_status hm_copy_pages(const hm_kv_cache *from, const hm_kv_cache *to, int64_t layers, const int32_t *copies, int64_t n, void *stream);
+
+/* What neighbouring rows of a step share of their pages, once per step for hm_shared_attention of all layers. Rows, positions, requests and block_table
+ * [R, W] (ld_table) as for hm_paged_attention.
+ *   shared [rows]     leading tokens that row t reads from the same pages as row t - 1, 0 for the first: those of the blocks before the first
+ *                     whose entries differ, at most as many as the shorter of the two sees; 0 next to a row that has no request or position in the table
+ *   plan              hm_share_plan_bytes(rows) bytes, 16-byte aligned, for the calls of the same rows, heads, table and positions; not made for any call yet: zeros
+ * Rows that share pages should follow each other, those that share most next to each other. window: as for hm_paged_attention. rows up to HM_SHARE_MAX_ROWS,
+ * q_heads a multiple of kv_heads, up to 128 times; 5 * rows * kv_heads * (W * page_size / 64 + 2) below 2^31. */
+#define HM_SHARE_MAX_ROWS 4096
+size_t hm_share_plan_bytes(int64_t rows);
+hm_status hm_share_plan(const int32_t *block_table, int64_t ld_table, int64_t R, int64_t W, int64_t page_size, const int32_t *positions, const int32_t *requests,
+                        int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t window, int32_t *shared, void *plan, size_t plan_bytes, void *stream);
+
+/* hm_paged_attention where rows share pages: keys and values that a plan found to be shared are read once for all rows that share them, in up to three levels
+ * (a system prompt, under it prompts, under each its samples), in steps of 64 tokens. The result is that of hm_paged_attention with the plan's window. The
+ * plan is of a call of hm_share_plan with the same rows, heads, block_table, positions and requests; rows of one that is not come out as NaN or wrong,
+ * nothing outside the arrays is read. The workspace is hm_shared_attention_workspace_bytes, as there. */
+size_t hm_shared_attention_workspace_bytes(const hm_kv_cache *cache, int64_t q_heads, int64_t rows);
+hm_status hm_shared_attention(const hm_kv_cache *cache, void *out, int64_t ldo, const void *q, int64_t ldq, int64_t rows, int64_t q_heads,
+                              const int32_t *block_table, int64_t ld_table, int64_t R, int64_t W, const int32_t *positions, const int32_t *requests, float scale,
+                              const void *plan, size_t plan_bytes, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------
  * Nonfinite scan (the merged FFN's failure check).
  * ------------------------------------------------------------------------- */
 
