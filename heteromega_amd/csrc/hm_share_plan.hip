@@ -19,8 +19,6 @@ namespace hm {
 namespace {
 
 constexpr int kShareStep = 64; // tokens: less is not worth a part of its own
-constexpr int kPlanThreads = 1024;
-
 struct RowKeys {
     int32_t request, first, end; // end 0: none
 };
@@ -104,127 +102,140 @@ struct Depths {
         }
         return p - base;
     }
-    // The boundary that stands for the segment of boundary i's depth.
-    __device__ __forceinline__ int first_alike(int i) const { return nearest<false, true>(nearest<true, false>(i, at(i)), at(i)); }
 };
 
-// One workgroup.
-__global__ void __launch_bounds__(kPlanThreads) share_plan_kernel(SharePlanArgs a) {
+__device__ __forceinline__ Count count_of(const SharePlanArgs &a, const ShareSegment &s) {
+    if (s.tiles == 0) {
+        return Count{0, 0, 0, 0, 0};
+    }
+    return s.rows * a.group_heads <= kNarrowCols ? Count{1, s.tiles * a.kv_heads, 0, 0, s.rows} : Count{0, 0, 1, s.tiles * a.kv_heads * s.chunks(), s.rows};
+}
+
+__device__ __forceinline__ SharePath path_of(const ShareSegment &s, int line, int t) {
+    if (s.tiles == 0) {
+        return SharePath{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+    const int row = t - s.row0, chunk = row / s.chunk;
+    return SharePath{s.tiles, line, s.tile0 + chunk * s.tiles, s.chunks() * s.tiles, s.slot0, s.rows, row, row - chunk * s.chunk};
+}
+
+// One workgroup, of PER rows a thread at most.
+template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share_plan_kernel(SharePlanArgs a) {
     extern __shared__ int32_t lds[];
-    __shared__ Count waves[kPlanThreads / 64];
+    __shared__ Count waves[THREADS / 64];
+    constexpr int kDropped = kShareLevels;
     const int R = static_cast<int>(a.rows), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Depths depth{lds, a.tree_base};
-    int32_t *parent = lds + 2 * a.tree_base, *level = parent + R, *record = level + R, *lo = record + R;
-    const ShareWorkspace ws = carve_share(a.plan, a.rows);
+    int32_t *alike = lds + max(2 * a.tree_base, 3 * R), *parent = alike + R, *level = parent + R, *record = level + R, *lo = record + R;
+    const ShareWorkspace ws = carve_share(a.plan, a.rows, a.runs);
+    const auto row_of = [&](int j) { return j * THREADS + static_cast<int>(threadIdx.x); };
 
-    for (int i = threadIdx.x; i < a.tree_base; i += kPlanThreads) {
+    for (int i = threadIdx.x; i < a.tree_base; i += THREADS) {
         lds[a.tree_base + i] = i > 0 && i < R ? a.shared[i] / kShareStep : 0;
+    }
+    RowKeys keys[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int i = row_of(j);
+        keys[j] = i < R ? row_keys(a, i) : RowKeys{0, 0, 0};
+        if (i < R) {
+            record[i] = keys[j].first; // for the windows' beginnings, until it has its own use
+        }
     }
     __syncthreads();
     for (int n = a.tree_base >> 1; n > 0; n >>= 1) {
-        for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+        for (int i = threadIdx.x; i < n; i += THREADS) {
             lds[n + i] = min(lds[2 * (n + i)], lds[2 * (n + i) + 1]);
         }
         __syncthreads();
     }
-    // ---- the segments of boundaries: level -1: the boundary stands for none ----
-    for (int i = threadIdx.x; i < R; i += kPlanThreads) {
-        parent[i] = -1, level[i] = -1;
-        const int32_t v = depth.at(i);
-        if (v == 0 || depth.first_alike(i) != i) {
-            continue;
-        }
-        const int from = depth.nearest<true, false>(i, v), to = depth.nearest<false, false>(i, v);
-        const int32_t above = max(depth.at(from), depth.at(to));
-        parent[i] = above == 0 ? -1 : depth.first_alike(depth.at(from) == above ? from : to);
-        level[i] = 0;
-        int32_t begin = above * kShareStep;
-        if (a.window > 0) {
-            for (int t = from; t < to; ++t) {
-                begin = max(begin, (row_keys(a, t).first + 15) & ~15);
-            }
-        }
-        lo[i] = begin;
-    }
-    __syncthreads();
-    int32_t levels[HM_SHARE_MAX_ROWS / kPlanThreads];
+    // ---- the segments of boundaries ----
+    int from[PER], to[PER];
 #pragma unroll
-    for (int j = 0; j < HM_SHARE_MAX_ROWS / kPlanThreads; ++j) {
-        const int i = j * kPlanThreads + static_cast<int>(threadIdx.x);
-        levels[j] = -1;
-        if (i < R && level[i] == 0) {
-            levels[j] = 0;
-            for (int p = parent[i]; p >= 0 && levels[j] < kShareLevels; p = parent[p]) {
-                ++levels[j];
-            }
+    for (int j = 0; j < PER; ++j) {
+        const int i = row_of(j);
+        const int32_t v = i < R ? depth.at(i) : 0;
+        from[j] = to[j] = 0;
+        if (v > 0) {
+            from[j] = depth.nearest<true, false>(i, v), to[j] = depth.nearest<false, false>(i, v);
+            alike[i] = depth.nearest<false, true>(from[j], v); // the boundary that stands for the segment
         }
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < HM_SHARE_MAX_ROWS / kPlanThreads; ++j) {
-        const int i = j * kPlanThreads + static_cast<int>(threadIdx.x);
-        if (i < R) {
-            level[i] = levels[j];
+    for (int j = 0; j < PER; ++j) {
+        const int i = row_of(j);
+        if (i < R && depth.at(i) > 0 && alike[i] == i) {
+            const int32_t above = max(depth.at(from[j]), depth.at(to[j]));
+            parent[i] = above == 0 ? -1 : alike[depth.at(from[j]) == above ? from[j] : to[j]];
+            int32_t begin = above * kShareStep;
+            if (a.window > 0) {
+                for (int t = from[j]; t < to[j]; ++t) {
+                    begin = max(begin, (record[t] + 15) & ~15);
+                }
+            }
+            lo[i] = begin;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) { // the number of segments that each is within, or that there are too many
+        const int i = row_of(j);
+        if (i < R && depth.at(i) > 0 && alike[i] == i) {
+            int n = 0;
+            for (int p = parent[i]; p >= 0 && n < kDropped; p = parent[p]) {
+                ++n;
+            }
+            level[i] = n;
         }
     }
     __syncthreads();
 
-    // ---- segments: of rows, what their windows leave before the shared ones, and of boundaries ----
-    const auto shared_of = [&](int t) { // the innermost segment that row t is in, or -1
-        const int32_t before = depth.at(t), after = t + 1 < R ? depth.at(t + 1) : 0;
-        if (max(before, after) == 0) {
-            return -1;
+    // ---- segments of each row: its own, what its window leaves before the shared ones, and the boundary's before it ----
+    ShareSegment segments[PER][3];
+    int inner[PER]; // the innermost segment that the row is in, or -1
+    Count own{0, 0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int t = row_of(j);
+        inner[j] = -1;
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            segments[j][n] = ShareSegment{t, 1, 0, 0, 0, 0, 0, 1};
         }
-        int i = depth.first_alike(before >= after ? t : t + 1);
-        while (level[i] >= kShareLevels) {
-            i = parent[i];
-        }
-        return i;
-    };
-    const auto segment_of = [&](int e) {
-        ShareSegment s{0, 0, 0, 0, 0, 0, 0, 1};
-        if (e < 2 * R) {
-            const int t = e < R ? e : e - R;
-            const RowKeys k = row_keys(a, t);
-            s.row0 = t, s.rows = 1;
-            int i = shared_of(t);
+        if (t < R) {
+            const int32_t before = depth.at(t), after = t + 1 < R ? depth.at(t + 1) : 0;
+            if (max(before, after) > 0) {
+                inner[j] = alike[before >= after ? t : t + 1];
+                while (level[inner[j]] >= kDropped) {
+                    inner[j] = parent[inner[j]];
+                }
+            }
             int32_t covered = INT32_MAX; // the first key of a shared segment
-            const int32_t own = i >= 0 ? depth.at(i) * kShareStep : 0;
-            for (; i >= 0; i = parent[i]) {
+            for (int i = inner[j]; i >= 0; i = parent[i]) {
                 covered = lo[i] < depth.at(i) * kShareStep ? lo[i] : covered;
             }
-            if (e < R) {
-                s.lo = covered == INT32_MAX ? k.first : own, s.hi = k.end;
-            } else {
-                s.lo = k.first, s.hi = covered == INT32_MAX ? 0 : covered;
+            segments[j][0].lo = covered == INT32_MAX ? keys[j].first : depth.at(inner[j]) * kShareStep;
+            segments[j][0].hi = keys[j].end;
+            segments[j][1].lo = keys[j].first;
+            segments[j][1].hi = covered == INT32_MAX ? 0 : covered;
+            if (before > 0 && alike[t] == t && level[t] < kDropped) {
+                segments[j][2].row0 = from[j], segments[j][2].rows = to[j] - from[j];
+                segments[j][2].lo = lo[t], segments[j][2].hi = before * kShareStep;
             }
-        } else if (const int i = e - 2 * R; level[i] >= 0 && level[i] < kShareLevels) {
-            const int32_t v = depth.at(i);
-            s.row0 = depth.nearest<true, false>(i, v);
-            s.rows = depth.nearest<false, false>(i, v) - s.row0;
-            s.lo = lo[i], s.hi = v * kShareStep;
         }
-        const int columns = s.rows * a.group_heads;
-        const int tile = columns <= kNarrowCols ? kNarrowTile : kWideTile;
-        s.tiles = s.lo < s.hi ? (s.hi - s.start() + tile - 1) / tile : 0;
-        if (columns > kNarrowCols) {
-            const int most = kWideCols / a.group_heads, chunks = (s.rows + most - 1) / most;
-            s.chunk = (s.rows + chunks - 1) / chunks;
-        } else {
-            s.chunk = s.rows > 0 ? s.rows : 1;
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            ShareSegment &s = segments[j][n];
+            const int columns = s.rows * a.group_heads, tile = columns <= kNarrowCols ? kNarrowTile : kWideTile;
+            s.tiles = s.lo < s.hi ? (s.hi - s.start() + tile - 1) / tile : 0;
+            s.chunk = s.rows;
+            if (columns > kNarrowCols) {
+                const int most = kWideCols / a.group_heads, chunks = (s.rows + most - 1) / most;
+                s.chunk = (s.rows + chunks - 1) / chunks;
+            }
+            own = own + count_of(a, s);
         }
-        return s;
-    };
-    const auto count_of = [&](const ShareSegment &s) {
-        if (s.tiles == 0) {
-            return Count{0, 0, 0, 0, 0};
-        }
-        return s.rows * a.group_heads <= kNarrowCols ? Count{1, s.tiles * a.kv_heads, 0, 0, s.rows} : Count{0, 0, 1, s.tiles * a.kv_heads * s.chunks(), s.rows};
-    };
-    const int all = 3 * R, per = (all + kPlanThreads - 1) / kPlanThreads, e0 = static_cast<int>(threadIdx.x) * per, e1 = min(e0 + per, all);
-    Count own{0, 0, 0, 0, 0};
-    for (int e = e0; e < e1; ++e) {
-        own = own + count_of(segment_of(e));
     }
     Count upto = own;
 #pragma unroll
@@ -242,65 +253,102 @@ __global__ void __launch_bounds__(kPlanThreads) share_plan_kernel(SharePlanArgs 
     if (lane == 0) {
         at = Count{0, 0, 0, 0, 0};
     }
-    __syncthreads();
+    __syncthreads(); // the depths are not read any more either: the lines' first tiles take their place
     Count total{0, 0, 0, 0, 0};
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
         at = w < wave ? at + waves[w] : at;
         total = total + waves[w];
     }
     if (threadIdx.x == 0) {
-        *ws.header = ShareHeader{{{total.narrow, total.narrow_tiles}, {total.wide, total.wide_tiles}}, R, a.group_heads, a.kv_heads, 0};
+        *ws.header = ShareHeader{{total.narrow_tiles, total.wide_tiles}, R, a.group_heads, a.kv_heads, a.runs, {0, 0}};
     }
-    for (int e = e0; e < e1; ++e) {
-        ShareSegment s = segment_of(e);
-        int32_t place = -1;
-        if (s.tiles > 0) {
-            const bool wide = s.rows * a.group_heads > kNarrowCols;
-            s.tile0 = wide ? at.wide_tiles : at.narrow_tiles;
-            s.slot0 = at.slots;
-            (wide ? ws.wide : ws.narrow)[wide ? at.wide : at.narrow] = s;
-            place = wide ? 2 * at.wide + 1 : 2 * at.narrow;
-        }
-        at = at + count_of(s);
-        if (e < 2 * R) {
-            ws.paths[(e < R ? e : e - R) * kPathEntries + (e < R ? 0 : 1)] = place;
-        } else {
-            record[e - 2 * R] = place;
+    int32_t *tile0[2] = {lds, lds + total.narrow};
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int t = row_of(j);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            ShareSegment &s = segments[j][n];
+            const int line = s.rows * a.group_heads > kNarrowCols ? 1 : 0, place = line == 1 ? at.wide : at.narrow;
+            if (s.tiles > 0) {
+                s.tile0 = line == 1 ? at.wide_tiles : at.narrow_tiles;
+                s.slot0 = at.slots;
+                ws.segments[line][place] = s;
+                tile0[line][place] = s.tile0;
+                at = at + count_of(a, s);
+            }
+            if (n < 2 && t < R) {
+                ws.paths[t * kPathEntries + n] = path_of(s, line, t);
+            }
+            if (n == 2 && t < R) {
+                record[t] = s.tiles > 0 ? 2 * place + line : -1;
+            }
         }
     }
     __syncthreads();
-    for (int t = threadIdx.x; t < R; t += kPlanThreads) {
-        int i = shared_of(t);
-        for (int j = 2; j < kPathEntries; ++j) {
-            ws.paths[t * kPathEntries + j] = i >= 0 ? record[i] : -1;
-            i = i >= 0 ? parent[i] : -1;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int t = row_of(j);
+        if (t < R) {
+            int i = inner[j];
+            for (int n = 2; n < kPathEntries; ++n) {
+                SharePath p{0, 0, 0, 0, 0, 0, 0, 0};
+                if (i >= 0 && record[i] >= 0) {
+                    p = path_of(ws.segments[record[i] & 1][record[i] >> 1], record[i] & 1, t);
+                }
+                ws.paths[t * kPathEntries + n] = p;
+                i = i >= 0 ? parent[i] : -1;
+            }
         }
     }
+    // ---- where the runs begin ----
+    for (int i = threadIdx.x; i < (kAttentionWaves + 1) * a.runs; i += THREADS) {
+        const int line = i < kAttentionWaves * a.runs ? 0 : 1, w = line == 0 ? i : i - kAttentionWaves * a.runs;
+        const int count = line == 0 ? total.narrow : total.wide, tiles = line == 0 ? total.narrow_tiles : total.wide_tiles;
+        const int x = Runs::deal(tiles, runs_of(line, a.runs)).begin(w);
+        int first = 0, last = count - 1; // the last segment that begins at x or before it
+        while (first < last) {
+            const int mid = (first + last + 1) >> 1;
+            if (tile0[line][mid] <= x) {
+                first = mid;
+            } else {
+                last = mid - 1;
+            }
+        }
+        ws.starts[line][w] = first;
+    }
+}
+
+template <int THREADS, int PER> hipError_t launch_plan(const SharePlanArgs &a, hipStream_t stream) {
+    const size_t lds = 4 * (static_cast<size_t>(std::max<int64_t>(2 * a.tree_base, 3 * a.rows)) + 5 * static_cast<size_t>(a.rows));
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&share_plan_kernel<THREADS, PER>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                 static_cast<int>(lds));
+        if (e != hipSuccess) {
+            return e;
+        }
+    }
+    hipLaunchKernelGGL((share_plan_kernel<THREADS, PER>), dim3(1), dim3(THREADS), lds, stream, a);
+    return hipGetLastError();
 }
 
 } // namespace
 
-size_t share_plan_workspace(int64_t rows) { return static_cast<size_t>(share_plan_bytes(rows)); }
+size_t share_plan_workspace(int64_t rows) { return static_cast<size_t>(share_plan_bytes(rows, share_runs())); }
 
 hipError_t launch_share_plan(SharePlanArgs a, hipStream_t stream) {
+    a.runs = share_runs();
     a.tree_base = 2;
     while (a.tree_base < a.rows + 1) {
         a.tree_base *= 2;
-    }
-    const size_t lds = 4 * (2 * static_cast<size_t>(a.tree_base) + 4 * static_cast<size_t>(a.rows));
-    if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&share_plan_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
-        if (e != hipSuccess) {
-            return e;
-        }
     }
     hipLaunchKernelGGL(shared_tokens_kernel, dim3(static_cast<unsigned>((a.rows + 3) / 4)), dim3(256), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {
         return e;
     }
-    hipLaunchKernelGGL(share_plan_kernel, dim3(1), dim3(kPlanThreads), lds, stream, a);
-    return hipGetLastError();
+    return a.rows <= 256 ? launch_plan<256, 1>(a, stream) : a.rows <= 1024 ? launch_plan<1024, 1>(a, stream) : launch_plan<1024, HM_SHARE_MAX_ROWS / 1024>(a, stream);
 }
 
 } // namespace hm

@@ -10,22 +10,14 @@
 // the one and half with the other, so that reads and products overlap.
 #include "hm_shared_attention.hpp"
 
-#include <algorithm>
-
 namespace hm {
-namespace {
-
-int64_t workgroups(int64_t head_dim) { return (head_dim > 128 ? 1 : 2) * device_topology().cus; }
-
-} // namespace
-
 size_t shared_attention_workspace(int64_t rows, int64_t q_heads, int64_t head_dim) {
-    const int64_t columns = shared_columns(rows, q_heads, workgroups(head_dim));
+    const int64_t columns = shared_columns(rows, q_heads, share_runs());
     return static_cast<size_t>((columns + 1) / 2 * 2 * 8 + columns * head_dim * 4);
 }
 
 hipError_t launch_shared_attention(SharedAttentionArgs a, hipStream_t stream) {
-    a.runs = static_cast<int>(workgroups(a.head_dim));
+    a.runs = share_runs();
     return a.dtype == HM_FP16 ? launch_shared_attention_f16(a, stream) : launch_shared_attention_bf16(a, stream);
 }
 

@@ -6,10 +6,15 @@
 
 namespace hm {
 
-constexpr int kShareLevels = 3;                 // shared segments that a row may be in, one within the other
-constexpr int kPathEntries = kShareLevels + 2;  // of a row: its own keys, those that its window leaves before the shared ones, and the shared segments
-constexpr int kNarrowCols = 16, kNarrowTile = 128; // units of up to 16 columns: tiles of 32 keys per wave
-constexpr int kWideCols = 128, kWideTile = 64;     // units of more: 32 columns per wave, which share tiles of 64 keys
+constexpr int kShareLevels = 3;                // shared segments that a row may be in, one within the other
+constexpr int kPathEntries = kShareLevels + 2; // of a row: its own keys, those that its window leaves before the shared ones, and the shared segments
+constexpr int kNarrowCols = 16, kNarrowTile = 32; // units of up to 16 columns: a wave's, in tiles of 32 keys
+constexpr int kWideCols = 128, kWideTile = 64;    // units of more: a workgroup's, 32 columns per wave, in tiles of 64 keys
+
+// Runs of the two lines (below), narrow and wide: two workgroups per CU, with a wave each for the narrow line's. (With heads of 256 they follow each other.)
+inline int share_runs() { return 2 * device_topology().cus; }
+__host__ __device__ __forceinline__ int runs_of(int line, int runs) { return line == 0 ? kAttentionWaves * runs : runs; }
+__host__ __device__ __forceinline__ int cols_of(int line) { return line == 0 ? kNarrowCols : kWideCols; }
 
 // Rows [row0, row0 + rows) that see keys [lo, hi) in the same pages, as a place in one of two lines of tiles: those of narrow units, whose
 // rows x query heads of a key head are at most kNarrowCols columns, and of wide ones. A segment has a unit for each key head and, in turn, each `chunk`
@@ -23,33 +28,40 @@ struct ShareSegment {
     __host__ __device__ int chunks() const { return (rows + chunk - 1) / chunk; }
 };
 
-// What the segments of a line come to.
-struct ShareLine {
-    int32_t segments, tiles;
+// What a row has of a segment, for the join: its unit of key head 0 begins at `tile` of its line, and further ones per_head tiles behind; row: in the
+// segment, in_chunk: in the unit. tiles 0: nothing.
+struct SharePath {
+    int32_t tiles, line, tile, per_head;
+    int32_t slot0, rows, row, in_chunk;
 };
 
-// What a plan was made for: a call that does not fit it finds no segments.
+// What a plan was made for, and how many tiles its lines have: a call that does not fit it finds none.
 struct ShareHeader {
-    ShareLine lines[2]; // narrow, wide
-    int32_t rows, group_heads, kv_heads, spare;
+    int32_t tiles[2]; // narrow, wide
+    int32_t rows, group_heads, kv_heads, runs, spare[2];
+
+    __host__ __device__ bool fits(int64_t n, int group, int heads, int r) const { return rows == n && group_heads == group && kv_heads == heads && runs == r; }
 };
 
 // Memory of a plan. A line's segments are those with tiles, in the order of the line.
 struct ShareWorkspace {
     ShareHeader *header;
-    int32_t *paths;         // [rows][kPathEntries]: 2 * segment + line of the row's segments, -1: none
-    ShareSegment *narrow;   // [3 rows]
-    ShareSegment *wide;     // [3 rows]
+    ShareSegment *segments[2]; // [3 rows]: narrow, wide
+    SharePath *paths;          // [rows][kPathEntries]
+    int32_t *starts[2];        // [runs_of]: the segment that each run begins in
 };
 
-__host__ __device__ __forceinline__ int64_t share_plan_bytes(int64_t rows) {
-    return sizeof(ShareHeader) + (rows * kPathEntries * 4 + 31) / 32 * 32 + 6 * rows * static_cast<int64_t>(sizeof(ShareSegment));
+__host__ __device__ __forceinline__ int64_t share_plan_bytes(int64_t rows, int runs) {
+    return sizeof(ShareHeader) + 6 * rows * static_cast<int64_t>(sizeof(ShareSegment)) + rows * kPathEntries * static_cast<int64_t>(sizeof(SharePath)) +
+           (kAttentionWaves + 1) * static_cast<int64_t>(runs) * 4;
 }
 
-__host__ __device__ __forceinline__ ShareWorkspace carve_share(void *p, int64_t rows) {
-    uint8_t *b = static_cast<uint8_t *>(p);
-    ShareSegment *segments = reinterpret_cast<ShareSegment *>(b + sizeof(ShareHeader) + (rows * kPathEntries * 4 + 31) / 32 * 32);
-    return {reinterpret_cast<ShareHeader *>(b), reinterpret_cast<int32_t *>(b + sizeof(ShareHeader)), segments, segments + 3 * rows};
+__host__ __device__ __forceinline__ ShareWorkspace carve_share(void *p, int64_t rows, int runs) {
+    ShareHeader *header = static_cast<ShareHeader *>(p);
+    ShareSegment *segments = reinterpret_cast<ShareSegment *>(header + 1);
+    SharePath *paths = reinterpret_cast<SharePath *>(segments + 6 * rows);
+    int32_t *starts = reinterpret_cast<int32_t *>(paths + rows * kPathEntries);
+    return {header, {segments, segments + 3 * rows}, paths, {starts, starts + kAttentionWaves * runs}};
 }
 
 // The parts of units: a run of a line leaves at most one unit that it does not finish, whose part goes to the run's own columns; the parts that end a unit
@@ -59,8 +71,8 @@ struct SharedParts {
     float *o;      // [columns][D]
 };
 
-__host__ __device__ __forceinline__ int64_t shared_columns(int64_t rows, int64_t q_heads, int64_t runs) {
-    return rows * kPathEntries * q_heads + runs * (kNarrowCols + kWideCols);
+__host__ __device__ __forceinline__ int64_t shared_columns(int64_t rows, int64_t q_heads, int runs) {
+    return rows * kPathEntries * q_heads + static_cast<int64_t>(runs) * (kAttentionWaves * kNarrowCols + kWideCols);
 }
 
 __host__ __device__ __forceinline__ SharedParts carve_parts(void *p, int64_t columns) {
@@ -69,8 +81,8 @@ __host__ __device__ __forceinline__ SharedParts carve_parts(void *p, int64_t col
 }
 
 // First column of run w's unfinished unit in a line, behind the row slots'.
-__host__ __device__ __forceinline__ int64_t run_column(int64_t rows, int64_t q_heads, int64_t runs, int line, int64_t w) {
-    return rows * kPathEntries * q_heads + (line == 0 ? w * kNarrowCols : runs * kNarrowCols + w * kWideCols);
+__host__ __device__ __forceinline__ int64_t run_column(int64_t rows, int64_t q_heads, int runs, int line, int64_t w) {
+    return rows * kPathEntries * q_heads + (line == 0 ? w * kNarrowCols : static_cast<int64_t>(runs) * kAttentionWaves * kNarrowCols + w * kWideCols);
 }
 
 struct SharedAttentionArgs : PagedAttentionArgs {

@@ -8,30 +8,12 @@
 namespace hm {
 namespace {
 
-// The segment that tile x of a line lies in, found by 64 lanes at a time: the last one that begins at x or before it.
-__device__ __forceinline__ int segment_at(const ShareSegment *segments, int count, int x) {
-    const int lane = threadIdx.x & 63;
-    int from = 0;
-    while (count > 1) {
-        const int step = (count + 63) / 64, at = lane * step;
-        const uint64_t who = __ballot(at < count && segments[from + min(at, count - 1)].tile0 <= x); // lane 0's always does
-        const int last = 63 - static_cast<int>(__builtin_clzll(who | 1));
-        from += last * step;
-        count = min(step, count - last * step);
-    }
-    return uniform(from);
-}
-
 __device__ __forceinline__ ShareSegment uniform_segment(const ShareSegment *p) {
     const ShareSegment s = *p;
     return {uniform(s.row0), uniform(s.rows), uniform(s.lo), uniform(s.hi), uniform(s.tile0), uniform(s.tiles), uniform(s.slot0), uniform(s.chunk)};
 }
 
-__device__ __forceinline__ bool fits(const ShareWorkspace &plan, const SharedAttentionArgs &a) {
-    return plan.header->rows == static_cast<int32_t>(a.rows) && plan.header->group_heads == a.group_heads && plan.header->kv_heads == a.kv_heads;
-}
-
-// A unit's tiles [tile0, tile1) as a workgroup works on them.
+// A unit's tiles [tile0, tile1).
 struct Work {
     ShareSegment s;
     int kv_head, row, rows; // row: first, behind the segment's
@@ -87,17 +69,17 @@ struct Pages {
     }
 };
 
-// A unit of up to 16 columns: each of the four waves takes 32 keys of a tile, and the waves join over LDS.
-template <class T, int D> __device__ __forceinline__ void narrow_work(const SharedAttentionArgs &a, const Work &k, uint8_t *lds, float2 (&wave_stats)[kAttentionWaves][16]) {
+// A unit of up to 16 columns, by one wave, 32 keys at a time: with up to 128 units on a CU one after the other, waves go on to their next by themselves.
+template <class T, int D> __device__ __forceinline__ void narrow_work(const SharedAttentionArgs &a, const Work &k, uint8_t *lds) {
     using S = Shape<T, D>;
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
     const int col = lane & 15, quad = lane >> 4;
     const int columns = k.rows * a.group_heads, start = k.s.start(), lo = k.s.lo, hi = k.s.hi;
     const Pages at(a, k.s.row0, k.kv_head);
     const Pieces<D> pieces(lane, at.row_bytes);
-    const uint32_t to_lds = wave * S::kRegion + pieces.lds_offset();
-    const uint32_t k_lds = wave * S::kRegion + col * S::kRowBytes + quad * 16;
-    const uint32_t v_lds = wave * S::kRegion + (4 * quad + (col >> 2)) * S::kRowBytes + (col & 3) * 8;
+    const uint32_t to_lds = pieces.lds_offset();
+    const uint32_t k_lds = col * S::kRowBytes + quad * 16;
+    const uint32_t v_lds = (4 * quad + (col >> 2)) * S::kRowBytes + (col & 3) * 8;
     const float c_scale = a.scale * 1.4426950408889634f;
 
     u32x4_t q[S::kSteps];
@@ -121,14 +103,14 @@ template <class T, int D> __device__ __forceinline__ void narrow_work(const Shar
     const auto page_ids = [&](int tile) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const int key = start + tile * kNarrowTile + wave * kWaveKeys + 16 * s;
+            const int key = start + tile * kNarrowTile + 16 * s;
             id[s] = at.page_of(key, hi);
         }
     };
     const auto request = [&](int tile) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const int key = start + tile * kNarrowTile + wave * kWaveKeys + 16 * s;
+            const int key = start + tile * kNarrowTile + 16 * s;
             const int32_t page = uniform(id[s]);
             int seen = max(0, min(16, hi - key));
             if (static_cast<uint32_t>(page) >= at.pages) {
@@ -152,10 +134,7 @@ template <class T, int D> __device__ __forceinline__ void narrow_work(const Shar
     request(k.tile0);
     page_ids(min(k.tile0 + 1, k.tile1 - 1));
     for (int tile = k.tile0; tile < k.tile1; ++tile) {
-        const int key0 = start + tile * kNarrowTile + wave * kWaveKeys;
-        if (key0 >= hi) {
-            break; // only the segment's last tile has waves without keys
-        }
+        const int key0 = start + tile * kNarrowTile;
         if (key0 < lo) { // values before the first key count as zero, whatever they are
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
@@ -200,7 +179,7 @@ template <class T, int D> __device__ __forceinline__ void narrow_work(const Shar
         for (int e = 0; e < 8; ++e) {
             p[e] = score[e >> 2][e & 3] * c_scale;
         }
-        if (key0 < lo || key0 + kWaveKeys > hi) {
+        if (key0 < lo || key0 + kNarrowTile > hi) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int key = key0 + 16 * (e >> 2) + 4 * quad + (e & 3);
@@ -246,60 +225,47 @@ template <class T, int D> __device__ __forceinline__ void narrow_work(const Shar
         }
     }
 
-    // ---- the waves' parts joined ----
     const SharedParts parts = carve_parts(a.workspace, shared_columns(a.rows, a.q_heads, a.runs));
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (poisoned) {
-        l = NAN;
-    }
-    if (quad == 0) {
-        wave_stats[wave][col] = make_float2(m, l);
-    }
-    __syncthreads();
-    {
-        float top = -INFINITY;
+    if (live) {
 #pragma unroll
-        for (int i = 0; i < kAttentionWaves; ++i) {
-            top = fmaxf(top, wave_stats[i][col].x);
+        for (int i = 0; i < S::kDTiles; ++i) {
+            *reinterpret_cast<float4_t *>(parts.o + (k.part + col) * D + 16 * i + 4 * quad) = o[i];
         }
-        const float f = top == -INFINITY ? 0.0f : exp2_fast(m - top);
-        float *mine = reinterpret_cast<float *>(lds + wave * S::kRegion);
-        if (live) {
-#pragma unroll
-            for (int i = 0; i < S::kDTiles; ++i) {
-                *reinterpret_cast<float4_t *>(mine + col * S::kORow + 16 * i + 4 * quad) = o[i] * f;
-            }
+        if (quad == 0) {
+            parts.stats[k.part + col] = make_float2(m, poisoned ? NAN : l);
         }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < columns * (D / 4); i += kThreads) {
-        const int j = i / (D / 4), d = (i - j * (D / 4)) * 4;
-        float top = -INFINITY, sum = 0.0f;
-        float4_t v = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < kAttentionWaves; ++w) {
-            top = fmaxf(top, wave_stats[w][j].x);
-        }
-#pragma unroll
-        for (int w = 0; w < kAttentionWaves; ++w) {
-            const float2 st = wave_stats[w][j];
-            sum += st.y * (top == -INFINITY ? 1.0f : exp2_fast(st.x - top));
-            v += *reinterpret_cast<const float4_t *>(reinterpret_cast<const float *>(lds + w * S::kRegion) + j * S::kORow + d);
-        }
-        *reinterpret_cast<float4_t *>(parts.o + (k.part + j) * D + d) = v;
-        if (d == 0) {
-            parts.stats[k.part + j] = make_float2(top, sum);
-        }
-    }
-    __syncthreads(); // the next unit takes the regions
 }
+
+// Two weights, each as an upper half cut off below it and a lower one that is rounded: less work than split(), for products that bound the time. The lower half has
+// 2^-23 of the weight too much, so that it is positive even where the upper one is exact: an infinite value then gives an infinite output.
+template <class T> struct Halves;
+template <> struct Halves<BF16> {
+    static __device__ __forceinline__ void split(float2_t p, uint32_t &upper, uint32_t &lower) {
+        const uint32_t p0 = __float_as_uint(p[0]), p1 = __float_as_uint(p[1]);
+        upper = __builtin_amdgcn_perm(p1, p0, 0x07060302u);
+        const float2_t rest{__builtin_fmaf(p[0], 1.0f + 0x1p-23f, -__uint_as_float(p0 & 0xFFFF0000u)),
+                            __builtin_fmaf(p[1], 1.0f + 0x1p-23f, -__uint_as_float(p1 & 0xFFFF0000u))};
+        lower = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, Split<BF16>::pair_t));
+    }
+};
+template <> struct Halves<F16> {
+    static __device__ __forceinline__ void split(float2_t p, uint32_t &upper, uint32_t &lower) {
+        const Split<F16>::pair_t cut = __builtin_bit_cast(Split<F16>::pair_t, __builtin_amdgcn_cvt_pkrtz(p[0], p[1]));
+        upper = __builtin_bit_cast(uint32_t, cut);
+        const float2_t rest{__builtin_fmaf(p[0], 1.0f + 0x1p-23f, -static_cast<float>(cut[0])), __builtin_fmaf(p[1], 1.0f + 0x1p-23f, -static_cast<float>(cut[1]))};
+        lower = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, Split<F16>::pair_t));
+    }
+};
 
 // A unit of more columns: 16 CT of each wave, up to 128 in all; the waves share tiles of 64 keys, of which each brings a quarter into LDS. Two buffers, one
 // barrier a tile.
 template <class T, int D, int CT> __device__ __forceinline__ void wide_work(const SharedAttentionArgs &a, const Work &k, uint8_t *lds) {
     using S = Shape<T, D>;
     constexpr int kTileBytes = kWideTile * S::kRowBytes; // of keys, or values
+    constexpr int kSubs = kWideTile / 16;
     // The maximum follows only when a score passes it by more than a factor 2^kSlack, and is one of the scores before their factor
     // (hm_paged_attention_prompt.hpp).
     constexpr float kSlack = 3.0f, kTop = Split<T>::kTop - (Split<T>::kTop > 0.0f ? kSlack : 0.0f);
@@ -392,67 +358,82 @@ template <class T, int D, int CT> __device__ __forceinline__ void wide_work(cons
         if (!works) {
             continue;
         }
-        const bool some_masked = key0 < lo || key0 + kWideTile > hi;
+        float4_t score[CT][kSubs];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+#pragma unroll
+            for (int s = 0; s < kSubs; ++s) {
+                score[c][s] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < S::kSteps; ++i) {
+#pragma unroll
+            for (int s = 0; s < kSubs; ++s) {
+                const uint4 kk = *reinterpret_cast<const uint4 *>(k_tile + k_lds + s * 16 * S::kRowBytes + 64 * i);
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    score[c][s] = T::mfma16(kk, __builtin_bit_cast(uint4, q[c][i]), score[c][s]);
+                }
+            }
+        }
+        if (key0 < lo || key0 + kWideTile > hi) {
+            __builtin_amdgcn_sched_barrier(0); // keeps this a branch
+#pragma unroll
+            for (int e = 0; e < 4 * kSubs; ++e) {
+                const int key = key0 + 16 * (e >> 2) + 4 * quad + (e & 3);
+                if (key < lo || key >= hi) {
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) {
+                        score[c][e >> 2][e & 3] = -INFINITY;
+                    }
+                }
+            }
+        }
+        float top[CT];
+        bool follow = false;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            top[c] = score[c][0][0];
+#pragma unroll
+            for (int e = 1; e < 4 * kSubs; ++e) {
+                top[c] = fmaxf(top[c], score[c][e >> 2][e & 3]);
+            }
+            follow |= top[c] > m[c] + slack;
+        }
+        if (__any(follow)) {
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                top[c] = fmaxf(top[c], __shfl_xor(top[c], 16));
+                top[c] = fmaxf(top[c], __shfl_xor(top[c], 32));
+                const float m_new = fmaxf(m[c], top[c]);
+                const float f = m_new == -INFINITY ? 1.0f : exp2_fast((m[c] - m_new) * c_scale);
+                m[c] = m_new;
+                l[c] *= f;
+#pragma unroll
+                for (int i = 0; i < S::kDTiles; ++i) {
+                    o[c][i] *= f;
+                }
+            }
+        }
+        // One straight piece from here on, so that the second half's weights are worked out beside the first half's products.
 #pragma unroll
         for (int h = 0; h < 2; ++h) { // 32 keys at a time
             const uint32_t half_lds = h * 32 * S::kRowBytes;
-            float4_t score[CT][2];
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                score[c][0] = score[c][1] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            }
-#pragma unroll
-            for (int i = 0; i < S::kSteps; ++i) {
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const uint4 kk = *reinterpret_cast<const uint4 *>(k_tile + k_lds + half_lds + s * 16 * S::kRowBytes + 64 * i);
-#pragma unroll
-                    for (int c = 0; c < CT; ++c) {
-                        score[c][s] = T::mfma16(kk, __builtin_bit_cast(uint4, q[c][i]), score[c][s]);
-                    }
-                }
-            }
             u32x4_t upper[CT], lower[CT];
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
-                if (some_masked) {
-                    __builtin_amdgcn_sched_barrier(0); // keeps this a branch
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int key = key0 + 32 * h + 16 * (e >> 2) + 4 * quad + (e & 3);
-                        if (key < lo || key >= hi) {
-                            score[c][e >> 2][e & 3] = -INFINITY;
-                        }
-                    }
-                }
-                float top = score[c][0][0];
-#pragma unroll
-                for (int e = 1; e < 8; ++e) {
-                    top = fmaxf(top, score[c][e >> 2][e & 3]);
-                }
-                if (__any(top > m[c] + slack)) {
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    const float m_new = fmaxf(m[c], top);
-                    const float f = m_new == -INFINITY ? 1.0f : exp2_fast((m[c] - m_new) * c_scale);
-                    m[c] = m_new;
-                    l[c] *= f;
-#pragma unroll
-                    for (int i = 0; i < S::kDTiles; ++i) {
-                        o[c][i] *= f;
-                    }
-                }
                 const float m_used = m[c] == -INFINITY ? 0.0f : m[c];
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
                     float2_t p;
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
-                        p[n] = exp2_fast(__builtin_fmaf(score[c][e >> 2][(e & 3) + n] - m_used, c_scale, kTop));
+                        p[n] = exp2_fast(__builtin_fmaf(score[c][2 * h + (e >> 2)][(e & 3) + n] - m_used, c_scale, kTop));
                         l[c] += p[n];
                     }
                     uint32_t u, v;
-                    split<T>(p, u, v);
+                    Halves<T>::split(p, u, v);
                     upper[c][e / 2] = u, lower[c][e / 2] = v;
                 }
             }
@@ -493,102 +474,104 @@ template <class T, int D, int CT> __device__ __forceinline__ void wide_work(cons
     __syncthreads(); // the next unit takes the buffers
 }
 
-// A run of each line per workgroup. Half of the workgroups begin with the wide line, which the matrix cores bound, half with the
-// narrow one, which the memory bounds.
+// A run of the wide line per workgroup and one of the narrow line per wave. Half of the workgroups begin with the wide line, which the matrix cores bound,
+// half with the narrow one, which the memory bounds.
 template <class T, int D> __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) shared_attention_kernel(SharedAttentionArgs a) {
     using S = Shape<T, D>;
     constexpr int kNarrowBytes = kAttentionWaves * S::kRegion, kWideBytes = 4 * kWideTile * S::kRowBytes;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kNarrowBytes > kWideBytes ? kNarrowBytes : kWideBytes];
-    __shared__ float2 wave_stats[kAttentionWaves][16];
-    const ShareWorkspace plan = carve_share(a.plan, a.rows);
-    if (!fits(plan, a)) {
+    const ShareWorkspace plan = carve_share(a.plan, a.rows, a.runs);
+    const int wave = uniform(threadIdx.x >> 6);
+    const int wide_start = plan.starts[1][blockIdx.x], narrow_start = plan.starts[0][blockIdx.x * kAttentionWaves + wave];
+    const ShareHeader header = *plan.header;
+    if (!header.fits(a.rows, a.group_heads, a.kv_heads, a.runs)) {
         return;
     }
-    const int w = blockIdx.x;
-    const bool wide_first = 2 * w < a.runs;
+    const bool wide_first = 2 * static_cast<int>(blockIdx.x) < a.runs;
 #pragma unroll 1
     for (int turn = 0; turn < 2; ++turn) {
-        const int line = (turn == 0) == wide_first ? 1 : 0;
-        const ShareLine all{uniform(plan.header->lines[line].segments), uniform(plan.header->lines[line].tiles)};
-        const Runs runs = Runs::deal(all.tiles, a.runs);
-        int x = runs.begin(w);
-        const int x_end = runs.begin(w + 1);
-        if (x >= x_end) {
-            continue;
-        }
-        const ShareSegment *segments = line == 1 ? plan.wide : plan.narrow;
-        int at = segment_at(segments, all.segments, x);
-        while (x < x_end) {
-            if (line == 0) {
-                narrow_work<T, D>(a, next_work<0>(a, segments, at, x, x_end, w), lds, wave_stats);
-            } else {
-                const Work k = next_work<1>(a, segments, at, x, x_end, w);
+        if ((turn == 0) == wide_first) {
+            const Runs runs = Runs::deal(uniform(header.tiles[1]), a.runs);
+            const int w = blockIdx.x, x_end = runs.begin(w + 1);
+            int x = runs.begin(w), at = uniform(wide_start);
+            if (x < x_end && turn == 1) {
+                __syncthreads(); // the narrow units' regions are free
+            }
+            while (x < x_end) {
+                const Work k = next_work<1>(a, plan.segments[1], at, x, x_end, w);
                 if (k.rows * a.group_heads > 64) {
                     wide_work<T, D, 2>(a, k, lds);
                 } else {
                     wide_work<T, D, 1>(a, k, lds);
                 }
             }
+        } else {
+            const Runs runs = Runs::deal(uniform(header.tiles[0]), kAttentionWaves * a.runs);
+            const int w = blockIdx.x * kAttentionWaves + wave, x_end = runs.begin(w + 1);
+            int x = runs.begin(w), at = uniform(narrow_start);
+            while (x < x_end) {
+                narrow_work<T, D>(a, next_work<0>(a, plan.segments[0], at, x, x_end, w), lds + wave * S::kRegion);
+            }
         }
     }
 }
 
-// A column's parts joined: those of the segments on its row's path, each of the runs that its unit lies in.
-template <class T, int D, int THREADS> __global__ void __launch_bounds__(THREADS) shared_join_kernel(SharedAttentionArgs a) {
-    constexpr int kItems = D / 4, kLanes = THREADS / kItems, kAhead = 4;
-    struct Span { // the parts of one unit: of runs first..last, that of the last at `end`
-        int64_t run0, end;
-        int count;
-    };
-    __shared__ Span spans[kPathEntries];
-    __shared__ float4_t acc[kLanes][kItems];
-    __shared__ float2 stat[kLanes];
-    const int64_t t = blockIdx.x / a.q_heads;
-    const int head = static_cast<int>(blockIdx.x - t * a.q_heads);
+// Columns joined, by THREADS threads each: the parts of the segments on the row's path, each of the runs that its unit lies in.
+template <class T, int D, int THREADS> __global__ void __launch_bounds__(256) shared_join_kernel(SharedAttentionArgs a) {
+    constexpr int kItems = D / 4, kLanes = THREADS / kItems, kAhead = 4, kColumns = 256 / THREADS;
+    __shared__ float4_t acc[kColumns][kLanes][kItems];
+    __shared__ float2 stat[kColumns][kLanes];
+    const int mine = THREADS == 64 ? uniform(threadIdx.x >> 6) : 0, thread = threadIdx.x % THREADS;
+    const uint32_t column = blockIdx.x * kColumns + mine; // rows and heads are below 2^12 and 2^17
+    const int64_t t = column / static_cast<uint32_t>(a.q_heads);
+    if (t >= a.rows) {
+        return;
+    }
+    const int head = static_cast<int>(column - static_cast<uint32_t>(t) * a.q_heads), kv_head = head / a.group_heads, in_group = head - kv_head * a.group_heads;
+    const ShareWorkspace plan = carve_share(a.plan, a.rows, a.runs);
+    const ShareHeader header = *plan.header;
+    const int lane = threadIdx.x & 63;
+    const SharePath p = plan.paths[t * kPathEntries + min(lane, kPathEntries - 1)];
     const Keys keys = keys_of(a, t);
     if (keys.request < 0) {
         return;
     }
-    uint16_t *out = a.out + t * a.ldo + static_cast<int64_t>(head) * D;
-    const ShareWorkspace plan = carve_share(a.plan, a.rows);
-    const SharedParts parts = carve_parts(a.workspace, shared_columns(a.rows, a.q_heads, a.runs));
-    if (threadIdx.x < kPathEntries) {
-        const int ref = fits(plan, a) ? plan.paths[t * kPathEntries + threadIdx.x] : -1;
-        Span span{0, 0, 0};
-        if (ref >= 0) {
-            const int line = ref & 1;
-            const ShareSegment s = (line ? plan.wide : plan.narrow)[ref >> 1];
-            const Runs runs = Runs::deal(plan.header->lines[line].tiles, a.runs);
-            const int kv_head = head / a.group_heads, row = static_cast<int>(t) - s.row0, chunks = s.chunks(), chunk = row / s.chunk;
-            const int tile = s.tile0 + (kv_head * chunks + chunk) * s.tiles;
-            const int w0 = runs.of(tile), w1 = runs.of(tile + s.tiles - 1);
-            const int in_unit = (row - chunk * s.chunk) * a.group_heads + head - kv_head * a.group_heads;
-            span.run0 = run_column(a.rows, a.q_heads, a.runs, line, w0) + in_unit;
-            span.end = static_cast<int64_t>(s.slot0) * a.q_heads + (static_cast<int64_t>(kv_head) * s.rows + row) * a.group_heads + head - kv_head * a.group_heads;
-            span.count = (w1 - w0 + 1) * 2 + line;
-        }
-        spans[threadIdx.x] = span;
+    // The parts of each segment's unit, a lane each: of runs w0, w0 + 1 and so on, the last one at `end`.
+    int own_count = 0;
+    int64_t own_first = 0, own_end = 0;
+    if (lane < kPathEntries && p.tiles > 0 && header.fits(a.rows, a.group_heads, a.kv_heads, a.runs)) {
+        const Runs runs = Runs::deal(p.line == 0 ? header.tiles[0] : header.tiles[1], runs_of(p.line, a.runs));
+        const int tile = p.tile + kv_head * p.per_head, w0 = runs.of(tile);
+        own_count = runs.of(tile + p.tiles - 1) - w0 + 1;
+        own_first = run_column(a.rows, a.q_heads, a.runs, p.line, w0) + p.in_chunk * a.group_heads + in_group;
+        own_end = static_cast<int64_t>(p.slot0) * a.q_heads + (static_cast<int64_t>(kv_head) * p.rows + p.row) * a.group_heads + in_group;
     }
-    __syncthreads();
-    int total = 0;
+    const auto of64 = [](int64_t v, int i) {
+        const uint32_t low = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), i), high = __builtin_amdgcn_readlane(static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32), i);
+        return static_cast<int64_t>(static_cast<uint64_t>(high) << 32 | low);
+    };
+    int count[kPathEntries], step[kPathEntries], total = 0;
+    int64_t first[kPathEntries], end[kPathEntries];
 #pragma unroll
     for (int i = 0; i < kPathEntries; ++i) {
-        total += spans[i].count >> 1;
+        count[i] = __builtin_amdgcn_readlane(own_count, i);
+        step[i] = cols_of(__builtin_amdgcn_readlane(p.line, i));
+        first[i] = of64(own_first, i), end[i] = of64(own_end, i);
+        total += count[i];
     }
-    const auto column_of = [&](int p) {
-        int64_t column = 0;
+    const auto column_of = [&](int part) {
+        int64_t at = 0;
 #pragma unroll
         for (int i = 0; i < kPathEntries; ++i) {
-            const Span &s = spans[i];
-            const int n = s.count >> 1;
-            if (p >= 0 && p < n) {
-                column = p == n - 1 ? s.end : s.run0 + p * ((s.count & 1) ? kWideCols : kNarrowCols);
+            if (part >= 0 && part < count[i]) {
+                at = part == count[i] - 1 ? end[i] : first[i] + part * step[i];
             }
-            p -= n;
+            part -= count[i];
         }
-        return column;
+        return at;
     };
-    const int y = threadIdx.x / kItems, e = threadIdx.x - y * kItems;
+    const SharedParts parts = carve_parts(a.workspace, shared_columns(a.rows, a.q_heads, a.runs));
+    const int y = thread / kItems, e = thread - y * kItems;
     float m = -INFINITY, l = 0.0f;
     float4_t v = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
     if (y < kLanes) {
@@ -598,9 +581,9 @@ template <class T, int D, int THREADS> __global__ void __launch_bounds__(THREADS
             float top = m;
 #pragma unroll
             for (int n = 0; n < kAhead; ++n) {
-                const int64_t column = column_of(min(i + n * kLanes, total - 1));
-                st[n] = parts.stats[column];
-                o[n] = *reinterpret_cast<const float4_t *>(parts.o + column * D + 4 * e);
+                const int64_t from = column_of(min(i + n * kLanes, total - 1));
+                st[n] = parts.stats[from];
+                o[n] = *reinterpret_cast<const float4_t *>(parts.o + from * D + 4 * e);
             }
 #pragma unroll
             for (int n = 0; n < kAhead; ++n) {
@@ -620,27 +603,31 @@ template <class T, int D, int THREADS> __global__ void __launch_bounds__(THREADS
             }
             m = top;
         }
-        acc[y][e] = v;
+        acc[mine][y][e] = v;
         if (e == 0) {
-            stat[y] = make_float2(m, l);
+            stat[mine][y] = make_float2(m, l);
         }
     }
-    __syncthreads();
+    if constexpr (THREADS > 64) {
+        __syncthreads();
+    } else {
+        __builtin_amdgcn_wave_barrier(); // a wave's LDS accesses are carried out in order
+    }
     if (y == 0) {
         float top = -INFINITY, sum = 0.0f;
         float4_t all = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < kLanes; ++i) {
-            top = fmaxf(top, stat[i].x);
+            top = fmaxf(top, stat[mine][i].x);
         }
 #pragma unroll
         for (int i = 0; i < kLanes; ++i) {
-            const float f = exp2_fast(stat[i].x - (top == -INFINITY ? 0.0f : top));
-            all += acc[i][e] * f;
-            sum += stat[i].y * f;
+            const float f = exp2_fast(stat[mine][i].x - (top == -INFINITY ? 0.0f : top));
+            all += acc[mine][i][e] * f;
+            sum += stat[mine][i].y * f;
         }
         const float over = keys.bad ? NAN : keys.end == 0 ? 1.0f : sum; // a row that sees no key is zero
-        store4<T>(out + 4 * e, all / over);
+        store4<T>(a.out + t * a.ldo + static_cast<int64_t>(head) * D + 4 * e, all / over);
     }
 }
 
@@ -650,7 +637,13 @@ template <class T, int D> hipError_t launch_shared(const SharedAttentionArgs &a,
     if (e != hipSuccess) {
         return e;
     }
-    hipLaunchKernelGGL((shared_join_kernel<T, D, 256>), dim3(static_cast<unsigned>(a.rows * a.q_heads)), dim3(256), 0, stream, a);
+    // A wave per column where there are enough columns for the card.
+    const int64_t columns = a.rows * a.q_heads;
+    if (D == 256 || columns <= 2 * a.runs) {
+        hipLaunchKernelGGL((shared_join_kernel<T, D, 256>), dim3(static_cast<unsigned>(columns)), dim3(256), 0, stream, a);
+    } else {
+        hipLaunchKernelGGL((shared_join_kernel<T, D, D == 256 ? 256 : 64>), dim3(static_cast<unsigned>((columns + 3) / 4)), dim3(256), 0, stream, a);
+    }
     return hipGetLastError();
 }
 

@@ -33,53 +33,69 @@ def as_table(rows, width, ids=None):
 
 
 def decode(share):
-    """(segments of the narrow and the wide line, paths) of a plan, from its memory."""
+    """(segments of the narrow and the wide line, their tiles, paths [rows, 5, 8], where the runs begin) of a plan, from its memory."""
     raw = share._plan
-    skip = (-raw.data_ptr()) % 256
-    words = raw[skip:skip + raw.numel() // 256 * 256 - 256 if skip else raw.numel() // 4 * 4].cpu().numpy()
+    words = raw[(-raw.data_ptr()) % 256:].cpu().numpy()
     words = words[:len(words) // 4 * 4].view(np.int32)
-    rows = share.rows
-    head = words[:8]
-    paths = words[8:8 + 5 * rows].reshape(rows, 5)
-    at = 8 + -(-5 * rows * 4 // 32) * 8
-    lines = words[at:at + 48 * rows].reshape(2, 3 * rows, 8)
-    assert head[4:7].tolist() == [rows, share.q_heads // share.kv_heads, share.kv_heads]
-    return [lines[i, :head[2 * i]] for i in range(2)], [int(head[1]), int(head[3])], paths
+    rows, head = share.rows, words[:8]
+    assert head[2:5].tolist() == [rows, share.q_heads // share.kv_heads, share.kv_heads]
+    lines = words[8:8 + 48 * rows].reshape(2, 3 * rows, 8)
+    paths = words[8 + 48 * rows:8 + 88 * rows].reshape(rows, 5, 8)
+    runs = int(head[5])
+    starts = words[8 + 88 * rows:8 + 88 * rows + 5 * runs]
+    counts = []
+    for i in range(2):  # as many as have the line's tiles
+        at = n = 0
+        while at < head[i]:
+            at += int(lines[i, n, 5]) * share.kv_heads * -(-int(lines[i, n, 1]) // int(lines[i, n, 7]))
+            n += 1
+        counts.append(n)
+    return [lines[i, :counts[i]] for i in range(2)], head[:2].tolist(), paths, [starts[:4 * runs], starts[4 * runs:]]
 
 
 def check_plan(share, table, positions, requests, ps):
-    lines, tiles, paths = decode(share)
+    lines, tiles, paths, starts = decode(share)
     group, window = share.q_heads // share.kv_heads, share.window
-    slots = []
+    slots, begins = [], []
     for i, line in enumerate(lines):
-        at = 0
+        at, begin = 0, []
         for row0, rows, lo, hi, tile0, n, slot0, chunk in line.tolist():
             assert 0 <= row0 and rows > 0 and row0 + rows <= share.rows and 0 <= lo < hi and tile0 == at
-            assert (rows * group > 16) == (i == 1) and n == -(-(hi - lo // 16 * 16) // (64 if i else 128))
+            assert (rows * group > 16) == (i == 1) and n == -(-(hi - lo // 16 * 16) // (64 if i else 32))
             assert rows == 1 or lo % 16 == 0
             assert chunk >= 1 and (chunk * group <= 128 if i else chunk == rows)
+            begin.append(at)
             at += n * share.kv_heads * -(-rows // chunk)
             for u in range(row0 + 1, row0 + rows):  # all rows have these pages
                 q, r = (u, row0) if requests is None else (int(requests[u]), int(requests[row0]))
                 np.testing.assert_array_equal(table[q, lo // ps:-(-hi // ps)], table[r, lo // ps:-(-hi // ps)])
             slots.append((slot0, rows))
         assert at == tiles[i]
+        runs = len(starts[i])
+        per, longer = divmod(tiles[i], runs)
+        w = np.arange(runs)
+        x = w * per + np.minimum(w, longer)
+        some = x < tiles[i]
+        np.testing.assert_array_equal(starts[i][some], np.searchsorted(begin, x[some], side="right") - 1)
     slots.sort()
     at = 0
     for slot0, rows in slots:
         assert slot0 == at
         at += rows
     assert at <= 5 * share.rows
+    by_slot = {int(s[6]): s for line in lines for s in line}
     for t in range(share.rows):
         r = t if requests is None else int(requests[t])
         good = 0 <= r < table.shape[0] and 0 <= positions[t] < table.shape[1] * ps
         end = int(positions[t]) + 1 if good else 0
         first = max(0, end - window) if window else 0
-        refs = [p for p in paths[t].tolist() if p >= 0]
         keys = []
-        for p in refs:
-            row0, rows, lo, hi = lines[p & 1][p >> 1].tolist()[:4]
-            assert row0 <= t < row0 + rows
+        for n, line, tile, per_head, slot0, rows, row, in_chunk in paths[t].tolist():
+            if n == 0:
+                continue
+            row0, count, lo, hi, tile0, tiles_of, _, chunk = by_slot[slot0].tolist()
+            assert (n, rows, row, line) == (tiles_of, count, t - row0, int(count * group > 16)) and 0 <= row < rows and in_chunk == row % chunk
+            assert tile == tile0 + row // chunk * n and per_head == n * -(-rows // chunk)
             keys.append((lo, hi))
         keys.sort()
         at = first
@@ -87,9 +103,8 @@ def check_plan(share, table, positions, requests, ps):
             assert lo == at, (t, keys, first, end)
             at = hi
         assert at == end or (end == 0 and not keys), (t, keys, first, end)
-        if not window and good and paths[t, 0] >= 0:  # what the row keeps for itself
-            lo = lines[paths[t, 0] & 1][paths[t, 0] >> 1][2]
-            assert lo % STEP == 0
+        if not window and good and paths[t, 0, 0] > 0:  # what the row keeps for itself
+            assert by_slot[int(paths[t, 0, 4])][2] % STEP == 0
 
 
 def run(hm, device, rows, ends, ps, heads, requests=None, window=0, positions=None):
@@ -149,8 +164,8 @@ def test_nested_prompts(hm, device):
                 rows.append(list(range(100))[:64] + prompt + inner + [pages])
                 pages += 1
     share = run(hm, device, rows, [16 * len(r) - 5 for r in rows], 16, (32, 8))
-    lines, _, paths = decode(share)
-    assert (paths[:, 2:] >= 0).all() and len(lines[1]) == 1 + 6 and len(lines[0]) == 18 + 72
+    lines, _, paths, _ = decode(share)
+    assert (paths[:, 2:, 0] > 0).all() and len(lines[1]) == 1 + 6 and len(lines[0]) == 18 + 72
 
 
 def test_rows_of_requests_padding_and_bad_rows(hm, device):
