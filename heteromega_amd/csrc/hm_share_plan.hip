@@ -127,7 +127,7 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share
     const int R = static_cast<int>(a.rows), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Depths depth{lds, a.tree_base};
     int32_t *alike = lds + max(2 * a.tree_base, 3 * R), *parent = alike + R, *level = parent + R, *record = level + R, *lo = record + R;
-    const ShareWorkspace ws = carve_share(a.plan, a.rows, a.runs);
+    const ShareWorkspace ws = carve_share(a.plan, a.rows, a.groups);
     const auto row_of = [&](int j) { return j * THREADS + static_cast<int>(threadIdx.x); };
 
     for (int i = threadIdx.x; i < a.tree_base; i += THREADS) {
@@ -260,8 +260,10 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share
         at = w < wave ? at + waves[w] : at;
         total = total + waves[w];
     }
+    const ShareHeader header{{total.narrow_tiles, total.wide_tiles}, R, a.group_heads, a.kv_heads, a.groups,
+                             wide_groups(total.wide_tiles, a.groups), 0};
     if (threadIdx.x == 0) {
-        *ws.header = ShareHeader{{total.narrow_tiles, total.wide_tiles}, R, a.group_heads, a.kv_heads, a.runs, {0, 0}};
+        *ws.header = header;
     }
     int32_t *tile0[2] = {lds, lds + total.narrow};
 #pragma unroll
@@ -303,10 +305,11 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share
         }
     }
     // ---- where the runs begin ----
-    for (int i = threadIdx.x; i < (kAttentionWaves + 1) * a.runs; i += THREADS) {
-        const int line = i < kAttentionWaves * a.runs ? 0 : 1, w = line == 0 ? i : i - kAttentionWaves * a.runs;
+    const int narrow_runs = header.runs(0);
+    for (int i = threadIdx.x; i < narrow_runs + header.runs(1); i += THREADS) {
+        const int line = i < narrow_runs ? 0 : 1, w = line == 0 ? i : i - narrow_runs;
         const int count = line == 0 ? total.narrow : total.wide, tiles = line == 0 ? total.narrow_tiles : total.wide_tiles;
-        const int x = Runs::deal(tiles, runs_of(line, a.runs)).begin(w);
+        const int x = Runs::deal(tiles, header.runs(line)).begin(w);
         int first = 0, last = count - 1; // the last segment that begins at x or before it
         while (first < last) {
             const int mid = (first + last + 1) >> 1;
@@ -335,10 +338,10 @@ template <int THREADS, int PER> hipError_t launch_plan(const SharePlanArgs &a, h
 
 } // namespace
 
-size_t share_plan_workspace(int64_t rows) { return static_cast<size_t>(share_plan_bytes(rows, share_runs())); }
+size_t share_plan_workspace(int64_t rows) { return static_cast<size_t>(share_plan_bytes(rows, share_groups())); }
 
 hipError_t launch_share_plan(SharePlanArgs a, hipStream_t stream) {
-    a.runs = share_runs();
+    a.groups = share_groups();
     a.tree_base = 2;
     while (a.tree_base < a.rows + 1) {
         a.tree_base *= 2;

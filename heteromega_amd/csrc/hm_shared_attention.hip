@@ -12,12 +12,13 @@
 
 namespace hm {
 size_t shared_attention_workspace(int64_t rows, int64_t q_heads, int64_t head_dim) {
-    const int64_t columns = shared_columns(rows, q_heads, share_runs());
+    const int64_t columns = shared_columns(rows, q_heads, share_groups());
     return static_cast<size_t>((columns + 1) / 2 * 2 * 8 + columns * head_dim * 4);
 }
 
 hipError_t launch_shared_attention(SharedAttentionArgs a, hipStream_t stream) {
-    a.runs = share_runs();
+    a.groups = share_groups();
+    a.xcds = device_topology().xcds;
     return a.dtype == HM_FP16 ? launch_shared_attention_f16(a, stream) : launch_shared_attention_bf16(a, stream);
 }
 

@@ -9,12 +9,18 @@ namespace hm {
 constexpr int kShareLevels = 3;                // shared segments that a row may be in, one within the other
 constexpr int kPathEntries = kShareLevels + 2; // of a row: its own keys, those that its window leaves before the shared ones, and the shared segments
 constexpr int kNarrowCols = 16, kNarrowTile = 32; // units of up to 16 columns: a wave's, in tiles of 32 keys
-constexpr int kWideCols = 128, kWideTile = 64;    // units of more: a workgroup's, 32 columns per wave, in tiles of 64 keys
+constexpr int kWideCols = 128, kWideTile = 32; // units of more: a workgroup's, 32 columns per wave, in tiles of 32 keys
 
-// Runs of the two lines (below), narrow and wide: two workgroups per CU, with a wave each for the narrow line's. (With heads of 256 they follow each other.)
-inline int share_runs() { return 2 * device_topology().cus; }
-__host__ __device__ __forceinline__ int runs_of(int line, int runs) { return line == 0 ? kAttentionWaves * runs : runs; }
+// Workgroups, two per CU (with heads of 256 they follow each other). The first ones have a run of the wide line (below) each, the others' waves one of the
+// narrow line.
+inline int share_groups() { return 2 * device_topology().cus; }
 __host__ __device__ __forceinline__ int cols_of(int line) { return line == 0 ? kNarrowCols : kWideCols; }
+
+// The workgroups that the wide line gets: one per CU at most, since two are hardly faster and leave twice the parts, and no more than have four tiles each.
+__host__ __device__ __forceinline__ int wide_groups(int wide_tiles, int groups) {
+    const int most = (wide_tiles + 3) / 4;
+    return most < groups / 2 ? most : groups / 2;
+}
 
 // Rows [row0, row0 + rows) that see keys [lo, hi) in the same pages, as a place in one of two lines of tiles: those of narrow units, whose
 // rows x query heads of a key head are at most kNarrowCols columns, and of wide ones. A segment has a unit for each key head and, in turn, each `chunk`
@@ -38,9 +44,12 @@ struct SharePath {
 // What a plan was made for, and how many tiles its lines have: a call that does not fit it finds none.
 struct ShareHeader {
     int32_t tiles[2]; // narrow, wide
-    int32_t rows, group_heads, kv_heads, runs, spare[2];
+    int32_t rows, group_heads, kv_heads;
+    int32_t groups, wide; // workgroups, and those of the wide line
+    int32_t spare;
 
-    __host__ __device__ bool fits(int64_t n, int group, int heads, int r) const { return rows == n && group_heads == group && kv_heads == heads && runs == r; }
+    __host__ __device__ bool fits(int64_t n, int group, int heads, int g) const { return rows == n && group_heads == group && kv_heads == heads && groups == g; }
+    __host__ __device__ int runs(int line) const { return line == 0 ? kAttentionWaves * (groups - wide) : wide; }
 };
 
 // Memory of a plan. A line's segments are those with tiles, in the order of the line.
@@ -48,20 +57,20 @@ struct ShareWorkspace {
     ShareHeader *header;
     ShareSegment *segments[2]; // [3 rows]: narrow, wide
     SharePath *paths;          // [rows][kPathEntries]
-    int32_t *starts[2];        // [runs_of]: the segment that each run begins in
+    int32_t *starts[2];        // [runs]: the segment that each run begins in
 };
 
-__host__ __device__ __forceinline__ int64_t share_plan_bytes(int64_t rows, int runs) {
+__host__ __device__ __forceinline__ int64_t share_plan_bytes(int64_t rows, int groups) {
     return sizeof(ShareHeader) + 6 * rows * static_cast<int64_t>(sizeof(ShareSegment)) + rows * kPathEntries * static_cast<int64_t>(sizeof(SharePath)) +
-           (kAttentionWaves + 1) * static_cast<int64_t>(runs) * 4;
+           (kAttentionWaves + 1) * static_cast<int64_t>(groups) * 4;
 }
 
-__host__ __device__ __forceinline__ ShareWorkspace carve_share(void *p, int64_t rows, int runs) {
+__host__ __device__ __forceinline__ ShareWorkspace carve_share(void *p, int64_t rows, int groups) {
     ShareHeader *header = static_cast<ShareHeader *>(p);
     ShareSegment *segments = reinterpret_cast<ShareSegment *>(header + 1);
     SharePath *paths = reinterpret_cast<SharePath *>(segments + 6 * rows);
     int32_t *starts = reinterpret_cast<int32_t *>(paths + rows * kPathEntries);
-    return {header, {segments, segments + 3 * rows}, paths, {starts, starts + kAttentionWaves * runs}};
+    return {header, {segments, segments + 3 * rows}, paths, {starts, starts + kAttentionWaves * groups}};
 }
 
 // The parts of units: a run of a line leaves at most one unit that it does not finish, whose part goes to the run's own columns; the parts that end a unit
@@ -71,8 +80,8 @@ struct SharedParts {
     float *o;      // [columns][D]
 };
 
-__host__ __device__ __forceinline__ int64_t shared_columns(int64_t rows, int64_t q_heads, int runs) {
-    return rows * kPathEntries * q_heads + static_cast<int64_t>(runs) * (kAttentionWaves * kNarrowCols + kWideCols);
+__host__ __device__ __forceinline__ int64_t shared_columns(int64_t rows, int64_t q_heads, int groups) {
+    return rows * kPathEntries * q_heads + static_cast<int64_t>(groups) * (kAttentionWaves * kNarrowCols + kWideCols);
 }
 
 __host__ __device__ __forceinline__ SharedParts carve_parts(void *p, int64_t columns) {
@@ -81,13 +90,13 @@ __host__ __device__ __forceinline__ SharedParts carve_parts(void *p, int64_t col
 }
 
 // First column of run w's unfinished unit in a line, behind the row slots'.
-__host__ __device__ __forceinline__ int64_t run_column(int64_t rows, int64_t q_heads, int runs, int line, int64_t w) {
-    return rows * kPathEntries * q_heads + (line == 0 ? w * kNarrowCols : static_cast<int64_t>(runs) * kAttentionWaves * kNarrowCols + w * kWideCols);
+__host__ __device__ __forceinline__ int64_t run_column(int64_t rows, int64_t q_heads, int groups, int line, int64_t w) {
+    return rows * kPathEntries * q_heads + (line == 0 ? w * kNarrowCols : static_cast<int64_t>(groups) * kAttentionWaves * kNarrowCols + w * kWideCols);
 }
 
 struct SharedAttentionArgs : PagedAttentionArgs {
     void *plan;
-    int runs;
+    int groups, xcds;
     int group_heads;
 };
 

@@ -5,6 +5,8 @@
 #include "hm_paged_attention_kernel.hpp"
 #include "hm_shared_attention.hpp"
 
+#include <type_traits>
+
 namespace hm {
 namespace {
 
@@ -33,7 +35,7 @@ template <int LINE> __device__ __forceinline__ Work next_work(const SharedAttent
     k.tile0 = x - k.s.tile0 - unit * k.s.tiles;
     k.tile1 = min(k.s.tiles, k.tile0 + (x_end - x));
     k.part = k.tile1 == k.s.tiles ? static_cast<int64_t>(k.s.slot0) * a.q_heads + (static_cast<int64_t>(k.kv_head) * k.s.rows + k.row) * a.group_heads
-                                  : run_column(a.rows, a.q_heads, a.runs, LINE, w);
+                                  : run_column(a.rows, a.q_heads, a.groups, LINE, w);
     x += k.tile1 - k.tile0;
     at += k.tile1 == k.s.tiles && unit + 1 == a.kv_heads * chunks;
     return k;
@@ -69,6 +71,20 @@ struct Pages {
     }
 };
 
+// The pages of 64 sub-tiles of 16 keys, a lane each, from one read of the table for all of them.
+struct PageIds {
+    int32_t ids;
+    int first; // sub-tile of lane 0
+
+    // Reads on from sub-tile `sub`; true if a page lies outside the cache.
+    __device__ __forceinline__ bool read(const Pages &at, int start, int hi, int sub) {
+        first = sub;
+        ids = at.page_of(start + 16 * (sub + static_cast<int>(threadIdx.x & 63)), hi);
+        return __any(static_cast<uint32_t>(ids) >= at.pages);
+    }
+    __device__ __forceinline__ int32_t of(int sub) const { return __builtin_amdgcn_readlane(ids, sub - first); }
+};
+
 // A unit of up to 16 columns, by one wave, 32 keys at a time: with up to 128 units on a CU one after the other, waves go on to their next by themselves.
 template <class T, int D> __device__ __forceinline__ void narrow_work(const SharedAttentionArgs &a, const Work &k, uint8_t *lds) {
     using S = Shape<T, D>;
@@ -99,24 +115,16 @@ template <class T, int D> __device__ __forceinline__ void narrow_work(const Shar
     bool poisoned = false; // a page outside the cache
 
     u32x4_t k_reg[2][S::kSteps], v_reg[2][S::kSteps];
-    int32_t id[2];
-    const auto page_ids = [&](int tile) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int key = start + tile * kNarrowTile + 16 * s;
-            id[s] = at.page_of(key, hi);
-        }
-    };
+    PageIds ids;
     const auto request = [&](int tile) {
+        if (2 * (tile - k.tile0) % 64 == 0) {
+            poisoned |= ids.read(at, start, hi, 2 * tile);
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const int key = start + tile * kNarrowTile + 16 * s;
-            const int32_t page = uniform(id[s]);
-            int seen = max(0, min(16, hi - key));
-            if (static_cast<uint32_t>(page) >= at.pages) {
-                poisoned |= seen > 0;
-                seen = 0;
-            }
+            const int32_t page = ids.of(2 * tile + s);
+            const int seen = static_cast<uint32_t>(page) < at.pages ? max(0, min(16, hi - key)) : 0;
             const uint32_t bytes = at.bytes<D>(seen);
             const int64_t from = at.offset(page, key, seen);
             const __amdgpu_buffer_rsrc_t kr = buffer_rsrc(at.k_head + from, bytes), vr = buffer_rsrc(at.v_head + from, bytes);
@@ -130,9 +138,7 @@ template <class T, int D> __device__ __forceinline__ void narrow_work(const Shar
             }
         }
     };
-    page_ids(k.tile0);
     request(k.tile0);
-    page_ids(min(k.tile0 + 1, k.tile1 - 1));
     for (int tile = k.tile0; tile < k.tile1; ++tile) {
         const int key0 = start + tile * kNarrowTile;
         if (key0 < lo) { // values before the first key count as zero, whatever they are
@@ -172,7 +178,6 @@ template <class T, int D> __device__ __forceinline__ void narrow_work(const Shar
         }
         if (tile + 1 < k.tile1) {
             request(tile + 1);
-            page_ids(min(tile + 2, k.tile1 - 1));
         }
         float p[8];
 #pragma unroll
@@ -225,7 +230,7 @@ template <class T, int D> __device__ __forceinline__ void narrow_work(const Shar
         }
     }
 
-    const SharedParts parts = carve_parts(a.workspace, shared_columns(a.rows, a.q_heads, a.runs));
+    const SharedParts parts = carve_parts(a.workspace, shared_columns(a.rows, a.q_heads, a.groups));
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (live) {
@@ -260,28 +265,64 @@ template <> struct Halves<F16> {
     }
 };
 
-// A unit of more columns: 16 CT of each wave, up to 128 in all; the waves share tiles of 64 keys, of which each brings a quarter into LDS. Two buffers, one
-// barrier a tile.
-template <class T, int D, int CT> __device__ __forceinline__ void wide_work(const SharedAttentionArgs &a, const Work &k, uint8_t *lds) {
+// Rows of keys and values in LDS as transfers leave them, without padding: 16-byte piece c of row r lies at piece c ^ key(r) or c ^ value(r) of its row, so that
+// 8 rows' pieces of the first product's operand, and 4 rows' pairs of pieces of the second's, lie in different banks.
+template <int D> struct Swizzle {
+    static constexpr int kPerRow = D / 8;
+    static constexpr int kKeys = D == 96 ? 1 : 2, kValues = D == 96 ? 2 : 4; // operands' addresses that are not a constant apart
+    static __device__ __forceinline__ int key(int r) { return D == 96 ? (r >> 1) & 3 : r & 7; }
+    static __device__ __forceinline__ int value(int r) { return D == 96 ? 2 * ((r >> 1) & 1) : 2 * (r & 3); }
+};
+
+// lds_dma16 without the compiler's knowledge: it would have every read of the ring wait for all transfers to it, and which are done is counted here. Bytes and
+// addresses are uniform; `to` is an LDS address. M0 has no other use in these kernels.
+__device__ __forceinline__ void ring_transfer(u32x4_t resource, uint32_t to, uint32_t offset) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(resource) : "memory");
+#else
+    (void)resource, (void)to, (void)offset;
+#endif
+}
+
+// Tiles of keys and values on the way or in use at once. In step n the first product takes the keys of tile n + 1, the second the values of tile n - 1, and the
+// weights of tile n are worked out beside them. What tile x brings is asked for kAhead steps before it is needed: keys in step x - 4, values in step x - 2, into
+// the places of tiles that were last read in the step before.
+constexpr int kRing = 4, kAhead = 3;
+template <int D> constexpr int kRingBytes = kRing * 2 * kWideTile * 2 * D;
+
+// A unit of more columns: 16 CT of each wave, up to 128 in all. The four waves share tiles of 32 keys, of which two waves bring the keys and two the values into LDS,
+// 16 rows each. The matrix cores bound it if the vector instructions run beside them, and for that they have to lie between the products in the
+// program, since the two waves of a SIMD hardly overlap otherwise (as many cycles as both kinds' sum were measured): hence the steps above.
+template <class T, int D, int CT> __device__ __forceinline__ void wide_work(const SharedAttentionArgs &a, const Work &k, uint8_t *ring) {
     using S = Shape<T, D>;
-    constexpr int kTileBytes = kWideTile * S::kRowBytes; // of keys, or values
-    constexpr int kSubs = kWideTile / 16;
+    using Z = Swizzle<D>;
+    constexpr int kRow = 2 * D, kPlane = kWideTile * kRow; // a tile's keys, or values
     // The maximum follows only when a score passes it by more than a factor 2^kSlack, and is one of the scores before their factor
-    // (hm_paged_attention_prompt.hpp).
-    constexpr float kSlack = 3.0f, kTop = Split<T>::kTop - (Split<T>::kTop > 0.0f ? kSlack : 0.0f);
+    // (hm_paged_attention_prompt.hpp). fp16 weights have 2^9 at the maximum, so that they end at 2^15 and lose what is below 2^-33 of it.
+    constexpr float kSlack = Split<T>::kTop > 0.0f ? 6.0f : 16.0f, kTop = Split<T>::kTop > 0.0f ? Split<T>::kTop - kSlack : 0.0f;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int col = lane & 15, quad = lane >> 4;
-    const int columns = k.rows * a.group_heads, start = k.s.start(), lo = k.s.lo, hi = k.s.hi;
+    const int columns = k.rows * a.group_heads, start = k.s.start() + k.tile0 * kWideTile, lo = k.s.lo, hi = min(k.s.hi, k.s.start() + k.tile1 * kWideTile);
+    const int tiles = k.tile1 - k.tile0;
     const Pages at(a, k.s.row0, k.kv_head);
-    const Pieces<D> pieces(lane, at.row_bytes);
-    const uint32_t to_lds = wave * 16 * S::kRowBytes + pieces.lds_offset();
-    const uint32_t k_lds = col * S::kRowBytes + quad * 16;
-    const uint32_t v_lds = (4 * quad + (col >> 2)) * S::kRowBytes + (col & 3) * 8;
+
+    // ---- pages and queries ----
+    int32_t ids[2]; // of 128 sub-tiles of 16 keys from first_id on, a lane each
+    int first_id = 0;
+    bool poisoned = false; // a page outside the cache
+    const auto read_ids = [&](int first) {
+        first_id = first;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            ids[i] = at.page_of(start + 16 * (first + 64 * i + lane), hi);
+        }
+    };
+    const auto check_ids = [&] { poisoned |= __any(static_cast<uint32_t>(ids[0]) >= at.pages || static_cast<uint32_t>(ids[1]) >= at.pages); };
+    read_ids(0);
     // The sign goes to the queries. Not zero: a masked score of -infinity times it must stay one.
     const float c_scale = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 0x1p-126f);
     const float slack = fminf(kSlack / c_scale, 0x1p126f); // of scores without the factor
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
-
     u32x4_t q[CT][S::kSteps];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -294,6 +335,53 @@ template <class T, int D, int CT> __device__ __forceinline__ void wide_work(cons
             q[c][s] = live ? *reinterpret_cast<const u32x4_t *>(q_row + 32 * s) ^ sign : u32x4_t{0, 0, 0, 0};
         }
     }
+    check_ids();
+    wait_vmcnt<0>(); // from here on only transfers are on the way
+
+    // ---- transfers: the wave's 16 rows of keys (waves 0 and 1) or values ----
+    const bool of_values = wave >= 2;
+    const int sub = wave & 1;
+    uint32_t from[S::kSteps]; // piece j * 64 + lane of the rows is the lane's of transfer j
+#pragma unroll
+    for (int j = 0; j < S::kSteps; ++j) {
+        const int r = (j * 64 + lane) / Z::kPerRow, c = (j * 64 + lane) % Z::kPerRow;
+        from[j] = r * at.row_bytes + (c ^ (of_values ? Z::value(r) : Z::key(r))) * 16;
+    }
+    const uint16_t *head = of_values ? at.v_head : at.k_head;
+    const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)ring)) + (of_values ? kPlane : 0) + sub * 16 * kRow;
+    const auto transfer = [&](int tile) { // zeros behind the last key, also of tiles that there are not: the counts stay what they are
+        const int key = start + tile * kWideTile + 16 * sub, i = 2 * tile + sub - first_id;
+        const int32_t page = i < 64 ? __builtin_amdgcn_readlane(ids[0], i) : __builtin_amdgcn_readlane(ids[1], i & 63);
+        const int seen = static_cast<uint32_t>(page) < at.pages ? max(0, min(16, hi - key)) : 0;
+        const uint64_t address = reinterpret_cast<uint64_t>(head + at.offset(page, key, seen));
+        const u32x4_t resource{static_cast<uint32_t>(uniform(static_cast<int>(address))), static_cast<uint32_t>(uniform(static_cast<int>(address >> 32))) & 0xFFFFu,
+                               at.bytes<D>(seen), 0x00020000u};
+#if defined(__HIP_DEVICE_COMPILE__)
+        asm volatile("s_nop 4" ::"s"(resource)); // vector instructions may have written it, and a load may read it 5 cycles later
+#endif
+#pragma unroll
+        for (int j = 0; j < S::kSteps; ++j) {
+            ring_transfer(resource, ring_at + (tile % kRing) * 2 * kPlane + j * 1024, from[j]);
+        }
+    };
+#pragma unroll
+    for (int x = 0; x < kAhead + 1; ++x) { // as if in steps -4 to -1
+        if (!of_values || x >= kAhead - 1) {
+            transfer(of_values ? x - 2 : x);
+        }
+    }
+
+    // ---- operands' addresses, and what is summed up ----
+    uint32_t k_lds[Z::kKeys], v_lds[Z::kValues];
+#pragma unroll
+    for (int i = 0; i < Z::kKeys; ++i) {
+        k_lds[i] = col * kRow + ((4 * i + quad) ^ Z::key(col)) * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < Z::kValues; ++i) {
+        const int r = 4 * quad + (col >> 2);
+        v_lds[i] = kPlane + r * kRow + ((2 * i + ((col & 3) >> 1)) ^ Z::value(r)) * 16 + (col & 1) * 8;
+    }
     float4_t o[CT][S::kDTiles];
     float m[CT], l[CT];
 #pragma unroll
@@ -304,83 +392,75 @@ template <class T, int D, int CT> __device__ __forceinline__ void wide_work(cons
         }
         m[c] = -INFINITY, l[c] = 0.0f;
     }
-    bool poisoned = false; // a page outside the cache
-
-    u32x4_t k_reg[S::kSteps], v_reg[S::kSteps];
-    int32_t ids = 0; // of sub-tile lane % 4: a vector load, since waits for LDS would wait for a scalar one too
-    const auto page_ids = [&](int tile) {
-        const int key = start + tile * kWideTile + 16 * (lane % kAttentionWaves);
-        ids = at.page_of(key, hi);
+    struct Weights {
+        u32x4_t upper[CT], lower[CT];
     };
-    const auto load = [&](int tile) { // the wave's sub-tile
-        poisoned |= __any(static_cast<uint32_t>(ids) >= at.pages);
-        const int32_t page = __builtin_amdgcn_readlane(ids, wave);
-        const int key = start + tile * kWideTile + 16 * wave;
-        const int seen = static_cast<uint32_t>(page) < at.pages ? max(0, min(16, hi - key)) : 0;
-        const uint32_t bytes = at.bytes<D>(seen);
-        const int64_t from = at.offset(page, key, seen);
-        const __amdgpu_buffer_rsrc_t kr = buffer_rsrc(at.k_head + from, bytes), vr = buffer_rsrc(at.v_head + from, bytes);
+    typedef float4_t Scores[CT][2];
+    const auto first_product = [&](int tile, Scores &score) __attribute__((always_inline)) {
+        const uint8_t *keys = ring + (tile % kRing) * 2 * kPlane;
 #pragma unroll
         for (int i = 0; i < S::kSteps; ++i) {
-            k_reg[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, pieces.offset(i), 0, 0);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const uint4 kk = *reinterpret_cast<const uint4 *>(keys + k_lds[i % Z::kKeys] + s * 16 * kRow + i / Z::kKeys * Z::kKeys * 64);
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    score[c][s] = T::mfma16(kk, __builtin_bit_cast(uint4, q[c][i]), i == 0 ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : score[c][s]);
+                }
+            }
         }
+    };
+    const auto second_product = [&](int tile, const Weights &w) __attribute__((always_inline)) {
+        const uint8_t *values = ring + (tile % kRing) * 2 * kPlane;
 #pragma unroll
-        for (int i = 0; i < S::kSteps; ++i) {
-            v_reg[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, pieces.offset(i), 0, 0);
+        for (int i = 0; i < S::kDTiles; ++i) {
+            uint2 half[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                half[s] = lds_read_transposed(values + v_lds[i % Z::kValues] + s * 16 * kRow + i / Z::kValues * Z::kValues * 32);
+            }
+            const uint4 vt = make_uint4(half[0].x, half[0].y, half[1].x, half[1].y);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                o[c][i] = T::mfma16(vt, __builtin_bit_cast(uint4, w.upper[c]), o[c][i]);
+            }
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                o[c][i] = T::mfma16(vt, __builtin_bit_cast(uint4, w.lower[c]), o[c][i]);
+            }
+        }
+    };
+    const auto clear_before = [&] { // values before the first key count as zero, whatever they are
+        if (lo > start && wave == 2) {
+            for (int j = lane; j < (lo - start) * Z::kPerRow; j += 64) {
+                *reinterpret_cast<u32x4_t *>(ring + kPlane + j * 16) = u32x4_t{0, 0, 0, 0};
+            }
         }
     };
     const bool works = 16 * wave * CT < columns;
-    page_ids(k.tile0);
-    load(k.tile0);
-    page_ids(min(k.tile0 + 1, k.tile1 - 1));
-    for (int tile = k.tile0; tile < k.tile1; ++tile) {
-        const int key0 = start + tile * kWideTile;
-        uint8_t *k_tile = lds + (tile & 1) * 2 * kTileBytes, *v_tile = k_tile + kTileBytes;
-        if (key0 < lo) { // values before the first key count as zero, whatever they are
-#pragma unroll
-            for (int i = 0; i < S::kSteps; ++i) {
-                if (key0 + 16 * wave + pieces.key(i) < lo) {
-                    v_reg[i] = u32x4_t{0, 0, 0, 0};
-                }
-            }
+    // Step n: scores of tile n in `score`, weights of tile n - 1 in `before`; leaves those of n + 1 and n.
+    const auto step = [&](auto first, int n, Scores &score, Scores &next, Weights &before, Weights &weights) __attribute__((always_inline)) {
+        constexpr bool kFirst = decltype(first)::value; // tile 0: there is none before
+        wait_vmcnt<(kAhead - 1) * S::kSteps>(); // the wave's transfers that this step needs are done, those of two steps may be on the way
+        if (n == 1) {
+            clear_before();
         }
-#pragma unroll
-        for (int i = 0; i < S::kSteps; ++i) {
-            *reinterpret_cast<u32x4_t *>(k_tile + to_lds + pieces.lds_step(i)) = k_reg[i];
-            *reinterpret_cast<u32x4_t *>(v_tile + to_lds + pieces.lds_step(i)) = v_reg[i];
+        lds_barrier();
+        const int wanted = n + (of_values ? kAhead - 1 : kAhead + 1);
+        if (2 * (wanted + 1) - first_id > 128) { // seldom: the pages of the next 60 tiles
+            read_ids(2 * (n + kAhead - 1));
+            check_ids();
+            wait_vmcnt<0>();
         }
-        // The buffer's readers of two tiles ago passed the barrier of the last one.
-        __syncthreads();
-        if (tile + 1 < k.tile1) {
-            load(tile + 1);
-            page_ids(min(tile + 2, k.tile1 - 1));
-        }
+        transfer(wanted);
         if (!works) {
-            continue;
+            return;
         }
-        float4_t score[CT][kSubs];
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-#pragma unroll
-            for (int s = 0; s < kSubs; ++s) {
-                score[c][s] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < S::kSteps; ++i) {
-#pragma unroll
-            for (int s = 0; s < kSubs; ++s) {
-                const uint4 kk = *reinterpret_cast<const uint4 *>(k_tile + k_lds + s * 16 * S::kRowBytes + 64 * i);
-#pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    score[c][s] = T::mfma16(kk, __builtin_bit_cast(uint4, q[c][i]), score[c][s]);
-                }
-            }
-        }
+        const int key0 = start + n * kWideTile;
         if (key0 < lo || key0 + kWideTile > hi) {
             __builtin_amdgcn_sched_barrier(0); // keeps this a branch
 #pragma unroll
-            for (int e = 0; e < 4 * kSubs; ++e) {
+            for (int e = 0; e < 8; ++e) {
                 const int key = key0 + 16 * (e >> 2) + 4 * quad + (e & 3);
                 if (key < lo || key >= hi) {
 #pragma unroll
@@ -396,12 +476,19 @@ template <class T, int D, int CT> __device__ __forceinline__ void wide_work(cons
         for (int c = 0; c < CT; ++c) {
             top[c] = score[c][0][0];
 #pragma unroll
-            for (int e = 1; e < 4 * kSubs; ++e) {
+            for (int e = 1; e < 8; ++e) {
                 top[c] = fmaxf(top[c], score[c][e >> 2][e & 3]);
             }
             follow |= top[c] > m[c] + slack;
         }
         if (__any(follow)) {
+            if constexpr (!kFirst) { // what is on the way is relative to the old maximum
+                second_product(n - 1, before);
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    before.upper[c] = before.lower[c] = u32x4_t{0, 0, 0, 0};
+                }
+            }
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
                 top[c] = fmaxf(top[c], __shfl_xor(top[c], 16));
@@ -416,11 +503,7 @@ template <class T, int D, int CT> __device__ __forceinline__ void wide_work(cons
                 }
             }
         }
-        // One straight piece from here on, so that the second half's weights are worked out beside the first half's products.
-#pragma unroll
-        for (int h = 0; h < 2; ++h) { // 32 keys at a time
-            const uint32_t half_lds = h * 32 * S::kRowBytes;
-            u32x4_t upper[CT], lower[CT];
+        const auto work_out = [&] {
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
                 const float m_used = m[c] == -INFINITY ? 0.0f : m[c];
@@ -428,33 +511,47 @@ template <class T, int D, int CT> __device__ __forceinline__ void wide_work(cons
                 for (int e = 0; e < 8; e += 2) {
                     float2_t p;
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        p[n] = exp2_fast(__builtin_fmaf(score[c][2 * h + (e >> 2)][(e & 3) + n] - m_used, c_scale, kTop));
-                        l[c] += p[n];
+                    for (int i = 0; i < 2; ++i) {
+                        p[i] = exp2_fast(__builtin_fmaf(score[c][e >> 2][(e & 3) + i] - m_used, c_scale, kTop));
+                        l[c] += p[i];
                     }
                     uint32_t u, v;
                     Halves<T>::split(p, u, v);
-                    upper[c][e / 2] = u, lower[c][e / 2] = v;
+                    weights.upper[c][e / 2] = u, weights.lower[c][e / 2] = v;
                 }
             }
-#pragma unroll
-            for (int i = 0; i < S::kDTiles; ++i) {
-                uint2 half[2];
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    half[s] = lds_read_transposed(v_tile + v_lds + half_lds + s * 16 * S::kRowBytes + i * 32);
-                }
-                const uint4 vt = make_uint4(half[0].x, half[0].y, half[1].x, half[1].y);
-#pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    o[c][i] = T::mfma16(vt, __builtin_bit_cast(uint4, upper[c]), o[c][i]);
-                    o[c][i] = T::mfma16(vt, __builtin_bit_cast(uint4, lower[c]), o[c][i]);
-                }
-            }
+        };
+        first_product(n + 1, next); // behind the last tile: of zeros
+        work_out();
+        if constexpr (!kFirst) {
+            second_product(n - 1, before);
+        }
+    };
+    Scores score_even, score_odd;
+    Weights even{}, odd{};
+    wait_vmcnt<kAhead * S::kSteps>(); // of keys: those of the first tile; of values: no more are on the way
+    lds_barrier();
+    if (works) {
+        first_product(0, score_even);
+    }
+    step(std::true_type{}, 0, score_even, score_odd, odd, even);
+#pragma unroll 1
+    for (int n = 1; n < tiles; n += 2) {
+        step(std::false_type{}, n, score_odd, score_even, even, odd);
+        if (n + 1 < tiles) {
+            step(std::false_type{}, n + 1, score_even, score_odd, odd, even);
         }
     }
+    wait_vmcnt<0>();
+    if (tiles == 1) {
+        clear_before();
+    }
+    lds_barrier();
+    if (works) {
+        second_product(tiles - 1, (tiles & 1) != 0 ? even : odd);
+    }
 
-    const SharedParts parts = carve_parts(a.workspace, shared_columns(a.rows, a.q_heads, a.runs));
+    const SharedParts parts = carve_parts(a.workspace, shared_columns(a.rows, a.q_heads, a.groups));
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         l[c] += __shfl_xor(l[c], 16);
@@ -471,48 +568,43 @@ template <class T, int D, int CT> __device__ __forceinline__ void wide_work(cons
             }
         }
     }
-    __syncthreads(); // the next unit takes the buffers
+    lds_barrier(); // the next unit takes the ring
 }
 
-// A run of the wide line per workgroup and one of the narrow line per wave. Half of the workgroups begin with the wide line, which the matrix cores bound,
-// half with the narrow one, which the memory bounds.
+// The first workgroups have a run of the wide line each, which the matrix cores bound; the waves of the others one each of the narrow line, which the
+// memory bounds. Where both are half, a CU has a workgroup of each.
 template <class T, int D> __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) shared_attention_kernel(SharedAttentionArgs a) {
     using S = Shape<T, D>;
-    constexpr int kNarrowBytes = kAttentionWaves * S::kRegion, kWideBytes = 4 * kWideTile * S::kRowBytes;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[kNarrowBytes > kWideBytes ? kNarrowBytes : kWideBytes];
-    const ShareWorkspace plan = carve_share(a.plan, a.rows, a.runs);
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kRingBytes<D>];
+    static_assert(kAttentionWaves * S::kRegion <= kRingBytes<D>, "narrow units' regions take the place of the ring");
+    const ShareWorkspace plan = carve_share(a.plan, a.rows, a.groups);
     const int wave = uniform(threadIdx.x >> 6);
-    const int wide_start = plan.starts[1][blockIdx.x], narrow_start = plan.starts[0][blockIdx.x * kAttentionWaves + wave];
     const ShareHeader header = *plan.header;
-    if (!header.fits(a.rows, a.group_heads, a.kv_heads, a.runs)) {
+    if (!header.fits(a.rows, a.group_heads, a.kv_heads, a.groups)) {
         return;
     }
-    const bool wide_first = 2 * static_cast<int>(blockIdx.x) < a.runs;
-#pragma unroll 1
-    for (int turn = 0; turn < 2; ++turn) {
-        if ((turn == 0) == wide_first) {
-            const Runs runs = Runs::deal(uniform(header.tiles[1]), a.runs);
-            const int w = blockIdx.x, x_end = runs.begin(w + 1);
-            int x = runs.begin(w), at = uniform(wide_start);
-            if (x < x_end && turn == 1) {
-                __syncthreads(); // the narrow units' regions are free
-            }
-            while (x < x_end) {
-                const Work k = next_work<1>(a, plan.segments[1], at, x, x_end, w);
-                if (k.rows * a.group_heads > 64) {
-                    wide_work<T, D, 2>(a, k, lds);
-                } else {
-                    wide_work<T, D, 1>(a, k, lds);
-                }
-            }
-        } else {
-            const Runs runs = Runs::deal(uniform(header.tiles[0]), kAttentionWaves * a.runs);
-            const int w = blockIdx.x * kAttentionWaves + wave, x_end = runs.begin(w + 1);
-            int x = runs.begin(w), at = uniform(narrow_start);
-            while (x < x_end) {
-                narrow_work<T, D>(a, next_work<0>(a, plan.segments[0], at, x, x_end, w), lds + wave * S::kRegion);
+    const int wide = uniform(header.wide), group = static_cast<int>(blockIdx.x) - wide;
+    if (group < 0) {
+        const Runs runs = Runs::deal(uniform(header.tiles[1]), wide);
+        // Runs that follow each other go to one XCD: those of a key head's chunks of rows read the same keys at the same time, and its L2 has them for all.
+        const int xcd = blockIdx.x % a.xcds, w = xcd * (wide / a.xcds) + min(xcd, wide % a.xcds) + static_cast<int>(blockIdx.x / a.xcds), x_end = runs.begin(w + 1);
+        int x = runs.begin(w), at = uniform(plan.starts[1][w]);
+        while (x < x_end) {
+            const Work k = next_work<1>(a, plan.segments[1], at, x, x_end, w);
+            if (k.rows * a.group_heads > 64) {
+                wide_work<T, D, 2>(a, k, lds);
+            } else {
+                wide_work<T, D, 1>(a, k, lds);
             }
         }
+        return;
+    }
+    const int groups = a.groups - wide, w = wave * groups + group; // few runs go to as many workgroups
+    const Runs runs = Runs::deal(uniform(header.tiles[0]), kAttentionWaves * groups);
+    const int x_end = runs.begin(w + 1);
+    int x = runs.begin(w), at = uniform(plan.starts[0][w]);
+    while (x < x_end) {
+        narrow_work<T, D>(a, next_work<0>(a, plan.segments[0], at, x, x_end, w), lds + wave * S::kRegion);
     }
 }
 
@@ -528,7 +620,7 @@ template <class T, int D, int THREADS> __global__ void __launch_bounds__(256) sh
         return;
     }
     const int head = static_cast<int>(column - static_cast<uint32_t>(t) * a.q_heads), kv_head = head / a.group_heads, in_group = head - kv_head * a.group_heads;
-    const ShareWorkspace plan = carve_share(a.plan, a.rows, a.runs);
+    const ShareWorkspace plan = carve_share(a.plan, a.rows, a.groups);
     const ShareHeader header = *plan.header;
     const int lane = threadIdx.x & 63;
     const SharePath p = plan.paths[t * kPathEntries + min(lane, kPathEntries - 1)];
@@ -539,11 +631,11 @@ template <class T, int D, int THREADS> __global__ void __launch_bounds__(256) sh
     // The parts of each segment's unit, a lane each: of runs w0, w0 + 1 and so on, the last one at `end`.
     int own_count = 0;
     int64_t own_first = 0, own_end = 0;
-    if (lane < kPathEntries && p.tiles > 0 && header.fits(a.rows, a.group_heads, a.kv_heads, a.runs)) {
-        const Runs runs = Runs::deal(p.line == 0 ? header.tiles[0] : header.tiles[1], runs_of(p.line, a.runs));
+    if (lane < kPathEntries && p.tiles > 0 && header.fits(a.rows, a.group_heads, a.kv_heads, a.groups)) {
+        const Runs runs = Runs::deal(p.line == 0 ? header.tiles[0] : header.tiles[1], header.runs(p.line));
         const int tile = p.tile + kv_head * p.per_head, w0 = runs.of(tile);
         own_count = runs.of(tile + p.tiles - 1) - w0 + 1;
-        own_first = run_column(a.rows, a.q_heads, a.runs, p.line, w0) + p.in_chunk * a.group_heads + in_group;
+        own_first = run_column(a.rows, a.q_heads, a.groups, p.line, w0) + p.in_chunk * a.group_heads + in_group;
         own_end = static_cast<int64_t>(p.slot0) * a.q_heads + (static_cast<int64_t>(kv_head) * p.rows + p.row) * a.group_heads + in_group;
     }
     const auto of64 = [](int64_t v, int i) {
@@ -570,7 +662,7 @@ template <class T, int D, int THREADS> __global__ void __launch_bounds__(256) sh
         }
         return at;
     };
-    const SharedParts parts = carve_parts(a.workspace, shared_columns(a.rows, a.q_heads, a.runs));
+    const SharedParts parts = carve_parts(a.workspace, shared_columns(a.rows, a.q_heads, a.groups));
     const int y = thread / kItems, e = thread - y * kItems;
     float m = -INFINITY, l = 0.0f;
     float4_t v = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -632,14 +724,14 @@ template <class T, int D, int THREADS> __global__ void __launch_bounds__(256) sh
 }
 
 template <class T, int D> hipError_t launch_shared(const SharedAttentionArgs &a, hipStream_t stream) {
-    hipLaunchKernelGGL((shared_attention_kernel<T, D>), dim3(static_cast<unsigned>(a.runs)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((shared_attention_kernel<T, D>), dim3(static_cast<unsigned>(a.groups)), dim3(kThreads), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {
         return e;
     }
     // A wave per column where there are enough columns for the card.
     const int64_t columns = a.rows * a.q_heads;
-    if (D == 256 || columns <= 2 * a.runs) {
+    if (D == 256 || columns <= 2 * a.groups) {
         hipLaunchKernelGGL((shared_join_kernel<T, D, 256>), dim3(static_cast<unsigned>(columns)), dim3(256), 0, stream, a);
     } else {
         hipLaunchKernelGGL((shared_join_kernel<T, D, D == 256 ? 256 : 64>), dim3(static_cast<unsigned>((columns + 3) / 4)), dim3(256), 0, stream, a);

@@ -41,8 +41,9 @@ def decode(share):
     assert head[2:5].tolist() == [rows, share.q_heads // share.kv_heads, share.kv_heads]
     lines = words[8:8 + 48 * rows].reshape(2, 3 * rows, 8)
     paths = words[8 + 48 * rows:8 + 88 * rows].reshape(rows, 5, 8)
-    runs = int(head[5])
-    starts = words[8 + 88 * rows:8 + 88 * rows + 5 * runs]
+    groups, wide = head[5:7].tolist()
+    starts = words[8 + 88 * rows:8 + 88 * rows + 5 * groups]
+    assert 0 <= wide <= groups // 2 and (wide > 0) == (head[1] > 0)
     counts = []
     for i in range(2):  # as many as have the line's tiles
         at = n = 0
@@ -50,7 +51,7 @@ def decode(share):
             at += int(lines[i, n, 5]) * share.kv_heads * -(-int(lines[i, n, 1]) // int(lines[i, n, 7]))
             n += 1
         counts.append(n)
-    return [lines[i, :counts[i]] for i in range(2)], head[:2].tolist(), paths, [starts[:4 * runs], starts[4 * runs:]]
+    return [lines[i, :counts[i]] for i in range(2)], head[:2].tolist(), paths, [starts[:4 * (groups - wide)], starts[4 * groups:4 * groups + wide]]
 
 
 def check_plan(share, table, positions, requests, ps):
@@ -61,7 +62,7 @@ def check_plan(share, table, positions, requests, ps):
         at, begin = 0, []
         for row0, rows, lo, hi, tile0, n, slot0, chunk in line.tolist():
             assert 0 <= row0 and rows > 0 and row0 + rows <= share.rows and 0 <= lo < hi and tile0 == at
-            assert (rows * group > 16) == (i == 1) and n == -(-(hi - lo // 16 * 16) // (64 if i else 32))
+            assert (rows * group > 16) == (i == 1) and n == -(-(hi - lo // 16 * 16) // 32)
             assert rows == 1 or lo % 16 == 0
             assert chunk >= 1 and (chunk * group <= 128 if i else chunk == rows)
             begin.append(at)
@@ -71,9 +72,9 @@ def check_plan(share, table, positions, requests, ps):
                 np.testing.assert_array_equal(table[q, lo // ps:-(-hi // ps)], table[r, lo // ps:-(-hi // ps)])
             slots.append((slot0, rows))
         assert at == tiles[i]
-        runs = len(starts[i])
+        runs = max(1, len(starts[i]))
         per, longer = divmod(tiles[i], runs)
-        w = np.arange(runs)
+        w = np.arange(len(starts[i]))
         x = w * per + np.minimum(w, longer)
         some = x < tiles[i]
         np.testing.assert_array_equal(starts[i][some], np.searchsorted(begin, x[some], side="right") - 1)
