@@ -261,7 +261,7 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share
         total = total + waves[w];
     }
     const ShareHeader header{{total.narrow_tiles, total.wide_tiles}, R, a.group_heads, a.kv_heads, a.groups,
-                             wide_groups(total.wide_tiles, a.groups), 0};
+                             wide_groups(total.wide_tiles, total.narrow_tiles, a.groups), 0};
     if (threadIdx.x == 0) {
         *ws.header = header;
     }

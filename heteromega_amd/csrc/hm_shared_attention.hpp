@@ -8,7 +8,7 @@ namespace hm {
 
 constexpr int kShareLevels = 3;                // shared segments that a row may be in, one within the other
 constexpr int kPathEntries = kShareLevels + 2; // of a row: its own keys, those that its window leaves before the shared ones, and the shared segments
-constexpr int kNarrowCols = 16, kNarrowTile = 32; // units of up to 16 columns: a wave's, in tiles of 32 keys
+constexpr int kNarrowCols = 32, kNarrowTile = 32; // units of up to 32 columns: a wave's, in tiles of 32 keys
 constexpr int kWideCols = 128, kWideTile = 32; // units of more: a workgroup's, 32 columns per wave, in tiles of 32 keys
 
 // Workgroups, two per CU (with heads of 256 they follow each other). The first ones have a run of the wide line (below) each, the others' waves one of the
@@ -16,9 +16,12 @@ constexpr int kWideCols = 128, kWideTile = 32; // units of more: a workgroup's, 
 inline int share_groups() { return 2 * device_topology().cus; }
 __host__ __device__ __forceinline__ int cols_of(int line) { return line == 0 ? kNarrowCols : kWideCols; }
 
-// The workgroups that the wide line gets: one per CU at most, since two are hardly faster and leave twice the parts, and no more than have four tiles each.
-__host__ __device__ __forceinline__ int wide_groups(int wide_tiles, int groups) {
-    const int most = (wide_tiles + 3) / 4;
+// The workgroups that the wide line gets: one per CU at most, since two are hardly faster and leave twice the parts, and no more than have four tiles each. A
+// wide run has one tile for each 512 narrow ones of the call, so that with many narrow tiles the wide line ends before the narrow one and leaves it most of the
+// card: the card reads 500 to 600 tiles of heads of 128 while a workgroup works on one wide tile. 256 rows whose 6.4k keys were shared by all and, mostly, by 8 took
+// 67 us so and 79 with a workgroup per CU; 16 384 keys shared by 128 rows with 1024 of their own 110 either way, and no less with fewer.
+__host__ __device__ __forceinline__ int wide_groups(int wide_tiles, int narrow_tiles, int groups) {
+    const int each = narrow_tiles > 4 * 512 ? narrow_tiles / 512 : 4, most = (wide_tiles + each - 1) / each;
     return most < groups / 2 ? most : groups / 2;
 }
 

@@ -85,8 +85,8 @@ struct PageIds {
     __device__ __forceinline__ int32_t of(int sub) const { return __builtin_amdgcn_readlane(ids, sub - first); }
 };
 
-// A unit of up to 16 columns, by one wave, 32 keys at a time: with up to 128 units on a CU one after the other, waves go on to their next by themselves.
-template <class T, int D> __device__ __forceinline__ void narrow_work(const SharedAttentionArgs &a, const Work &k, uint8_t *lds) {
+// A unit of up to 16 CT columns, by one wave, 32 keys at a time: with up to 128 units on a CU one after the other, waves go on to their next by themselves.
+template <class T, int D, int CT> __device__ __forceinline__ void narrow_work(const SharedAttentionArgs &a, const Work &k, uint8_t *lds) {
     using S = Shape<T, D>;
     const int lane = threadIdx.x & 63;
     const int col = lane & 15, quad = lane >> 4;
@@ -98,25 +98,31 @@ template <class T, int D> __device__ __forceinline__ void narrow_work(const Shar
     const uint32_t v_lds = (4 * quad + (col >> 2)) * S::kRowBytes + (col & 3) * 8;
     const float c_scale = a.scale * 1.4426950408889634f;
 
-    u32x4_t q[S::kSteps];
-    const int row = col / a.group_heads;
-    const bool live = col < columns;
-    const uint16_t *q_row = a.q + (live ? (k.s.row0 + row) * a.ldq + static_cast<int64_t>(k.kv_head * a.group_heads + col - row * a.group_heads) * D : 0) + 8 * quad;
+    u32x4_t q[CT][S::kSteps];
+    float4_t o[CT][S::kDTiles];
+    float m[CT], l[CT];
 #pragma unroll
-    for (int s = 0; s < S::kSteps; ++s) {
-        q[s] = live ? *reinterpret_cast<const u32x4_t *>(q_row + 32 * s) : u32x4_t{0, 0, 0, 0};
-    }
-    float4_t o[S::kDTiles];
+    for (int c = 0; c < CT; ++c) {
+        const int column = 16 * c + col, row = column / a.group_heads;
+        const bool live = column < columns;
+        const uint16_t *q_row =
+            a.q + (live ? (k.s.row0 + row) * a.ldq + static_cast<int64_t>(k.kv_head * a.group_heads + column - row * a.group_heads) * D : 0) + 8 * quad;
 #pragma unroll
-    for (int i = 0; i < S::kDTiles; ++i) {
-        o[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < S::kSteps; ++s) {
+            q[c][s] = live ? *reinterpret_cast<const u32x4_t *>(q_row + 32 * s) : u32x4_t{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < S::kDTiles; ++i) {
+            o[c][i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        m[c] = -INFINITY, l[c] = 0.0f;
     }
-    float m = -INFINITY, l = 0.0f;
     bool poisoned = false; // a page outside the cache
 
-    u32x4_t k_reg[2][S::kSteps], v_reg[2][S::kSteps];
+    constexpr int kTilesAhead = D == 64 ? 2 : 1; // 16 KB on the way for each wave keep the memory busy with one workgroup on a CU, 8 KB do not
+    u32x4_t k_reg[kTilesAhead][2][S::kSteps], v_reg[kTilesAhead][2][S::kSteps];
     PageIds ids;
-    const auto request = [&](int tile) {
+    const auto request = [&](int tile, auto &k_reg, auto &v_reg) __attribute__((always_inline)) {
         if (2 * (tile - k.tile0) % 64 == 0) {
             poisoned |= ids.read(at, start, hi, 2 * tile);
         }
@@ -138,8 +144,7 @@ template <class T, int D> __device__ __forceinline__ void narrow_work(const Shar
             }
         }
     };
-    request(k.tile0);
-    for (int tile = k.tile0; tile < k.tile1; ++tile) {
+    const auto step = [&](int tile, auto &k_reg, auto &v_reg) __attribute__((always_inline)) {
         const int key0 = start + tile * kNarrowTile;
         if (key0 < lo) { // values before the first key count as zero, whatever they are
 #pragma unroll
@@ -160,13 +165,20 @@ template <class T, int D> __device__ __forceinline__ void narrow_work(const Shar
                 *reinterpret_cast<u32x4_t *>(lds + to_lds + pieces.lds_step(i) + s * 16 * S::kRowBytes) = k_reg[s][i];
             }
         }
-        float4_t score[2] = {float4_t{0.0f, 0.0f, 0.0f, 0.0f}, float4_t{0.0f, 0.0f, 0.0f, 0.0f}};
+        float4_t score[CT][2];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            score[c][0] = score[c][1] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        }
 #pragma unroll
         for (int i = 0; i < S::kSteps; ++i) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 const uint4 kk = *reinterpret_cast<const uint4 *>(lds + k_lds + s * 16 * S::kRowBytes + 64 * i);
-                score[s] = T::mfma16(kk, __builtin_bit_cast(uint4, q[i]), score[s]);
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    score[c][s] = T::mfma16(kk, __builtin_bit_cast(uint4, q[c][i]), score[c][s]);
+                }
             }
         }
 #pragma unroll
@@ -176,46 +188,49 @@ template <class T, int D> __device__ __forceinline__ void narrow_work(const Shar
                 *reinterpret_cast<u32x4_t *>(lds + to_lds + pieces.lds_step(i) + s * 16 * S::kRowBytes) = v_reg[s][i];
             }
         }
-        if (tile + 1 < k.tile1) {
-            request(tile + 1);
+        if (tile + kTilesAhead < k.tile1) {
+            request(tile + kTilesAhead, k_reg, v_reg);
         }
-        float p[8];
+        u32x4_t upper[CT], lower[CT];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            p[e] = score[e >> 2][e & 3] * c_scale;
-        }
-        if (key0 < lo || key0 + kNarrowTile > hi) {
+        for (int c = 0; c < CT; ++c) {
+            float p[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int key = key0 + 16 * (e >> 2) + 4 * quad + (e & 3);
-                p[e] = key >= lo && key < hi ? p[e] : -INFINITY;
+                p[e] = score[c][e >> 2][e & 3] * c_scale;
             }
-        }
-        float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        if (__any(top > m)) {
-            const float m_new = fmaxf(m, top);
-            const float f = m_new == -INFINITY ? 1.0f : exp2_fast(m - m_new);
-            m = m_new;
-            l *= f;
+            if (key0 < lo || key0 + kNarrowTile > hi) {
 #pragma unroll
-            for (int i = 0; i < S::kDTiles; ++i) {
-                o[i] *= f;
+                for (int e = 0; e < 8; ++e) {
+                    const int key = key0 + 16 * (e >> 2) + 4 * quad + (e & 3);
+                    p[e] = key >= lo && key < hi ? p[e] : -INFINITY;
+                }
             }
-        }
-        const float m_used = m == -INFINITY ? 0.0f : m - Split<T>::kTop;
+            float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            if (__any(top > m[c])) {
+                const float m_new = fmaxf(m[c], top);
+                const float f = m_new == -INFINITY ? 1.0f : exp2_fast(m[c] - m_new);
+                m[c] = m_new;
+                l[c] *= f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            p[e] = exp2_fast(p[e] - m_used);
-            l += p[e];
-        }
-        u32x4_t upper, lower;
+                for (int i = 0; i < S::kDTiles; ++i) {
+                    o[c][i] *= f;
+                }
+            }
+            const float m_used = m[c] == -INFINITY ? 0.0f : m[c] - Split<T>::kTop;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            uint32_t u, v;
-            split<T>(float2_t{p[2 * e], p[2 * e + 1]}, u, v);
-            upper[e] = u, lower[e] = v;
+            for (int e = 0; e < 8; ++e) {
+                p[e] = exp2_fast(p[e] - m_used);
+                l[c] += p[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t u, v;
+                split<T>(float2_t{p[2 * e], p[2 * e + 1]}, u, v);
+                upper[c][e] = u, lower[c][e] = v;
+            }
         }
 #pragma unroll
         for (int i = 0; i < S::kDTiles; ++i) {
@@ -225,21 +240,43 @@ template <class T, int D> __device__ __forceinline__ void narrow_work(const Shar
                 half[s] = lds_read_transposed(lds + v_lds + s * 16 * S::kRowBytes + i * 32);
             }
             const uint4 vt = make_uint4(half[0].x, half[0].y, half[1].x, half[1].y);
-            o[i] = T::mfma16(vt, __builtin_bit_cast(uint4, upper), o[i]);
-            o[i] = T::mfma16(vt, __builtin_bit_cast(uint4, lower), o[i]);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                o[c][i] = T::mfma16(vt, __builtin_bit_cast(uint4, upper[c]), o[c][i]);
+                o[c][i] = T::mfma16(vt, __builtin_bit_cast(uint4, lower[c]), o[c][i]);
+            }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kTilesAhead; ++i) {
+        if (k.tile0 + i < k.tile1) {
+            request(k.tile0 + i, k_reg[i], v_reg[i]);
+        }
+    }
+#pragma unroll 1
+    for (int tile = k.tile0; tile < k.tile1; tile += kTilesAhead) {
+#pragma unroll
+        for (int i = 0; i < kTilesAhead; ++i) {
+            if (i == 0 || tile + i < k.tile1) {
+                step(tile + i, k_reg[i], v_reg[i]);
+            }
         }
     }
 
     const SharedParts parts = carve_parts(a.workspace, shared_columns(a.rows, a.q_heads, a.groups));
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if (live) {
 #pragma unroll
-        for (int i = 0; i < S::kDTiles; ++i) {
-            *reinterpret_cast<float4_t *>(parts.o + (k.part + col) * D + 16 * i + 4 * quad) = o[i];
-        }
-        if (quad == 0) {
-            parts.stats[k.part + col] = make_float2(m, poisoned ? NAN : l);
+    for (int c = 0; c < CT; ++c) {
+        const int column = 16 * c + col;
+        l[c] += __shfl_xor(l[c], 16);
+        l[c] += __shfl_xor(l[c], 32);
+        if (column < columns) {
+#pragma unroll
+            for (int i = 0; i < S::kDTiles; ++i) {
+                *reinterpret_cast<float4_t *>(parts.o + (k.part + column) * D + 16 * i + 4 * quad) = o[c][i];
+            }
+            if (quad == 0) {
+                parts.stats[k.part + column] = make_float2(m[c], poisoned ? NAN : l[c]);
+            }
         }
     }
 }
@@ -266,13 +303,25 @@ template <> struct Halves<F16> {
 };
 
 // Rows of keys and values in LDS as transfers leave them, without padding: 16-byte piece c of row r lies at piece c ^ key(r) or c ^ value(r) of its row, so that
-// 8 rows' pieces of the first product's operand, and 4 rows' pairs of pieces of the second's, lie in different banks.
+// the pieces that 16 lanes read at a time of 16 rows (keys), and 32 or 16 lanes of 4 rows (values), lie in different banks.
 template <int D> struct Swizzle {
     static constexpr int kPerRow = D / 8;
-    static constexpr int kKeys = D == 96 ? 1 : 2, kValues = D == 96 ? 2 : 4; // operands' addresses that are not a constant apart
-    static __device__ __forceinline__ int key(int r) { return D == 96 ? (r >> 1) & 3 : r & 7; }
-    static __device__ __forceinline__ int value(int r) { return D == 96 ? 2 * ((r >> 1) & 1) : 2 * (r & 3); }
+    // Operands whose addresses are not a constant apart.
+    static constexpr int kKeys = D == 64 ? 4 : D == 96 ? 2 : 8, kValues = D == 64 ? 2 : D == 96 ? 1 : 4;
+    static __device__ __forceinline__ int key(int r) { return D == 64 ? (r >> 1) & 7 : D == 96 ? (r >> 2) & 3 : r & 15; }
+    static __device__ __forceinline__ int value(int r) { return D == 64 ? 2 * (r & 3) : D == 96 ? r & 2 : 4 * (r & 1) + 5 * (r & 2); }
 };
+
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+// 32 x 32 x 16: lane L has row (or column) L & 31 of the operands, elements 8 (L >> 5) on; of the result column L & 31, rows 8 (i / 4) + 4 (L >> 5) + i % 4.
+template <class T> __device__ __forceinline__ float16_t mfma32(uint4 x, uint4 y, float16_t c);
+template <> __device__ __forceinline__ float16_t mfma32<F16>(uint4 x, uint4 y, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, x), __builtin_bit_cast(half8_t, y), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ float16_t mfma32<BF16>(uint4 x, uint4 y, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, x), __builtin_bit_cast(bf16x8_t, y), c, 0, 0, 0);
+}
 
 // lds_dma16 without the compiler's knowledge: it would have every read of the ring wait for all transfers to it, and which are done is counted here. Bytes and
 // addresses are uniform; `to` is an LDS address. M0 has no other use in these kernels.
@@ -290,18 +339,22 @@ __device__ __forceinline__ void ring_transfer(u32x4_t resource, uint32_t to, uin
 constexpr int kRing = 4, kAhead = 3;
 template <int D> constexpr int kRingBytes = kRing * 2 * kWideTile * 2 * D;
 
-// A unit of more columns: 16 CT of each wave, up to 128 in all. The four waves share tiles of 32 keys, of which two waves bring the keys and two the values into LDS,
-// 16 rows each. The matrix cores bound it if the vector instructions run beside them, and for that they have to lie between the products in the
-// program, since the two waves of a SIMD hardly overlap otherwise (as many cycles as both kinds' sum were measured): hence the steps above.
-template <class T, int D, int CT> __device__ __forceinline__ void wide_work(const SharedAttentionArgs &a, const Work &k, uint8_t *ring) {
+// A unit of more columns, up to 128: 32 of each wave. The four waves share tiles of 32 keys, of which two waves bring the keys and two the values into LDS,
+// 16 rows each. The matrix cores bound it if the vector instructions run beside them, and for that they have to lie between the products in the program: hence the
+// steps above. Products of 32 x 32 leave them more room than those of 16 x 16 (three vector instructions for each 16 cycles of a product take 30 % longer
+// than the products alone, next to 16 x 16 ones 20 to 60 %).
+//   S^T [key, column] = K Q^T     A = K, 16 elements of 32 keys; B = Q^T, in registers
+//   O^T [d, column] += V^T P^T    A = V^T, 32 elements of 16 keys, read transposed; B = P^T, as it leaves S^T: keys 16 t + 4 (L >> 5) + j and 8 behind them
+template <class T, int D> __device__ __forceinline__ void wide_work(const SharedAttentionArgs &a, const Work &k, uint8_t *ring) {
     using S = Shape<T, D>;
     using Z = Swizzle<D>;
     constexpr int kRow = 2 * D, kPlane = kWideTile * kRow; // a tile's keys, or values
+    constexpr int kKeySteps = D / 16, kBlocks = D / 32;    // of the first product, and of the second's rows
     // The maximum follows only when a score passes it by more than a factor 2^kSlack, and is one of the scores before their factor
     // (hm_paged_attention_prompt.hpp). fp16 weights have 2^9 at the maximum, so that they end at 2^15 and lose what is below 2^-33 of it.
     constexpr float kSlack = Split<T>::kTop > 0.0f ? 6.0f : 16.0f, kTop = Split<T>::kTop > 0.0f ? Split<T>::kTop - kSlack : 0.0f;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-    const int col = lane & 15, quad = lane >> 4;
+    const int col = lane & 31, side = lane >> 5;
     const int columns = k.rows * a.group_heads, start = k.s.start() + k.tile0 * kWideTile, lo = k.s.lo, hi = min(k.s.hi, k.s.start() + k.tile1 * kWideTile);
     const int tiles = k.tile1 - k.tile0;
     const Pages at(a, k.s.row0, k.kv_head);
@@ -323,16 +376,16 @@ template <class T, int D, int CT> __device__ __forceinline__ void wide_work(cons
     const float c_scale = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 0x1p-126f);
     const float slack = fminf(kSlack / c_scale, 0x1p126f); // of scores without the factor
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
-    u32x4_t q[CT][S::kSteps];
-#pragma unroll
-    for (int c = 0; c < CT; ++c) {
-        const int j = 16 * (wave * CT + c) + col, row = j / a.group_heads;
-        const bool live = j < columns;
+    const int column = 32 * wave + col;
+    const bool live = column < columns;
+    u32x4_t q[kKeySteps];
+    {
+        const int row = column / a.group_heads;
         const uint16_t *q_row =
-            a.q + (live ? (k.s.row0 + k.row + row) * a.ldq + static_cast<int64_t>(k.kv_head * a.group_heads + j - row * a.group_heads) * D : 0) + 8 * quad;
+            a.q + (live ? (k.s.row0 + k.row + row) * a.ldq + static_cast<int64_t>(k.kv_head * a.group_heads + column - row * a.group_heads) * D : 0) + 8 * side;
 #pragma unroll
-        for (int s = 0; s < S::kSteps; ++s) {
-            q[c][s] = live ? *reinterpret_cast<const u32x4_t *>(q_row + 32 * s) ^ sign : u32x4_t{0, 0, 0, 0};
+        for (int i = 0; i < kKeySteps; ++i) {
+            q[i] = live ? *reinterpret_cast<const u32x4_t *>(q_row + 16 * i) ^ sign : u32x4_t{0, 0, 0, 0};
         }
     }
     check_ids();
@@ -345,7 +398,7 @@ template <class T, int D, int CT> __device__ __forceinline__ void wide_work(cons
 #pragma unroll
     for (int j = 0; j < S::kSteps; ++j) {
         const int r = (j * 64 + lane) / Z::kPerRow, c = (j * 64 + lane) % Z::kPerRow;
-        from[j] = r * at.row_bytes + (c ^ (of_values ? Z::value(r) : Z::key(r))) * 16;
+        from[j] = r * at.row_bytes + (c ^ (of_values ? Z::value(r) : Z::key(16 * sub + r))) * 16;
     }
     const uint16_t *head = of_values ? at.v_head : at.k_head;
     const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)ring)) + (of_values ? kPlane : 0) + sub * 16 * kRow;
@@ -375,58 +428,43 @@ template <class T, int D, int CT> __device__ __forceinline__ void wide_work(cons
     uint32_t k_lds[Z::kKeys], v_lds[Z::kValues];
 #pragma unroll
     for (int i = 0; i < Z::kKeys; ++i) {
-        k_lds[i] = col * kRow + ((4 * i + quad) ^ Z::key(col)) * 16;
+        k_lds[i] = col * kRow + ((2 * i + side) ^ Z::key(col)) * 16;
     }
 #pragma unroll
     for (int i = 0; i < Z::kValues; ++i) {
-        const int r = 4 * quad + (col >> 2);
-        v_lds[i] = kPlane + r * kRow + ((2 * i + ((col & 3) >> 1)) ^ Z::value(r)) * 16 + (col & 1) * 8;
+        const int r = 4 * side + ((lane & 15) >> 2);
+        v_lds[i] = kPlane + r * kRow + ((4 * i + 2 * (lane >> 4 & 1) + ((lane & 3) >> 1)) ^ Z::value(r)) * 16 + (lane & 1) * 8;
     }
-    float4_t o[CT][S::kDTiles];
-    float m[CT], l[CT];
+    float16_t o[kBlocks];
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-#pragma unroll
-        for (int i = 0; i < S::kDTiles; ++i) {
-            o[c][i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-        m[c] = -INFINITY, l[c] = 0.0f;
+    for (int i = 0; i < kBlocks; ++i) {
+        o[i] = float16_t{};
     }
+    float m = -INFINITY, l = 0.0f;
     struct Weights {
-        u32x4_t upper[CT], lower[CT];
+        u32x4_t upper[2], lower[2];
     };
-    typedef float4_t Scores[CT][2];
-    const auto first_product = [&](int tile, Scores &score) __attribute__((always_inline)) {
-        const uint8_t *keys = ring + (tile % kRing) * 2 * kPlane;
+    const auto first_product = [&](int place, float16_t &score) __attribute__((always_inline)) {
+        score = float16_t{};
 #pragma unroll
-        for (int i = 0; i < S::kSteps; ++i) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const uint4 kk = *reinterpret_cast<const uint4 *>(keys + k_lds[i % Z::kKeys] + s * 16 * kRow + i / Z::kKeys * Z::kKeys * 64);
-#pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    score[c][s] = T::mfma16(kk, __builtin_bit_cast(uint4, q[c][i]), i == 0 ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : score[c][s]);
-                }
-            }
+        for (int i = 0; i < kKeySteps; ++i) {
+            const uint4 kk = *reinterpret_cast<const uint4 *>(ring + place * 2 * kPlane + k_lds[i % Z::kKeys] + i / Z::kKeys * Z::kKeys * 32);
+            score = mfma32<T>(kk, __builtin_bit_cast(uint4, q[i]), score);
         }
     };
-    const auto second_product = [&](int tile, const Weights &w) __attribute__((always_inline)) {
-        const uint8_t *values = ring + (tile % kRing) * 2 * kPlane;
+    const auto second_product = [&](int place, const Weights &w) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < S::kDTiles; ++i) {
-            uint2 half[2];
+        for (int t = 0; t < 2; ++t) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                half[s] = lds_read_transposed(values + v_lds[i % Z::kValues] + s * 16 * kRow + i / Z::kValues * Z::kValues * 32);
-            }
-            const uint4 vt = make_uint4(half[0].x, half[0].y, half[1].x, half[1].y);
+            for (int i = 0; i < kBlocks; ++i) {
+                uint2 half[2];
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                o[c][i] = T::mfma16(vt, __builtin_bit_cast(uint4, w.upper[c]), o[c][i]);
-            }
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                o[c][i] = T::mfma16(vt, __builtin_bit_cast(uint4, w.lower[c]), o[c][i]);
+                for (int s = 0; s < 2; ++s) {
+                    half[s] = lds_read_transposed(ring + place * 2 * kPlane + v_lds[i % Z::kValues] + (16 * t + 8 * s) * kRow + i / Z::kValues * Z::kValues * 64);
+                }
+                const uint4 vt = make_uint4(half[0].x, half[0].y, half[1].x, half[1].y);
+                o[i] = mfma32<T>(vt, __builtin_bit_cast(uint4, w.upper[t]), o[i]);
+                o[i] = mfma32<T>(vt, __builtin_bit_cast(uint4, w.lower[t]), o[i]);
             }
         }
     };
@@ -437,10 +475,11 @@ template <class T, int D, int CT> __device__ __forceinline__ void wide_work(cons
             }
         }
     };
-    const bool works = 16 * wave * CT < columns;
-    // Step n: scores of tile n in `score`, weights of tile n - 1 in `before`; leaves those of n + 1 and n.
-    const auto step = [&](auto first, int n, Scores &score, Scores &next, Weights &before, Weights &weights) __attribute__((always_inline)) {
+    const bool works = 32 * wave < columns;
+    // Step n, with n % kRing = place: scores of tile n in `score`, weights of tile n - 1 in `before`; leaves those of n + 1 and n.
+    const auto step = [&](auto first, int n, auto place, float16_t &score, float16_t &next, Weights &before, Weights &weights) __attribute__((always_inline)) {
         constexpr bool kFirst = decltype(first)::value; // tile 0: there is none before
+        constexpr int kPlace = decltype(place)::value;
         wait_vmcnt<(kAhead - 1) * S::kSteps>(); // the wave's transfers that this step needs are done, those of two steps may be on the way
         if (n == 1) {
             clear_before();
@@ -460,86 +499,68 @@ template <class T, int D, int CT> __device__ __forceinline__ void wide_work(cons
         if (key0 < lo || key0 + kWideTile > hi) {
             __builtin_amdgcn_sched_barrier(0); // keeps this a branch
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int key = key0 + 16 * (e >> 2) + 4 * quad + (e & 3);
-                if (key < lo || key >= hi) {
-#pragma unroll
-                    for (int c = 0; c < CT; ++c) {
-                        score[c][e >> 2][e & 3] = -INFINITY;
-                    }
-                }
+            for (int e = 0; e < 16; ++e) {
+                const int key = key0 + 8 * (e >> 2) + 4 * side + (e & 3);
+                score[e] = key < lo || key >= hi ? -INFINITY : score[e];
             }
         }
-        float top[CT];
-        bool follow = false;
+        float top = score[0];
 #pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            top[c] = score[c][0][0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) {
-                top[c] = fmaxf(top[c], score[c][e >> 2][e & 3]);
-            }
-            follow |= top[c] > m[c] + slack;
+        for (int e = 1; e < 16; ++e) {
+            top = fmaxf(top, score[e]);
         }
-        if (__any(follow)) {
+        if (__any(top > m + slack)) {
             if constexpr (!kFirst) { // what is on the way is relative to the old maximum
-                second_product(n - 1, before);
-#pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    before.upper[c] = before.lower[c] = u32x4_t{0, 0, 0, 0};
-                }
+                second_product((kPlace + kRing - 1) % kRing, before);
+                before = Weights{};
             }
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float m_new = fmaxf(m, top);
+            const float f = m_new == -INFINITY ? 1.0f : exp2_fast((m - m_new) * c_scale);
+            m = m_new;
+            l *= f;
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                top[c] = fmaxf(top[c], __shfl_xor(top[c], 16));
-                top[c] = fmaxf(top[c], __shfl_xor(top[c], 32));
-                const float m_new = fmaxf(m[c], top[c]);
-                const float f = m_new == -INFINITY ? 1.0f : exp2_fast((m[c] - m_new) * c_scale);
-                m[c] = m_new;
-                l[c] *= f;
-#pragma unroll
-                for (int i = 0; i < S::kDTiles; ++i) {
-                    o[c][i] *= f;
-                }
+            for (int i = 0; i < kBlocks; ++i) {
+                o[i] *= f;
             }
         }
-        const auto work_out = [&] {
+        first_product((kPlace + 1) % kRing, next); // behind the last tile: of zeros
+        const float m_used = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                const float m_used = m[c] == -INFINITY ? 0.0f : m[c];
+        for (int e = 0; e < 16; e += 2) {
+            float2_t p;
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    float2_t p;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        p[i] = exp2_fast(__builtin_fmaf(score[c][e >> 2][(e & 3) + i] - m_used, c_scale, kTop));
-                        l[c] += p[i];
-                    }
-                    uint32_t u, v;
-                    Halves<T>::split(p, u, v);
-                    weights.upper[c][e / 2] = u, weights.lower[c][e / 2] = v;
-                }
+            for (int i = 0; i < 2; ++i) {
+                p[i] = exp2_fast(__builtin_fmaf(score[e + i] - m_used, c_scale, kTop));
+                l += p[i];
             }
-        };
-        first_product(n + 1, next); // behind the last tile: of zeros
-        work_out();
+            uint32_t u, v;
+            Halves<T>::split(p, u, v);
+            weights.upper[e >> 3][(e & 7) / 2] = u, weights.lower[e >> 3][(e & 7) / 2] = v;
+        }
         if constexpr (!kFirst) {
-            second_product(n - 1, before);
+            second_product((kPlace + kRing - 1) % kRing, before);
         }
     };
-    Scores score_even, score_odd;
+    float16_t score_even, score_odd;
     Weights even{}, odd{};
     wait_vmcnt<kAhead * S::kSteps>(); // of keys: those of the first tile; of values: no more are on the way
     lds_barrier();
     if (works) {
         first_product(0, score_even);
     }
-    step(std::true_type{}, 0, score_even, score_odd, odd, even);
+    step(std::true_type{}, 0, std::integral_constant<int, 0>{}, score_even, score_odd, odd, even);
 #pragma unroll 1
-    for (int n = 1; n < tiles; n += 2) {
-        step(std::false_type{}, n, score_odd, score_even, even, odd);
+    for (int n = 1; n < tiles; n += kRing) {
+        step(std::false_type{}, n, std::integral_constant<int, 1>{}, score_odd, score_even, even, odd);
         if (n + 1 < tiles) {
-            step(std::false_type{}, n + 1, score_even, score_odd, odd, even);
+            step(std::false_type{}, n + 1, std::integral_constant<int, 2>{}, score_even, score_odd, odd, even);
+        }
+        if (n + 2 < tiles) {
+            step(std::false_type{}, n + 2, std::integral_constant<int, 3>{}, score_odd, score_even, even, odd);
+        }
+        if (n + 3 < tiles) {
+            step(std::false_type{}, n + 3, std::integral_constant<int, 0>{}, score_even, score_odd, odd, even);
         }
     }
     wait_vmcnt<0>();
@@ -548,24 +569,23 @@ template <class T, int D, int CT> __device__ __forceinline__ void wide_work(cons
     }
     lds_barrier();
     if (works) {
-        second_product(tiles - 1, (tiles & 1) != 0 ? even : odd);
+        second_product((tiles - 1) % kRing, (tiles & 1) != 0 ? even : odd);
     }
 
     const SharedParts parts = carve_parts(a.workspace, shared_columns(a.rows, a.q_heads, a.groups));
+    l += __shfl_xor(l, 32);
+    if (live) {
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-        l[c] += __shfl_xor(l[c], 16);
-        l[c] += __shfl_xor(l[c], 32);
-        const int j = 16 * (wave * CT + c) + col;
-        if (j < columns) {
+        for (int i = 0; i < kBlocks; ++i) {
 #pragma unroll
-            for (int i = 0; i < S::kDTiles; ++i) {
-                *reinterpret_cast<float4_t *>(parts.o + (k.part + j) * D + 16 * i + 4 * quad) = o[c][i];
+            for (int e = 0; e < 4; ++e) {
+                *reinterpret_cast<float4_t *>(parts.o + (k.part + column) * D + 32 * i + 8 * e + 4 * side) =
+                    float4_t{o[i][4 * e], o[i][4 * e + 1], o[i][4 * e + 2], o[i][4 * e + 3]};
             }
-            if (quad == 0) {
-                // relative to the maximum as narrow units have it: with the factor, and with weights from 2^Split::kTop down
-                parts.stats[k.part + j] = make_float2(m[c] * c_scale + (Split<T>::kTop - kTop), poisoned ? NAN : l[c]);
-            }
+        }
+        if (side == 0) {
+            // relative to the maximum as narrow units have it: with the factor, and with weights from 2^Split::kTop down
+            parts.stats[k.part + column] = make_float2(m * c_scale + (Split<T>::kTop - kTop), poisoned ? NAN : l);
         }
     }
     lds_barrier(); // the next unit takes the ring
@@ -590,12 +610,7 @@ template <class T, int D> __global__ void __launch_bounds__(kThreads, D <= 128 ?
         const int xcd = blockIdx.x % a.xcds, w = xcd * (wide / a.xcds) + min(xcd, wide % a.xcds) + static_cast<int>(blockIdx.x / a.xcds), x_end = runs.begin(w + 1);
         int x = runs.begin(w), at = uniform(plan.starts[1][w]);
         while (x < x_end) {
-            const Work k = next_work<1>(a, plan.segments[1], at, x, x_end, w);
-            if (k.rows * a.group_heads > 64) {
-                wide_work<T, D, 2>(a, k, lds);
-            } else {
-                wide_work<T, D, 1>(a, k, lds);
-            }
+            wide_work<T, D>(a, next_work<1>(a, plan.segments[1], at, x, x_end, w), lds);
         }
         return;
     }
@@ -604,7 +619,12 @@ template <class T, int D> __global__ void __launch_bounds__(kThreads, D <= 128 ?
     const int x_end = runs.begin(w + 1);
     int x = runs.begin(w), at = uniform(plan.starts[0][w]);
     while (x < x_end) {
-        narrow_work<T, D>(a, next_work<0>(a, plan.segments[0], at, x, x_end, w), lds + wave * S::kRegion);
+        const Work k = next_work<0>(a, plan.segments[0], at, x, x_end, w);
+        if (k.rows * a.group_heads <= 16) {
+            narrow_work<T, D, 1>(a, k, lds + wave * S::kRegion);
+        } else {
+            narrow_work<T, D, 2>(a, k, lds + wave * S::kRegion);
+        }
     }
 }
 

@@ -62,7 +62,7 @@ def check_plan(share, table, positions, requests, ps):
         at, begin = 0, []
         for row0, rows, lo, hi, tile0, n, slot0, chunk in line.tolist():
             assert 0 <= row0 and rows > 0 and row0 + rows <= share.rows and 0 <= lo < hi and tile0 == at
-            assert (rows * group > 16) == (i == 1) and n == -(-(hi - lo // 16 * 16) // 32)
+            assert (rows * group > 32) == (i == 1) and n == -(-(hi - lo // 16 * 16) // 32)
             assert rows == 1 or lo % 16 == 0
             assert chunk >= 1 and (chunk * group <= 128 if i else chunk == rows)
             begin.append(at)
@@ -95,7 +95,7 @@ def check_plan(share, table, positions, requests, ps):
             if n == 0:
                 continue
             row0, count, lo, hi, tile0, tiles_of, _, chunk = by_slot[slot0].tolist()
-            assert (n, rows, row, line) == (tiles_of, count, t - row0, int(count * group > 16)) and 0 <= row < rows and in_chunk == row % chunk
+            assert (n, rows, row, line) == (tiles_of, count, t - row0, int(count * group > 32)) and 0 <= row < rows and in_chunk == row % chunk
             assert tile == tile0 + row // chunk * n and per_head == n * -(-rows // chunk)
             keys.append((lo, hi))
         keys.sort()
