@@ -1,23 +1,28 @@
 // Beam search's selection: of the continuations of a request's beams the k best, by score + logit - log(sum of exp(logits)).
 //
-// Bound by memory: the logits are read once (2 bytes each in 16 bits), 64 requests of 4 beams and 152064 tokens 78 MB. A wave takes 64 bytes a lane of one row
-// into registers and works out its maximum, the sum of exp relative to it and its k best tokens; a second launch, a workgroup per request, joins the
-// waves' sums in fp64 and picks the k best of all their candidates. Candidates of one row are compared by their logits, which are exact; those of
-// different rows by fp64 scores, since their sums' errors (about 1e-8 relative: fp32 sums of 32 terms, joined in fp64) should not decide which comes first.
+// Bound by memory and, nearly as much, by the instructions of a first launch, which reads the logits once: 64 requests of 4 beams and 152064 tokens have 78 MB of
+// them in 16 bits. A wave takes 32 elements a lane of one row into registers and works out its maximum, the sum of exp relative to it and its k best tokens. A
+// second launch, a workgroup per request, joins the waves' sums and picks the k best of their candidates. It is bound by latency: of the waves' best ones only
+// those that reach the k-th score's bound are looked at closely. With all candidates compared it took 26 to 34 us, so 7. Candidates of one row are compared by their
+// logits, which are exact; those of different rows by fp64 scores, so that rounding adds no ties.
 //
 // The k best of a wave's 2048: the k-th largest of the 64 lanes' maxima, found by sorting them over the lanes, is a bound that at least k elements reach and
-// seldom many more; those go to a list in LDS and are ranked by counting who comes before. Many equal or badly spread elements overflow the list;
-// then the best are taken one after the other.
+// seldom many more; those go to a list in LDS and are ranked by counting who comes before. (The least of k or more groups' maxima is quicker to find, but
+// almost three times as many reach it: 37 us instead of 21 for the case above. 64 elements a lane, with fewer sorts, took 40.) Many equal or badly spread
+// elements overflow the list; then the best are taken one after the other.
 #include "hm_device.hpp"
 #include "hm_internal.hpp"
+
+#include <algorithm>
 
 namespace hm {
 namespace {
 
-constexpr int kVectors = 4;    // 16-byte loads of a lane
-constexpr int kList = 192;     // candidates that a wave's list holds
-constexpr int kJoinThreads = 256;
-constexpr int kJoinList = 1024;
+constexpr int kList = 192;       // candidates that a wave's list holds
+constexpr int kJoinList = 1024;  // and that of a request
+constexpr int kJoinParts = 1024; // parts that are looked at at once
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 struct Fp32 {
     static __device__ __forceinline__ float to_float(uint32_t bits) { return __uint_as_float(bits); }
@@ -25,19 +30,14 @@ struct Fp32 {
 
 template <class T> struct Elements {
     static constexpr int kOf16Bytes = 8;
-    static __device__ __forceinline__ float get(const uint4 &v, int i) {
-        const uint32_t w = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
-        return T::to_float(i & 1 ? w >> 16 : w & 0xFFFFu);
-    }
+    static __device__ __forceinline__ float get(const u32x4_t &v, int i) { return T::to_float(i & 1 ? v[i / 2] >> 16 : v[i / 2] & 0xFFFFu); }
 };
 template <> struct Elements<Fp32> {
     static constexpr int kOf16Bytes = 4;
-    static __device__ __forceinline__ float get(const uint4 &v, int i) { return __uint_as_float(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w); }
+    static __device__ __forceinline__ float get(const u32x4_t &v, int i) { return __uint_as_float(v[i]); }
 };
 
-template <class T> constexpr int wave_elements() { return 64 * kVectors * Elements<T>::kOf16Bytes; }
-
-struct Candidate {
+struct alignas(8) Candidate {
     float logit;
     int32_t token;
 };
@@ -57,55 +57,90 @@ __device__ __forceinline__ bool is_open(const BeamSelectArgs &a, int64_t row) {
     return (a.ended == nullptr || a.ended[row] == 0) && fabsf(a.scores[row]) < INFINITY;
 }
 
-// The k-th largest value of the lanes': sorted downwards over the lanes.
-__device__ __forceinline__ float kth_of_lanes(float v, int k) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int size = 2; size <= 64; size <<= 1) {
-#pragma unroll
-        for (int step = size >> 1; step > 0; step >>= 1) {
-            const float other = __shfl_xor(v, step);
-            const bool keep_more = ((lane & step) == 0) == ((lane & size) == 0 || size == 64);
-            v = keep_more ? fmaxf(v, other) : fminf(v, other);
-        }
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+
+// The values of a lane and of the one whose number has bit STEP changed, in either order, without passing through LDS.
+template <int STEP> __device__ __forceinline__ float2 both(float v) {
+    if constexpr (STEP <= 8) { // quad_perm, row_half_mirror (^ 7) of quad_perm (^ 3), row_ror
+        return make_float2(v, STEP == 1 ? dpp<0xB1>(v) : STEP == 2 ? dpp<0x4E>(v) : STEP == 4 ? dpp<0x141>(dpp<0x1B>(v)) : dpp<0x128>(v));
+    } else {
+        typedef unsigned pair_t __attribute__((ext_vector_type(2)));
+        const unsigned bits = __float_as_uint(v);
+        const pair_t p = STEP == 16 ? __builtin_bit_cast(pair_t, __builtin_amdgcn_permlane16_swap(bits, bits, false, false))
+                                    : __builtin_bit_cast(pair_t, __builtin_amdgcn_permlane32_swap(bits, bits, false, false));
+        return make_float2(__uint_as_float(p.x), __uint_as_float(p.y));
     }
-    return __shfl(v, k - 1);
+}
+
+template <int STEP = 1, class F> __device__ __forceinline__ float over_lanes(float v, F f) {
+    const float2 p = both<STEP>(v);
+    v = f(p.x, p.y);
+    if constexpr (STEP < 32) {
+        v = over_lanes<2 * STEP>(v, f);
+    }
+    return v;
+}
+
+// Steps of a bitonic sort downwards over the lanes: runs of SIZE sorted, from pairs STEP lanes apart.
+template <int SIZE, int STEP> __device__ __forceinline__ float sort_steps(float v, int lane) {
+    const float2 p = both<STEP>(v);
+    const float more = fmaxf(p.x, p.y), less = fminf(p.x, p.y);
+    v = ((lane & STEP) == 0) == ((lane & SIZE) == 0 || SIZE == 64) ? more : less;
+    if constexpr (STEP > 1) {
+        return sort_steps<SIZE, STEP / 2>(v, lane);
+    } else if constexpr (SIZE < 64) {
+        return sort_steps<2 * SIZE, SIZE>(v, lane);
+    } else {
+        return v;
+    }
+}
+
+// The k-th largest value of the lanes'.
+__device__ __forceinline__ float kth_of_lanes(float v, int k) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sort_steps<2, 1>(v, threadIdx.x & 63)), k - 1));
 }
 
 __device__ __forceinline__ bool before(float v, int32_t token, float w, int32_t other) { return v > w || (v == w && token < other); }
 
-template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(BeamSelectArgs a) {
+// A wave per part of a row: V 16-byte loads a lane.
+template <class T, int V> __global__ void __launch_bounds__(256, 4) beam_parts_kernel(BeamSelectArgs a) {
     using E = Elements<T>;
-    constexpr int kOne = E::kOf16Bytes, kMine = kVectors * kOne;
+    constexpr int kOne = E::kOf16Bytes, kMine = V * kOne;
     __shared__ Candidate list[4][kList];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int64_t row = blockIdx.y;
     const int part = static_cast<int>(blockIdx.x) * 4 + wave;
-    if (part >= a.parts || !is_open(a, row)) {
+    if (part >= a.parts) {
         return;
     }
     // 16-byte pieces from the one on that holds the row's first element: what lies around the row's elements in its first and last piece is read, not used.
     const int64_t bytes = 16 / kOne, start = reinterpret_cast<int64_t>(a.logits) + row * a.ld * bytes;
-    const int skip = static_cast<int>(start & 15) / static_cast<int>(bytes);
-    const uint4 *pieces = reinterpret_cast<const uint4 *>(start & ~int64_t(15));
-    const int vocabulary = static_cast<int>(a.vocabulary), last_piece = (vocabulary + skip - 1) / kOne;
-    const int first = part * (64 * kVectors);
-    uint4 raw[kVectors];
+    const int skip = uniform(static_cast<int>(start & 15) / static_cast<int>(bytes));
+    const int vocabulary = static_cast<int>(a.vocabulary), pieces = (vocabulary + skip + kOne - 1) / kOne;
+    const int first = part * (64 * V);
+    void *const from_piece = reinterpret_cast<void *>((start & ~int64_t(15)) + static_cast<int64_t>(first) * 16);
+    const __amdgpu_buffer_rsrc_t resource = __builtin_amdgcn_make_buffer_rsrc(from_piece, 0, uniform(min(64 * V, pieces - first) * 16), 0x00020000);
+    if (!is_open(a, row)) {
+        return;
+    }
+    u32x4_t raw[V];
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-        const int piece = first + i * 64 + lane;
-        raw[i] = piece <= last_piece ? pieces[piece] : uint4{};
+    for (int i = 0; i < V; ++i) { // behind the last piece: zeros
+        raw[i] = __builtin_amdgcn_raw_buffer_load_b128(resource, lane * 16, i * 1024, 0);
     }
     float x[kMine];
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
+    for (int i = 0; i < V; ++i) {
 #pragma unroll
         for (int e = 0; e < kOne; ++e) {
             x[i * kOne + e] = E::get(raw[i], e);
         }
     }
-    const auto token_of = [&](int j) { return (first + j / kOne * 64 + lane) * kOne + j % kOne - skip; };
-    if (first == 0 || first + kVectors * 64 > last_piece) { // elements that are not the row's
+    int first_token = (first + lane) * kOne - skip;
+    const auto token_of = [&](int j) { return first_token + j / kOne * 64 * kOne + j % kOne; };
+    if (first == 0 || first + V * 64 >= pieces) { // elements that are not the row's
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
             const int token = token_of(j);
@@ -117,31 +152,32 @@ template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(Beam
     for (int j = 1; j < kMine; ++j) {
         most = fmaxf(most, x[j]);
     }
-    float top = most;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        top = fmaxf(top, __shfl_xor(top, off));
-    }
+    const int k = a.k;
+    const float top = over_lanes(most, [](float v, float w) { return fmaxf(v, w); });
     // An infinity or NaN among the logits makes the sum NaN.
     const float from = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kMine; ++j) {
-        sum += __builtin_amdgcn_exp2f((x[j] - from) * 1.4426950408889634f);
-    }
+    for (int i = 0; i < V; ++i) {
+        float some = 0.0f;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        sum += __shfl_xor(sum, off);
+        for (int e = 0; e < kOne; ++e) {
+            some += __builtin_amdgcn_exp2f((x[i * kOne + e] - from) * 1.4426950408889634f);
+        }
+        sum += some;
     }
+    sum = over_lanes(sum, [](float v, float w) { return v + w; });
     const BeamWorkspace ws = carve_beam(a.workspace, a.rows, a.parts);
     const int64_t at = row * a.parts + part;
     if (lane == 0) {
         ws.stats[at] = make_float2(top, sum);
     }
-    const int k = a.k;
     Candidate *out = ws.candidates + at * k;
     const float bound = fmaxf(kth_of_lanes(most, k), -3.4028234663852886e38f); // -infinity is no candidate
     Candidate *mine = list[wave];
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("" : "+v"(first_token)); // the tokens are worked out again rather than kept in registers
+#endif
     int count = 0;
 #pragma unroll
     for (int j = 0; j < kMine; ++j) {
@@ -156,10 +192,29 @@ template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(Beam
         }
     }
     __builtin_amdgcn_wave_barrier(); // a wave's LDS accesses are carried out in order
+    if (count <= 64) {
+        const Candidate c = lane < count ? mine[lane] : Candidate{-INFINITY, -1};
+        // in the order of the values, equal ones (zeros of either sign, too) by token
+        const uint32_t bits = __float_as_uint(c.logit + 0.0f), upper = bits ^ ((bits >> 31) != 0 ? 0xFFFFFFFFu : 0x80000000u), lower = ~static_cast<uint32_t>(c.token);
+        const uint64_t key = static_cast<uint64_t>(upper) << 32 | lower;
+        int rank = 0;
+        for (int j = 0; j < count; ++j) {
+            const uint32_t u = __builtin_amdgcn_readlane(upper, j), v = __builtin_amdgcn_readlane(lower, j);
+            rank += (static_cast<uint64_t>(u) << 32 | v) > key;
+        }
+        if (lane < count && rank < k) {
+            out[rank] = c;
+        }
+        if (lane >= count && lane < k) {
+            out[lane] = Candidate{-INFINITY, -1};
+        }
+        return;
+    }
     if (count <= kList) {
         for (int i = lane; i < count; i += 64) {
             const Candidate c = mine[i];
             int rank = 0;
+#pragma unroll 4
             for (int j = 0; j < count; ++j) {
                 const Candidate d = mine[j];
                 rank += before(d.logit, d.token, c.logit, c.token);
@@ -168,21 +223,23 @@ template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(Beam
                 out[rank] = c;
             }
         }
-        for (int i = count + lane; i < k; i += 64) {
-            out[i] = Candidate{-INFINITY, -1};
-        }
         return;
     }
     float last = INFINITY;
     int32_t last_token = -1;
-    for (int i = 0; i < k; ++i) { // the best behind the last one taken
+    for (int i = 0; i < k; ++i) { // the best behind the last one taken, from memory: seldom, and little code
         float best = -INFINITY;
         int32_t token = INT32_MAX;
+#pragma unroll 1
+        for (int j = 0; j < V; ++j) {
+            const u32x4_t piece = __builtin_amdgcn_raw_buffer_load_b128(resource, lane * 16, j * 1024, 0);
 #pragma unroll
-        for (int j = 0; j < kMine; ++j) {
-            const int32_t t = token_of(j);
-            if (before(last, last_token, x[j], t) && before(x[j], t, best, token)) {
-                best = x[j], token = t;
+            for (int e = 0; e < kOne; ++e) {
+                const int32_t t = token_of(j * kOne + e);
+                const float v = t >= 0 && t < vocabulary ? E::get(piece, e) : -INFINITY;
+                if (before(last, last_token, v, t) && before(v, t, best, token)) {
+                    best = v, token = t;
+                }
             }
         }
 #pragma unroll
@@ -212,107 +269,125 @@ __device__ __forceinline__ bool before(const Scored &a, const Scored &b) {
     return a.score > b.score || (a.score == b.score && (a.beam < b.beam || (a.beam == b.beam && before(a.logit, a.token, b.logit, b.token))));
 }
 
+__device__ __forceinline__ Scored better(const Scored &a, const Scored &b) { // by fields: the whole would be picked in memory
+    const bool first = before(a, b);
+    return Scored{first ? a.score : b.score, first ? a.beam : b.beam, first ? a.logit : b.logit, first ? a.token : b.token};
+}
+
 constexpr Scored kNone{-INFINITY, INT32_MAX, -INFINITY, INT32_MAX};
 
-// A workgroup per request.
-__global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(BeamSelectArgs a) {
+__device__ __forceinline__ float rounded_down(double v) {
+    const float f = static_cast<float>(v);
+    return static_cast<double>(f) > v ? nextafterf(f, -INFINITY) : f;
+}
+
+// A workgroup per request. The scores of the parts' best candidates bound the k-th score from below, and only parts whose best one reaches that bound are looked at
+// more closely: about k of them.
+template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kernel(BeamSelectArgs a) {
+    constexpr int kWaves = THREADS / 64, kHeld = 2;
     __shared__ double norm[HM_BEAM_MAX_BEAMS], base[HM_BEAM_MAX_BEAMS]; // base NaN: the row has no candidates from its logits
     __shared__ uint8_t was_ended[HM_BEAM_MAX_BEAMS];
-    __shared__ double maxima[kJoinThreads];
+    __shared__ float maxima[kWaves][64];
+    __shared__ float best_of[kJoinParts]; // parts' best scores, rounded down; of the first ones
+    __shared__ int32_t work[kJoinParts];
     __shared__ Scored list[kJoinList];
-    __shared__ Scored wave_best[kJoinThreads / 64];
-    __shared__ int listed;
-    __shared__ double bound_at;
+    __shared__ Scored wave_best[kWaves];
+    __shared__ int listed, works;
+    __shared__ double next_bound;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int beams = a.beams, k = a.k, parts = a.parts;
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * beams;
     const BeamWorkspace ws = carve_beam(a.workspace, a.rows, parts);
-    for (int beam = wave; beam < beams; beam += kJoinThreads / 64) {
+    float own = -INFINITY; // the best of those parts that are the lane's: part i of all beams' is lane i % 64's
+    for (int beam = wave; beam < beams; beam += kWaves) {
         const int64_t row = row0 + beam;
-        const bool open = is_open(a, row);
+        const int shift = (lane - beam * parts) & 63;
+        const float2 *stats = ws.stats + row * parts;
+        float2 held[kHeld];
+#pragma unroll
+        for (int n = 0; n < kHeld; ++n) { // of a row that is not open they are not there, and not used
+            const int i = shift + 64 * n;
+            held[n] = stats[min(i, parts - 1)];
+            held[n] = i < parts ? held[n] : make_float2(-INFINITY, 0.0f);
+        }
+        const float score = a.scores[row];
+        const bool ended = a.ended != nullptr && a.ended[row] != 0, open = !ended && fabsf(score) < INFINITY;
         float top = -INFINITY;
         bool odd = false;
-        for (int i = lane; open && i < parts; i += 64) {
-            const float2 st = ws.stats[row * parts + i];
-            top = fmaxf(top, st.x);
-            odd |= !(st.y < INFINITY);
-        }
+        const auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) {
-            top = fmaxf(top, __shfl_xor(top, off));
+            for (int n = 0; n < kHeld; ++n) {
+                f(shift + 64 * n, held[n]);
+            }
+            for (int i = shift + 64 * kHeld; i < parts; i += 64) {
+                f(i, stats[i]);
+            }
+        };
+        float sum = 0.0f;
+        if (open) {
+            each([&](int, float2 st) {
+                top = fmaxf(top, st.x);
+                odd |= !(st.y < INFINITY);
+            });
+            top = over_lanes(top, [](float v, float w) { return fmaxf(v, w); });
+            each([&](int, float2 st) { sum += st.y == 0.0f ? 0.0f : st.y * __builtin_amdgcn_exp2f((st.x - top) * 1.4426950408889634f); });
+            sum = over_lanes(sum, [](float v, float w) { return v + w; });
+            odd = __any(odd) || !(fabsf(top) < INFINITY);
         }
-        double sum = 0.0;
-        for (int i = lane; open && i < parts; i += 64) {
-            const float2 st = ws.stats[row * parts + i];
-            sum += st.y == 0.0f ? 0.0 : static_cast<double>(st.y) * exp(static_cast<double>(st.x) - static_cast<double>(top));
-        }
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) {
-            sum += __shfl_xor(sum, off);
-        }
-        odd = __any(odd) || !(fabsf(top) < INFINITY);
+        const double of_row = static_cast<double>(top) + log(static_cast<double>(sum)), from = (open && odd) || !(fabsf(score) < INFINITY) ? NAN : static_cast<double>(score);
         if (lane == 0) {
-            const float score = a.scores[row];
-            const bool ended = a.ended != nullptr && a.ended[row] != 0;
-            norm[beam] = static_cast<double>(top) + log(sum);
-            base[beam] = open && odd ? NAN : fabsf(score) < INFINITY ? static_cast<double>(score) : NAN;
+            norm[beam] = of_row;
+            base[beam] = from;
             was_ended[beam] = ended;
         }
+        const auto put_best = [&](int i, float v) {
+            own = fmaxf(own, v);
+            if (beam * parts + i < kJoinParts) {
+                best_of[beam * parts + i] = v;
+            }
+        };
+        each([&](int i, float2 st) {
+            if (i < parts) {
+                // an ended beam goes on as it is, once
+                put_best(i, from != from ? -INFINITY : ended ? (i == 0 ? score : -INFINITY) : rounded_down(from + (static_cast<double>(st.x) - of_row)));
+            }
+        });
     }
-    if (threadIdx.x == 0) {
-        listed = 0;
-    }
+    maxima[wave][lane] = own;
     __syncthreads();
-    // Candidate i of the request's, all rows' parts' k; one that is not there has a score of -infinity.
-    const int per_row = parts * k;
-    const int64_t all = static_cast<int64_t>(beams) * per_row;
-    const auto scored = [&](int64_t i) {
-        const int beam = static_cast<int>(i / per_row);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        own = fmaxf(own, maxima[w][lane]);
+    }
+    const int all = beams * parts;
+    const auto best_score = [&](int i) {
+        if (i < kJoinParts) {
+            return best_of[i];
+        }
+        const int beam = i / parts, part = i - beam * parts;
+        return base[beam] != base[beam]    ? -INFINITY
+               : was_ended[beam] != 0 ? (part == 0 ? static_cast<float>(base[beam]) : -INFINITY)
+                                      : rounded_down(base[beam] + (static_cast<double>(ws.stats[(row0 + beam) * parts + part].x) - norm[beam]));
+    };
+    // Candidate `place` of a part, as the rows' sums have it; one that is not there has a score of -infinity.
+    const auto scored = [&](int i, int place) {
+        const int beam = i / parts, part = i - beam * parts;
         Scored s = kNone;
         if (base[beam] != base[beam]) {
             return s;
         }
-        const int in_row = static_cast<int>(i - static_cast<int64_t>(beam) * per_row);
-        if (was_ended[beam] != 0) { // goes on as it is, once
-            if (in_row == 0) {
+        if (was_ended[beam] != 0) {
+            if (part == 0 && place == 0) {
                 s = Scored{base[beam], beam, 0.0f, a.end_token};
             }
             return s;
         }
-        const Candidate c = ws.candidates[(row0 + beam) * per_row + in_row];
+        const Candidate c = __builtin_bit_cast(Candidate, *reinterpret_cast<const uint2 *>(ws.candidates + ((row0 + beam) * parts + part) * k + place));
         if (c.token >= 0) {
             s = Scored{base[beam] + (static_cast<double>(c.logit) - norm[beam]), beam, c.logit, c.token};
         }
         return s;
     };
-    double most = -INFINITY;
-    for (int64_t i = threadIdx.x; i < all; i += kJoinThreads) {
-        most = fmax(most, scored(i).score);
-    }
-    maxima[threadIdx.x] = most;
-    __syncthreads();
-    {
-        // The k-th largest of the threads' maxima, ties counted one by one: a bound that at least k candidates reach.
-        int rank = 0;
-        for (int i = 0; i < kJoinThreads; ++i) {
-            rank += maxima[i] > most || (maxima[i] == most && i < static_cast<int>(threadIdx.x));
-        }
-        if (rank == k - 1) {
-            bound_at = most;
-        }
-    }
-    __syncthreads();
-    const double bound = bound_at;
-    for (int64_t i = threadIdx.x; i < all; i += kJoinThreads) {
-        const Scored s = scored(i);
-        if (s.score >= bound && s.score > -INFINITY) {
-            const int place = atomicAdd(&listed, 1);
-            if (place < kJoinList) {
-                list[place] = s;
-            }
-        }
-    }
-    __syncthreads();
     const auto put = [&](int rank, const Scored &s) {
         const int64_t to = static_cast<int64_t>(blockIdx.x) * k + rank;
         const bool some = s.score > -INFINITY;
@@ -321,44 +396,87 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(BeamSelectArgs 
         a.scores_out[to] = some ? static_cast<float>(s.score) : -INFINITY;
         a.ended_out[to] = !some || was_ended[s.beam] != 0 || s.token == a.end_token;
     };
-    const int count = listed;
-    if (count <= kJoinList) {
-        for (int i = threadIdx.x; i < count; i += kJoinThreads) {
+    double bound = kth_of_lanes(own, k);
+    for (;;) {
+        __syncthreads(); // the list's last readers are done
+        if (threadIdx.x == 0) {
+            listed = 0;
+        }
+        for (int i0 = 0; i0 < all; i0 += kJoinParts) {
+            if (threadIdx.x == 0) {
+                works = 0;
+            }
+            __syncthreads();
+            for (int i = i0 + threadIdx.x; i < min(all, i0 + kJoinParts); i += THREADS) {
+                const float v = best_score(i);
+                if (v > -INFINITY && static_cast<double>(v) >= rounded_down(bound)) {
+                    work[atomicAdd(&works, 1)] = i;
+                }
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < works * k; i += THREADS) {
+                const int w = i / k;
+                const Scored s = scored(work[w], i - w * k);
+                if (s.score >= bound && s.score > -INFINITY) {
+                    const int place = atomicAdd(&listed, 1);
+                    if (place < kJoinList) {
+                        list[place] = s;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        const int count = min(listed, kJoinList);
+        const bool whole = listed <= kJoinList;
+        for (int i = threadIdx.x; i < count; i += THREADS) {
             const Scored s = list[i];
             int rank = 0;
+#pragma unroll 2
             for (int j = 0; j < count; ++j) {
                 rank += before(list[j], s);
             }
-            if (rank < k) {
+            if (whole && rank < k) {
                 put(rank, s);
             }
+            if (!whole && rank == k - 1) {
+                next_bound = s.score;
+            }
         }
-        for (int i = count + threadIdx.x; i < k; i += kJoinThreads) {
-            put(i, kNone);
+        if (whole) {
+            for (int i = count + threadIdx.x; i < k; i += THREADS) {
+                put(i, kNone);
+            }
+            return;
         }
-        return;
+        // Too many: the k-th best of those listed is a better bound, unless they are equal.
+        __syncthreads();
+        if (!(next_bound > bound)) {
+            break;
+        }
+        bound = next_bound;
     }
     Scored last{INFINITY, -1, INFINITY, -1};
     for (int i = 0; i < k; ++i) { // the best behind the last one taken
         Scored best = kNone;
-        for (int64_t j = threadIdx.x; j < all; j += kJoinThreads) {
-            const Scored s = scored(j);
-            if (before(last, s) && before(s, best)) {
-                best = s;
+        for (int64_t j = threadIdx.x; j < static_cast<int64_t>(all) * k; j += THREADS) {
+            const int part = static_cast<int>(j / k);
+            const Scored s = scored(part, static_cast<int>(j - static_cast<int64_t>(part) * k));
+            if (before(last, s)) {
+                best = better(s, best);
             }
         }
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) {
             const Scored other{__shfl_xor(best.score, off), __shfl_xor(best.beam, off), __shfl_xor(best.logit, off), __shfl_xor(best.token, off)};
-            best = before(other, best) ? other : best;
+            best = better(other, best);
         }
         if (lane == 0) {
             wave_best[wave] = best;
         }
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kJoinThreads / 64; ++w) {
-            best = before(wave_best[w], best) ? wave_best[w] : best;
+        for (int w = 0; w < kWaves; ++w) {
+            best = better(wave_best[w], best);
         }
         if (threadIdx.x == 0) {
             put(i, best);
@@ -368,35 +486,59 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(BeamSelectArgs 
     }
 }
 
-int64_t parts_of(int64_t vocabulary, int dtype) { // the row may begin within a piece
-    const int64_t one = dtype == HM_LOGITS_FP32 ? 4 : 8;
-    return (vocabulary + one - 1 + 64 * kVectors * one - 1) / (64 * kVectors * one);
+// 16-byte loads of a lane: 32 elements where the logits give each SIMD eight such waves, else a quarter, so that there are more waves.
+template <class T> constexpr int kManyLoads = 32 / Elements<T>::kOf16Bytes;
+constexpr int64_t kManyLogits = int64_t(8) * 1024 * 2048;
+
+bool many_loads(int64_t rows, int64_t vocabulary) { return rows * vocabulary >= kManyLogits; }
+
+int64_t parts_of(int64_t vocabulary, int dtype, bool many) { // the row may begin within a piece
+    const int64_t one = dtype == HM_LOGITS_FP32 ? 4 : 8, in_part = many ? 2048 : 512;
+    return (vocabulary + one - 1 + in_part - 1) / in_part;
+}
+
+template <class T> void launch_parts(const BeamSelectArgs &a, hipStream_t stream) {
+    constexpr int kMany = kManyLoads<T>;
+    const dim3 grid(static_cast<unsigned>((a.parts + 3) / 4), static_cast<unsigned>(a.rows));
+    if (many_loads(a.rows, a.vocabulary)) {
+        hipLaunchKernelGGL((beam_parts_kernel<T, kMany>), grid, dim3(256), 0, stream, a);
+    } else {
+        hipLaunchKernelGGL((beam_parts_kernel<T, kMany / 4>), grid, dim3(256), 0, stream, a);
+    }
 }
 
 } // namespace
 
 size_t beam_select_workspace(int64_t rows, int64_t vocabulary, int64_t k, int dtype) {
-    return static_cast<size_t>(rows * parts_of(vocabulary, dtype)) * (sizeof(float2) + static_cast<size_t>(k) * sizeof(Candidate));
+    int64_t parts = rows * parts_of(vocabulary, dtype, many_loads(rows, vocabulary));
+    if (many_loads(rows, vocabulary)) { // enough for calls of fewer rows, whose parts are shorter
+        parts = std::max(parts, (kManyLogits - 1) / vocabulary * parts_of(vocabulary, dtype, false));
+    }
+    return static_cast<size_t>(parts) * (sizeof(float2) + static_cast<size_t>(k) * sizeof(Candidate));
 }
 
 hipError_t launch_beam_select(BeamSelectArgs a, hipStream_t stream) {
-    a.parts = static_cast<int>(parts_of(a.vocabulary, a.dtype));
-    const dim3 grid(static_cast<unsigned>((a.parts + 3) / 4), static_cast<unsigned>(a.rows));
+    a.parts = static_cast<int>(parts_of(a.vocabulary, a.dtype, many_loads(a.rows, a.vocabulary)));
     switch (a.dtype) {
     case HM_FP16:
-        hipLaunchKernelGGL((beam_parts_kernel<F16>), grid, dim3(256), 0, stream, a);
+        launch_parts<F16>(a, stream);
         break;
     case HM_BF16:
-        hipLaunchKernelGGL((beam_parts_kernel<BF16>), grid, dim3(256), 0, stream, a);
+        launch_parts<BF16>(a, stream);
         break;
     default:
-        hipLaunchKernelGGL((beam_parts_kernel<Fp32>), grid, dim3(256), 0, stream, a);
+        launch_parts<Fp32>(a, stream);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {
         return e;
     }
-    hipLaunchKernelGGL(beam_join_kernel, dim3(static_cast<unsigned>(a.rows / a.beams)), dim3(kJoinThreads), 0, stream, a);
+    const dim3 requests(static_cast<unsigned>(a.rows / a.beams));
+    if (a.beams <= 4) {
+        hipLaunchKernelGGL((beam_join_kernel<256>), requests, dim3(256), 0, stream, a);
+    } else {
+        hipLaunchKernelGGL((beam_join_kernel<1024>), requests, dim3(1024), 0, stream, a);
+    }
     return hipGetLastError();
 }
 

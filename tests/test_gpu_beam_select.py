@@ -71,6 +71,22 @@ def test_beams(hm, device, dtype, requests, beams, k):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("requests,beams,k,vocabulary", [(300, 2, 4, 30001), (150, 1, 8, 131075), (1, 256, 16, 66000), (9, 64, 64, 32000), (128, 4, 1, 40003)])
+def test_many_logits(hm, device, dtype, requests, beams, k, vocabulary):
+    logits, scores = _inputs(device, k, requests * beams, vocabulary, dtype)
+    ended = torch.rand(requests * beams, device=device, generator=torch.Generator(device=device).manual_seed(2)) < 0.3
+    _check(hm, device, logits, scores, ended, 5, beams, k)
+
+
+@pytest.mark.parametrize("beams,vocabulary", [(256, 70), (256, 1000), (200, 1025), (37, 64)])
+@pytest.mark.parametrize("k", [16, 64])
+def test_many_beams_of_few_logits(hm, device, beams, vocabulary, k):
+    logits, scores = _inputs(device, beams, beams, vocabulary, "fp16")
+    _check(hm, device, logits, scores, None, -1, beams, k)
+    _check(hm, device, logits, torch.zeros_like(scores), None, -1, beams, k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_of_any_alignment(hm, device, dtype):
     for ld, at in ((5003, 0), (5003, 1), (5001, 3), (5016, 7), (5000, 0)):
         big, scores = _inputs(device, at, 8, ld, dtype)
