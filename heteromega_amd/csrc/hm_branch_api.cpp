@@ -232,7 +232,7 @@ hm_status hm_share_plan(const int32_t *block_table, int64_t ld_table, int64_t R,
         return st;
     }
     const hm::SharePlanArgs a{block_table, ld_table, R, W, log2_of(page_size), positions, requests, rows, static_cast<int>(q_heads / kv_heads),
-                              static_cast<int>(kv_heads), window, shared, plan, 0, 0};
+                              static_cast<int>(kv_heads), window, shared, plan, 0};
     return launched(hm::launch_share_plan(a, reinterpret_cast<hipStream_t>(stream)), what);
 }
 

@@ -323,7 +323,7 @@ struct SharePlanArgs {
     int64_t window;
     int32_t *shared;
     void *plan;
-    int tree_base, groups; // set by the launch
+    int groups; // set by the launch
 };
 size_t share_plan_workspace(int64_t rows);
 hipError_t launch_share_plan(SharePlanArgs a, hipStream_t stream);

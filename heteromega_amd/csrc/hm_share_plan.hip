@@ -2,7 +2,7 @@
 //
 // shared[t], the leading tokens that rows t - 1 and t read from the same pages, is found by comparing their table rows, a wave per row. In units of kShareStep
 // tokens it is the depth of the boundary between the rows, and the segments are the tree of its intervals: rows between two boundaries of less depth than v
-// share v steps, of which their parent's are the lowest. Each boundary finds the nearest ones of less depth by a tree of minima in LDS; the first of those
+// share v steps, of which their parent's are the lowest. Each boundary finds the nearest ones of less depth, within its wave and then among the others' minima; the first of those
 // with the same depth and interval stands for the segment. Segments in more than kShareLevels others are left out: their keys stay with the rows
 // or segments within them.
 //
@@ -69,96 +69,133 @@ __global__ void __launch_bounds__(256) shared_tokens_kernel(SharePlanArgs a) {
     }
 }
 
+// What a row's segments take of the lines: segments and tiles of the narrow and the wide one, and slots. Two words, for the sums over rows.
 struct Count {
-    int32_t narrow, narrow_tiles, wide, wide_tiles, slots;
+    uint64_t places, tiles; // narrow, wide << 16, slots << 32; narrow, wide << 32
+
+    __device__ __forceinline__ int narrow() const { return static_cast<int>(places & 0xFFFF); }
+    __device__ __forceinline__ int wide() const { return static_cast<int>(places >> 16 & 0xFFFF); }
+    __device__ __forceinline__ int slots() const { return static_cast<int>(places >> 32); }
+    __device__ __forceinline__ int narrow_tiles() const { return static_cast<int>(tiles); }
+    __device__ __forceinline__ int wide_tiles() const { return static_cast<int>(tiles >> 32); }
 };
 
-__device__ __forceinline__ Count operator+(const Count &a, const Count &b) {
-    return {a.narrow + b.narrow, a.narrow_tiles + b.narrow_tiles, a.wide + b.wide, a.wide_tiles + b.wide_tiles, a.slots + b.slots};
-}
+__device__ __forceinline__ Count operator+(const Count &a, const Count &b) { return {a.places + b.places, a.tiles + b.tiles}; }
 
-// Depths of the boundaries 0..R (of rows t - 1 and t; none at the ends), with the minima of pairs, pairs of pairs and so on above them.
+// n / d for n below 2^13: (n + 1/2) / d lies 2^-14 of itself or more from whole numbers, and the roundings are off by 2^-22.
+__device__ __forceinline__ int quotient(int n, int d) { return static_cast<int>((static_cast<float>(n) + 0.5f) * __builtin_amdgcn_rcpf(static_cast<float>(d))); }
+
+// Depths of the boundaries 0..R (of rows t - 1 and t; none at the ends), in chunks of 64, with each chunk's minima up to a boundary and from it on. The last chunk
+// is filled up with depths of 0.
 struct Depths {
-    int32_t *tree;
-    int base;
+    int32_t *depth, *upto, *onward;
+    int count, chunks;
 
-    __device__ __forceinline__ int32_t at(int i) const { return tree[base + i]; }
-    // The nearest boundary before i (BACK) or after it with a depth below v, or not above it (EQUAL). There is one: the ends have depth 0.
-    template <bool BACK, bool EQUAL> __device__ __forceinline__ int nearest(int i, int32_t v) const {
-        const auto fits = [&](int p) { return EQUAL ? tree[p] <= v : tree[p] < v; };
-        int p = base + i;
-        while (p > 1) {
-            if ((p & 1) == (BACK ? 1 : 0) && fits(BACK ? p - 1 : p + 1)) {
-                p = BACK ? p - 1 : p + 1;
-                break;
-            }
-            p >>= 1;
+    __device__ __forceinline__ int32_t at(int i) const { return depth[i]; }
+    // A wave's 64 boundaries, of chunk c.
+    __device__ __forceinline__ void set(int c, int32_t v) const {
+        const int lane = threadIdx.x & 63, i = 64 * c + lane;
+        int32_t up = v, on = v;
+#pragma unroll 1
+        for (int off = 1; off < 64; off <<= 1) {
+            const int32_t x = __shfl_up(up, off), y = __shfl_down(on, off);
+            up = lane >= off ? min(up, x) : up;
+            on = lane + off < 64 ? min(on, y) : on;
         }
-        while (p < base) {
-            p = 2 * p + (BACK ? 1 : 0);
-            if (!fits(p)) {
-                p += BACK ? -1 : 1;
+        depth[i] = v, upto[i] = up, onward[i] = on;
+    }
+    // The nearest boundaries before the lane's, of chunk c, and after it with a depth below its own, v > 0. There are some: the ends have depth 0.
+    __device__ __forceinline__ int2 nearest(int c, int32_t v) const {
+        const int lane = threadIdx.x & 63;
+        uint32_t low = 0, high = 0; // a bit per lane
+#pragma unroll 4
+        for (int j = 31; j >= 0; --j) {
+            low = low + low + (__builtin_amdgcn_readlane(v, j) < v ? 1 : 0);
+            high = high + high + (__builtin_amdgcn_readlane(v, j + 32) < v ? 1 : 0);
+        }
+        const uint64_t less = static_cast<uint64_t>(high) << 32 | low;
+        const uint64_t before = less & ((uint64_t(1) << lane) - 1), after = less >> lane; // the lane's own bit is 0
+        // in other chunks: first which, then where
+        int left = -1, right = -1;
+#pragma unroll 1
+        for (int d = c - 1; d >= 0 && __any(v > 0 && before == 0 && left < 0); --d) {
+            left = left < 0 && onward[64 * d] < v ? d : left;
+        }
+#pragma unroll 1
+        for (int d = c + 1; d < chunks && __any(v > 0 && after == 0 && right < 0); ++d) {
+            right = right < 0 && onward[64 * d] < v ? d : right;
+        }
+        int last = 0, first = 0; // of those behind it, one is less deep; of those up to it, none
+        if (__any(v > 0 && (before == 0 || after == 0))) {
+#pragma unroll 1
+            for (int step = 32; step > 0; step >>= 1) {
+                last += onward[64 * max(left, 0) + last + step] < v ? step : 0;
+                first += upto[64 * max(right, 0) + first + step - 1] >= v ? step : 0;
             }
         }
-        return p - base;
+        return make_int2(before != 0 ? 64 * c + 63 - __clzll(before) : 64 * max(left, 0) + last,
+                         after != 0 ? 64 * c + lane + __ffsll(static_cast<unsigned long long>(after)) - 1 : right >= 0 ? 64 * right + min(first, 63) : count);
     }
 };
-
-__device__ __forceinline__ Count count_of(const SharePlanArgs &a, const ShareSegment &s) {
-    if (s.tiles == 0) {
-        return Count{0, 0, 0, 0, 0};
-    }
-    return s.rows * a.group_heads <= kNarrowCols ? Count{1, s.tiles * a.kv_heads, 0, 0, s.rows} : Count{0, 0, 1, s.tiles * a.kv_heads * s.chunks(), s.rows};
-}
-
-__device__ __forceinline__ SharePath path_of(const ShareSegment &s, int line, int t) {
-    if (s.tiles == 0) {
-        return SharePath{0, 0, 0, 0, 0, 0, 0, 0};
-    }
-    const int row = t - s.row0, chunk = row / s.chunk;
-    return SharePath{s.tiles, line, s.tile0 + chunk * s.tiles, s.chunks() * s.tiles, s.slot0, s.rows, row, row - chunk * s.chunk};
-}
 
 // One workgroup, of PER rows a thread at most.
 template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share_plan_kernel(SharePlanArgs a) {
     extern __shared__ int32_t lds[];
     __shared__ Count waves[THREADS / 64];
-    constexpr int kDropped = kShareLevels;
+    constexpr int kDropped = kShareLevels, kOfWide = 1 << 16;
     const int R = static_cast<int>(a.rows), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Depths depth{lds, a.tree_base};
-    int32_t *alike = lds + max(2 * a.tree_base, 3 * R), *parent = alike + R, *level = parent + R, *record = level + R, *lo = record + R;
+    const int chunks = (R + 63) / 64;
+    const Depths depth{lds, lds + 64 * chunks + 1, lds + 128 * chunks + 1, R, chunks};
+    int32_t *alike = lds + 192 * chunks + 1, *parent = alike + R, *level = parent + R, *record = level + R, *lo = record + R;
+    int32_t *by_begin = parent, *by_end = level; // before parents and levels are known; ends from 1 on
+    int32_t *marks = lo + R;                      // of each run
     const ShareWorkspace ws = carve_share(a.plan, a.rows, a.groups);
     const auto row_of = [&](int j) { return j * THREADS + static_cast<int>(threadIdx.x); };
 
-    for (int i = threadIdx.x; i < a.tree_base; i += THREADS) {
-        lds[a.tree_base + i] = i > 0 && i < R ? a.shared[i] / kShareStep : 0;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < 2 * R; i += THREADS) {
+        by_begin[i] = INT32_MAX;
+    }
+#pragma unroll 1
+    for (int i = threadIdx.x; i < (kAttentionWaves + 1) * a.groups; i += THREADS) {
+        marks[i] = 0;
     }
     RowKeys keys[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int i = row_of(j);
+        const int32_t tokens = i > 0 && i < R ? a.shared[i] : 0;
         keys[j] = i < R ? row_keys(a, i) : RowKeys{0, 0, 0};
         if (i < R) {
             record[i] = keys[j].first; // for the windows' beginnings, until it has its own use
         }
+        if (i - lane < R) {
+            depth.set(i / 64, tokens / kShareStep);
+        }
+    }
+    if (threadIdx.x == 0) {
+        depth.depth[64 * chunks] = 0;
     }
     __syncthreads();
-    for (int n = a.tree_base >> 1; n > 0; n >>= 1) {
-        for (int i = threadIdx.x; i < n; i += THREADS) {
-            lds[n + i] = min(lds[2 * (n + i)], lds[2 * (n + i) + 1]);
-        }
-        __syncthreads();
-    }
     // ---- the segments of boundaries ----
     int from[PER], to[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int i = row_of(j);
         const int32_t v = i < R ? depth.at(i) : 0;
-        from[j] = to[j] = 0;
+        const int2 ends = depth.nearest(uniform(i / 64), v);
+        from[j] = ends.x, to[j] = ends.y;
         if (v > 0) {
-            from[j] = depth.nearest<true, false>(i, v), to[j] = depth.nearest<false, false>(i, v);
-            alike[i] = depth.nearest<false, true>(from[j], v); // the boundary that stands for the segment
+            // One segment alone begins at a boundary and ends at one that is not deeper, and one alone ends at a boundary and begins at a less deep one.
+            atomicMin(depth.at(from[j]) >= depth.at(to[j]) ? &by_begin[from[j]] : &by_end[to[j] - 1], i);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int i = row_of(j);
+        if (i < R && depth.at(i) > 0) { // the first boundary as deep stands for the segment
+            alike[i] = depth.at(from[j]) >= depth.at(to[j]) ? by_begin[from[j]] : by_end[to[j] - 1];
         }
     }
     __syncthreads();
@@ -170,6 +207,7 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share
             parent[i] = above == 0 ? -1 : alike[depth.at(from[j]) == above ? from[j] : to[j]];
             int32_t begin = above * kShareStep;
             if (a.window > 0) {
+#pragma unroll 1
                 for (int t = from[j]; t < to[j]; ++t) {
                     begin = max(begin, (record[t] + 15) & ~15);
                 }
@@ -183,6 +221,7 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share
         const int i = row_of(j);
         if (i < R && depth.at(i) > 0 && alike[i] == i) {
             int n = 0;
+#pragma unroll 1
             for (int p = parent[i]; p >= 0 && n < kDropped; p = parent[p]) {
                 ++n;
             }
@@ -192,99 +231,117 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share
     __syncthreads();
 
     // ---- segments of each row: its own, what its window leaves before the shared ones, and the boundary's before it ----
-    ShareSegment segments[PER][3];
-    int inner[PER]; // the innermost segment that the row is in, or -1
-    Count own{0, 0, 0, 0, 0};
+    int inner[PER];     // the innermost segment that the row is in, or -1
+    int32_t covered[PER]; // the first key of a shared segment
+    Count own{0, 0};
+    const auto segment_of = [&](int j, int n) __attribute__((always_inline)) {
+        const int t = row_of(j);
+        ShareSegment s{t, 1, 0, 0, 0, 0, 0, 1};
+        const bool alone = covered[j] == INT32_MAX;
+        if (n == 0) {
+            s.lo = alone ? keys[j].first : depth.at(inner[j]) * kShareStep;
+            s.hi = keys[j].end;
+        } else if (n == 1) {
+            s.lo = keys[j].first;
+            s.hi = alone ? 0 : covered[j];
+        } else if (t < R && depth.at(t) > 0 && alike[t] == t && level[t] < kDropped) {
+            s.row0 = from[j], s.rows = to[j] - from[j];
+            s.lo = lo[t], s.hi = depth.at(t) * kShareStep;
+        }
+        static_assert(kNarrowTile == kWideTile, "of one length");
+        s.tiles = s.lo < s.hi ? (s.hi - s.start() + kNarrowTile - 1) / kNarrowTile : 0;
+        s.chunk = s.rows;
+        return s;
+    };
+    // Splits the rows of a wide segment evenly; what the segment takes of the lines.
+    const auto take = [&](ShareSegment &s) __attribute__((always_inline)) {
+        const bool wide = s.rows * a.group_heads > kNarrowCols;
+        int chunks = 1;
+        if (wide) {
+            const int most = kWideCols / a.group_heads;
+            chunks = quotient(s.rows + most - 1, most);
+            s.chunk = quotient(s.rows + chunks - 1, chunks);
+            chunks = quotient(s.rows + s.chunk - 1, s.chunk);
+        }
+        const uint64_t some = s.tiles > 0 ? 1 : 0;
+        const uint64_t tiles = static_cast<uint32_t>(s.tiles) * static_cast<uint32_t>(a.kv_heads * chunks);
+        return Count{some << (wide ? 16 : 0) | static_cast<uint64_t>(some != 0 ? s.rows : 0) << 32, tiles << (wide ? 32 : 0)};
+    };
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int t = row_of(j);
-        inner[j] = -1;
-#pragma unroll
-        for (int n = 0; n < 3; ++n) {
-            segments[j][n] = ShareSegment{t, 1, 0, 0, 0, 0, 0, 1};
-        }
+        inner[j] = -1, covered[j] = INT32_MAX;
         if (t < R) {
             const int32_t before = depth.at(t), after = t + 1 < R ? depth.at(t + 1) : 0;
             if (max(before, after) > 0) {
-                inner[j] = alike[before >= after ? t : t + 1];
-                while (level[inner[j]] >= kDropped) {
-                    inner[j] = parent[inner[j]];
+                int i = alike[before >= after ? t : t + 1];
+                while (level[i] >= kDropped) {
+                    i = parent[i];
+                }
+                inner[j] = i;
+#pragma unroll 1
+                for (; i >= 0; i = parent[i]) {
+                    covered[j] = lo[i] < depth.at(i) * kShareStep ? lo[i] : covered[j];
                 }
             }
-            int32_t covered = INT32_MAX; // the first key of a shared segment
-            for (int i = inner[j]; i >= 0; i = parent[i]) {
-                covered = lo[i] < depth.at(i) * kShareStep ? lo[i] : covered;
-            }
-            segments[j][0].lo = covered == INT32_MAX ? keys[j].first : depth.at(inner[j]) * kShareStep;
-            segments[j][0].hi = keys[j].end;
-            segments[j][1].lo = keys[j].first;
-            segments[j][1].hi = covered == INT32_MAX ? 0 : covered;
-            if (before > 0 && alike[t] == t && level[t] < kDropped) {
-                segments[j][2].row0 = from[j], segments[j][2].rows = to[j] - from[j];
-                segments[j][2].lo = lo[t], segments[j][2].hi = before * kShareStep;
-            }
         }
-#pragma unroll
+#pragma unroll 1
         for (int n = 0; n < 3; ++n) {
-            ShareSegment &s = segments[j][n];
-            const int columns = s.rows * a.group_heads, tile = columns <= kNarrowCols ? kNarrowTile : kWideTile;
-            s.tiles = s.lo < s.hi ? (s.hi - s.start() + tile - 1) / tile : 0;
-            s.chunk = s.rows;
-            if (columns > kNarrowCols) {
-                const int most = kWideCols / a.group_heads, chunks = (s.rows + most - 1) / most;
-                s.chunk = (s.rows + chunks - 1) / chunks;
-            }
-            own = own + count_of(a, s);
+            ShareSegment s = segment_of(j, n);
+            own = own + take(s);
         }
     }
     Count upto = own;
-#pragma unroll
+#pragma unroll 1
     for (int off = 1; off < 64; off <<= 1) {
-        const Count v{__shfl_up(upto.narrow, off), __shfl_up(upto.narrow_tiles, off), __shfl_up(upto.wide, off), __shfl_up(upto.wide_tiles, off),
-                      __shfl_up(upto.slots, off)};
-        if (lane >= off) {
-            upto = upto + v;
-        }
+        const Count v{__shfl_up(upto.places, off), __shfl_up(upto.tiles, off)};
+        upto = lane >= off ? upto + v : upto;
     }
     if (lane == 63) {
         waves[wave] = upto;
     }
-    Count at{__shfl_up(upto.narrow, 1), __shfl_up(upto.narrow_tiles, 1), __shfl_up(upto.wide, 1), __shfl_up(upto.wide_tiles, 1), __shfl_up(upto.slots, 1)};
-    if (lane == 0) {
-        at = Count{0, 0, 0, 0, 0};
-    }
-    __syncthreads(); // the depths are not read any more either: the lines' first tiles take their place
-    Count total{0, 0, 0, 0, 0};
-#pragma unroll
+    __syncthreads();
+    Count at{upto.places - own.places, upto.tiles - own.tiles}, total{0, 0};
+#pragma unroll 1
     for (int w = 0; w < THREADS / 64; ++w) {
         at = w < wave ? at + waves[w] : at;
         total = total + waves[w];
     }
-    const ShareHeader header{{total.narrow_tiles, total.wide_tiles}, R, a.group_heads, a.kv_heads, a.groups,
-                             wide_groups(total.wide_tiles, total.narrow_tiles, a.groups), 0};
+    const ShareHeader header{{total.narrow_tiles(), total.wide_tiles()}, R, a.group_heads, a.kv_heads, a.groups,
+                             wide_groups(total.wide_tiles(), total.narrow_tiles(), a.groups), 0};
     if (threadIdx.x == 0) {
         *ws.header = header;
     }
-    int32_t *tile0[2] = {lds, lds + total.narrow};
+    const int narrow_runs = header.runs(0), runs = narrow_runs + header.runs(1);
+    const Runs narrow = Runs::deal(header.tiles[0], narrow_runs), wide = Runs::deal(header.tiles[1], max(header.wide, 1));
+    ShareSegment *lines = ws.segments[0];
+    const int wide_at = static_cast<int>(ws.segments[1] - lines); // no arrays indexed by the line: they would be in memory
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int t = row_of(j);
-#pragma unroll
+#pragma unroll 1
         for (int n = 0; n < 3; ++n) {
-            ShareSegment &s = segments[j][n];
-            const int line = s.rows * a.group_heads > kNarrowCols ? 1 : 0, place = line == 1 ? at.wide : at.narrow;
-            if (s.tiles > 0) {
-                s.tile0 = line == 1 ? at.wide_tiles : at.narrow_tiles;
-                s.slot0 = at.slots;
-                ws.segments[line][place] = s;
-                tile0[line][place] = s.tile0;
-                at = at + count_of(a, s);
+            ShareSegment s = segment_of(j, n);
+            const Count c = take(s);
+            const bool some = s.tiles > 0, is_wide = s.rows * a.group_heads > kNarrowCols;
+            const int place = is_wide ? at.wide() : at.narrow();
+            s.tile0 = is_wide ? at.wide_tiles() : at.narrow_tiles();
+            s.slot0 = at.slots();
+            at = at + c;
+            if (some) {
+                lines[place + (is_wide ? wide_at : 0)] = s;
+                // the first run that begins in the segment or behind it; several may have the same, of which the last counts
+                const Runs &of = is_wide ? wide : narrow;
+                const int w = s.tile0 > 0 ? of.of(s.tile0 - 1) + 1 : 0;
+                if (w < (is_wide ? header.wide : narrow_runs)) {
+                    atomicMax(&marks[is_wide ? narrow_runs + w : w], is_wide ? kOfWide + place : place);
+                }
             }
-            if (n < 2 && t < R) {
-                ws.paths[t * kPathEntries + n] = path_of(s, line, t);
+            if (n < 2 && t < R) { // a unit of one row for each key head
+                ws.paths[n * R + t] = some ? SharePath{s.tiles, is_wide ? 1 : 0, s.tile0, s.tiles, s.slot0, 1, 0, 0} : SharePath{0, 0, 0, 0, 0, 0, 0, 0};
             }
             if (n == 2 && t < R) {
-                record[t] = s.tiles > 0 ? 2 * place + line : -1;
+                record[t] = some ? 2 * place + (is_wide ? 1 : 0) : -1;
             }
         }
     }
@@ -293,38 +350,60 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share
     for (int j = 0; j < PER; ++j) {
         const int t = row_of(j);
         if (t < R) {
+            int which[kShareLevels];
+            ShareSegment s[kShareLevels];
             int i = inner[j];
-            for (int n = 2; n < kPathEntries; ++n) {
-                SharePath p{0, 0, 0, 0, 0, 0, 0, 0};
-                if (i >= 0 && record[i] >= 0) {
-                    p = path_of(ws.segments[record[i] & 1][record[i] >> 1], record[i] & 1, t);
-                }
-                ws.paths[t * kPathEntries + n] = p;
+#pragma unroll
+            for (int n = 0; n < kShareLevels; ++n) {
+                which[n] = i >= 0 ? record[i] : -1;
                 i = i >= 0 ? parent[i] : -1;
+            }
+#pragma unroll
+            for (int n = 0; n < kShareLevels; ++n) { // all read at once
+                s[n] = lines[(max(which[n], 0) >> 1) + ((max(which[n], 0) & 1) != 0 ? wide_at : 0)];
+            }
+#pragma unroll
+            for (int n = 0; n < kShareLevels; ++n) {
+                const int row = t - s[n].row0, chunk = quotient(row, s[n].chunk), chunks = quotient(s[n].rows + s[n].chunk - 1, s[n].chunk);
+                ws.paths[(2 + n) * R + t] = which[n] >= 0 ? SharePath{s[n].tiles, which[n] & 1, s[n].tile0 + chunk * s[n].tiles, chunks * s[n].tiles, s[n].slot0, s[n].rows, row,
+                                                                      row - chunk * s[n].chunk}
+                                                          : SharePath{0, 0, 0, 0, 0, 0, 0, 0};
             }
         }
     }
-    // ---- where the runs begin ----
-    const int narrow_runs = header.runs(0);
-    for (int i = threadIdx.x; i < narrow_runs + header.runs(1); i += THREADS) {
-        const int line = i < narrow_runs ? 0 : 1, w = line == 0 ? i : i - narrow_runs;
-        const int count = line == 0 ? total.narrow : total.wide, tiles = line == 0 ? total.narrow_tiles : total.wide_tiles;
-        const int x = Runs::deal(tiles, header.runs(line)).begin(w);
-        int first = 0, last = count - 1; // the last segment that begins at x or before it
-        while (first < last) {
-            const int mid = (first + last + 1) >> 1;
-            if (tile0[line][mid] <= x) {
-                first = mid;
-            } else {
-                last = mid - 1;
-            }
-        }
-        ws.starts[line][w] = first;
+    // ---- where the runs begin: the last segment marked up to each ----
+    const int each = (runs + THREADS - 1) / THREADS, first = min(static_cast<int>(threadIdx.x) * each, runs), last = min(first + each, runs);
+    int here = 0;
+#pragma unroll 4
+    for (int i = first; i < last; ++i) {
+        here = max(here, marks[i]);
+    }
+#pragma unroll 1
+    for (int off = 1; off < 64; off <<= 1) {
+        const int v = __shfl_up(here, off);
+        here = lane >= off ? max(here, v) : here;
+    }
+    if (lane == 63) {
+        waves[wave].places = here;
+    }
+    const int before = __shfl_up(here, 1);
+    here = lane > 0 ? before : 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int w = 0; w < wave; ++w) {
+        here = max(here, static_cast<int>(waves[w].places));
+    }
+    int32_t *starts = ws.starts[0];
+    const int wide_starts = static_cast<int>(ws.starts[1] - starts);
+#pragma unroll 1
+    for (int i = first; i < last; ++i) {
+        here = max(here, marks[i]);
+        starts[i < narrow_runs ? i : wide_starts + i - narrow_runs] = here & (kOfWide - 1);
     }
 }
 
 template <int THREADS, int PER> hipError_t launch_plan(const SharePlanArgs &a, hipStream_t stream) {
-    const size_t lds = 4 * (static_cast<size_t>(std::max<int64_t>(2 * a.tree_base, 3 * a.rows)) + 5 * static_cast<size_t>(a.rows));
+    const size_t lds = 4 * static_cast<size_t>(1 + 3 * ((a.rows + 63) / 64 * 64) + 5 * a.rows + (kAttentionWaves + 1) * a.groups);
     if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&share_plan_kernel<THREADS, PER>), hipFuncAttributeMaxDynamicSharedMemorySize,
                                                  static_cast<int>(lds));
@@ -342,10 +421,6 @@ size_t share_plan_workspace(int64_t rows) { return static_cast<size_t>(share_pla
 
 hipError_t launch_share_plan(SharePlanArgs a, hipStream_t stream) {
     a.groups = share_groups();
-    a.tree_base = 2;
-    while (a.tree_base < a.rows + 1) {
-        a.tree_base *= 2;
-    }
     hipLaunchKernelGGL(shared_tokens_kernel, dim3(static_cast<unsigned>((a.rows + 3) / 4)), dim3(256), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {

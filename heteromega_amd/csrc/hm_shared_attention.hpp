@@ -59,7 +59,7 @@ struct ShareHeader {
 struct ShareWorkspace {
     ShareHeader *header;
     ShareSegment *segments[2]; // [3 rows]: narrow, wide
-    SharePath *paths;          // [rows][kPathEntries]
+    SharePath *paths;          // [kPathEntries][rows]
     int32_t *starts[2];        // [runs]: the segment that each run begins in
 };
 

@@ -643,7 +643,7 @@ template <class T, int D, int THREADS> __global__ void __launch_bounds__(256) sh
     const ShareWorkspace plan = carve_share(a.plan, a.rows, a.groups);
     const ShareHeader header = *plan.header;
     const int lane = threadIdx.x & 63;
-    const SharePath p = plan.paths[t * kPathEntries + min(lane, kPathEntries - 1)];
+    const SharePath p = plan.paths[min(lane, kPathEntries - 1) * a.rows + t];
     const Keys keys = keys_of(a, t);
     if (keys.request < 0) {
         return;

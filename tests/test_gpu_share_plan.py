@@ -40,7 +40,7 @@ def decode(share):
     rows, head = share.rows, words[:8]
     assert head[2:5].tolist() == [rows, share.q_heads // share.kv_heads, share.kv_heads]
     lines = words[8:8 + 48 * rows].reshape(2, 3 * rows, 8)
-    paths = words[8 + 48 * rows:8 + 88 * rows].reshape(rows, 5, 8)
+    paths = words[8 + 48 * rows:8 + 88 * rows].reshape(5, rows, 8).transpose(1, 0, 2)
     groups, wide = head[5:7].tolist()
     starts = words[8 + 88 * rows:8 + 88 * rows + 5 * groups]
     assert 0 <= wide <= groups // 2 and (wide > 0) == (head[1] > 0)
