@@ -144,7 +144,7 @@ def copy_pages(caches, copies, to=None, stream=None):
 
 
 class SharePlan:
-    """What share_plan finds for a step of up to `rows` rows, kept from step to step (a captured step's layers read it): shared [rows], the leading tokens
+    """What share_plan finds for a step of `rows` rows, kept from step to step (a captured step's layers read it): shared [rows], the leading tokens
     that a row reads from the same pages as the row before it, and what shared_attention of these heads, page size and window works on."""
 
     def __init__(self, rows, page_size, q_heads, kv_heads, device="cuda", window=0):

@@ -121,7 +121,7 @@ template <class T, int V> __global__ void __launch_bounds__(256, 4) beam_parts_k
     const int vocabulary = static_cast<int>(a.vocabulary), pieces = (vocabulary + skip + kOne - 1) / kOne;
     const int first = part * (64 * V);
     void *const from_piece = reinterpret_cast<void *>((start & ~int64_t(15)) + static_cast<int64_t>(first) * 16);
-    const __amdgpu_buffer_rsrc_t resource = __builtin_amdgcn_make_buffer_rsrc(from_piece, 0, uniform(min(64 * V, pieces - first) * 16), 0x00020000);
+    const __amdgpu_buffer_rsrc_t resource = __builtin_amdgcn_make_buffer_rsrc(from_piece, 0, uniform(max(0, min(64 * V, pieces - first)) * 16), 0x00020000);
     if (!is_open(a, row)) {
         return;
     }

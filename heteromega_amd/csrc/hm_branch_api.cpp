@@ -53,9 +53,10 @@ hm_status check_share(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t W
     if (q_heads / kv_heads > hm::kWideCols) {
         return set_error(HM_UNSUPPORTED, "%s: at most %d query heads to a key head, got %lld", what, hm::kWideCols, static_cast<long long>(q_heads / kv_heads));
     }
-    const int64_t tiles = (W * page_size / 64 + 2) * kv_heads; // all tiles are counted in 32 bits
+    static_assert(hm::kNarrowTile == 32 && hm::kWideTile == 32, "the refusal names their length");
+    const int64_t tiles = (W * page_size / 32 + 2) * kv_heads; // all tiles are counted in 32 bits
     if (tiles > INT32_MAX || 5 * rows > INT32_MAX / tiles) {
-        return set_error(HM_UNSUPPORTED, "%s: 5 * rows * key heads * (W * page_size / 64 + 2) must stay below 2^31 (fewer rows per call)", what);
+        return set_error(HM_UNSUPPORTED, "%s: 5 * rows * key heads * (W * page_size / 32 + 2) must stay below 2^31 (fewer rows per call)", what);
     }
     return HM_OK;
 }

@@ -464,8 +464,8 @@ hm_status hm_paged_attention(const hm_kv_cache *cache, void *out, int64_t ldo, c
  *   tokens [R, k], scores_out [R, k]
  *   ended_out [R, k]  1 if its row had ended or its token is end_token
  * Logits of -infinity are no continuations, nor are those of a row whose score is not finite (-infinity: a beam that is not in use yet) or among whose
- * logits are NaN or +infinity. Where fewer than k are left: parent and token -1, score -infinity, ended 1. Sums are fp32 over 32 logits and fp64 from there on, candidates
- * of different rows are compared in fp64. end_token: -1 for none, if `ended` is NULL. beams up to HM_BEAM_MAX_BEAMS, k up to HM_BEAM_MAX_K. With k = beams,
+ * logits are NaN or +infinity. Where fewer than k are left: parent and token -1, score -infinity, ended 1. Sums are fp32, a row's in the same order
+ * each time, their logarithms and the comparison of different rows' candidates fp64. end_token: -1 for none, if `ended` is NULL. beams up to HM_BEAM_MAX_BEAMS, k up to HM_BEAM_MAX_K. With k = beams,
  * scores_out may be scores and ended_out may be ended; other arrays must not overlap. Workspace (16-byte aligned, nothing in it has to start at zero):
  * hm_beam_select_workspace_bytes. */
 #define HM_LOGITS_FP32 2
@@ -523,7 +523,7 @@ hm_status hm_copy_pages(const hm_kv_cache *from, const hm_kv_cache *to, int64_t 
  *                     whose entries differ, at most as many as the shorter of the two sees; 0 next to a row that has no request or position in the table
  *   plan              hm_share_plan_bytes(rows) bytes, 16-byte aligned, for the calls of the same rows, heads, table and positions; not made for any call yet: zeros
  * Rows that share pages should follow each other, those that share most next to each other. window: as for hm_paged_attention. rows up to HM_SHARE_MAX_ROWS,
- * q_heads a multiple of kv_heads, up to 128 times; 5 * rows * kv_heads * (W * page_size / 64 + 2) below 2^31. */
+ * q_heads a multiple of kv_heads, up to 128 times; 5 * rows * kv_heads * (W * page_size / 32 + 2) below 2^31. */
 #define HM_SHARE_MAX_ROWS 4096
 size_t hm_share_plan_bytes(int64_t rows);
 hm_status hm_share_plan(const int32_t *block_table, int64_t ld_table, int64_t R, int64_t W, int64_t page_size, const int32_t *positions, const int32_t *requests,

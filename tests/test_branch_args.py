@@ -69,6 +69,11 @@ def test_share_plans_that_are_refused(hm, over, status):
     assert _call("hm_share_plan", SHARE, over) == status
 
 
+def test_share_plans_count_tiles_of_32_keys_in_31_bits(hm):
+    # 5 * rows * key heads * (W * page_size / 32 + 2) is 2^31 and more from W = 104856 on: 52429 tiles and two, 2 heads, 4096 rows
+    assert _call("hm_share_plan", SHARE, dict(rows=4096, R=4096, W=104856, ld=104856, bytes=1 << 30)) == hm._lib.HM_UNSUPPORTED
+
+
 def _shared(hm, cache=None, **over):
     f = dict(out=FAKE, ldo=512, q=FAKE, ldq=512, rows=3, q_heads=8, table=FAKE, ld=5, R=3, W=5, positions=FAKE, requests=None, scale=0.125, plan=FAKE, plan_bytes=1 << 20,
              ws=FAKE, wb=1 << 40, stream=None)
@@ -111,6 +116,14 @@ def test_shapes_that_are_unsupported(hm):
         assert _shared(hm, ctypes.byref(_cache(hm, **over)), ldq=1 << 20, ldo=1 << 20) == hm._lib.HM_UNSUPPORTED
     c = ctypes.byref(_cache(hm, kv_heads=65536))
     assert _shared(hm, c, q_heads=65536, W=2 ** 26, ld=2 ** 26) == hm._lib.HM_UNSUPPORTED
+
+
+def test_a_workspace_for_many_requests_is_enough_for_fewer(hm):
+    of = hm._lib.load().hm_beam_select_workspace_bytes
+    for dtype in (hm._lib.HM_FP16, hm._lib.HM_BF16, hm._lib.HM_LOGITS_FP32):
+        for v in (1, 1000, 32003, 152064, 2 ** 22 + 1):
+            sizes = [of(r, 4, v, 8, dtype) for r in range(1, 300)]
+            assert sizes[0] > 0 and sizes == sorted(sizes)
 
 
 def test_workspace_bytes(hm):
