@@ -8,16 +8,16 @@
 //
 // The k best of a wave's 2048: the k-th largest of the 64 lanes' maxima, found by sorting them over the lanes, is a bound that at least k elements reach and
 // seldom many more; those go to a list in LDS and are ranked by counting who comes before. (The least of k or more groups' maxima is quicker to find, but
-// almost three times as many reach it: 37 us instead of 21 for the case above. 64 elements a lane, with fewer sorts, took 40.) Many equal or badly spread
+// almost three times as many reach it: 37 us instead of 21 for the case above. 64 elements a lane, with fewer sorts, took 25 at three waves a SIMD; 8 or 16 of them
+// for few logits gain less here than the second launch loses by more parts.) Many equal or badly spread
 // elements overflow the list; then the best are taken one after the other.
 #include "hm_device.hpp"
 #include "hm_internal.hpp"
 
-#include <algorithm>
-
 namespace hm {
 namespace {
 
+constexpr int kElements = 32;    // of a lane
 constexpr int kList = 192;       // candidates that a wave's list holds
 constexpr int kJoinList = 1024;  // and that of a request
 constexpr int kJoinParts = 1024; // parts that are looked at at once
@@ -104,10 +104,10 @@ __device__ __forceinline__ float kth_of_lanes(float v, int k) {
 
 __device__ __forceinline__ bool before(float v, int32_t token, float w, int32_t other) { return v > w || (v == w && token < other); }
 
-// A wave per part of a row: V 16-byte loads a lane.
-template <class T, int V> __global__ void __launch_bounds__(256, 4) beam_parts_kernel(BeamSelectArgs a) {
+// A wave per part of a row.
+template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(BeamSelectArgs a) {
     using E = Elements<T>;
-    constexpr int kOne = E::kOf16Bytes, kMine = V * kOne;
+    constexpr int kOne = E::kOf16Bytes, V = kElements / kOne;
     __shared__ Candidate list[4][kList];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int64_t row = blockIdx.y;
@@ -130,7 +130,7 @@ template <class T, int V> __global__ void __launch_bounds__(256, 4) beam_parts_k
     for (int i = 0; i < V; ++i) { // behind the last piece: zeros
         raw[i] = __builtin_amdgcn_raw_buffer_load_b128(resource, lane * 16, i * 1024, 0);
     }
-    float x[kMine];
+    float x[kElements];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
 #pragma unroll
@@ -142,14 +142,14 @@ template <class T, int V> __global__ void __launch_bounds__(256, 4) beam_parts_k
     const auto token_of = [&](int j) { return first_token + j / kOne * 64 * kOne + j % kOne; };
     if (first == 0 || first + V * 64 >= pieces) { // elements that are not the row's
 #pragma unroll
-        for (int j = 0; j < kMine; ++j) {
+        for (int j = 0; j < kElements; ++j) {
             const int token = token_of(j);
             x[j] = token >= 0 && token < vocabulary ? x[j] : -INFINITY;
         }
     }
     float most = x[0];
 #pragma unroll
-    for (int j = 1; j < kMine; ++j) {
+    for (int j = 1; j < kElements; ++j) {
         most = fmaxf(most, x[j]);
     }
     const int k = a.k;
@@ -180,7 +180,7 @@ template <class T, int V> __global__ void __launch_bounds__(256, 4) beam_parts_k
 #endif
     int count = 0;
 #pragma unroll
-    for (int j = 0; j < kMine; ++j) {
+    for (int j = 0; j < kElements; ++j) {
         const bool in = x[j] >= bound;
         const uint64_t who = __ballot(in);
         if (who != 0) {
@@ -486,48 +486,29 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
     }
 }
 
-// 16-byte loads of a lane: 32 elements where the logits give each SIMD eight such waves, else a quarter, so that there are more waves.
-template <class T> constexpr int kManyLoads = 32 / Elements<T>::kOf16Bytes;
-constexpr int64_t kManyLogits = int64_t(8) * 1024 * 2048;
-
-bool many_loads(int64_t rows, int64_t vocabulary) { return rows * vocabulary >= kManyLogits; }
-
-int64_t parts_of(int64_t vocabulary, int dtype, bool many) { // the row may begin within a piece
-    const int64_t one = dtype == HM_LOGITS_FP32 ? 4 : 8, in_part = many ? 2048 : 512;
+int64_t parts_of(int64_t vocabulary, int dtype) { // the row may begin within a piece
+    const int64_t one = dtype == HM_LOGITS_FP32 ? 4 : 8, in_part = 64 * kElements;
     return (vocabulary + one - 1 + in_part - 1) / in_part;
-}
-
-template <class T> void launch_parts(const BeamSelectArgs &a, hipStream_t stream) {
-    constexpr int kMany = kManyLoads<T>;
-    const dim3 grid(static_cast<unsigned>((a.parts + 3) / 4), static_cast<unsigned>(a.rows));
-    if (many_loads(a.rows, a.vocabulary)) {
-        hipLaunchKernelGGL((beam_parts_kernel<T, kMany>), grid, dim3(256), 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((beam_parts_kernel<T, kMany / 4>), grid, dim3(256), 0, stream, a);
-    }
 }
 
 } // namespace
 
 size_t beam_select_workspace(int64_t rows, int64_t vocabulary, int64_t k, int dtype) {
-    int64_t parts = rows * parts_of(vocabulary, dtype, many_loads(rows, vocabulary));
-    if (many_loads(rows, vocabulary)) { // enough for calls of fewer rows, whose parts are shorter
-        parts = std::max(parts, (kManyLogits - 1) / vocabulary * parts_of(vocabulary, dtype, false));
-    }
-    return static_cast<size_t>(parts) * (sizeof(float2) + static_cast<size_t>(k) * sizeof(Candidate));
+    return static_cast<size_t>(rows * parts_of(vocabulary, dtype)) * (sizeof(float2) + static_cast<size_t>(k) * sizeof(Candidate));
 }
 
 hipError_t launch_beam_select(BeamSelectArgs a, hipStream_t stream) {
-    a.parts = static_cast<int>(parts_of(a.vocabulary, a.dtype, many_loads(a.rows, a.vocabulary)));
+    a.parts = static_cast<int>(parts_of(a.vocabulary, a.dtype));
+    const dim3 grid(static_cast<unsigned>((a.parts + 3) / 4), static_cast<unsigned>(a.rows));
     switch (a.dtype) {
     case HM_FP16:
-        launch_parts<F16>(a, stream);
+        hipLaunchKernelGGL((beam_parts_kernel<F16>), grid, dim3(256), 0, stream, a);
         break;
     case HM_BF16:
-        launch_parts<BF16>(a, stream);
+        hipLaunchKernelGGL((beam_parts_kernel<BF16>), grid, dim3(256), 0, stream, a);
         break;
     default:
-        launch_parts<Fp32>(a, stream);
+        hipLaunchKernelGGL((beam_parts_kernel<Fp32>), grid, dim3(256), 0, stream, a);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {

@@ -501,6 +501,7 @@ constexpr int kCopyAhead = 4;   // 16-byte loads of a lane
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
+// Bound by memory: 373 us for the large cache of the compaction (4.9 TB/s read and written), 38 for 32 requests' pages of 16; 41 with one load of a lane at a time.
 // A wave per piece: 16 tokens of one page and head; blockIdx.y: layer, and keys or values. The lanes read the entries of a wave's next 64 pieces at once, so
 // that lists that are mostly empty are soon passed over.
 __global__ void __launch_bounds__(256) copy_pages_kernel(CopyPagesArgs a) {

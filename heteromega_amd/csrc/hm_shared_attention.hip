@@ -4,10 +4,14 @@
 // rows, whose query heads are the columns of the matrix products, and gives each column a maximum m, a sum l and an output o relative to it; a second launch joins
 // the parts of a column: out = sum of o 2^(m - M) / sum of l 2^(m - M).
 //
-// Up to 16 columns a segment is bound by the reads of its keys and values, as a row of its own is; it is worked on as in hm_paged_attention.hip, four waves to a tile
-// of 128 keys. With more, the four waves share tiles of 64 keys and have up to 32 columns each, as for the rows of prompts; from about 128 columns the matrix
-// cores bound it. The tiles of each kind lie in a line that is cut into equal runs, one of each for every workgroup, and half of the workgroups begin with
-// the one and half with the other, so that reads and products overlap.
+// Up to 32 columns a segment is bound by the reads of its keys and values, as a row of its own is. A wave has a unit (a segment and key head) to itself, in tiles of
+// 32 keys that pass through its registers and its part of LDS, and the next tile is on the way meanwhile. With more, up to 128 columns, the four waves of a workgroup
+// have 32 each and share tiles of 32 keys; from about 128 columns the matrix cores bound it, and it is worked on as a pipeline of transfers, products and weights.
+// (Units of 17 to 32 columns as wide ones, of which one wave in four had work: 88 us instead of 81 at 256 rows in groups of 8 with 4 query heads to a key head.) The tiles of each kind lie in a line that is cut into equal runs. The first workgroups, one per CU at most, have a run of the wide line each, the waves of the
+// others one of the narrow line, so that a CU has work that reads and work that multiplies.
+//
+// 128 rows, 32 / 8 heads of 128, bf16: 16 384 keys shared by all 84 us (410 TFLOP/s; the products of both halves of the weights are 615), 65 536 keys 253 (543 and 815;
+// a large product reaches 1199); up to 1024 keys of its own for each row 63 us (4.7 TB/s); both 110.
 #include "hm_shared_attention.hpp"
 
 namespace hm {
