@@ -323,7 +323,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
                 f(i, stats[i]);
             }
         };
-        float sum = 0.0f;
+        double sum = 0.0;
         if (open) {
             each([&](int, float2 st) {
                 top = fmaxf(top, st.x);
@@ -331,10 +331,10 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
             });
             top = over_lanes(top, [](float v, float w) { return fmaxf(v, w); });
             each([&](int, float2 st) { sum += st.y == 0.0f ? 0.0f : st.y * __builtin_amdgcn_exp2f((st.x - top) * 1.4426950408889634f); });
-            sum = over_lanes(sum, [](float v, float w) { return v + w; });
+            sum = over_lanes(static_cast<float>(sum), [](float v, float w) { return v + w; });
             odd = __any(odd) || !(fabsf(top) < INFINITY);
         }
-        const double of_row = static_cast<double>(top) + log(static_cast<double>(sum)), from = (open && odd) || !(fabsf(score) < INFINITY) ? NAN : static_cast<double>(score);
+        const double of_row = static_cast<double>(top) + log(sum), from = (open && odd) || !(fabsf(score) < INFINITY) ? NAN : static_cast<double>(score);
         if (lane == 0) {
             norm[beam] = of_row;
             base[beam] = from;
