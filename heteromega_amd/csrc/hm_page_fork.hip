@@ -509,8 +509,8 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(CopyPagesArgs a) {
     const int layer = blockIdx.y >> 1;
     const uint16_t *from = (blockIdx.y & 1) ? a.from_v[layer] : a.from_k[layer];
     uint16_t *to = (blockIdx.y & 1) ? a.to_v[layer] : a.to_k[layer];
-    const int per_page = a.kv_heads << (a.page_shift - 4), row_pieces = a.head_dim / 8, per_step = 64 / row_pieces;
-    const int in_step = lane / row_pieces, at = (lane - in_step * row_pieces) * 8, first_token = in_step < per_step ? in_step : kCopyTokens;
+    const int per_page = a.kv_heads << (a.page_shift - 4), row_pieces = a.head_dim / 8, per_step = max(64 / row_pieces, 1);
+    const int in_step = lane / row_pieces, first_piece = lane - in_step * row_pieces, first_token = in_step < per_step ? in_step : kCopyTokens;
     const int64_t pieces = a.count * per_page, step = static_cast<int64_t>(gridDim.x) * 4;
     for (int64_t p0 = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); p0 < pieces; p0 += 64 * step) {
         const int64_t p = p0 + lane * step;
@@ -527,19 +527,21 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(CopyPagesArgs a) {
             const int i = static_cast<int>(__builtin_ctzll(left));
             const int64_t in_from = __builtin_amdgcn_readlane(source, i) * a.from_page, in_to = __builtin_amdgcn_readlane(target, i) * a.to_page;
             const int at_head = __builtin_amdgcn_readlane(head, i), at_token = __builtin_amdgcn_readlane(t0, i);
-            const uint16_t *f = from + in_from + at_head * a.from_head + at_token * a.from_token + at;
-            uint16_t *t = to + in_to + at_head * a.to_head + at_token * a.to_token + at;
+            const uint16_t *f = from + in_from + at_head * a.from_head + at_token * a.from_token;
+            uint16_t *t = to + in_to + at_head * a.to_head + at_token * a.to_token;
             const int tokens = __builtin_amdgcn_readlane(count, i);
-            for (int token = first_token; token < tokens; token += kCopyAhead * per_step) { // all loads before the first store, which may be to their place, for what the compiler knows
-                u32x4_t v[kCopyAhead];
+            for (int at = 8 * first_piece; at < a.head_dim; at += 512) { // once, but for heads of more than 512
+                for (int token = first_token; token < tokens; token += kCopyAhead * per_step) {
+                    u32x4_t v[kCopyAhead]; // all loads before the first store, which may be to their place, for what the compiler knows
 #pragma unroll
-                for (int n = 0; n < kCopyAhead; ++n) {
-                    v[n] = *reinterpret_cast<const u32x4_t *>(f + min(token + n * per_step, tokens - 1) * a.from_token);
-                }
+                    for (int n = 0; n < kCopyAhead; ++n) {
+                        v[n] = *reinterpret_cast<const u32x4_t *>(f + min(token + n * per_step, tokens - 1) * a.from_token + at);
+                    }
 #pragma unroll
-                for (int n = 0; n < kCopyAhead; ++n) {
-                    if (token + n * per_step < tokens) {
-                        *reinterpret_cast<u32x4_t *>(t + (token + n * per_step) * a.to_token) = v[n];
+                    for (int n = 0; n < kCopyAhead; ++n) {
+                        if (token + n * per_step < tokens) {
+                            *reinterpret_cast<u32x4_t *>(t + (token + n * per_step) * a.to_token + at) = v[n];
+                        }
                     }
                 }
             }
@@ -555,7 +557,10 @@ hipError_t launch_page_fork(const PageForkArgs &a, hipStream_t stream) {
     if (a.requests_count <= 64) {
         return launch_fork<64, 1>(a, kMaxChunks, stream);
     }
-    return a.requests_count <= 1024 ? launch_fork<256, 4>(a, 512, stream) : launch_fork<1024, kMaxRequests / 1024>(a, 256, stream);
+    if (a.requests_count <= 256) {
+        return launch_fork<256, 1>(a, 512, stream);
+    }
+    return a.requests_count <= 1024 ? launch_fork<1024, 1>(a, 512, stream) : launch_fork<1024, kMaxRequests / 1024>(a, 256, stream);
 }
 
 size_t page_compact_workspace(int64_t pages) { return 4 * static_cast<size_t>(4 + 2 * ((pages + 31) / 32)); }

@@ -337,6 +337,11 @@ def test_copies_of_pages(hm, device, dtype, heads, ps, d):
     hm.copy_pages(caches[0], torch.full((5, 3), -1, dtype=torch.int32, device=device))
 
 
+@pytest.mark.parametrize("d", [16, 32, 48, 80, 112, 144, 256, 272, 512, 528, 1040])
+def test_copies_of_rows_of_any_width(hm, device, d):
+    test_copies_of_pages(hm, device, torch.bfloat16, 2, 32, d)
+
+
 def test_copies_of_many_layers_and_entries(hm, device):
     layers, pages, ps = 70, 40, 16
     caches = [hm.PagedCache.empty(pages, ps, 1, 64, torch.float16, device) for _ in range(layers)]
