@@ -103,6 +103,33 @@ def test_columns_of_wide_units(hm, device, dtype, heads, rows):
     Call(hm, device, rows, table, ends, 16, heads, 64, dtype).check(f"{rows} rows, {heads} heads")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("heads,rows", [((8, 2), 5), ((5, 1), 6), ((32, 4), 4), ((17, 1), 1), ((24, 1), 1), ((3, 3), 30)])
+def test_units_of_17_to_32_columns(hm, device, dtype, d, heads, rows):
+    for window in (0, 90):
+        table, ends = prompts(2, rows, 64, 320, 50, 16)
+        Call(hm, device, rows, table, ends, 16, heads, d, dtype, window=window).check(f"{rows} rows, {heads} heads of {d}, window {window}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [6, 8])
+def test_infinities_and_nan_in_units_of_24_and_32_columns(hm, device, dtype, rows):
+    test_infinities_and_nan(hm, device, dtype, rows)
+
+
+@pytest.mark.parametrize("dtype,d,heads,rows,keys", [("bf16", 64, (32, 8), 128, 37000), ("fp16", 128, (64, 8), 120, 20016), ("bf16", 256, (32, 8), 100, 20000)])
+def test_wide_runs_of_many_tiles(hm, device, dtype, d, heads, rows, keys):
+    # about 150 tiles for each of 256 runs, of which the pages of 64 are read at a time
+    table, ends = prompts(1, rows, keys // 16 * 16, 0, 200, 16)
+    c = Call(hm, device, 4, table, ends, 16, heads, d, dtype)
+    got = c()
+    same = hm.paged_attention(torch.zeros_like(c.q), c.q, c.cache, *c.on[:2])
+    torch.cuda.synchronize()
+    step = 2 * ref.half_step(c.q.dtype) * (same.float().abs().amax(-1, keepdim=True) + 1e-3)  # as below
+    assert ((got.float() - same.float()).abs() <= step).all()
+
+
 def test_long_keys_are_split_over_the_card(hm, device):
     for dtype, rows, heads, d in (("bf16", 2, (8, 2), 128), ("fp16", 30, (8, 2), 64), ("bf16", 40, (4, 1), 128), ("fp16", 3, (2, 1), 256)):
         table, ends = prompts(1, rows, 20000, 0, 300, 16)
