@@ -109,34 +109,42 @@ struct Depths {
     // The nearest boundaries before the lane's, of chunk c, and after it with a depth below its own, v > 0. There are some: the ends have depth 0.
     __device__ __forceinline__ int2 nearest(int c, int32_t v) const {
         const int lane = threadIdx.x & 63;
-        uint32_t low = 0, high = 0; // a bit per lane
-#pragma unroll 4
-        for (int j = 31; j >= 0; --j) {
-            low = low + low + (__builtin_amdgcn_readlane(v, j) < v ? 1 : 0);
-            high = high + high + (__builtin_amdgcn_readlane(v, j + 32) < v ? 1 : 0);
+        // Within the chunk by halves: minima of the 2^n boundaries behind each lane and before it, then the longest ways over boundaries that are no less deep.
+        // What lies outside the chunk counts as less deep.
+        int32_t back[6], ahead[6];
+#pragma unroll
+        for (int n = 0; n < 6; ++n) {
+            const int32_t b = __shfl_up(n == 0 ? v : back[n - 1], n == 0 ? 1 : 1 << (n - 1)), f = __shfl_down(n == 0 ? v : ahead[n - 1], n == 0 ? 1 : 1 << (n - 1));
+            back[n] = lane < 1 << n ? -1 : n == 0 ? b : min(back[n - 1], b);
+            ahead[n] = lane + (1 << n) > 63 ? -1 : n == 0 ? f : min(ahead[n - 1], f);
         }
-        const uint64_t less = static_cast<uint64_t>(high) << 32 | low;
-        const uint64_t before = less & ((uint64_t(1) << lane) - 1), after = less >> lane; // the lane's own bit is 0
+        int p = lane, q = lane;
+#pragma unroll
+        for (int n = 5; n >= 0; --n) {
+            const int32_t b = __shfl(back[n], p), f = __shfl(ahead[n], q);
+            p -= b >= v ? 1 << n : 0;
+            q += f >= v ? 1 << n : 0;
+        }
+        const bool before = p > 0, after = q < 63; // it is the next one then
         // in other chunks: first which, then where
         int left = -1, right = -1;
 #pragma unroll 1
-        for (int d = c - 1; d >= 0 && __any(v > 0 && before == 0 && left < 0); --d) {
+        for (int d = c - 1; d >= 0 && __any(v > 0 && !before && left < 0); --d) {
             left = left < 0 && onward[64 * d] < v ? d : left;
         }
 #pragma unroll 1
-        for (int d = c + 1; d < chunks && __any(v > 0 && after == 0 && right < 0); ++d) {
+        for (int d = c + 1; d < chunks && __any(v > 0 && !after && right < 0); ++d) {
             right = right < 0 && onward[64 * d] < v ? d : right;
         }
         int last = 0, first = 0; // of those behind it, one is less deep; of those up to it, none
-        if (__any(v > 0 && (before == 0 || after == 0))) {
+        if (__any(v > 0 && (!before || !after))) {
 #pragma unroll 1
             for (int step = 32; step > 0; step >>= 1) {
                 last += onward[64 * max(left, 0) + last + step] < v ? step : 0;
                 first += upto[64 * max(right, 0) + first + step - 1] >= v ? step : 0;
             }
         }
-        return make_int2(before != 0 ? 64 * c + 63 - __clzll(before) : 64 * max(left, 0) + last,
-                         after != 0 ? 64 * c + lane + __ffsll(static_cast<unsigned long long>(after)) - 1 : right >= 0 ? 64 * right + min(first, 63) : count);
+        return make_int2(before ? 64 * c + p - 1 : 64 * max(left, 0) + last, after ? 64 * c + q + 1 : right >= 0 ? 64 * right + min(first, 63) : count);
     }
 };
 
@@ -288,7 +296,7 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share
             }
         }
 #pragma unroll 1
-        for (int n = 0; n < 3; ++n) {
+        for (int n = 0; n < 3; n += a.window > 0 || n > 0 ? 1 : 2) {
             ShareSegment s = segment_of(j, n);
             own = own + take(s);
         }
@@ -322,7 +330,7 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share
     for (int j = 0; j < PER; ++j) {
         const int t = row_of(j);
 #pragma unroll 1
-        for (int n = 0; n < 3; ++n) {
+        for (int n = 0; n < 3; n += a.window > 0 || n > 0 ? 1 : 2) {
             ShareSegment s = segment_of(j, n);
             const Count c = take(s);
             const bool some = s.tiles > 0, is_wide = s.rows * a.group_heads > kNarrowCols;
@@ -338,6 +346,9 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share
                 if (w < (is_wide ? header.wide : narrow_runs)) {
                     atomicMax(&marks[is_wide ? narrow_runs + w : w], is_wide ? kOfWide + place : place);
                 }
+            }
+            if (n == 0 && t < R && a.window == 0) { // then no keys are left before the shared ones
+                ws.paths[R + t] = SharePath{0, 0, 0, 0, 0, 0, 0, 0};
             }
             if (n < 2 && t < R) { // a unit of one row for each key head
                 ws.paths[n * R + t] = some ? SharePath{s.tiles, is_wide ? 1 : 0, s.tile0, s.tiles, s.slot0, 1, 0, 0} : SharePath{0, 0, 0, 0, 0, 0, 0, 0};
