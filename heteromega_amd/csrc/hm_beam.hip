@@ -57,26 +57,24 @@ __device__ __forceinline__ bool is_open(const BeamSelectArgs &a, int64_t row) {
     return (a.ended == nullptr || a.ended[row] == 0) && fabsf(a.scores[row]) < INFINITY;
 }
 
-template <int CTRL> __device__ __forceinline__ float dpp(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
-}
+template <int CTRL> __device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_mov_dpp(v, CTRL, 0xF, 0xF, true); }
 
 // The values of a lane and of the one whose number has bit STEP changed, in either order, without passing through LDS.
-template <int STEP> __device__ __forceinline__ float2 both(float v) {
+template <int STEP> __device__ __forceinline__ int2 both(int v) {
     if constexpr (STEP <= 8) { // quad_perm, row_half_mirror (^ 7) of quad_perm (^ 3), row_ror
-        return make_float2(v, STEP == 1 ? dpp<0xB1>(v) : STEP == 2 ? dpp<0x4E>(v) : STEP == 4 ? dpp<0x141>(dpp<0x1B>(v)) : dpp<0x128>(v));
+        return make_int2(v, STEP == 1 ? dpp<0xB1>(v) : STEP == 2 ? dpp<0x4E>(v) : STEP == 4 ? dpp<0x141>(dpp<0x1B>(v)) : dpp<0x128>(v));
     } else {
         typedef unsigned pair_t __attribute__((ext_vector_type(2)));
-        const unsigned bits = __float_as_uint(v);
+        const unsigned bits = static_cast<unsigned>(v);
         const pair_t p = STEP == 16 ? __builtin_bit_cast(pair_t, __builtin_amdgcn_permlane16_swap(bits, bits, false, false))
                                     : __builtin_bit_cast(pair_t, __builtin_amdgcn_permlane32_swap(bits, bits, false, false));
-        return make_float2(__uint_as_float(p.x), __uint_as_float(p.y));
+        return make_int2(static_cast<int>(p.x), static_cast<int>(p.y));
     }
 }
 
 template <int STEP = 1, class F> __device__ __forceinline__ float over_lanes(float v, F f) {
-    const float2 p = both<STEP>(v);
-    v = f(p.x, p.y);
+    const int2 p = both<STEP>(__float_as_int(v));
+    v = f(__int_as_float(p.x), __int_as_float(p.y));
     if constexpr (STEP < 32) {
         v = over_lanes<2 * STEP>(v, f);
     }
@@ -84,9 +82,9 @@ template <int STEP = 1, class F> __device__ __forceinline__ float over_lanes(flo
 }
 
 // Steps of a bitonic sort downwards over the lanes: runs of SIZE sorted, from pairs STEP lanes apart.
-template <int SIZE, int STEP> __device__ __forceinline__ float sort_steps(float v, int lane) {
-    const float2 p = both<STEP>(v);
-    const float more = fmaxf(p.x, p.y), less = fminf(p.x, p.y);
+template <int SIZE, int STEP> __device__ __forceinline__ int sort_steps(int v, int lane) {
+    const int2 p = both<STEP>(v);
+    const int more = max(p.x, p.y), less = min(p.x, p.y);
     v = ((lane & STEP) == 0) == ((lane & SIZE) == 0 || SIZE == 64) ? more : less;
     if constexpr (STEP > 1) {
         return sort_steps<SIZE, STEP / 2>(v, lane);
@@ -97,10 +95,14 @@ template <int SIZE, int STEP> __device__ __forceinline__ float sort_steps(float 
     }
 }
 
-// The k-th largest value of the lanes'.
-__device__ __forceinline__ float kth_of_lanes(float v, int k) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sort_steps<2, 1>(v, threadIdx.x & 63)), k - 1));
-}
+// The lanes' values sorted downwards, as whole numbers of the same order: those take one instruction each where floats are made quiet first.
+struct Sorted {
+    int keys;
+
+    static __device__ __forceinline__ int key_of(int bits) { return bits ^ (bits >> 31 & 0x7FFFFFFF); }
+    __device__ __forceinline__ explicit Sorted(float v) : keys(sort_steps<2, 1>(key_of(__float_as_int(v)), threadIdx.x & 63)) {}
+    __device__ __forceinline__ float at(int i) const { return __int_as_float(key_of(__builtin_amdgcn_readlane(keys, i))); }
+};
 
 __device__ __forceinline__ bool before(float v, int32_t token, float w, int32_t other) { return v > w || (v == w && token < other); }
 
@@ -153,7 +155,8 @@ template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(Beam
         most = fmaxf(most, x[j]);
     }
     const int k = a.k;
-    const float top = over_lanes(most, [](float v, float w) { return fmaxf(v, w); });
+    const Sorted best(most);
+    const float top = best.at(0);
     // An infinity or NaN among the logits makes the sum NaN.
     const float from = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
@@ -173,7 +176,7 @@ template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(Beam
         ws.stats[at] = make_float2(top, sum);
     }
     Candidate *out = ws.candidates + at * k;
-    const float bound = fmaxf(kth_of_lanes(most, k), -3.4028234663852886e38f); // -infinity is no candidate
+    const float bound = fmaxf(best.at(k - 1), -3.4028234663852886e38f); // -infinity is no candidate
     Candidate *mine = list[wave];
 #if defined(__HIP_DEVICE_COMPILE__)
     asm volatile("" : "+v"(first_token)); // the tokens are worked out again rather than kept in registers
@@ -396,7 +399,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
         a.scores_out[to] = some ? static_cast<float>(s.score) : -INFINITY;
         a.ended_out[to] = !some || was_ended[s.beam] != 0 || s.token == a.end_token;
     };
-    double bound = kth_of_lanes(own, k);
+    double bound = Sorted(own).at(k - 1);
     for (;;) {
         __syncthreads(); // the list's last readers are done
         if (threadIdx.x == 0) {
