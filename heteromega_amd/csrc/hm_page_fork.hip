@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(256) compact_mark_kernel(PageCompactArgs a) {
 }
 
 constexpr int kCountedWords = 8 * 1024;    // a bit per page, in LDS
-constexpr int kCountedEntries = 128 * 1024; // of the table
+constexpr int kCountedEntries = 48 * 1024; // of the table, at least 64 a request
 
 // The sums of the words' bits, in one workgroup. MARK: after the bits are set, in LDS, which takes the place of the two launches before.
 template <bool MARK> __global__ void __launch_bounds__(1024) compact_sum_kernel(PageCompactArgs a) {
@@ -554,6 +554,8 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(CopyPagesArgs a) {
 size_t page_fork_workspace(int64_t requests, int64_t width) { return 16 + 4 * static_cast<size_t>(kMaxChunks + width + 2 * requests); }
 
 hipError_t launch_page_fork(const PageForkArgs &a, hipStream_t stream) {
+    // A thread per request where a workgroup has them: 256 requests 11.3 us with 256 threads and 12.7 with 1024, 512 of the mixed case's 15 with 1024 and
+    // 18 with four to a thread; up to 64, one wave 10.9 and four 11.1.
     if (a.requests_count <= 64) {
         return launch_fork<64, 1>(a, kMaxChunks, stream);
     }
@@ -571,8 +573,9 @@ hipError_t launch_page_compact(const PageCompactArgs &a, hipStream_t stream) {
     const unsigned requests = static_cast<unsigned>(std::min<int64_t>(a.requests_count, 4 * cus));
     const unsigned wide = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((a.width + 255) / 256, 4 * cus / requests)));
     const unsigned ids = static_cast<unsigned>(std::min<int64_t>(4 * cus, (a.pages + 255) / 256));
-    // One workgroup marks a table of up to 128 thousand entries sooner than two more launches take (each about 4.7 us).
-    if (words <= kCountedWords && a.requests_count * a.width <= kCountedEntries) {
+    // One workgroup marks a small table sooner than two more launches take: 4096 entries 10.1 us instead of 14.6, 24 576 13.7 instead of 18.2; 65 536 entries
+    // of 512 requests 20.1 either way, of 1024 requests 23.7 instead of 20.5, and 131 072 32 instead of 23.
+    if (words <= kCountedWords && a.requests_count * std::max<int64_t>(a.width, 64) <= kCountedEntries) {
         hipLaunchKernelGGL(compact_sum_kernel<true>, dim3(1), dim3(1024), 4 * static_cast<size_t>(words), stream, a);
     } else {
         hipLaunchKernelGGL(compact_clear_kernel, dim3(clear), dim3(256), 0, stream, a);
