@@ -3,14 +3,14 @@
 // Bound by memory and, nearly as much, by the instructions of a first launch, which reads the logits once: 64 requests of 4 beams and 152064 tokens have 78 MB of
 // them in 16 bits. A wave takes 32 elements a lane of one row into registers and works out its maximum, the sum of exp relative to it and its k best tokens. A
 // second launch, a workgroup per request, joins the waves' sums and picks the k best of their candidates. It is bound by latency: of the waves' best ones only
-// those that reach the k-th score's bound are looked at closely. With all candidates compared it took 26 to 34 us, so 7. Candidates of one row are compared by their
+// those that reach the k-th score's bound are looked at closely. With all candidates compared it took 26 to 34 us, so 5.5. Candidates of one row are compared by their
 // logits, which are exact; those of different rows by fp64 scores, so that rounding adds no ties.
 //
-// The k best of a wave's 2048: the k-th largest of the 64 lanes' maxima, found by sorting them over the lanes, is a bound that at least k elements reach and
-// seldom many more; those go to a list in LDS and are ranked by counting who comes before. (The least of k or more groups' maxima is quicker to find, but
-// almost three times as many reach it: 37 us instead of 21 for the case above. 64 elements a lane, with fewer sorts, took 25 at three waves a SIMD; 8 or 16 of them
-// for few logits gain less here than the second launch loses by more parts.) Many equal or badly spread
-// elements overflow the list; then the best are taken one after the other.
+// The k best of a wave's 2048: the k-th largest of the 64 lanes' maxima (above k = 32, of 128 halves' maxima), found by sorting them over the lanes, is a bound that at
+// least k elements reach and seldom many more; those go to a list in LDS and are ranked by counting who comes before. (The least of k or more groups' maxima is
+// quicker to find, but almost three times as many reach it: 37 us instead of 21 for the case above. 64 elements a lane, with fewer sorts, took 25 at three waves a
+// SIMD; 8 or 16 of them for few logits gain less here than the second launch loses by more parts.) Many equal or badly spread elements overflow the list; then the
+// best are taken one after the other. A request's candidates are ranked in the same way, after a second and third bound where there are many.
 #include "hm_device.hpp"
 #include "hm_internal.hpp"
 
@@ -18,9 +18,10 @@ namespace hm {
 namespace {
 
 constexpr int kElements = 32;    // of a lane
-constexpr int kList = 512;       // candidates that a wave's list holds: at k = 64 about 300 reach the bound
+constexpr int kList = 256;       // candidates that a wave's list holds
 constexpr int kJoinList = 1024;  // and that of a request
 constexpr int kJoinParts = 1024; // parts that are looked at at once
+constexpr int kRanked = 128;     // candidates that are ranked without a look for a better bound
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
@@ -37,14 +38,19 @@ template <> struct Elements<Fp32> {
     static __device__ __forceinline__ float get(const u32x4_t &v, int i) { return __uint_as_float(v[i]); }
 };
 
-struct alignas(8) Candidate {
-    float logit;
-    int32_t token;
-};
+// A logit and its token as one whole number, in the order of candidates of a row: larger logits first (zeros of either sign are equal), of equal ones lower tokens.
+// 0: none.
+typedef uint64_t Candidate;
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const uint32_t bits = __float_as_uint(v + 0.0f);
+    return bits ^ ((bits >> 31) != 0 ? 0xFFFFFFFFu : 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float((key >> 31) != 0 ? key ^ 0x80000000u : ~key); }
+__device__ __forceinline__ Candidate candidate(float logit, int32_t token) { return static_cast<uint64_t>(ordered(logit)) << 32 | ~static_cast<uint32_t>(token); }
 
 struct BeamWorkspace {
     float2 *stats;         // [rows][parts]: maximum, and sum of exp(logit - maximum)
-    Candidate *candidates; // [rows][parts][k], best first; tokens of -1 behind the last
+    Candidate *candidates; // [rows][parts][k], best first
 };
 
 __host__ __device__ __forceinline__ BeamWorkspace carve_beam(void *p, int64_t rows, int64_t parts) {
@@ -104,8 +110,6 @@ struct Sorted {
     __device__ __forceinline__ float at(int i) const { return __int_as_float(key_of(__builtin_amdgcn_readlane(keys, i))); }
 };
 
-__device__ __forceinline__ bool before(float v, int32_t token, float w, int32_t other) { return v > w || (v == w && token < other); }
-
 // A wave per part of a row.
 template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(BeamSelectArgs a) {
     using E = Elements<T>;
@@ -149,14 +153,18 @@ template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(Beam
             x[j] = token >= 0 && token < vocabulary ? x[j] : -INFINITY;
         }
     }
-    float most = x[0];
+    float half[2] = {x[0], x[kOne / 2]}; // of the halves of each 16 bytes, so that short rows have both
 #pragma unroll
     for (int j = 1; j < kElements; ++j) {
-        most = fmaxf(most, x[j]);
+        half[j % kOne / (kOne / 2)] = fmaxf(half[j % kOne / (kOne / 2)], x[j]);
     }
     const int k = a.k;
-    const Sorted best(most);
+    Sorted best(fmaxf(half[0], half[1]));
     const float top = best.at(0);
+    if (k > 32) { // the best 64 of the lanes' halves' maxima: the bound that 64 of 64 maxima give is reached by 300 elements, this one by 90
+        const Sorted first(half[0]), second(half[1]);
+        best.keys = sort_steps<2, 1>(max(first.keys, __shfl(second.keys, 63 - lane)), lane);
+    }
     // An infinity or NaN among the logits makes the sum NaN.
     const float from = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
@@ -189,50 +197,57 @@ template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(Beam
         if (who != 0) {
             const int place = count + __popcll(who & ((uint64_t(1) << lane) - 1));
             if (in && place < kList) {
-                mine[place] = Candidate{x[j], token_of(j)};
+                mine[place] = candidate(x[j], token_of(j));
             }
             count += __popcll(who);
         }
     }
     __builtin_amdgcn_wave_barrier(); // a wave's LDS accesses are carried out in order
+    for (int i = count + lane; i < k; i += 64) {
+        out[i] = 0;
+    }
     if (count <= 64) {
-        const Candidate c = lane < count ? mine[lane] : Candidate{-INFINITY, -1};
-        // in the order of the values, equal ones (zeros of either sign, too) by token
-        const uint32_t bits = __float_as_uint(c.logit + 0.0f), upper = bits ^ ((bits >> 31) != 0 ? 0xFFFFFFFFu : 0x80000000u), lower = ~static_cast<uint32_t>(c.token);
-        const uint64_t key = static_cast<uint64_t>(upper) << 32 | lower;
+        const Candidate c = lane < count ? mine[lane] : 0;
+        const uint32_t upper = static_cast<uint32_t>(c >> 32), lower = static_cast<uint32_t>(c);
         int rank = 0;
         for (int j = 0; j < count; ++j) {
             const uint32_t u = __builtin_amdgcn_readlane(upper, j), v = __builtin_amdgcn_readlane(lower, j);
-            rank += (static_cast<uint64_t>(u) << 32 | v) > key;
+            rank += (static_cast<uint64_t>(u) << 32 | v) > c;
         }
         if (lane < count && rank < k) {
             out[rank] = c;
         }
-        if (lane >= count && lane < k) {
-            out[lane] = Candidate{-INFINITY, -1};
-        }
         return;
     }
     if (count <= kList) {
-        for (int i = lane; i < count; i += 64) {
-            const Candidate c = mine[i];
-            int rank = 0;
-#pragma unroll 4
-            for (int j = 0; j < count; ++j) {
-                const Candidate d = mine[j];
-                rank += before(d.logit, d.token, c.logit, c.token);
+        Candidate own[kList / 64];
+        int rank[kList / 64];
+#pragma unroll
+        for (int i = 0; i < kList / 64; ++i) {
+            own[i] = 64 * i + lane < count ? mine[64 * i + lane] : 0;
+            rank[i] = 0;
+        }
+#pragma unroll 2
+        for (int j = 0; j < count; ++j) {
+            const Candidate c = mine[j];
+#pragma unroll
+            for (int i = 0; i < kList / 64; ++i) {
+                if (64 * i < count) {
+                    rank[i] += c > own[i];
+                }
             }
-            if (rank < k) {
-                out[rank] = c;
+        }
+#pragma unroll
+        for (int i = 0; i < kList / 64; ++i) {
+            if (64 * i + lane < count && rank[i] < k) {
+                out[rank[i]] = own[i];
             }
         }
         return;
     }
-    float last = INFINITY;
-    int32_t last_token = -1;
+    Candidate last = ~Candidate(0);
     for (int i = 0; i < k; ++i) { // the best behind the last one taken, from memory: seldom, and little code
-        float best = -INFINITY;
-        int32_t token = INT32_MAX;
+        Candidate best = 0;
 #pragma unroll 1
         for (int j = 0; j < V; ++j) {
             const u32x4_t piece = __builtin_amdgcn_raw_buffer_load_b128(resource, lane * 16, j * 1024, 0);
@@ -240,44 +255,45 @@ template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(Beam
             for (int e = 0; e < kOne; ++e) {
                 const int32_t t = token_of(j * kOne + e);
                 const float v = t >= 0 && t < vocabulary ? E::get(piece, e) : -INFINITY;
-                if (before(last, last_token, v, t) && before(v, t, best, token)) {
-                    best = v, token = t;
-                }
+                const Candidate c = v > -INFINITY ? candidate(v, t) : 0;
+                best = c < last && c > best ? c : best;
             }
         }
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) {
-            const float v = __shfl_xor(best, off);
-            const int32_t t = __shfl_xor(token, off);
-            if (before(v, t, best, token)) {
-                best = v, token = t;
-            }
+            const Candidate other = __shfl_xor(static_cast<unsigned long long>(best), off);
+            best = other > best ? other : best;
         }
         if (lane == 0) {
-            out[i] = best == -INFINITY ? Candidate{-INFINITY, -1} : Candidate{best, token};
+            out[i] = best;
         }
-        last = best, last_token = token;
+        last = best;
     }
 }
 
-struct Scored {
-    double score;
-    int32_t beam;
-    float logit;
-    int32_t token;
-};
+// A request's candidate in the order of the results: by score, then lower beams first, then as candidates of a row, which rounded scores may make equal (next to a
+// sum of 1e38, say). {0, 0}: none.
+struct alignas(16) Scored {
+    uint64_t score, rest; // rest: 8 bits of the beam, 32 of the logit, 24 of the token
 
-// Where the scores' rounding makes equals of a row's logits (next to a sum of 1e38, say), these still tell them apart.
-__device__ __forceinline__ bool before(const Scored &a, const Scored &b) {
-    return a.score > b.score || (a.score == b.score && (a.beam < b.beam || (a.beam == b.beam && before(a.logit, a.token, b.logit, b.token))));
-}
+    static __device__ __forceinline__ Scored of(double score, int beam, float logit, int32_t token) {
+        const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(score + 0.0));
+        return {bits ^ ((bits >> 63) != 0 ? ~uint64_t(0) : uint64_t(1) << 63),
+                static_cast<uint64_t>(255 - beam) << 56 | static_cast<uint64_t>(ordered(logit)) << 24 | (0xFFFFFFu - static_cast<uint32_t>(token))};
+    }
+    __device__ __forceinline__ double value() const { return __longlong_as_double(static_cast<long long>((score >> 63) != 0 ? score ^ uint64_t(1) << 63 : ~score)); }
+    __device__ __forceinline__ int beam() const { return 255 - static_cast<int>(rest >> 56); }
+    __device__ __forceinline__ int32_t token() const { return static_cast<int32_t>(0xFFFFFFu - (static_cast<uint32_t>(rest) & 0xFFFFFFu)); }
+    __device__ __forceinline__ bool some() const { return score != 0; }
+};
+static_assert(HM_BEAM_MAX_BEAMS <= 256, "a beam has 8 bits");
+
+__device__ __forceinline__ bool before(const Scored &a, const Scored &b) { return a.score > b.score || (a.score == b.score && a.rest > b.rest); }
 
 __device__ __forceinline__ Scored better(const Scored &a, const Scored &b) { // by fields: the whole would be picked in memory
     const bool first = before(a, b);
-    return Scored{first ? a.score : b.score, first ? a.beam : b.beam, first ? a.logit : b.logit, first ? a.token : b.token};
+    return Scored{first ? a.score : b.score, first ? a.rest : b.rest};
 }
-
-constexpr Scored kNone{-INFINITY, INT32_MAX, -INFINITY, INT32_MAX};
 
 __device__ __forceinline__ float rounded_down(double v) {
     const float f = static_cast<float>(v);
@@ -372,33 +388,32 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
                : was_ended[beam] != 0 ? (part == 0 ? static_cast<float>(base[beam]) : -INFINITY)
                                       : rounded_down(base[beam] + (static_cast<double>(ws.stats[(row0 + beam) * parts + part].x) - norm[beam]));
     };
-    // Candidate `place` of a part, as the rows' sums have it; one that is not there has a score of -infinity.
+    // Candidate `place` of a part, as the rows' sums have it, or none.
     const auto scored = [&](int i, int place) {
         const int beam = i / parts, part = i - beam * parts;
-        Scored s = kNone;
         if (base[beam] != base[beam]) {
-            return s;
+            return Scored{0, 0};
         }
         if (was_ended[beam] != 0) {
-            if (part == 0 && place == 0) {
-                s = Scored{base[beam], beam, 0.0f, a.end_token};
-            }
-            return s;
+            return part == 0 && place == 0 ? Scored::of(base[beam], beam, 0.0f, a.end_token) : Scored{0, 0};
         }
-        const Candidate c = __builtin_bit_cast(Candidate, *reinterpret_cast<const uint2 *>(ws.candidates + ((row0 + beam) * parts + part) * k + place));
-        if (c.token >= 0) {
-            s = Scored{base[beam] + (static_cast<double>(c.logit) - norm[beam]), beam, c.logit, c.token};
-        }
-        return s;
+        const Candidate c = ws.candidates[((row0 + beam) * parts + part) * k + place];
+        const float logit = value_of(static_cast<uint32_t>(c >> 32));
+        return c != 0 ? Scored::of(base[beam] + (static_cast<double>(logit) - norm[beam]), beam, logit, static_cast<int32_t>(~static_cast<uint32_t>(c))) : Scored{0, 0};
     };
     const auto put = [&](int rank, const Scored &s) {
         const int64_t to = static_cast<int64_t>(blockIdx.x) * k + rank;
-        const bool some = s.score > -INFINITY;
-        a.parents[to] = some ? static_cast<int32_t>(row0) + s.beam : -1;
-        a.tokens[to] = some ? s.token : -1;
-        a.scores_out[to] = some ? static_cast<float>(s.score) : -INFINITY;
-        a.ended_out[to] = !some || was_ended[s.beam] != 0 || s.token == a.end_token;
+        const bool some = s.some();
+        a.parents[to] = some ? static_cast<int32_t>(row0) + s.beam() : -1;
+        a.tokens[to] = some ? s.token() : -1;
+        a.scores_out[to] = some ? static_cast<float>(s.value()) : -INFINITY;
+        a.ended_out[to] = !some || was_ended[s.beam()] != 0 || s.token() == a.end_token;
     };
+    if (all < 64) { // so few parts that their second, third and further best ones count
+        const int place = lane / all;
+        const Scored s = place < k ? scored(lane - place * all, place) : Scored{0, 0};
+        own = s.some() ? rounded_down(s.value()) : -INFINITY;
+    }
     double bound = Sorted(own).at(k - 1);
     for (;;) {
         __syncthreads(); // the list's last readers are done
@@ -420,7 +435,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
             for (int i = threadIdx.x; i < works * k; i += THREADS) {
                 const int w = i / k;
                 const Scored s = scored(work[w], i - w * k);
-                if (s.score >= bound && s.score > -INFINITY) {
+                if (s.some() && s.value() >= bound) {
                     const int place = atomicAdd(&listed, 1);
                     if (place < kJoinList) {
                         list[place] = s;
@@ -431,6 +446,23 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
         }
         const int count = min(listed, kJoinList);
         const bool whole = listed <= kJoinList;
+        if (count > kRanked + 4 * k) { // ranking takes the square of the number: the k-th of the lanes' best ones listed is a better bound, unless there are many equal ones
+            float most = -INFINITY;
+            for (int i = threadIdx.x; i < count; i += THREADS) {
+                most = fmaxf(most, rounded_down(list[i].value()));
+            }
+            maxima[wave][lane] = most;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                most = fmaxf(most, maxima[w][lane]);
+            }
+            const double next = Sorted(most).at(k - 1);
+            if (next > bound) {
+                bound = next;
+                continue;
+            }
+        }
         for (int i = threadIdx.x; i < count; i += THREADS) {
             const Scored s = list[i];
             int rank = 0;
@@ -442,12 +474,12 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
                 put(rank, s);
             }
             if (!whole && rank == k - 1) {
-                next_bound = s.score;
+                next_bound = s.value();
             }
         }
         if (whole) {
             for (int i = count + threadIdx.x; i < k; i += THREADS) {
-                put(i, kNone);
+                put(i, Scored{0, 0});
             }
             return;
         }
@@ -458,9 +490,9 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
         }
         bound = next_bound;
     }
-    Scored last{INFINITY, -1, INFINITY, -1};
+    Scored last{~uint64_t(0), ~uint64_t(0)};
     for (int i = 0; i < k; ++i) { // the best behind the last one taken
-        Scored best = kNone;
+        Scored best{0, 0};
         for (int64_t j = threadIdx.x; j < static_cast<int64_t>(all) * k; j += THREADS) {
             const int part = static_cast<int>(j / k);
             const Scored s = scored(part, static_cast<int>(j - static_cast<int64_t>(part) * k));
@@ -470,7 +502,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
         }
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) {
-            const Scored other{__shfl_xor(best.score, off), __shfl_xor(best.beam, off), __shfl_xor(best.logit, off), __shfl_xor(best.token, off)};
+            const Scored other{__shfl_xor(static_cast<unsigned long long>(best.score), off), __shfl_xor(static_cast<unsigned long long>(best.rest), off)};
             best = better(other, best);
         }
         if (lane == 0) {
