@@ -71,13 +71,14 @@ __global__ void __launch_bounds__(256) shared_tokens_kernel(SharePlanArgs a) {
     }
 }
 
-// What a row's segments take of the lines: segments and tiles of the narrow and the wide one, and slots. Two words, for the sums over rows.
+// What a row's segments take of the lines: segments and tiles of the narrow and the wide one, slots, and chunks of the wide one. Two words, for the sums over rows.
 struct Count {
-    uint64_t places, tiles; // narrow, wide << 16, slots << 32; narrow, wide << 32
+    uint64_t places, tiles; // narrow, wide << 16, slots << 32, chunks << 48 (at most five for a row); narrow, wide << 32
 
     __device__ __forceinline__ int narrow() const { return static_cast<int>(places & 0xFFFF); }
     __device__ __forceinline__ int wide() const { return static_cast<int>(places >> 16 & 0xFFFF); }
-    __device__ __forceinline__ int slots() const { return static_cast<int>(places >> 32); }
+    __device__ __forceinline__ int slots() const { return static_cast<int>(places >> 32 & 0xFFFF); }
+    __device__ __forceinline__ int chunks() const { return static_cast<int>(places >> 48); }
     __device__ __forceinline__ int narrow_tiles() const { return static_cast<int>(tiles); }
     __device__ __forceinline__ int wide_tiles() const { return static_cast<int>(tiles >> 32); }
 };
@@ -275,7 +276,8 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share
         }
         const uint64_t some = s.tiles > 0 ? 1 : 0;
         const uint64_t tiles = static_cast<uint32_t>(s.tiles) * static_cast<uint32_t>(a.kv_heads * chunks);
-        return Count{some << (wide ? 16 : 0) | static_cast<uint64_t>(some != 0 ? s.rows : 0) << 32, tiles << (wide ? 32 : 0)};
+        const uint64_t of_wide = wide ? chunks : 0;
+        return Count{some << (wide ? 16 : 0) | (some != 0 ? static_cast<uint64_t>(s.rows) << 32 | of_wide << 48 : 0), tiles << (wide ? 32 : 0)};
     };
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
@@ -318,7 +320,7 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share
         total = total + waves[w];
     }
     const ShareHeader header{{total.narrow_tiles(), total.wide_tiles()}, R, a.group_heads, a.kv_heads, a.groups,
-                             wide_groups(total.wide_tiles(), total.narrow_tiles(), a.groups), 0};
+                             wide_groups(total.wide_tiles(), static_cast<int64_t>(total.chunks()) * a.kv_heads, total.narrow_tiles(), a.groups), 0};
     if (threadIdx.x == 0) {
         *ws.header = header;
     }

@@ -19,10 +19,14 @@ __host__ __device__ __forceinline__ int cols_of(int line) { return line == 0 ? k
 // The workgroups that the wide line gets: one per CU at most, since two are hardly faster and leave twice the parts, and no more than have four tiles each. A
 // wide run has one tile for each 512 narrow ones of the call, so that with many narrow tiles the wide line ends before the narrow one and leaves it most of the
 // card: the card reads 500 to 600 tiles of heads of 128 while a workgroup works on one wide tile. 256 rows whose 6.4k keys were shared by all and, mostly, by 8 took
-// 67 us so and 79 with a workgroup per CU; 16 384 keys shared by 128 rows with 1024 of their own 110 either way, and no less with fewer.
-__host__ __device__ __forceinline__ int wide_groups(int wide_tiles, int narrow_tiles, int groups) {
-    const int each = narrow_tiles > 4 * 512 ? narrow_tiles / 512 : 4, most = (wide_tiles + each - 1) / each;
-    return most < groups / 2 ? most : groups / 2;
+// 67 us so and 79 with a workgroup per CU; 16 384 keys shared by 128 rows with 1024 of their own 110 either way, and no less with fewer. To begin and end a
+// unit takes a workgroup as long as about eight tiles, which counts where units are short: 84 rows of 32 key heads under a window of 30 keys, with 32 units of a tile or
+// two, took 45 us with four of them for each workgroup and 19 with one; 126 rows on 358 keys and 2193 of their own 133 and 94.
+__host__ __device__ __forceinline__ int wide_groups(int wide_tiles, int64_t wide_units, int narrow_tiles, int groups) {
+    const int each = narrow_tiles / 512, long_each = each > 4 ? each : 4, short_each = each > 9 ? each : 9;
+    const int64_t of_long = (static_cast<int64_t>(wide_tiles) + long_each - 1) / long_each, of_short = (wide_tiles + 8 * wide_units + short_each - 1) / short_each;
+    const int64_t most = of_long > of_short ? of_long : of_short < wide_tiles ? of_short : wide_tiles;
+    return most < groups / 2 ? static_cast<int>(most) : groups / 2;
 }
 
 // Rows [row0, row0 + rows) that see keys [lo, hi) in the same pages, as a place in one of two lines of tiles: those of narrow units, whose

@@ -10,10 +10,24 @@
 namespace hm {
 namespace {
 
-__device__ __forceinline__ ShareSegment uniform_segment(const ShareSegment *p) {
-    const ShareSegment s = *p;
-    return {uniform(s.row0), uniform(s.rows), uniform(s.lo), uniform(s.hi), uniform(s.tile0), uniform(s.tiles), uniform(s.slot0), uniform(s.chunk)};
-}
+// A run's segments, the next one on the way: one of its numbers a lane. The one behind the line's last is read too, and not used: other memory of the plan.
+struct Segments {
+    const ShareSegment *line;
+    int at;
+    int32_t next;
+
+    __device__ __forceinline__ Segments(const ShareSegment *l, int first) : line(l), at(first) { read(); }
+    __device__ __forceinline__ void read() { next = reinterpret_cast<const int32_t *>(line + at)[threadIdx.x & 7]; }
+    __device__ __forceinline__ ShareSegment take() const {
+        const auto of = [&](int i) { return __builtin_amdgcn_readlane(next, i); };
+        return {of(0), of(1), of(2), of(3), of(4), of(5), of(6), of(7)};
+    }
+    __device__ __forceinline__ void move_on() {
+        ++at;
+        read();
+    }
+};
+static_assert(sizeof(ShareSegment) == 32, "eight numbers");
 
 // A unit's tiles [tile0, tile1).
 struct Work {
@@ -24,9 +38,9 @@ struct Work {
 };
 
 // The next work of a run [x, x_end) of a line; moves x on.
-template <int LINE> __device__ __forceinline__ Work next_work(const SharedAttentionArgs &a, const ShareSegment *segments, int &at, int &x, int x_end, int w) {
+template <int LINE> __device__ __forceinline__ Work next_work(const SharedAttentionArgs &a, Segments &segments, int &x, int x_end, int w) {
     Work k;
-    k.s = uniform_segment(segments + at);
+    k.s = segments.take();
     const int chunks = LINE == 0 ? 1 : k.s.chunks();
     const int unit = uniform(static_cast<uint32_t>(x - k.s.tile0) / static_cast<uint32_t>(k.s.tiles));
     k.kv_head = LINE == 0 ? unit : unit / chunks;
@@ -37,7 +51,9 @@ template <int LINE> __device__ __forceinline__ Work next_work(const SharedAttent
     k.part = k.tile1 == k.s.tiles ? static_cast<int64_t>(k.s.slot0) * a.q_heads + (static_cast<int64_t>(k.kv_head) * k.s.rows + k.row) * a.group_heads
                                   : run_column(a.rows, a.q_heads, a.groups, LINE, w);
     x += k.tile1 - k.tile0;
-    at += k.tile1 == k.s.tiles && unit + 1 == a.kv_heads * chunks;
+    if (k.tile1 == k.s.tiles && unit + 1 == a.kv_heads * chunks) {
+        segments.move_on();
+    }
     return k;
 }
 
@@ -71,22 +87,25 @@ struct Pages {
     }
 };
 
-// The pages of 64 sub-tiles of 16 keys, a lane each, from one read of the table for all of them.
+// The pages of 64 sub-tiles of 16 keys, a lane each, from one read of the table for all of them. They stay from a unit to the next, which mostly is of the same rows
+// and another key head.
 struct PageIds {
-    int32_t ids;
-    int first; // sub-tile of lane 0
+    int32_t ids = 0;
+    int first = -1, row = -1, start = 0; // sub-tile of lane 0, and whose keys
+    bool bad = false;                    // a page outside the cache
 
-    // Reads on from sub-tile `sub`; true if a page lies outside the cache.
-    __device__ __forceinline__ bool read(const Pages &at, int start, int hi, int sub) {
-        first = sub;
-        ids = at.page_of(start + 16 * (sub + static_cast<int>(threadIdx.x & 63)), hi);
-        return __any(static_cast<uint32_t>(ids) >= at.pages);
+    __device__ __forceinline__ void read(const Pages &at, const ShareSegment &s, int sub) {
+        if (first != sub || row != s.row0 || start != s.start()) {
+            first = sub, row = s.row0, start = s.start();
+            ids = at.page_of(start + 16 * (sub + static_cast<int>(threadIdx.x & 63)), s.hi);
+            bad = __any(static_cast<uint32_t>(ids) >= at.pages);
+        }
     }
     __device__ __forceinline__ int32_t of(int sub) const { return __builtin_amdgcn_readlane(ids, sub - first); }
 };
 
 // A unit of up to 16 CT columns, by one wave, 32 keys at a time: with up to 128 units on a CU one after the other, waves go on to their next by themselves.
-template <class T, int D, int CT> __device__ __forceinline__ void narrow_work(const SharedAttentionArgs &a, const Work &k, uint8_t *lds) {
+template <class T, int D, int CT> __device__ __forceinline__ void narrow_work(const SharedAttentionArgs &a, const Work &k, uint8_t *lds, PageIds &ids) {
     using S = Shape<T, D>;
     const int lane = threadIdx.x & 63;
     const int col = lane & 15, quad = lane >> 4;
@@ -121,10 +140,10 @@ template <class T, int D, int CT> __device__ __forceinline__ void narrow_work(co
 
     constexpr int kTilesAhead = D == 64 ? 2 : 1; // 16 KB on the way for each wave keep the memory busy with one workgroup on a CU, 8 KB do not
     u32x4_t k_reg[kTilesAhead][2][S::kSteps], v_reg[kTilesAhead][2][S::kSteps];
-    PageIds ids;
     const auto request = [&](int tile, auto &k_reg, auto &v_reg) __attribute__((always_inline)) {
         if (2 * (tile - k.tile0) % 64 == 0) {
-            poisoned |= ids.read(at, start, hi, 2 * tile);
+            ids.read(at, k.s, 2 * tile);
+            poisoned |= ids.bad;
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -608,22 +627,28 @@ template <class T, int D> __global__ void __launch_bounds__(kThreads, D <= 128 ?
         const Runs runs = Runs::deal(uniform(header.tiles[1]), wide);
         // Runs that follow each other go to one XCD: those of a key head's chunks of rows read the same keys at the same time, and its L2 has them for all.
         const int xcd = blockIdx.x % a.xcds, w = xcd * (wide / a.xcds) + min(xcd, wide % a.xcds) + static_cast<int>(blockIdx.x / a.xcds), x_end = runs.begin(w + 1);
-        int x = runs.begin(w), at = uniform(plan.starts[1][w]);
+        int x = runs.begin(w);
+        Segments segments(plan.segments[1], uniform(plan.starts[1][w]));
         while (x < x_end) {
-            wide_work<T, D>(a, next_work<1>(a, plan.segments[1], at, x, x_end, w), lds);
+            wide_work<T, D>(a, next_work<1>(a, segments, x, x_end, w), lds);
         }
         return;
     }
     const int groups = a.groups - wide, w = wave * groups + group; // few runs go to as many workgroups
     const Runs runs = Runs::deal(uniform(header.tiles[0]), kAttentionWaves * groups);
     const int x_end = runs.begin(w + 1);
-    int x = runs.begin(w), at = uniform(plan.starts[0][w]);
+    int x = runs.begin(w);
+    if (x == x_end) {
+        return;
+    }
+    Segments segments(plan.segments[0], uniform(plan.starts[0][w]));
+    PageIds ids;
     while (x < x_end) {
-        const Work k = next_work<0>(a, plan.segments[0], at, x, x_end, w);
+        const Work k = next_work<0>(a, segments, x, x_end, w);
         if (k.rows * a.group_heads <= 16) {
-            narrow_work<T, D, 1>(a, k, lds + wave * S::kRegion);
+            narrow_work<T, D, 1>(a, k, lds + wave * S::kRegion, ids);
         } else {
-            narrow_work<T, D, 2>(a, k, lds + wave * S::kRegion);
+            narrow_work<T, D, 2>(a, k, lds + wave * S::kRegion, ids);
         }
     }
 }
