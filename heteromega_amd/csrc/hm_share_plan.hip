@@ -319,12 +319,13 @@ template <int THREADS, int PER> __global__ void __launch_bounds__(THREADS) share
         at = w < wave ? at + waves[w] : at;
         total = total + waves[w];
     }
-    const ShareHeader header{{total.narrow_tiles(), total.wide_tiles()}, R, a.group_heads, a.kv_heads, a.groups,
-                             wide_groups(total.wide_tiles(), static_cast<int64_t>(total.chunks()) * a.kv_heads, total.narrow_tiles(), a.groups), 0};
+    const int of_wide = wide_groups(total.wide_tiles(), static_cast<int64_t>(total.chunks()) * a.kv_heads, total.narrow_tiles(), a.groups);
+    const ShareHeader header{{total.narrow_tiles(), total.wide_tiles()}, R, a.group_heads, a.kv_heads, a.groups, of_wide,
+                             hm::narrow_runs(total.narrow_tiles(), static_cast<int64_t>(total.narrow()) * a.kv_heads, of_wide, a.groups)};
     if (threadIdx.x == 0) {
         *ws.header = header;
     }
-    const int narrow_runs = header.runs(0), runs = narrow_runs + header.runs(1);
+    const int narrow_runs = header.narrow, runs = narrow_runs + header.wide;
     const Runs narrow = Runs::deal(header.tiles[0], narrow_runs), wide = Runs::deal(header.tiles[1], max(header.wide, 1));
     ShareSegment *lines = ws.segments[0];
     const int wide_at = static_cast<int>(ws.segments[1] - lines); // no arrays indexed by the line: they would be in memory

@@ -29,6 +29,14 @@ __host__ __device__ __forceinline__ int wide_groups(int wide_tiles, int64_t wide
     return most < groups / 2 ? static_cast<int>(most) : groups / 2;
 }
 
+// And the narrow line's runs, of one wave each: of two tiles at least where units have eight or more on the average, since each run leaves a part to join (3 rows of 8628
+// shared keys, 28 / 4 heads of 128: 21.5 us, and 24.9 with runs of a tile; 16 rows of 1156 keys, 40 / 8 heads: 18.6 and 21.8), else of one (255 rows of 48 keys, 32 / 8
+// heads: 15.2 us, and 17.6 with two).
+__host__ __device__ __forceinline__ int narrow_runs(int narrow_tiles, int64_t narrow_units, int wide, int groups) {
+    const int most = kAttentionWaves * (groups - wide), wanted = narrow_tiles >= 8 * narrow_units ? narrow_tiles / 2 : narrow_tiles, some = wanted > groups ? wanted : groups;
+    return some < most ? some : most;
+}
+
 // Rows [row0, row0 + rows) that see keys [lo, hi) in the same pages, as a place in one of two lines of tiles: those of narrow units, whose
 // rows x query heads of a key head are at most kNarrowCols columns, and of wide ones. A segment has a unit for each key head and, in turn, each `chunk`
 // rows. Its units' results lie behind each other from row slot0 on.
@@ -52,11 +60,10 @@ struct SharePath {
 struct ShareHeader {
     int32_t tiles[2]; // narrow, wide
     int32_t rows, group_heads, kv_heads;
-    int32_t groups, wide; // workgroups, and those of the wide line
-    int32_t spare;
+    int32_t groups, wide, narrow; // workgroups, those of the wide line, and the narrow line's runs
 
     __host__ __device__ bool fits(int64_t n, int group, int heads, int g) const { return rows == n && group_heads == group && kv_heads == heads && groups == g; }
-    __host__ __device__ int runs(int line) const { return line == 0 ? kAttentionWaves * (groups - wide) : wide; }
+    __host__ __device__ int runs(int line) const { return line == 0 ? narrow : wide; }
 };
 
 // Memory of a plan. A line's segments are those with tiles, in the order of the line.

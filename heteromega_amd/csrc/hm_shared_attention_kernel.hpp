@@ -635,7 +635,10 @@ template <class T, int D> __global__ void __launch_bounds__(kThreads, D <= 128 ?
         return;
     }
     const int groups = a.groups - wide, w = wave * groups + group; // few runs go to as many workgroups
-    const Runs runs = Runs::deal(uniform(header.tiles[0]), kAttentionWaves * groups);
+    if (w >= uniform(header.narrow)) {
+        return;
+    }
+    const Runs runs = Runs::deal(uniform(header.tiles[0]), uniform(header.narrow));
     const int x_end = runs.begin(w + 1);
     int x = runs.begin(w);
     if (x == x_end) {

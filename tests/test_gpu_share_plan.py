@@ -41,9 +41,9 @@ def decode(share):
     assert head[2:5].tolist() == [rows, share.q_heads // share.kv_heads, share.kv_heads]
     lines = words[8:8 + 48 * rows].reshape(2, 3 * rows, 8)
     paths = words[8 + 48 * rows:8 + 88 * rows].reshape(5, rows, 8).transpose(1, 0, 2)
-    groups, wide = head[5:7].tolist()
+    groups, wide, narrow = head[5:8].tolist()
     starts = words[8 + 88 * rows:8 + 88 * rows + 5 * groups]
-    assert 0 <= wide <= groups // 2 and (wide > 0) == (head[1] > 0)
+    assert 0 <= wide <= groups // 2 and (wide > 0) == (head[1] > 0) and 0 < narrow <= 4 * (groups - wide)
     counts = []
     for i in range(2):  # as many as have the line's tiles
         at = n = 0
@@ -51,7 +51,7 @@ def decode(share):
             at += int(lines[i, n, 5]) * share.kv_heads * -(-int(lines[i, n, 1]) // int(lines[i, n, 7]))
             n += 1
         counts.append(n)
-    return [lines[i, :counts[i]] for i in range(2)], head[:2].tolist(), paths, [starts[:4 * (groups - wide)], starts[4 * groups:4 * groups + wide]]
+    return [lines[i, :counts[i]] for i in range(2)], head[:2].tolist(), paths, [starts[:narrow], starts[4 * groups:4 * groups + wide]]
 
 
 def check_plan(share, table, positions, requests, ps):
