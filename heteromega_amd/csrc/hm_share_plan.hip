@@ -10,7 +10,7 @@
 // earlier windows have before that are a row's own.
 //
 // Bound by latency: the launch, and about four reads of the table one after the other for each 4096 tokens that two rows share; then one workgroup's steps, each of
-// which waits for LDS, and with 1024 rows for the issue of four waves' instructions to a SIMD: 9 us for 64 rows, 17 for 1024. A tree of minima for the nearest
+// which waits for LDS, and with 1024 rows for the issue of four waves' instructions to a SIMD: 9 us for 64 rows, 18 for 1024. A tree of minima for the nearest
 // boundaries took 3 us more of either, a search per run for the segment that it begins in 2 to 5 us, arrays indexed by the line (in scratch memory) 2 us.
 #include "hm_device.hpp"
 #include "hm_shared_attention.hpp"

@@ -11,7 +11,7 @@
 // others one of the narrow line, so that a CU has work that reads and work that multiplies.
 //
 // 128 rows, 32 / 8 heads of 128, bf16: 16 384 keys shared by all 84 us (410 TFLOP/s; the products of both halves of the weights are 615), 65 536 keys 253 (543 and 815;
-// a large product reaches 1199); up to 1024 keys of its own for each row 63 us (4.7 TB/s); both 110.
+// a large product reaches 1199); up to 1024 keys of its own for each row 61 us (4.9 TB/s); both 110.
 #include "hm_shared_attention.hpp"
 
 namespace hm {

@@ -23,10 +23,11 @@ __host__ __device__ __forceinline__ int cols_of(int line) { return line == 0 ? k
 // unit takes a workgroup as long as about eight tiles, which counts where units are short: 84 rows of 32 key heads under a window of 30 keys, with 32 units of a tile or
 // two, took 45 us with four of them for each workgroup and 19 with one; 126 rows on 358 keys and 2193 of their own 133 and 94.
 __host__ __device__ __forceinline__ int wide_groups(int wide_tiles, int64_t wide_units, int narrow_tiles, int groups) {
-    const int each = narrow_tiles / 512, long_each = each > 4 ? each : 4, short_each = each > 9 ? each : 9;
-    const int64_t of_long = (static_cast<int64_t>(wide_tiles) + long_each - 1) / long_each, of_short = (wide_tiles + 8 * wide_units + short_each - 1) / short_each;
-    const int64_t most = of_long > of_short ? of_long : of_short < wide_tiles ? of_short : wide_tiles;
-    return most < groups / 2 ? static_cast<int>(most) : groups / 2;
+    const uint32_t each = static_cast<uint32_t>(narrow_tiles) / 512, long_each = each > 4 ? each : 4, short_each = each > 9 ? each : 9;
+    const uint32_t tiles = static_cast<uint32_t>(wide_tiles), units = wide_units < 1 << 24 ? static_cast<uint32_t>(wide_units) : 1u << 24; // more are enough for all
+    const uint32_t of_long = (tiles + long_each - 1) / long_each, of_short = (tiles + 8 * units + short_each - 1) / short_each;
+    const uint32_t most = of_long > of_short ? of_long : of_short < tiles ? of_short : tiles;
+    return most < static_cast<uint32_t>(groups / 2) ? static_cast<int>(most) : groups / 2;
 }
 
 // And the narrow line's runs, of one wave each: of two tiles at least where units have eight or more on the average, since each run leaves a part to join (3 rows of 8628
