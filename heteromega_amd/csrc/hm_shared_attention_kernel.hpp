@@ -91,12 +91,12 @@ struct Pages {
 // and another key head.
 struct PageIds {
     int32_t ids = 0;
-    int first = -1, row = -1, start = 0; // sub-tile of lane 0, and whose keys
+    int first = -1, row = -1, start = 0, end = 0; // sub-tile of lane 0, and whose keys
     bool bad = false;                    // a page outside the cache
 
     __device__ __forceinline__ void read(const Pages &at, const ShareSegment &s, int sub) {
-        if (first != sub || row != s.row0 || start != s.start()) {
-            first = sub, row = s.row0, start = s.start();
+        if (first != sub || row != s.row0 || start != s.start() || end != s.hi) {
+            first = sub, row = s.row0, start = s.start(), end = s.hi;
             ids = at.page_of(start + 16 * (sub + static_cast<int>(threadIdx.x & 63)), s.hi);
             bad = __any(static_cast<uint32_t>(ids) >= at.pages);
         }
