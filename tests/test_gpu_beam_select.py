@@ -141,6 +141,19 @@ def test_rows_without_candidates(hm, device, dtype):
     _check(hm, device, _inputs(device, 5, 12, 4100, dtype)[0], scores, None, -1, 4, 4)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_largest_vocabulary(hm, device, dtype):
+    v = 2 ** 24
+    logits = torch.full((2, v), -math.inf, dtype=DTYPES[dtype], device=device)
+    logits[0, 0] = logits[0, v - 1] = logits[1, 12345] = 1
+    step = hm.BeamStep(1, 2, 4, v, device)
+    hm.beam_select(step, logits, torch.zeros(2, device=device), end_token=v - 1)
+    torch.cuda.synchronize()
+    assert step.parents.tolist() == [[1, 0, 0, -1]] and step.tokens.tolist() == [[12345, 0, v - 1, -1]] and step.ended.tolist() == [[False, False, True, True]]
+    want = torch.tensor([0, -math.log(2), -math.log(2), -math.inf])
+    assert torch.equal(step.scores.cpu()[0, 3], want[3]) and (step.scores.cpu()[0, :3] - want[:3]).abs().max() <= 4 * 2.0 ** -24
+
+
 def test_extreme_logits(hm, device):
     for dtype in DTYPES:
         logits, scores = _inputs(device, 6, 4, 3000, dtype, 100.0)
