@@ -4,7 +4,8 @@
 // them in 16 bits. A wave takes 32 elements a lane of one row into registers and works out its maximum, the sum of exp relative to it and its k best tokens. A
 // second launch, a workgroup per request, joins the waves' sums and picks the k best of their candidates. It is bound by latency: of the waves' best ones only
 // those that reach the k-th score's bound are looked at closely. With all candidates compared it took 26 to 34 us, so 5.5. Candidates of one row are compared by their
-// logits, which are exact; those of different rows by fp64 scores, so that rounding adds no ties.
+// logits, which are exact; those of different rows by fp64 scores, so that rounding adds no ties. Nor may it take any away: which lane sums which tokens, and in
+// which order the sums are joined, goes by the token alone, whichever beam a row is and wherever it begins in memory, so that equal rows have one sum, to the last bit.
 //
 // The k best of a wave's 2048: the k-th largest of the 64 lanes' maxima (above k = 32, of 128 halves' maxima), found by sorting them over the lanes, is a bound that at
 // least k elements reach and seldom many more; those go to a list in LDS and are ranked by counting who comes before. (The least of k or more groups' maxima is
@@ -24,6 +25,9 @@ constexpr int kJoinParts = 1024; // parts that are looked at at once
 constexpr int kRanked = 128;     // candidates that are ranked without a look for a better bound
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+struct __attribute__((packed)) Unaligned {
+    u32x4_t v;
+};
 
 struct Fp32 {
     static __device__ __forceinline__ float to_float(uint32_t bits) { return __uint_as_float(bits); }
@@ -32,10 +36,15 @@ struct Fp32 {
 template <class T> struct Elements {
     static constexpr int kOf16Bytes = 8;
     static __device__ __forceinline__ float get(const u32x4_t &v, int i) { return T::to_float(i & 1 ? v[i / 2] >> 16 : v[i / 2] & 0xFFFFu); }
+    // Element `at` of a row in the place of the i-th, which was zero.
+    static __device__ __forceinline__ void put(u32x4_t &v, int i, const uint8_t *row, int at) {
+        v[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(row)[at]) << (i & 1 ? 16 : 0);
+    }
 };
 template <> struct Elements<Fp32> {
     static constexpr int kOf16Bytes = 4;
     static __device__ __forceinline__ float get(const u32x4_t &v, int i) { return __uint_as_float(v[i]); }
+    static __device__ __forceinline__ void put(u32x4_t &v, int i, const uint8_t *row, int at) { v[i] = reinterpret_cast<const uint32_t *>(row)[at]; }
 };
 
 // A logit and its token as one whole number, in the order of candidates of a row: larger logits first (zeros of either sign are equal), of equal ones lower tokens.
@@ -76,6 +85,15 @@ template <int STEP> __device__ __forceinline__ int2 both(int v) {
                                     : __builtin_bit_cast(pair_t, __builtin_amdgcn_permlane32_swap(bits, bits, false, false));
         return make_int2(static_cast<int>(p.x), static_cast<int>(p.y));
     }
+}
+
+template <int STEP = 1> __device__ __forceinline__ double sum_over_lanes(double v) {
+    const int2 low = both<STEP>(__double2loint(v)), high = both<STEP>(__double2hiint(v));
+    v = __hiloint2double(high.x, low.x) + __hiloint2double(high.y, low.y);
+    if constexpr (STEP < 32) {
+        v = sum_over_lanes<2 * STEP>(v);
+    }
+    return v;
 }
 
 template <int STEP = 1, class F> __device__ __forceinline__ float over_lanes(float v, F f) {
@@ -121,20 +139,43 @@ template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(Beam
     if (part >= a.parts) {
         return;
     }
-    // 16-byte pieces from the one on that holds the row's first element: what lies around the row's elements in its first and last piece is read, not used.
-    const int64_t bytes = 16 / kOne, start = reinterpret_cast<int64_t>(a.logits) + row * a.ld * bytes;
-    const int skip = uniform(static_cast<int>(start & 15) / static_cast<int>(bytes));
-    const int vocabulary = static_cast<int>(a.vocabulary), pieces = (vocabulary + skip + kOne - 1) / kOne;
-    const int first = part * (64 * V);
-    void *const from_piece = reinterpret_cast<void *>((start & ~int64_t(15)) + static_cast<int64_t>(first) * 16);
-    const __amdgpu_buffer_rsrc_t resource = __builtin_amdgcn_make_buffer_rsrc(from_piece, 0, uniform(max(0, min(64 * V, pieces - first)) * 16), 0x00020000);
     if (!is_open(a, row)) {
         return;
     }
-    u32x4_t raw[V];
+    // Pieces of 16 bytes from the row's first element on, which is aligned to its type alone: loads of any alignment take no longer (64 requests of 4 beams, bf16:
+    // 152 061 tokens 25.5 us, 152 064 26.0).
+    const int vocabulary = static_cast<int>(a.vocabulary), first = part * (64 * V);
+    const uint8_t *const from_row = static_cast<const uint8_t *>(a.logits) + row * a.ld * (16 / kOne);
+    int first_token = (first + lane) * kOne;
+    const auto token_of = [&](int j) { return first_token + j / kOne * 64 * kOne + j % kOne; };
+    const auto piece_of = [&](int i) __attribute__((always_inline)) { // zeros behind the row's end
+        const int token = token_of(i * kOne);
+        u32x4_t piece{0, 0, 0, 0};
+        if (token + kOne <= vocabulary) {
+            piece = reinterpret_cast<const Unaligned *>(from_row + static_cast<int64_t>(token) * (16 / kOne))->v;
+        } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) { // behind the last piece: zeros
-        raw[i] = __builtin_amdgcn_raw_buffer_load_b128(resource, lane * 16, i * 1024, 0);
+            for (int e = 0; e < kOne - 1; ++e) {
+                if (token + e < vocabulary) {
+                    E::put(piece, e, from_row, token + e);
+                }
+            }
+        }
+        return piece;
+    };
+    const bool inside = (first + 64 * V) * kOne <= vocabulary;
+    u32x4_t raw[V];
+    if (inside) {
+        const Unaligned *pieces = reinterpret_cast<const Unaligned *>(from_row + static_cast<int64_t>(first) * 16) + lane;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            raw[i] = pieces[64 * i].v;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            raw[i] = piece_of(i);
+        }
     }
     float x[kElements];
 #pragma unroll
@@ -144,13 +185,10 @@ template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(Beam
             x[i * kOne + e] = E::get(raw[i], e);
         }
     }
-    int first_token = (first + lane) * kOne - skip;
-    const auto token_of = [&](int j) { return first_token + j / kOne * 64 * kOne + j % kOne; };
-    if (first == 0 || first + V * 64 >= pieces) { // elements that are not the row's
+    if (!inside) {
 #pragma unroll
         for (int j = 0; j < kElements; ++j) {
-            const int token = token_of(j);
-            x[j] = token >= 0 && token < vocabulary ? x[j] : -INFINITY;
+            x[j] = token_of(j) < vocabulary ? x[j] : -INFINITY;
         }
     }
     float half[2] = {x[0], x[kOne / 2]}; // of the halves of each 16 bytes, so that short rows have both
@@ -250,11 +288,11 @@ template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(Beam
         Candidate best = 0;
 #pragma unroll 1
         for (int j = 0; j < V; ++j) {
-            const u32x4_t piece = __builtin_amdgcn_raw_buffer_load_b128(resource, lane * 16, j * 1024, 0);
+            const u32x4_t piece = piece_of(j);
 #pragma unroll
             for (int e = 0; e < kOne; ++e) {
                 const int32_t t = token_of(j * kOne + e);
-                const float v = t >= 0 && t < vocabulary ? E::get(piece, e) : -INFINITY;
+                const float v = t < vocabulary ? E::get(piece, e) : -INFINITY;
                 const Candidate c = v > -INFINITY ? candidate(v, t) : 0;
                 best = c < last && c > best ? c : best;
             }
@@ -320,12 +358,11 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
     float own = -INFINITY; // the best of those parts that are the lane's: part i of all beams' is lane i % 64's
     for (int beam = wave; beam < beams; beam += kWaves) {
         const int64_t row = row0 + beam;
-        const int shift = (lane - beam * parts) & 63;
         const float2 *stats = ws.stats + row * parts;
         float2 held[kHeld];
 #pragma unroll
         for (int n = 0; n < kHeld; ++n) { // of a row that is not open they are not there, and not used
-            const int i = shift + 64 * n;
+            const int i = lane + 64 * n;
             held[n] = stats[min(i, parts - 1)];
             held[n] = i < parts ? held[n] : make_float2(-INFINITY, 0.0f);
         }
@@ -336,9 +373,9 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
         const auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
             for (int n = 0; n < kHeld; ++n) {
-                f(shift + 64 * n, held[n]);
+                f(lane + 64 * n, held[n]);
             }
-            for (int i = shift + 64 * kHeld; i < parts; i += 64) {
+            for (int i = lane + 64 * kHeld; i < parts; i += 64) {
                 f(i, stats[i]);
             }
         };
@@ -350,7 +387,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
             });
             top = over_lanes(top, [](float v, float w) { return fmaxf(v, w); });
             each([&](int, float2 st) { sum += st.y == 0.0f ? 0.0f : st.y * __builtin_amdgcn_exp2f((st.x - top) * 1.4426950408889634f); });
-            sum = over_lanes(static_cast<float>(sum), [](float v, float w) { return v + w; });
+            sum = sum_over_lanes(sum);
             odd = __any(odd) || !(fabsf(top) < INFINITY);
         }
         const double of_row = static_cast<double>(top) + log(sum), from = (open && odd) || !(fabsf(score) < INFINITY) ? NAN : static_cast<double>(score);
@@ -359,8 +396,9 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
             base[beam] = from;
             was_ended[beam] = ended;
         }
+        float best = -INFINITY;
         const auto put_best = [&](int i, float v) {
-            own = fmaxf(own, v);
+            best = fmaxf(best, v);
             if (beam * parts + i < kJoinParts) {
                 best_of[beam * parts + i] = v;
             }
@@ -371,6 +409,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
                 put_best(i, from != from ? -INFINITY : ended ? (i == 0 ? score : -INFINITY) : rounded_down(from + (static_cast<double>(st.x) - of_row)));
             }
         });
+        own = fmaxf(own, __shfl(best, (lane - beam * parts) & 63));
     }
     maxima[wave][lane] = own;
     __syncthreads();
@@ -521,19 +560,16 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
     }
 }
 
-int64_t parts_of(int64_t vocabulary, int dtype) { // the row may begin within a piece
-    const int64_t one = dtype == HM_LOGITS_FP32 ? 4 : 8, in_part = 64 * kElements;
-    return (vocabulary + one - 1 + in_part - 1) / in_part;
-}
+int64_t parts_of(int64_t vocabulary) { return (vocabulary + 64 * kElements - 1) / (64 * kElements); }
 
 } // namespace
 
-size_t beam_select_workspace(int64_t rows, int64_t vocabulary, int64_t k, int dtype) {
-    return static_cast<size_t>(rows * parts_of(vocabulary, dtype)) * (sizeof(float2) + static_cast<size_t>(k) * sizeof(Candidate));
+size_t beam_select_workspace(int64_t rows, int64_t vocabulary, int64_t k) {
+    return static_cast<size_t>(rows * parts_of(vocabulary)) * (sizeof(float2) + static_cast<size_t>(k) * sizeof(Candidate));
 }
 
 hipError_t launch_beam_select(BeamSelectArgs a, hipStream_t stream) {
-    a.parts = static_cast<int>(parts_of(a.vocabulary, a.dtype));
+    a.parts = static_cast<int>(parts_of(a.vocabulary));
     const dim3 grid(static_cast<unsigned>((a.parts + 3) / 4), static_cast<unsigned>(a.rows));
     switch (a.dtype) {
     case HM_FP16:

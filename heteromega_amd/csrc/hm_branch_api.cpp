@@ -81,7 +81,7 @@ size_t hm_beam_select_workspace_bytes(int64_t R, int64_t beams, int64_t V, int64
     if (check_beams(R, beams, V, k, logits_dtype, "hm_beam_select_workspace_bytes") != HM_OK) {
         return 0;
     }
-    return hm::beam_select_workspace(R * beams, V, k, logits_dtype);
+    return hm::beam_select_workspace(R * beams, V, k);
 }
 
 hm_status hm_beam_select(const void *logits, int64_t ld, int32_t logits_dtype, const float *scores, const uint8_t *ended, int64_t end_token, int64_t R,
@@ -104,7 +104,7 @@ hm_status hm_beam_select(const void *logits, int64_t ld, int32_t logits_dtype, c
     if (k != beams && (scores_out == scores || ended_out == ended)) {
         return set_error(HM_INVALID_ARGUMENT, "%s: results may take the place of scores and ended only where k is the number of beams", what);
     }
-    if ((st = check_workspace(workspace, workspace_bytes, hm::beam_select_workspace(R * beams, V, k, logits_dtype), what)) != HM_OK) {
+    if ((st = check_workspace(workspace, workspace_bytes, hm::beam_select_workspace(R * beams, V, k), what)) != HM_OK) {
         return st;
     }
     const hm::BeamSelectArgs a{logits, ld, logits_dtype, scores, ended, static_cast<int32_t>(end_token), R * beams, static_cast<int>(beams), V,

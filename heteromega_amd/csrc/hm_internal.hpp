@@ -309,7 +309,7 @@ struct BeamSelectArgs {
     void *workspace;
     int parts; // waves of a row; set by the launch
 };
-size_t beam_select_workspace(int64_t rows, int64_t vocabulary, int64_t k, int dtype);
+size_t beam_select_workspace(int64_t rows, int64_t vocabulary, int64_t k);
 hipError_t launch_beam_select(BeamSelectArgs a, hipStream_t stream);
 
 // What rows share (hm_share_plan).

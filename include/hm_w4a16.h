@@ -464,8 +464,9 @@ hm_status hm_paged_attention(const hm_kv_cache *cache, void *out, int64_t ldo, c
  *   tokens [R, k], scores_out [R, k]
  *   ended_out [R, k]  1 if its row had ended or its token is end_token
  * Logits of -infinity are no continuations, nor are those of a row whose score is not finite (-infinity: a beam that is not in use yet) or among whose
- * logits are NaN or +infinity. Where fewer than k are left: parent and token -1, score -infinity, ended 1. Sums are fp32, a row's in the same order
- * each time, their logarithms and the comparison of different rows' candidates fp64. end_token: -1 for none, if `ended` is NULL. beams up to HM_BEAM_MAX_BEAMS, k up to HM_BEAM_MAX_K. With k = beams,
+ * logits are NaN or +infinity. Where fewer than k are left: parent and token -1, score -infinity, ended 1. Sums are fp32 over 2048 tokens and fp64 over
+ * those sums, as are their logarithms and the comparison of different rows' candidates. Their order goes by the token alone: rows of the same logits have the
+ * same sum, whichever beams they are and wherever they begin in memory, so that their equal scores are equal here too. end_token: -1 for none, if `ended` is NULL. beams up to HM_BEAM_MAX_BEAMS, k up to HM_BEAM_MAX_K. With k = beams,
  * scores_out may be scores and ended_out may be ended; other arrays must not overlap. Workspace (16-byte aligned, nothing in it has to start at zero):
  * hm_beam_select_workspace_bytes. */
 #define HM_LOGITS_FP32 2
