@@ -71,7 +71,7 @@ hm_status check_table(const int32_t *table, int64_t ld, int64_t R, int64_t W, in
         return set_error(HM_INVALID_ARGUMENT, "%s: block_table must be [R > 0, W > 0] with a leading dimension >= W, got [%lld, %lld], %lld", what,
                          static_cast<long long>(R), static_cast<long long>(W), static_cast<long long>(ld));
     }
-    // Positions are 32-bit; the attention's tiles may begin up to 15 tokens early and end up to 127 late.
+    // Positions are 32-bit; the attention's tiles may begin up to 15 tokens early and end up to 160 late.
     if (W > (INT32_MAX - 256) / page_size) {
         return set_error(HM_UNSUPPORTED, "%s: W * page_size must stay below 2^31 - 256 tokens, got %lld * %lld", what, static_cast<long long>(W),
                          static_cast<long long>(page_size));

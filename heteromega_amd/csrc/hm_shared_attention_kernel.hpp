@@ -67,7 +67,10 @@ struct Pages {
     int capacity;
     bool there;
 
-    __device__ __forceinline__ int32_t page_of(int key, int hi) const { return key >= hi ? 0 : there && key < capacity ? table[key >> shift] : -1; }
+    // Page numbers are read for up to 2032 keys behind the last one, which may be at the end of 31 bits: the key has 32.
+    __device__ __forceinline__ int32_t page_of(uint32_t key, int hi) const {
+        return key >= static_cast<uint32_t>(hi) ? 0 : there && key < static_cast<uint32_t>(capacity) ? table[key >> shift] : -1;
+    }
     __device__ __forceinline__ Pages(const SharedAttentionArgs &a, int64_t row, int kv_head) {
         // The plan's requests and keys are those of its call, whose table this call's should be: one that is not there is poisoned.
         const int64_t request = a.requests != nullptr ? a.requests[row] : row;
@@ -97,7 +100,7 @@ struct PageIds {
     __device__ __forceinline__ void read(const Pages &at, const ShareSegment &s, int sub) {
         if (first != sub || row != s.row0 || start != s.start() || end != s.hi) {
             first = sub, row = s.row0, start = s.start(), end = s.hi;
-            ids = at.page_of(start + 16 * (sub + static_cast<int>(threadIdx.x & 63)), s.hi);
+            ids = at.page_of(static_cast<uint32_t>(start) + 16 * (static_cast<uint32_t>(sub) + (threadIdx.x & 63)), s.hi);
             bad = __any(static_cast<uint32_t>(ids) >= at.pages);
         }
     }
@@ -386,7 +389,7 @@ template <class T, int D> __device__ __forceinline__ void wide_work(const Shared
         first_id = first;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            ids[i] = at.page_of(start + 16 * (first + 64 * i + lane), hi);
+            ids[i] = at.page_of(static_cast<uint32_t>(start) + 16 * static_cast<uint32_t>(first + 64 * i + lane), hi);
         }
     };
     const auto check_ids = [&] { poisoned |= __any(static_cast<uint32_t>(ids[0]) >= at.pages || static_cast<uint32_t>(ids[1]) >= at.pages); };
