@@ -105,14 +105,17 @@ class PagedCache:
         with _guard(self.device):
             return _workspace(self.attention_workspace_bytes(q_heads), self.device, stream)
 
-
     def shared_attention_workspace_bytes(self, q_heads, rows):
         return _lib.load().hm_shared_attention_workspace_bytes(self._ref, q_heads, rows)
 
     def shared_attention_workspace(self, q_heads, rows, stream=None):
-        """A workspace for shared_attention calls of so many rows on one stream, for any lengths."""
+        """A workspace for shared_attention calls of up to so many rows on one stream, for any lengths."""
         with _guard(self.device):
-            return _workspace(self.shared_attention_workspace_bytes(q_heads, rows), self.device, stream)
+            nbytes = self.shared_attention_workspace_bytes(q_heads, rows)
+            if nbytes == 0:
+                raise ValueError(f"PagedCache.shared_attention_workspace: shared_attention takes up to 4096 rows and query heads that are a multiple of the key heads, got {rows} "
+                                 f"rows, {q_heads} and {self.kv_heads} heads")
+            return _workspace(nbytes, self.device, stream)
 
 
 class PagePlan:
@@ -180,7 +183,7 @@ class _Scratch:
 
     def __init__(self, rows, linear, attention):
         self.rows, self.linear, self.attention, self.captured = rows, linear, attention, False
-        self.shared = None  # shared_attention's workspace, for as many rows as the buffers have
+        self.shared, self.shared_rows, self.shared_captured = None, 0, False  # shared_attention's workspace, for the most rows of such a step
 
 
 class AttnLayer:
@@ -210,7 +213,7 @@ class AttnLayer:
 
     def _scratch(self, rows, cache, stream, shared=False):
         """(normed or projected rows, Q/K/V rows, attention rows, workspaces) of calls on this stream, grown as needed. shared: the attention's workspace is
-        shared_attention's."""
+        shared_attention's, which grows with the rows of such calls alone (32 heads of 128: 73 MB for 64 rows, 409 MB for 4096)."""
         key = _stream(stream, self.device)
         kept = self._buffers.get(key)
         with _on(stream, self.device):
@@ -222,17 +225,24 @@ class AttnLayer:
                 linear = max(w.workspace_bytes(m) for w in (self.wqkv, self.wo) for m in (rows, min(rows, 16)))
                 # attention's workspace does not depend on the rows
                 attention = cache.attention_workspace(self.q_heads) if kept is None else kept.attention
-                kept = self._buffers[key] = _Scratch((new(self.hidden), new(self.wqkv.n), new(self.wo.k)), _workspace(linear, self.device, None), attention)
-            if shared and kept.shared is None:
-                kept.shared = cache.shared_attention_workspace(self.q_heads, kept.rows[0].size(0))
+                before, kept = kept, _Scratch((new(self.hidden), new(self.wqkv.n), new(self.wo.k)), _workspace(linear, self.device, None), attention)
+                self._buffers[key] = kept
+                if before is not None:
+                    kept.shared, kept.shared_rows, kept.shared_captured = before.shared, before.shared_rows, before.shared_captured
+            if shared and kept.shared_rows < rows:
+                if kept.shared_captured:
+                    self._outgrown.append(kept.shared)
+                kept.shared = None  # goes back before the next one is taken
+                kept.shared, kept.shared_rows, kept.shared_captured = cache.shared_attention_workspace(self.q_heads, rows), rows, False
         kept.captured |= capturing
+        kept.shared_captured |= capturing and shared
         return tuple(t[:rows] for t in kept.rows) + (kept.linear, kept.shared if shared else kept.attention)
 
     def block_forward(self, x, norm_weight, cache, plan, block_table, eps=1e-5, stream=None, share=None):
         """In place: x [rows, hidden] += attention(RMSNorm(x) * norm_weight) Wo. The rows are those of `plan` (page_plan of this step): their keys and values
         are written to `cache` first, and each row sees its request's tokens up to its own. Rows that the plan left empty stay as they are. share: share_plan of this
-        step's positions and requests, where rows share pages (up to 4096 rows, the layer's heads and window). The buffers in between are the stream's, also those of a step that was captured on it: such steps, wherever they are replayed, and other calls on the stream must not run at the same
-        time."""
+        step's positions and requests, where rows share pages (up to 4096 rows, the layer's heads and window). The buffers in between are the stream's, also those
+        of a step that was captured on it: such steps, wherever they are replayed, and other calls on the stream must not run at the same time."""
         rows = plan.slots.size(0)
         if x.dim() != 2 or x.size(0) != rows or x.size(1) != self.hidden or x.stride(1) != 1 or x.dtype != self.dtype:
             raise ValueError(f"AttnLayer.block_forward: x must be {self.dtype} [{rows}, {self.hidden}]")
