@@ -373,8 +373,9 @@ template <class T, int D> __device__ __forceinline__ void wide_work(const Shared
     constexpr int kRow = 2 * D, kPlane = kWideTile * kRow; // a tile's keys, or values
     constexpr int kKeySteps = D / 16, kBlocks = D / 32;    // of the first product, and of the second's rows
     // The maximum follows only when a score passes it by more than a factor 2^kSlack, and is one of the scores before their factor
-    // (hm_paged_attention_prompt.hpp). fp16 weights have 2^9 at the maximum, so that they end at 2^15 and lose what is below 2^-33 of it.
-    constexpr float kSlack = Split<T>::kTop > 0.0f ? 6.0f : 16.0f, kTop = Split<T>::kTop > 0.0f ? Split<T>::kTop - kSlack : 0.0f;
+    // (hm_paged_attention_prompt.hpp). Weights end at 2^Split::kTop all the same, so that values may be as large as in narrow units: fp16 ones have 2^9 at the maximum
+    // and lose what is below 2^-33 of it, bf16 ones 2^-16 and 2^-110.
+    constexpr float kSlack = Split<T>::kTop > 0.0f ? 6.0f : 16.0f, kTop = Split<T>::kTop - kSlack;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int col = lane & 31, side = lane >> 5;
     const int columns = k.rows * a.group_heads, start = k.s.start() + k.tile0 * kWideTile, lo = k.s.lo, hi = min(k.s.hi, k.s.start() + k.tile1 * kWideTile);

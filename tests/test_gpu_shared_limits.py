@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import attention_ref as ref
+from test_gpu_shared_attention import Call, prompts
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +69,17 @@ def test_all_keys_of_the_longest_table(hm, device, dtype, heads):
     want = 2 * 2.0 ** (torch.arange(64, device=device) % 3)
     off = (out.double() - want).abs() / want
     assert off.max() <= ref.half_step(TYPES[dtype]) + 2048 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("rows", [3, 40])
+def test_values_near_the_end_of_bf16(hm, device, d, rows):
+    # Scores rise by 15 powers of two behind the first keys, which is less than the maximum has to follow at once; weights times values stay below 2^128 all the same.
+    table, ends = prompts(1, rows, 320, 0, 60, 16)
+    c = Call(hm, device, rows, table, ends, 16, (8, 2), d, "bf16", scale=math.log(2.0))
+    c.cache.k.zero_()
+    c.cache.k[[int(p) for p in c.table[0, 2:20]], :, :, 0] = 15
+    c.cache.v.mul_(2.0 ** 116)  # of 380 normal numbers: sums below 2^127
+    c.q.zero_()
+    c.q[..., 0] = 1
+    c.check(f"{rows} rows, heads of {d}")
