@@ -345,11 +345,31 @@ template <> __device__ __forceinline__ float16_t mfma32<BF16>(uint4 x, uint4 y, 
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, x), __builtin_bit_cast(bf16x8_t, y), c, 0, 0, 0);
 }
 
-// lds_dma16 without the compiler's knowledge: it would have every read of the ring wait for all transfers to it, and which are done is counted here. Bytes and
-// addresses are uniform; `to` is an LDS address. M0 has no other use in these kernels.
-__device__ __forceinline__ void ring_transfer(u32x4_t resource, uint32_t to, uint32_t offset) {
+// N transfers of lds_dma16 to 1024 bytes each, without the compiler's knowledge: it would have every read of the ring wait for all transfers to it, and which are
+// done is counted here. Bytes and addresses are uniform; `to` is an LDS address. M0, which the compiler does not let be named as changed, is left as it was.
+template <int N> __device__ __forceinline__ void ring_transfer(u32x4_t resource, uint32_t to, const uint32_t *offset) {
+    static_assert(N >= 2 && N <= 4, "of the heads' sizes");
 #if defined(__HIP_DEVICE_COMPILE__)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(resource) : "memory");
+    uint32_t before;
+#define HM_FIRST "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %2, 0 offen lds\n\t"
+#define HM_NEXT(OFFSET) "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 " OFFSET ", %2, 0 offen lds\n\t"
+#define HM_LAST "s_mov_b32 m0, %0"
+    if constexpr (N == 2) {
+        asm volatile(HM_FIRST HM_NEXT("%4") HM_LAST : "=&s"(before) : "s"(to), "s"(resource), "v"(offset[0]), "v"(offset[1]) : "memory", "scc");
+    } else if constexpr (N == 3) {
+        asm volatile(HM_FIRST HM_NEXT("%4") HM_NEXT("%5") HM_LAST
+                     : "=&s"(before)
+                     : "s"(to), "s"(resource), "v"(offset[0]), "v"(offset[1]), "v"(offset[2])
+                     : "memory", "scc");
+    } else {
+        asm volatile(HM_FIRST HM_NEXT("%4") HM_NEXT("%5") HM_NEXT("%6") HM_LAST
+                     : "=&s"(before)
+                     : "s"(to), "s"(resource), "v"(offset[0]), "v"(offset[1]), "v"(offset[2]), "v"(offset[3])
+                     : "memory", "scc");
+    }
+#undef HM_FIRST
+#undef HM_NEXT
+#undef HM_LAST
 #else
     (void)resource, (void)to, (void)offset;
 #endif
@@ -435,9 +455,10 @@ template <class T, int D> __device__ __forceinline__ void wide_work(const Shared
 #if defined(__HIP_DEVICE_COMPILE__)
         asm volatile("s_nop 4" ::"s"(resource)); // vector instructions may have written it, and a load may read it 5 cycles later
 #endif
+        constexpr int kAtOnce = S::kSteps < 4 ? S::kSteps : 4;
 #pragma unroll
-        for (int j = 0; j < S::kSteps; ++j) {
-            ring_transfer(resource, ring_at + (tile % kRing) * 2 * kPlane + j * 1024, from[j]);
+        for (int j = 0; j < S::kSteps; j += kAtOnce) {
+            ring_transfer<kAtOnce>(resource, ring_at + (tile % kRing) * 2 * kPlane + j * 1024, from + j);
         }
     };
 #pragma unroll
