@@ -112,7 +112,7 @@ hm_status hm_beam_select(const void *logits, int64_t ld, int32_t logits_dtype, c
     return launched(hm::launch_beam_select(a, reinterpret_cast<hipStream_t>(stream)), what);
 }
 
-size_t hm_page_fork_workspace_bytes(int64_t R, int64_t W) { return R <= 0 || W <= 0 ? 0 : hm::page_fork_workspace(R, W); }
+size_t hm_page_fork_workspace_bytes(int64_t R, int64_t W) { return R <= 0 || W <= 0 ? 0 : hm::page_fork_workspace(R); }
 
 hm_status hm_page_fork(const int32_t *sources, const int32_t *keep, const int32_t *lengths, int64_t R, const int32_t *block_table, int64_t ld_table,
                        int32_t *table_out, int64_t ld_out, int64_t W, int64_t page_size, int32_t *free_pages, int64_t Q, const int64_t *queue_in,
@@ -129,7 +129,7 @@ hm_status hm_page_fork(const int32_t *sources, const int32_t *keep, const int32_
     if (sources == nullptr || lengths == nullptr || copies == nullptr || lengths_out == nullptr) {
         return set_error(HM_INVALID_ARGUMENT, "%s: null pointer", what);
     }
-    if ((st = check_workspace(workspace, workspace_bytes, hm::page_fork_workspace(R, W), what)) != HM_OK) {
+    if ((st = check_workspace(workspace, workspace_bytes, hm::page_fork_workspace(R), what)) != HM_OK) {
         return st;
     }
     const hm::PageForkArgs a{sources, keep, lengths, R, block_table, ld_table, table_out, ld_out, W, log2_of(page_size), free_pages, Q, queue_in,

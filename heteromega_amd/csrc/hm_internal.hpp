@@ -253,7 +253,7 @@ struct PageForkArgs {
     void *workspace;
     int hash_bits; // set by the launch
 };
-size_t page_fork_workspace(int64_t requests, int64_t width);
+size_t page_fork_workspace(int64_t requests);
 hipError_t launch_page_fork(const PageForkArgs &a, hipStream_t stream);
 
 // Pages in use moved below a limit (hm_page_compact).

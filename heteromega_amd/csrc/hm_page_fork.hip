@@ -23,15 +23,14 @@ constexpr int kMaxChunks = 1024; // of columns
 struct ForkWorkspace {
     int64_t *queue;   // [2]: head, tail
     int32_t *chunks;  // [kMaxChunks]: pages that come free in each chunk of columns
-    int32_t *columns; // [W]: and in each column
     int32_t *lengths; // [R]
     int32_t *fresh;   // [R]: whether the request's last page is to be a fresh one
 };
 
-__host__ __device__ __forceinline__ ForkWorkspace carve_fork(void *p, int64_t requests, int64_t width) {
+__host__ __device__ __forceinline__ ForkWorkspace carve_fork(void *p, int64_t requests) {
     uint8_t *b = static_cast<uint8_t *>(p);
-    int32_t *chunks = reinterpret_cast<int32_t *>(b + 16), *columns = chunks + kMaxChunks, *lengths = columns + width;
-    return {reinterpret_cast<int64_t *>(b), chunks, columns, lengths, lengths + requests};
+    int32_t *chunks = reinterpret_cast<int32_t *>(b + 16), *lengths = chunks + kMaxChunks;
+    return {reinterpret_cast<int64_t *>(b), chunks, lengths, lengths + requests};
 }
 
 // Exclusive sum of v over the workgroup's threads; *total: over all of them.
@@ -80,11 +79,6 @@ __device__ __forceinline__ int place_of(int32_t *keys, int bits, int32_t page) {
     }
 }
 
-// A step's requests as all workgroups see them, in LDS.
-struct ForkRequests {
-    int32_t *length, *after, *source; // tokens before and after, and the source or -1
-};
-
 // THREADS threads of at most PER requests each, a chunk of columns per workgroup. APPLY: the second launch.
 template <int THREADS, int PER, bool APPLY> __global__ void __launch_bounds__(THREADS) fork_kernel(PageForkArgs a) {
     extern __shared__ int32_t lds[];
@@ -93,8 +87,8 @@ template <int THREADS, int PER, bool APPLY> __global__ void __launch_bounds__(TH
     constexpr int kNobody = INT32_MAX;
     const int R = static_cast<int>(a.requests_count), shift = a.page_shift, bits = a.hash_bits;
     const int32_t page_tokens = 1 << shift;
-    const ForkWorkspace ws = carve_fork(a.workspace, a.requests_count, a.width);
-    int32_t *length = lds, *after = length + R, *source = after + R;
+    const ForkWorkspace ws = carve_fork(a.workspace, a.requests_count);
+    int32_t *length = lds, *after = length + R, *source = after + R; // tokens before and after, and the source or -1
     int32_t *keys = source + R, *holder = keys + (1 << bits), *owner = holder + (1 << bits);
     const int32_t *lengths = APPLY ? ws.lengths : a.lengths;
     const int per = (R + THREADS - 1) / THREADS, r0 = static_cast<int>(threadIdx.x) * per;
@@ -274,9 +268,6 @@ template <int THREADS, int PER, bool APPLY> __global__ void __launch_bounds__(TH
                 if (i < per && r < R && (after[r] & (page_tokens - 1)) != 0 && b == after[r] >> shift) {
                     ws.fresh[r] = held_at[i] >= 0 && holder[held_at[i]] != rank[i];
                 }
-            }
-            if (threadIdx.x == 0) {
-                ws.columns[b] = total;
             }
             __syncthreads();
         }
@@ -551,7 +542,7 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(CopyPagesArgs a) {
 
 } // namespace
 
-size_t page_fork_workspace(int64_t requests, int64_t width) { return 16 + 4 * static_cast<size_t>(kMaxChunks + width + 2 * requests); }
+size_t page_fork_workspace(int64_t requests) { return 16 + 4 * static_cast<size_t>(kMaxChunks + 2 * requests); }
 
 hipError_t launch_page_fork(const PageForkArgs &a, hipStream_t stream) {
     // A thread per request where a workgroup has them: 256 requests 11.3 us with 256 threads and 12.7 with 1024, 512 of the mixed case's 15 with 1024 and
