@@ -76,7 +76,7 @@ def beam_select(step, logits, scores, ended=None, end_token=-1, stream=None):
 
 
 class PageFork:
-    """What page_fork works out for a block table [requests, width], kept from step to step: copies [requests, 3] (source page, target page, tokens; -1 behind the
+    """What page_fork works out for a block table [requests, up to width], kept from step to step: copies [requests, 3] (source page, target page, tokens; -1 behind the
     last) for copy_pages, lengths and queue after the call. Its workspace is its own: calls with one object must not run at the same time."""
 
     def __init__(self, requests, width, page_size, device="cuda"):
@@ -84,7 +84,7 @@ class PageFork:
         if min(requests, width) < 1:
             raise ValueError(f"PageFork: needs requests and a table of some pages, got {requests}, {width}")
         new = lambda shape, t: torch.full(shape, -1, dtype=t, device=device)
-        self.page_size = page_size
+        self.width, self.page_size = width, page_size
         self.copies, self.lengths, self.queue = new((requests, 3), torch.int32), new((requests,), torch.int32), new((4,), torch.int64)
         self._workspace = _new_workspace(_lib.load().hm_page_fork_workspace_bytes(requests, width), device)
 
@@ -95,6 +95,8 @@ def page_fork(fork, sources, lengths, block_table, free_pages, queue, keep=None,
     ring, listed in fork.copies for copy_pages of each layer's cache. block_table (or table_out) and free_pages are updated; lengths and counters after the call go to
     fork.lengths and fork.queue, or to lengths_out and queue_out, which may be lengths and queue. queue[2] is 1 where the call was refused as a whole (a bad
     source, keep or length, or too few pages or places in the ring), and then nothing has changed. Requests that share pages end here, not in page_plan."""
+    if block_table.dim() == 2 and block_table.size(1) > fork.width:
+        raise ValueError(f"page_fork: the fork is too small, made for {fork.width} blocks of each request, the table has {block_table.size(1)}")
     status = _host.page_fork(fork.copies, fork.lengths, fork.queue, fork._workspace, fork.page_size, sources, lengths, block_table, free_pages, queue, keep, table_out,
                              lengths_out, queue_out, stream)
     if status != _lib.HM_OK:
