@@ -19,6 +19,7 @@ namespace hm {
 namespace {
 
 constexpr int kElements = 32;    // of a lane
+constexpr float kLowest = -3.4028234663852886e38f;
 constexpr int kList = 256;       // candidates that a wave's list holds
 constexpr int kJoinList = 1024;  // and that of a request
 constexpr int kJoinParts = 1024; // parts that are looked at at once
@@ -222,7 +223,7 @@ template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(Beam
         ws.stats[at] = make_float2(top, sum);
     }
     Candidate *out = ws.candidates + at * k;
-    const float bound = fmaxf(best.at(k - 1), -3.4028234663852886e38f); // -infinity is no candidate
+    const float bound = fmaxf(best.at(k - 1), kLowest); // -infinity is no candidate
     Candidate *mine = list[wave];
 #if defined(__HIP_DEVICE_COMPILE__)
     asm volatile("" : "+v"(first_token)); // the tokens are worked out again rather than kept in registers
@@ -333,10 +334,14 @@ __device__ __forceinline__ Scored better(const Scored &a, const Scored &b) { // 
     return Scored{first ? a.score : b.score, first ? a.rest : b.rest};
 }
 
+// Scores as fp32 in their order, none above its score but for those below fp32's range, which are kLowest: -infinity stands for none.
 __device__ __forceinline__ float rounded_down(double v) {
     const float f = static_cast<float>(v);
-    return static_cast<double>(f) > v ? nextafterf(f, -INFINITY) : f;
+    return v > -INFINITY ? fmaxf(static_cast<double>(f) > v ? nextafterf(f, -INFINITY) : f, kLowest) : -INFINITY;
 }
+
+// The bound that such a score is.
+__device__ __forceinline__ double bound_of(float v) { return v > kLowest ? static_cast<double>(v) : -INFINITY; }
 
 // A workgroup per request. The scores of the parts' best candidates bound the k-th score from below, and only parts whose best one reaches that bound are looked at
 // more closely: about k of them.
@@ -453,7 +458,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
         const Scored s = place < k ? scored(lane - place * all, place) : Scored{0, 0};
         own = s.some() ? rounded_down(s.value()) : -INFINITY;
     }
-    double bound = Sorted(own).at(k - 1);
+    double bound = bound_of(Sorted(own).at(k - 1));
     for (;;) {
         __syncthreads(); // the list's last readers are done
         if (threadIdx.x == 0) {
@@ -496,7 +501,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) beam_join_kern
             for (int w = 0; w < kWaves; ++w) {
                 most = fmaxf(most, maxima[w][lane]);
             }
-            const double next = Sorted(most).at(k - 1);
+            const double next = bound_of(Sorted(most).at(k - 1));
             if (next > bound) {
                 bound = next;
                 continue;

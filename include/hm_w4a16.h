@@ -461,7 +461,7 @@ hm_status hm_paged_attention(const hm_kv_cache *cache, void *out, int64_t ldo, c
  * and of a row that has ended (ended [R * beams], 0 or 1; NULL: none) there is one, by end_token, at scores[i]. Per request, best first, equal scores by
  * the lower beam * V + token:
  *   parents [R, k]    row that it continues (hm_page_fork's sources, where k = beams and a row is a request there)
- *   tokens [R, k], scores_out [R, k]
+ *   tokens [R, k], scores_out [R, k] (a score below fp32's range is -infinity)
  *   ended_out [R, k]  1 if its row had ended or its token is end_token
  * Logits of -infinity are no continuations, nor are those of a row whose score is not finite (-infinity: a beam that is not in use yet) or among whose
  * logits are NaN or +infinity. Where fewer than k are left: parent and token -1, score -infinity, ended 1. Sums are fp32 over 2048 tokens and fp64 over

@@ -66,3 +66,20 @@ def test_a_row_has_one_score_wherever_it_lies(hm, device, dtype):
         torch.cuda.synchronize()
         seen.add(step.scores[0, 0].item())
     assert len(seen) == 1
+
+
+def test_scores_below_the_range_of_fp32(hm, device):
+    # Two beams that went on with a masked token, of the type's lowest value, and have one token each that is not: the next ones are masked again, the lowest first
+    lowest = torch.finfo(torch.float32).min
+    for v, token in ((5000, 3000), (9001, 0), (140000, 139999)):
+        for beams in (2, 3, 70):
+            logits = torch.full((beams, v), lowest, device=device)
+            logits[:, token] = 1.0
+            step = hm.BeamStep(1, beams, beams + 4, v, device) if beams < 60 else hm.BeamStep(1, beams, 64, v, device)
+            hm.beam_select(step, logits, torch.full((beams,), -3e38, device=device))
+            torch.cuda.synchronize()
+            print(f"below the range: {beams} beams, {v} tokens", flush=True)
+            masked = [t for t in range(6) if t != token]
+            want = ([(b, token) for b in range(beams)] + [(0, t) for t in masked])[:step.k]
+            assert list(zip(step.parents[0].tolist(), step.tokens[0].tolist())) == want
+            assert (step.scores[0, :min(beams, step.k)].double() + 3e38).abs().max() <= 2.0 ** -23 * 3e38 and (step.scores[0, beams:] == -math.inf).all()
