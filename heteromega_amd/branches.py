@@ -13,11 +13,12 @@ import math
 import torch
 
 from . import _lib
-from .attention import PagedCache, _guard, _host
+from .attention import PagedCache, _guard, _host, kPagePlanMaxRequests
 from .ffn import _call, _workspace
 
 kBeamMaxBeams = 256
 kBeamMaxK = 64
+kBeamMaxRows, kBeamMaxVocabulary = 65535, 1 << 24
 kShareMaxRows = 4096
 
 
@@ -49,6 +50,11 @@ def _new_workspace(nbytes, device):
         return _workspace(nbytes, device, None)
 
 
+def _check_page_size(what, page_size):
+    if not 16 <= page_size <= 1 << 30 or page_size & (page_size - 1):
+        raise ValueError(f"{what}: page_size must be a power of two from 16 to 2^30, got {page_size}")
+
+
 class BeamStep:
     """What beam_select works out for `requests` requests of `beams` beams each, kept from step to step: parents (rows of the logits), tokens, scores
     and ended [requests, k], best first. Its workspace is its own: calls with one step object must not run at the same time."""
@@ -57,6 +63,8 @@ class BeamStep:
         self.device = device = _device(device)
         if min(requests, beams, k, vocabulary) < 1 or beams > kBeamMaxBeams or k > kBeamMaxK:
             raise ValueError(f"BeamStep: needs requests, 1 to {kBeamMaxBeams} beams, k of 1 to {kBeamMaxK} and a vocabulary, got {requests}, {beams}, {k}, {vocabulary}")
+        if requests * beams > kBeamMaxRows or vocabulary > kBeamMaxVocabulary:
+            raise ValueError(f"BeamStep: at most {kBeamMaxRows} rows and {kBeamMaxVocabulary} tokens, got {requests} x {beams} and {vocabulary}")
         self.requests, self.beams, self.k, self.vocabulary = requests, beams, k, vocabulary
         new = lambda v, t: torch.full((requests, k), v, dtype=t, device=device)
         self.parents, self.tokens, self.scores, self.ended = new(-1, torch.int32), new(-1, torch.int32), new(-math.inf, torch.float32), new(True, torch.bool)
@@ -81,8 +89,9 @@ class PageFork:
 
     def __init__(self, requests, width, page_size, device="cuda"):
         self.device = device = _device(device)
-        if min(requests, width) < 1:
-            raise ValueError(f"PageFork: needs requests and a table of some pages, got {requests}, {width}")
+        if not 1 <= requests <= kPagePlanMaxRequests or width < 1:
+            raise ValueError(f"PageFork: needs 1 to {kPagePlanMaxRequests} requests and a table of some pages, got {requests}, {width}")
+        _check_page_size("PageFork", page_size)
         new = lambda shape, t: torch.full(shape, -1, dtype=t, device=device)
         self.width, self.page_size = width, page_size
         self.copies, self.lengths, self.queue = new((requests, 3), torch.int32), new((requests,), torch.int32), new((4,), torch.int64)
@@ -112,6 +121,7 @@ class PageCompact:
         self.device = device = _device(device)
         if pages < 1:
             raise ValueError(f"PageCompact: needs a cache of some pages, got {pages}")
+        _check_page_size("PageCompact", page_size)
         self.pages, self.page_size = pages, page_size
         self.copies = torch.full((max(1, pages // 2), 3), -1, dtype=torch.int32, device=device)
         self.queue = torch.full((4,), -1, dtype=torch.int64, device=device)
@@ -154,6 +164,7 @@ class SharePlan:
         if not 1 <= rows <= kShareMaxRows or kv_heads < 1 or q_heads < 1 or q_heads % kv_heads or q_heads // kv_heads > 128 or window < 0:
             raise ValueError(f"SharePlan: needs 1 to {kShareMaxRows} rows, query heads that are a multiple (up to 128) of the key heads and a window that is not negative, got "
                              f"{rows}, {q_heads}, {kv_heads}, {window}")
+        _check_page_size("SharePlan", page_size)
         self.rows, self.page_size, self.q_heads, self.kv_heads, self.window = rows, page_size, q_heads, kv_heads, window
         self.shared = torch.zeros(rows, dtype=torch.int32, device=device)
         self._plan = _new_workspace(_lib.load().hm_share_plan_bytes(rows), device)
@@ -182,5 +193,5 @@ def shared_attention(out, q, cache, block_table, positions, share, requests=None
     return out
 
 
-__all__ = ["kBeamMaxBeams", "kBeamMaxK", "kShareMaxRows", "BeamStep", "beam_select", "PageFork", "page_fork", "PageCompact", "page_compact", "copy_pages", "SharePlan",
+__all__ = ["kBeamMaxBeams", "kBeamMaxK", "kBeamMaxRows", "kBeamMaxVocabulary", "kShareMaxRows", "BeamStep", "beam_select", "PageFork", "page_fork", "PageCompact", "page_compact", "copy_pages", "SharePlan",
            "share_plan", "shared_attention"]
