@@ -347,11 +347,12 @@ template <> __device__ __forceinline__ float16_t mfma32<BF16>(uint4 x, uint4 y, 
 
 // N transfers of lds_dma16 to 1024 bytes each, without the compiler's knowledge: it would have every read of the ring wait for all transfers to it, and which are
 // done is counted here. Bytes and addresses are uniform; `to` is an LDS address. M0, which the compiler does not let be named as changed, is left as it was.
+// A vector instruction may write the resource right before (the compiler gets spilled scalars back that way), and a load may read it 5 cycles later: the block waits.
 template <int N> __device__ __forceinline__ void ring_transfer(u32x4_t resource, uint32_t to, const uint32_t *offset) {
     static_assert(N >= 2 && N <= 4, "of the heads' sizes");
 #if defined(__HIP_DEVICE_COMPILE__)
     uint32_t before;
-#define HM_FIRST "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %2, 0 offen lds\n\t"
+#define HM_FIRST "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %3, %2, 0 offen lds\n\t"
 #define HM_NEXT(OFFSET) "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 " OFFSET ", %2, 0 offen lds\n\t"
 #define HM_LAST "s_mov_b32 m0, %0"
     if constexpr (N == 2) {
@@ -452,9 +453,6 @@ template <class T, int D> __device__ __forceinline__ void wide_work(const Shared
         const uint64_t address = reinterpret_cast<uint64_t>(head + at.offset(page, key, seen));
         const u32x4_t resource{static_cast<uint32_t>(uniform(static_cast<int>(address))), static_cast<uint32_t>(uniform(static_cast<int>(address >> 32))) & 0xFFFFu,
                                at.bytes<D>(seen), 0x00020000u};
-#if defined(__HIP_DEVICE_COMPILE__)
-        asm volatile("s_nop 4" ::"s"(resource)); // vector instructions may have written it, and a load may read it 5 cycles later
-#endif
         constexpr int kAtOnce = S::kSteps < 4 ? S::kSteps : 4;
 #pragma unroll
         for (int j = 0; j < S::kSteps; j += kAtOnce) {
