@@ -154,7 +154,7 @@ template <class T> __global__ void __launch_bounds__(256) beam_parts_kernel(Beam
         u32x4_t piece{0, 0, 0, 0};
         if (token + kOne <= vocabulary) {
             piece = reinterpret_cast<const Unaligned *>(from_row + static_cast<int64_t>(token) * (16 / kOne))->v;
-        } else {
+        } else if (token < vocabulary) {
 #pragma unroll
             for (int e = 0; e < kOne - 1; ++e) {
                 if (token + e < vocabulary) {
