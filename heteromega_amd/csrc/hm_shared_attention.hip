@@ -10,8 +10,8 @@
 // (Units of 17 to 32 columns as wide ones, of which one wave in four had work: 88 us instead of 81 at 256 rows in groups of 8 with 4 query heads to a key head.) The tiles of each kind lie in a line that is cut into equal runs. The first workgroups, one per CU at most, have a run of the wide line each, the waves of the
 // others one of the narrow line, so that a CU has work that reads and work that multiplies.
 //
-// 128 rows, 32 / 8 heads of 128, bf16: 16 384 keys shared by all 84 us (410 TFLOP/s; the products of both halves of the weights are 615), 65 536 keys 253 (543 and 815;
-// a large product reaches 1199); up to 1024 keys of its own for each row 61 us (4.9 TB/s); both 110.
+// 128 rows, 32 / 8 heads of 128, bf16: 16 384 keys shared by all 81 us (424 TFLOP/s; the products of both halves of the weights are 636), 65 536 keys 248 (554 and 831;
+// a large product reaches 1199); up to 1024 keys of its own for each row 58 us (5.1 TB/s); both 95 to 107.
 #include "hm_shared_attention.hpp"
 
 namespace hm {

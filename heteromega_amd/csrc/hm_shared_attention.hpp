@@ -19,7 +19,7 @@ __host__ __device__ __forceinline__ int cols_of(int line) { return line == 0 ? k
 // The workgroups that the wide line gets: one per CU at most, since two are hardly faster and leave twice the parts, and no more than have four tiles each. A
 // wide run has one tile for each 512 narrow ones of the call, so that with many narrow tiles the wide line ends before the narrow one and leaves it most of the
 // card: the card reads 500 to 600 tiles of heads of 128 while a workgroup works on one wide tile. 256 rows whose 6.4k keys were shared by all and, mostly, by 8 took
-// 67 us so and 79 with a workgroup per CU; 16 384 keys shared by 128 rows with 1024 of their own 110 either way, and no less with fewer. To begin and end a
+// 67 us so and 79 with a workgroup per CU; 16 384 keys shared by 128 rows with 1024 of their own as long either way, and no less with fewer. To begin and end a
 // unit takes a workgroup as long as about eight tiles, which counts where units are short: 84 rows of 32 key heads under a window of 30 keys, with 32 units of a tile or
 // two, took 45 us with four of them for each workgroup and 19 with one; 126 rows on 358 keys and 2193 of their own 133 and 94.
 __host__ __device__ __forceinline__ int wide_groups(int wide_tiles, int64_t wide_units, int narrow_tiles, int groups) {
