@@ -232,7 +232,7 @@ class AttnLayer:
             if shared and kept.shared_rows < rows:
                 if kept.shared_captured:
                     self._outgrown.append(kept.shared)
-                kept.shared = None  # goes back before the next one is taken
+                kept.shared, kept.shared_rows = None, 0  # goes back before the next one is taken, which may fail
                 kept.shared, kept.shared_rows, kept.shared_captured = cache.shared_attention_workspace(self.q_heads, rows), rows, False
         kept.captured |= capturing
         kept.shared_captured |= capturing and shared

@@ -124,3 +124,18 @@ def test_workspaces_that_no_call_would_take_are_refused(hm, device, served):
     q = torch.zeros((REQUESTS, Q_HEADS, D), dtype=torch.bfloat16, device=device)
     with pytest.raises(ValueError):
         hm.shared_attention(torch.zeros_like(q), q, three, s.table, s.plan.positions, hm.SharePlan(REQUESTS, PS, Q_HEADS, KV_HEADS, device), s.plan.requests)
+
+
+def test_a_workspace_that_could_not_be_had_is_taken_again(hm, device, served):
+    model, s = served
+    layer, cache = model.attn[0], s.caches[0]
+    assert layer._scratch(40, cache, None, True)[-1] is _held(layer).shared
+
+    class Full:
+        def shared_attention_workspace(self, q_heads, rows):
+            raise torch.OutOfMemoryError
+
+    with pytest.raises(torch.OutOfMemoryError):
+        layer._scratch(80, Full(), None, True)
+    workspace = layer._scratch(REQUESTS, cache, None, True)[-1]
+    assert workspace is _held(layer).shared and workspace.numel() == cache.shared_attention_workspace_bytes(Q_HEADS, REQUESTS) + 256
